@@ -22,14 +22,14 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 OUT = PKG / "candle_fused_attn" / "libcfa.so"
 SOURCES = ["fwd_ffma.cu", "fwd_tc.cu", "bwd_ffma.cu", "bwd_tc.cu", "hd_ffma.cu", "linear_tc.cu",
-           "cfa_abi.cu", "cfa_noalloc.cu"]
+           "rotary.cu", "split_attn.cu", "cfa_abi.cu", "cfa_ops_abi.cu", "cfa_noalloc.cu"]
 HOST_DIR = PKG / "host"
 HOST_OUT = PKG / "candle_fused_attn" / "libcfa_host.so"
 HOST_SOURCES = ["tensor.cu", "candle_fused_attn.cpp"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
-    "-lineinfo", "-O3", "-std=c++17",
+    "-lineinfo", "-O3", "-std=c++17", "--threads", "0",
     "-Xcompiler", "-fPIC", "-shared",
     "-Xptxas", "-v",
 ]

@@ -29,6 +29,12 @@ Next to the path, the projection of the reference's training step (examples/tuto
   w [k, n], differentiable in both (dx = dy w^T, dw = x^T dy), on the tensor-core GEMM of the C ABI
   (`cfa_matmul_f32`); `matmul(a, b)` is the 2-D product itself.
 
+Beside the fused attention, without a counterpart in the crate:
+- `cross_attention(q, k, v, scale, key_lengths)`: queries over another sequence's keys (cross.py);
+- `rotary`, `rotary_qkv`, `rotary_frequencies`: rotary positions between the projection and the
+  attention (positions.py);
+- `paged_append`, `paged_attention`: a decoding step over a paged key-value cache (paged.py).
+
 Failure detection: every device-side wait of the kernels is bounded. An expired wait (results
 invalid) is written by the kernel into a page-locked host flag this module registers with the C
 ABI (`cfa_error_sink`), so the next call of any function here raises `FusedAttentionError`
@@ -57,6 +63,12 @@ __all__ = [
     "matmul",
     "broadcast_matmul",
     "HostPipeline",
+    "cross_attention",
+    "rotary",
+    "rotary_qkv",
+    "rotary_frequencies",
+    "paged_append",
+    "paged_attention",
 ]
 
 CUDA_HEAD_DIM = 64  # src/lib.rs:91
@@ -375,3 +387,6 @@ def broadcast_matmul(x: torch.Tensor, w: torch.Tensor) -> torch.Tensor:
 
 
 from .host_pipeline import HostPipeline  # noqa: E402  (uses _abi; public host-buffer API)
+from .cross import cross_attention  # noqa: E402  (these use the checks and launch helpers above)
+from .paged import paged_append, paged_attention  # noqa: E402
+from .positions import rotary, rotary_frequencies, rotary_qkv  # noqa: E402

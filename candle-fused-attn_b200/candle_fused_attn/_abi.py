@@ -26,6 +26,15 @@ CFA_ERR_WORKSPACE = 6
 CFA_ERR_LAUNCH = 7
 CFA_ERR_TIMEOUT = 8
 CFA_ERR_CUDA = 9
+CFA_ERR_PAGE = 10
+CFA_ERR_TYPE = 11
+CFA_ERR_HEADS = 12
+CFA_ERR_ROTARY = 13
+
+# include/cfa.h enum cfa_dtype
+CFA_F32 = 0
+CFA_F16 = 1
+CFA_BF16 = 2
 
 # Every symbol include/cfa.h declares.
 EXPORTS = (
@@ -52,6 +61,15 @@ EXPORTS = (
     "cfa_matmul_status",
     "cfa_fwd_f32_ffma",
     "cfa_bwd_f32_ffma",
+    "cfa_cross_fwd_f32",
+    "cfa_cross_bwd_workspace_bytes",
+    "cfa_cross_bwd_f32",
+    "cfa_cross_few_workspace_bytes",
+    "cfa_cross_few_f32",
+    "cfa_rotary",
+    "cfa_paged_append",
+    "cfa_paged_attention_workspace_bytes",
+    "cfa_paged_attention",
 )
 
 # Head dims the generic entry points (cfa_fwd_f32, cfa_bwd_f32) take; the _d64 ones take 64 only,
@@ -133,6 +151,33 @@ def load() -> ctypes.CDLL:
         fn = getattr(lib, name)
         fn.restype = ctypes.c_size_t
         fn.argtypes = [_i64, _i64, _i64, _i64]
+    _f, _d, _n = ctypes.c_float, ctypes.c_int, ctypes.c_size_t
+    lib.cfa_cross_fwd_f32.restype = ctypes.c_int
+    lib.cfa_cross_fwd_f32.argtypes = [_p, _strides, _p, _strides, _p, _strides, _p, _p, _p,
+                                      *[_i64] * 6, _f, _p]
+    lib.cfa_cross_bwd_workspace_bytes.restype = _n
+    lib.cfa_cross_bwd_workspace_bytes.argtypes = [_i64] * 6
+    lib.cfa_cross_bwd_f32.restype = ctypes.c_int
+    lib.cfa_cross_bwd_f32.argtypes = [_p, _strides, _p, _strides, _p, _strides, _p, _p, _p, _p,
+                                      _strides, _p, _p, _p, _n, *[_i64] * 6, _f, _p]
+    lib.cfa_cross_few_workspace_bytes.restype = _n
+    lib.cfa_cross_few_workspace_bytes.argtypes = [_i64] * 5
+    lib.cfa_cross_few_f32.restype = ctypes.c_int
+    lib.cfa_cross_few_f32.argtypes = [_p, _strides, _p, _strides, _p, _strides, _p, _p, _p, _n,
+                                      *[_i64] * 6, _f, _p]
+    lib.cfa_rotary.restype = ctypes.c_int
+    lib.cfa_rotary.argtypes = [_p, _strides, _p, _strides, _d, _p, _d, _strides, _i64, _p, _f,
+                               *[_i64] * 6, _d, _d, _p]
+    lib.cfa_paged_append.restype = ctypes.c_int
+    lib.cfa_paged_append.argtypes = [_p, _strides, _p, _strides, _p, _strides, _p, _strides, _d,
+                                     _p, _strides, _p, _strides, _d, _i64, _i64, _p, _i64, _i64,
+                                     _p, _p, _p, _f, *[_i64] * 6, _d, _p]
+    lib.cfa_paged_attention_workspace_bytes.restype = _n
+    lib.cfa_paged_attention_workspace_bytes.argtypes = [_i64] * 5
+    lib.cfa_paged_attention.restype = ctypes.c_int
+    lib.cfa_paged_attention.argtypes = [_p, _strides, _d, _p, _strides, _p, _strides, _d, _i64,
+                                        _i64, _p, _i64, _i64, _p, _p, _p, _p, _n, *[_i64] * 5, _f,
+                                        _p]
     _lib = lib
     return lib
 
@@ -290,3 +335,70 @@ def matmul(a_ptr, a_rs, a_cs, b_ptr, b_rs, b_cs, c_ptr, c_rs, m, n, k, ws_ptr, w
 
 def matmul_status(stream) -> int:
     return load().cfa_matmul_status(stream)
+
+
+def cross_fwd(q_ptr, qs, k_ptr, ks, v_ptr, vs, lengths_ptr, o_ptr, lse_ptr, b, h, hk, sq, sk, d,
+              scale, stream) -> int:
+    """cfa_cross_fwd_f32; returns the status."""
+    return load().cfa_cross_fwd_f32(
+        q_ptr, strides3(qs), k_ptr, strides3(ks), v_ptr, strides3(vs), lengths_ptr, o_ptr, lse_ptr,
+        b, h, hk, sq, sk, d, scale, stream)
+
+
+def cross_bwd_workspace_bytes(b, h, hk, sq, sk, d) -> int:
+    return int(load().cfa_cross_bwd_workspace_bytes(b, h, hk, sq, sk, d))
+
+
+def cross_bwd(q_ptr, qs, k_ptr, ks, v_ptr, vs, lengths_ptr, o_ptr, lse_ptr, do_ptr, dos, dq_ptr,
+              dkv_ptr, ws_ptr, ws_bytes, b, h, hk, sq, sk, d, scale, stream) -> int:
+    """cfa_cross_bwd_f32; returns the status."""
+    return load().cfa_cross_bwd_f32(
+        q_ptr, strides3(qs), k_ptr, strides3(ks), v_ptr, strides3(vs), lengths_ptr, o_ptr, lse_ptr,
+        do_ptr, strides3(dos), dq_ptr, dkv_ptr, ws_ptr, ws_bytes, b, h, hk, sq, sk, d, scale,
+        stream)
+
+
+def cross_few_workspace_bytes(b, h, sq, sk, d) -> int:
+    return int(load().cfa_cross_few_workspace_bytes(b, h, sq, sk, d))
+
+
+def cross_few(q_ptr, qs, k_ptr, ks, v_ptr, vs, lengths_ptr, o_ptr, ws_ptr, ws_bytes, b, h, hk, sq,
+              sk, d, scale, stream) -> int:
+    """cfa_cross_few_f32 (the forward for few query rows a key head); returns the status."""
+    return load().cfa_cross_few_f32(
+        q_ptr, strides3(qs), k_ptr, strides3(ks), v_ptr, strides3(vs), lengths_ptr, o_ptr, ws_ptr,
+        ws_bytes, b, h, hk, sq, sk, d, scale, stream)
+
+
+def rotary(x_ptr, xs, y_ptr, ys, dtype, pos_ptr, pos_bytes, pos_strides, first, freqs_ptr,
+           amplitude, b, h, rotated, s, d, rot, interleaved, inverse, stream) -> int:
+    """cfa_rotary; returns the status. `pos_strides`: (batch, seq), or None without positions."""
+    return load().cfa_rotary(
+        x_ptr, strides3(xs), y_ptr, strides3(ys), dtype, pos_ptr, pos_bytes,
+        None if pos_strides is None else (ctypes.c_int64 * 2)(*pos_strides), first, freqs_ptr,
+        amplitude, b, h, rotated, s, d, rot, int(interleaved), int(inverse), stream)
+
+
+def paged_append(q_ptr, qs, qo_ptr, qos, k_ptr, ks, v_ptr, vs, dtype, kc_ptr, kcs, vc_ptr, vcs,
+                 cache_dtype, pages, page_size, table_ptr, table_stride, table_width, lengths_ptr,
+                 new_ptr, freqs_ptr, amplitude, b, h, hk, s, d, rot, interleaved, stream) -> int:
+    """cfa_paged_append; returns the status. `qs`, `qos`: None without q."""
+    return load().cfa_paged_append(
+        q_ptr, None if qs is None else strides3(qs), qo_ptr, None if qos is None else strides3(qos),
+        k_ptr, strides3(ks), v_ptr, strides3(vs), dtype, kc_ptr, strides3(kcs), vc_ptr,
+        strides3(vcs), cache_dtype, pages, page_size, table_ptr, table_stride, table_width,
+        lengths_ptr, new_ptr, freqs_ptr, amplitude, b, h, hk, s, d, rot, int(interleaved), stream)
+
+
+def paged_attention_workspace_bytes(b, h, s, max_keys, d) -> int:
+    return int(load().cfa_paged_attention_workspace_bytes(b, h, s, max_keys, d))
+
+
+def paged_attention(q_ptr, qs, dtype, kc_ptr, kcs, vc_ptr, vcs, cache_dtype, pages, page_size,
+                    table_ptr, table_stride, table_width, lengths_ptr, new_ptr, o_ptr, ws_ptr,
+                    ws_bytes, b, h, hk, s, d, scale, stream) -> int:
+    """cfa_paged_attention; returns the status."""
+    return load().cfa_paged_attention(
+        q_ptr, strides3(qs), dtype, kc_ptr, strides3(kcs), vc_ptr, strides3(vcs), cache_dtype,
+        pages, page_size, table_ptr, table_stride, table_width, lengths_ptr, new_ptr, o_ptr,
+        ws_ptr, ws_bytes, b, h, hk, s, d, scale, stream)

@@ -230,9 +230,15 @@ __device__ __forceinline__ void bar_sync(int id, int count) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(count) : "memory");
 }
 
-template <bool CAUSAL, int HD>
+// CROSS (cross attention): the keys have a length of their own (a.Sk rows, the first
+// cross_keys(a, b) attended), and a key block belongs to a key head: it walks the query tiles of
+// every query head of the group, one head after the other, so dV and dK of a shared head are summed
+// in registers in that order. Key blocks past a batch element's length write zeros and take no part.
+// dQ and dK, dV go to buffers of their own (a.dq, a.dkv).
+template <bool CAUSAL, int HD, bool CROSS = false>
 __global__ void __launch_bounds__(NB, 1) bwd_tc_kernel(const BwdArgs a) {
   static_assert(HD == 64 || HD == 32, "head dims of the tensor-core backward");
+  static_assert(!(CAUSAL && CROSS), "cross attention has no causal mask");
   constexpr int KSD = HD / 16;  // K-steps of the products that reduce over the head dim
   constexpr int WIN = TailWindow<HD>::WIN;
   constexpr auto win4 = TailWindow<HD>::item;
@@ -262,8 +268,10 @@ __global__ void __launch_bounds__(NB, 1) bwd_tc_kernel(const BwdArgs a) {
   const int row = 32 * (w & 3) + lane;  // key row: TMEM lane (compute warps)
   const int cg = (w >> 2) & 3;          // column group: 16 queries (S, dP) or dims (dV, dK, dQ)
   const int S = a.S;
-  const int nkb = a.n_kblocks;
-  const int BH = a.B * a.H;
+  const int HU = CROSS ? a.Hk : a.H;  // heads that own key blocks
+  const int BH = a.B * HU;
+  int nkb = a.n_kblocks;  // key blocks of this (batch, head) that take part
+  if constexpr (CROSS) griddep_wait();  // the lengths may come from the previous kernels
   // The work item. With the dQ partials (no-wait path): the block index, (b, h)-major, so a
   // (b, h)'s key blocks run side by side and its last one finishes early. With the turn chain: a
   // ticket drawn after the prep kernel's wait, key-block-major -- a block waits only on key block
@@ -299,23 +307,61 @@ __global__ void __launch_bounds__(NB, 1) bwd_tc_kernel(const BwdArgs a) {
     part = g + 1 < nparts ? g + 1 : 0;
     ticket = a.tail_base + tail_r;
   }
-  const int kb = chain ? ticket / BH : ticket % nkb;
-  const int bh = chain ? ticket % BH : ticket / nkb;
-  const int b = bh / a.H, h = bh % a.H;
+  const int kb = chain ? ticket / BH : ticket % a.n_kblocks;
+  const int bh = chain ? ticket % BH : ticket / a.n_kblocks;
+  const int b = bh / HU, h = bh % HU;
   const int k0 = kb * KB;
-  const float* qp = a.q + b * a.q_sb + h * a.q_sh;
+  const int group = CROSS ? a.H / a.Hk : 1;  // query heads of the key block
+  const int h0 = h * group, nqt = (S + QT - 1) / QT;
+  int SK = S;  // keys
+  if constexpr (CROSS) {
+    SK = cross_keys(a, b);
+    nkb = (SK + KB - 1) / KB;
+    if (kb >= nkb) {  // no key of this block is attended: zeros, and no part in dQ's sums
+      griddep_launch_dependents();
+      if (part != 0) return;
+      constexpr int C4 = HD / 4;
+      const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
+      const int rows = min(KB, a.Sk - k0);
+      for (int f = tid; f < 2 * rows * C4; f += NB) {
+        const int which = f / (rows * C4), r = (f / C4) % rows;
+        reinterpret_cast<float4*>(
+            a.dkv + (((static_cast<int64_t>(b) * a.Sk + k0 + r) * 2 + which) * a.Hk + h) * HD)[f % C4] = zero;
+      }
+      if (kb == 0)  // no key at all: dQ = 0
+        for (int64_t f = tid; f < static_cast<int64_t>(S) * group * C4; f += NB)
+          reinterpret_cast<float4*>(a.dq + ((static_cast<int64_t>(b) * S + f / (group * C4)) * a.H + h0) *
+                                               HD)[f % (group * C4)] = zero;
+      return;
+    }
+  }
   const float* kp = a.k + b * a.k_sb + h * a.k_sh;
   const float* vp = a.v + b * a.v_sb + h * a.v_sh;
+  const float* qp = a.q + b * a.q_sb + h * a.q_sh;
   const float* gp = a.d_o + b * a.do_sb + h * a.do_sh;
   const float* lp = a.lse + static_cast<int64_t>(bh) * S;
   const float* dp = a.dsum + static_cast<int64_t>(bh) * S;
+  // The query head and first query of the block's tile t, and that head's operands.
+  auto tile_head = [&](int t) { return CROSS ? h0 + t / nqt : h; };
+  auto tile_q0 = [&](int t) { return (CROSS ? t % nqt : t) * QT; };
+  auto q_rows = [&](int t) { return CROSS ? a.q + b * a.q_sb + tile_head(t) * a.q_sh : qp; };
+  auto g_rows = [&](int t) { return CROSS ? a.d_o + b * a.do_sb + tile_head(t) * a.do_sh : gp; };
+  auto query_bh = [&](int t) {
+    return CROSS ? static_cast<int64_t>(b) * a.H + tile_head(t) : static_cast<int64_t>(bh);
+  };
   const int t_first = CAUSAL ? k0 / QT : 0;  // queries before the block's first key see none
-  const int n_all = (S + QT - 1) / QT - t_first;  // the key block's query tiles, >= 1 (k0 < S)
+  const int n_all = group * nqt - t_first;  // the key block's query tiles, >= 1 (k0 < SK)
   const int n_lo = part * n_all / nparts, n_hi = (part + 1) * n_all / nparts;
   const int t_begin = t_first + n_lo;  // this block's first query tile
-  int* turn = a.turn + static_cast<int64_t>(bh) * a.n_qtiles;  // turn chain: per 64-query tile
-  const int64_t row_stride = 3 * static_cast<int64_t>(a.H) * HD;  // dqkv floats per (b, s)
-  float* dq_base = a.dqkv + static_cast<int64_t>(b) * S * row_stride + h * HD;
+  // Turn chain: counters per 64-query tile of a query head.
+  int* turn = a.turn + (CROSS ? (static_cast<int64_t>(b) * a.H + h0) * nqt
+                              : static_cast<int64_t>(bh) * a.n_qtiles);
+  // dqkv (CROSS: dq) floats per (b, s), and a query head's dQ rows.
+  const int64_t row_stride = (CROSS ? 1 : 3) * static_cast<int64_t>(a.H) * HD;
+  float* dq_base = (CROSS ? a.dq : a.dqkv) + static_cast<int64_t>(b) * S * row_stride + h * HD;
+  auto dq_rows = [&](int head) {
+    return CROSS ? a.dq + static_cast<int64_t>(b) * S * row_stride + head * HD : dq_base;
+  };
   const int N = n_hi - n_lo;  // this block's query tiles, >= 1 (a.tail_parts <= n_all)
   bool err0 = false;
 
@@ -329,7 +375,7 @@ __global__ void __launch_bounds__(NB, 1) bwd_tc_kernel(const BwdArgs a) {
     tc::mbar_init(bar_p, NT / 32);
     tc::mbar_init(bar_dv, 1);
     tc::fence_mbar_init();
-    tc::mbar_arrive_expect_tx(bar_ld, 4u * HD * (2 * min(KB, S - k0) + 2 * min(QT, S - t_begin * QT)));
+    tc::mbar_arrive_expect_tx(bar_ld, 4u * HD * (2 * min(KB, SK - k0) + 2 * min(QT, S - tile_q0(t_begin))));
   }
   griddep_launch_dependents();
 
@@ -337,16 +383,17 @@ __global__ void __launch_bounds__(NB, 1) bwd_tc_kernel(const BwdArgs a) {
   // L / D buffer n % 2 (threads 0-127).
   auto stage_ld = [&](int n) {
     if (tid < 2 * QT) {
-      const int r = tid & 63, i = (t_begin + n) * QT + r;
+      const int r = tid & 63, i = tile_q0(t_begin + n) + r;
       const bool ok = i < S;
-      cp_async4(ld + (n & 1) * 128 + (tid < QT ? 0 : QT) + r, (tid < QT ? lp : dp) + (ok ? i : 0),
-                ok ? 4 : 0);
+      const float* src = CROSS ? (tid < QT ? a.lse : a.dsum) + query_bh(t_begin + n) * S
+                               : (tid < QT ? lp : dp);
+      cp_async4(ld + (n & 1) * 128 + (tid < QT ? 0 : QT) + r, src + (ok ? i : 0), ok ? 4 : 0);
     }
   };
   auto stage_tile = [&](int n) {
-    const int q0 = (t_begin + n) * QT;
-    stage_row_item<HD>(st, 0, tid, qp, a.q_ss, q0, S);
-    stage_row_item<HD>(st, 1, tid, gp, a.do_ss, q0, S);
+    const int q0 = tile_q0(t_begin + n);
+    stage_row_item<HD>(st, 0, tid, q_rows(t_begin + n), a.q_ss, q0, S);
+    stage_row_item<HD>(st, 1, tid, g_rows(t_begin + n), a.do_ss, q0, S);
     stage_ld(n);
   };
   // The block one wave later (work item + a.wave_ctas) starts by reading its key block's K, V rows
@@ -354,12 +401,13 @@ __global__ void __launch_bounds__(NB, 1) bwd_tc_kernel(const BwdArgs a) {
   // this wave computes and HBM is otherwise idle (one 256-byte row per thread).
   auto prefetch_next_wave = [&]() {
     const int nb = ticket + a.wave_ctas;
-    if (a.wave_ctas <= 0 || nparts > 1 || nb >= nkb * BH || tid >= 2 * KB + 2 * QT) return;
-    const int nkb2 = chain ? nb / BH : nb % nkb, nbh = chain ? nb % BH : nb / nkb;
-    const int nb_b = nbh / a.H, nb_h = nbh % a.H;
+    const int n_kb = a.n_kblocks;
+    if (a.wave_ctas <= 0 || nparts > 1 || nb >= n_kb * BH || tid >= 2 * KB + 2 * QT) return;
+    const int nkb2 = chain ? nb / BH : nb % n_kb, nbh = chain ? nb % BH : nb / n_kb;
+    const int nb_b = nbh / HU, nb_h = tid < 2 * KB ? nbh % HU : nbh % HU * group;
     const int r = tid < 2 * KB ? (tid & (KB - 1)) : (tid & (QT - 1));
     const int row = tid < 2 * KB ? nkb2 * KB + r : (CAUSAL ? nkb2 * KB : 0) + r;
-    if (row >= S) return;
+    if (row >= (CROSS && tid < 2 * KB ? a.Sk : S)) return;
     const float* src;
     if (tid < KB) src = a.k + nb_b * a.k_sb + nb_h * a.k_sh + static_cast<int64_t>(row) * a.k_ss;
     else if (tid < 2 * KB) src = a.v + nb_b * a.v_sb + nb_h * a.v_sh + static_cast<int64_t>(row) * a.v_ss;
@@ -381,11 +429,11 @@ __global__ void __launch_bounds__(NB, 1) bwd_tc_kernel(const BwdArgs a) {
   constexpr int LDP = 68;
   float* k_rows = reinterpret_cast<float*>(dSp);
   float* v_rows = k_rows + KB * LDP;
-  float* q_rows = reinterpret_cast<float*>(Qp + 3 * PART_Q);
-  float* o_rows = reinterpret_cast<float*>(dOp + 3 * PART_Q);
+  float* q_st = reinterpret_cast<float*>(Qp + 3 * PART_Q);
+  float* o_st = reinterpret_cast<float*>(dOp + 3 * PART_Q);
   static_assert(2 * KB * LDP * 4 <= 3 * PART_K + 2 * QT * 64 * 4 && QT * LDP * 4 <= 3 * PART_Q,
                 "prologue staging");
-  const int nk = min(KB, S - k0), nq = min(QT, S - t_begin * QT);
+  const int nk = min(KB, SK - k0), nq = min(QT, S - tile_q0(t_begin));
   __syncthreads();  // the mbarriers' initialisation
   if (mma_warp) {  // TMEM, by the warp that is idle while the rows travel (it also frees it)
     tc::tmem_alloc(tbase_p, TMEM_COLS);
@@ -401,9 +449,11 @@ __global__ void __launch_bounds__(NB, 1) bwd_tc_kernel(const BwdArgs a) {
         if (r < nk) tc::bulk_load(v_rows + r * LDP, vp + static_cast<int64_t>(k0 + r) * a.v_ss, 4 * HD, bar_ld);
       } else if (tid < 2 * KB + QT) {
         if (r < nq)
-          tc::bulk_load(q_rows + r * LDP, qp + static_cast<int64_t>(t_begin * QT + r) * a.q_ss, 4 * HD, bar_ld);
+          tc::bulk_load(q_st + r * LDP, q_rows(t_begin) + static_cast<int64_t>(tile_q0(t_begin) + r) * a.q_ss,
+                        4 * HD, bar_ld);
       } else if (r < nq) {
-        tc::bulk_load(o_rows + r * LDP, gp + static_cast<int64_t>(t_begin * QT + r) * a.do_ss, 4 * HD, bar_ld);
+        tc::bulk_load(o_st + r * LDP, g_rows(t_begin) + static_cast<int64_t>(tile_q0(t_begin) + r) * a.do_ss,
+                      4 * HD, bar_ld);
       }
     }
     griddep_wait();  // L, D, the cleared counters: the prep kernel's writes
@@ -413,8 +463,8 @@ __global__ void __launch_bounds__(NB, 1) bwd_tc_kernel(const BwdArgs a) {
     cp_async_wait_all();
     split_staged_row<HD>(Kp, PART_K, k_rows, tid, nk);
     split_staged_row<HD>(Kp, PART_K, k_rows, tid + NT, nk);
-    split_staged_row<HD>(Qp, PART_Q, q_rows, tid, nq);
-    split_staged_row<HD>(dOp, PART_Q, o_rows, tid, nq);
+    split_staged_row<HD>(Qp, PART_Q, q_st, tid, nq);
+    split_staged_row<HD>(dOp, PART_Q, o_st, tid, nq);
 #pragma unroll
     for (int c4 = 0; c4 < 4; ++c4) {
       const float4 u = row < nk && 16 * cg < HD
@@ -515,14 +565,14 @@ __global__ void __launch_bounds__(NB, 1) bwd_tc_kernel(const BwdArgs a) {
     if (N > 1) stage_tile(1);  // while the MMA warp issues T1(0)
     cp_async_commit();
     for (int n = 0; n < N; ++n) {
-      const int q0 = (t_begin + n) * QT;
+      const int q0 = tile_q0(t_begin + n);
       // (C1a) P^T for this thread's 16 queries, its parts into TMEM (pt_col) for dV -- while the
       // tensor core computes dP^T.
       err |= !tc::mbar_wait(bar_s, n & 1, WAIT_TIMEOUT_NS);
       tc::fence_after_sync();
       const float* Lt = ld + (n & 1) * 128;
       const float* Dt = Lt + QT;
-      const bool edge = (q0 + QT > S) || (k0 + KB > S) || (CAUSAL && k0 + KB - 1 > q0);
+      const bool edge = (q0 + QT > S) || (k0 + KB > SK) || (CAUSAL && k0 + KB - 1 > q0);
       float pr[16];
       tc::tmem_ld16(tbase + lane_sel + T_S + 16 * cg, pr);
       tc::tmem_wait_ld();
@@ -541,8 +591,8 @@ __global__ void __launch_bounds__(NB, 1) bwd_tc_kernel(const BwdArgs a) {
           tc::unpack2(mul2(fma2v(tc::pack2(pr[u], pr[u + 1]), nsc2, l2), nl2e2), x0, x1);
           float p0 = ex2(x0), p1 = ex2(x1);
           if (edge) {
-            if (!(q0 + ql < S && key < S && !(CAUSAL && key > q0 + ql))) p0 = 0.0f;
-            if (!(q0 + ql + 1 < S && key < S && !(CAUSAL && key > q0 + ql + 1))) p1 = 0.0f;
+            if (!(q0 + ql < S && key < SK && !(CAUSAL && key > q0 + ql))) p0 = 0.0f;
+            if (!(q0 + ql + 1 < S && key < SK && !(CAUSAL && key > q0 + ql + 1))) p1 = 0.0f;
           }
           pr[u] = p0;
           pr[u + 1] = p1;
@@ -631,7 +681,8 @@ __global__ void __launch_bounds__(NB, 1) bwd_tc_kernel(const BwdArgs a) {
         if (lane < 16 && qi < S && 16 * cg < HD && !err) {
           // Two 32-byte stores: whole L2 sectors (16-byte stores 256 bytes apart across the warp
           // each wrote half of 16 sectors).
-          float* dst = a.dq_part + ((static_cast<int64_t>(bh) * nkb + kb) * S + qi) * HD + 16 * cg;
+          float* dst = a.dq_part +
+                       ((query_bh(t_begin + n) * (CROSS ? a.n_kblocks : nkb) + kb) * S + qi) * HD + 16 * cg;
 #pragma unroll
           for (int c8 = 0; c8 < 2; ++c8) {
             float v[8];
@@ -659,7 +710,7 @@ __global__ void __launch_bounds__(NB, 1) bwd_tc_kernel(const BwdArgs a) {
           go = s_int[2 + (n & 1)] != 0;
         }
         if (go && lane < 16 && qi < S && 16 * cg < HD) {
-          float4* dst = reinterpret_cast<float4*>(dq_base + qi * row_stride + 16 * cg);
+          float4* dst = reinterpret_cast<float4*>(dq_rows(tile_head(t)) + qi * row_stride + 16 * cg);
 #pragma unroll
           for (int c4 = 0; c4 < 4; ++c4) {
             float4 v = make_float4(xb[4 * c4] + xs[4 * c4], xb[4 * c4 + 1] + xs[4 * c4 + 1],
@@ -771,12 +822,13 @@ __global__ void __launch_bounds__(NB, 1) bwd_tc_kernel(const BwdArgs a) {
     if (tid == 0 && !chain) count = atom_add_acq_rel(a.turn + bh, 1);
     // dV, dK rows out of shared memory: every 16 threads store one whole row.
     {
-      const int64_t row_stride = 3 * static_cast<int64_t>(a.H) * HD;
       for (int f = tid; f < 2 * KB * C4; f += NB) {
         const int which = f / (KB * C4), r = (f / C4) % KB, c4 = f % C4;
-        if (k0 + r < S) {
-          float* dst = a.dqkv + (static_cast<int64_t>(b) * S + k0 + r) * row_stride +
-                       (2 - which) * a.H * HD + h * HD;
+        if (k0 + r < (CROSS ? a.Sk : S)) {  // (CROSS: rows past the length hold zeros)
+          float* dst = CROSS ? a.dkv + (static_cast<int64_t>(b) * a.Sk + k0 + r) * 2 * a.Hk * HD +
+                                   (1 - which) * a.Hk * HD + h * HD
+                             : a.dqkv + (static_cast<int64_t>(b) * S + k0 + r) * row_stride +
+                                   (2 - which) * a.H * HD + h * HD;
           reinterpret_cast<float4*>(dst)[c4] =
               reinterpret_cast<const float4*>((which ? sk : sv) + r * LDS)[c4];
         }
@@ -785,36 +837,37 @@ __global__ void __launch_bounds__(NB, 1) bwd_tc_kernel(const BwdArgs a) {
     if (tid == 0) s_int[0] = count;
     __syncthreads();
     const int64_t part_bytes = static_cast<int64_t>(nkb) * S * HD * 4;
-    if (s_int[0] == nkb - 1 && part_bytes <= OFF_DS) {
-      // The (b, h)'s partials, contiguous [nkb][S][64], as one bulk copy into shared memory (the
-      // part buffers, free since the last T2; the dS^T buffer holds dV, dK), then summed there.
-      const float* part = a.dq_part + static_cast<int64_t>(bh) * nkb * S * HD;
-      const float* sp = reinterpret_cast<const float*>(sm);
-      if (tid == 0) {
-        tc::fence_async_global();  // the partials the count made visible, for the copy engine
-        tc::mbar_arrive_expect_tx(bar_ld, static_cast<uint32_t>(part_bytes));
-        tc::bulk_load(sm, part, static_cast<uint32_t>(part_bytes), bar_ld);
-      }
-      const bool ok = tc::mbar_wait(bar_ld, ld_phase & 1, WAIT_TIMEOUT_NS);
-      const int64_t row_stride = 3 * static_cast<int64_t>(a.H) * HD;
-      float* dq_base = a.dqkv + static_cast<int64_t>(b) * S * row_stride + h * HD;
-      // DETERMINISM: dQ = (((p0 + p1) + p2) + ...) * scale, as below.
-      for (int idx = tid; idx < S * C4 && ok; idx += NB) {
-        const int i = idx / C4, c4 = idx % C4;
-        const int last = CAUSAL ? min(nkb - 1, i / KB) : nkb - 1;
-        float4 v = reinterpret_cast<const float4*>(sp + i * HD)[c4];
-        for (int j = 1; j <= last; ++j) {
-          const float4 q = reinterpret_cast<const float4*>(sp + (j * S + i) * HD)[c4];
-          v = make_float4(v.x + q.x, v.y + q.y, v.z + q.z, v.w + q.w);
+    // (CROSS: head by head of the group, the partials of a head a.n_kblocks apart.)
+    for (int hq = h0; s_int[0] == nkb - 1 && hq < h0 + group; ++hq) {
+      const float* part = a.dq_part + (static_cast<int64_t>(b) * a.H + hq) * a.n_kblocks * S * HD;
+      float* dq_out = dq_rows(hq);
+      if (part_bytes <= OFF_DS) {
+        // The (b, h)'s partials, contiguous [nkb][S][64], as one bulk copy into shared memory (the
+        // part buffers, free since the last T2; the dS^T buffer holds dV, dK), then summed there.
+        const float* sp = reinterpret_cast<const float*>(sm);
+        if (CROSS && hq > h0) __syncthreads();  // the previous head's sums are read
+        if (tid == 0) {
+          tc::fence_async_global();  // the partials the count made visible, for the copy engine
+          tc::mbar_arrive_expect_tx(bar_ld, static_cast<uint32_t>(part_bytes));
+          tc::bulk_load(sm, part, static_cast<uint32_t>(part_bytes), bar_ld);
         }
-        reinterpret_cast<float4*>(dq_base + i * row_stride)[c4] =
-            make_float4(v.x * a.scale, v.y * a.scale, v.z * a.scale, v.w * a.scale);
+        const bool ok = tc::mbar_wait(bar_ld, ld_phase & 1, WAIT_TIMEOUT_NS);
+        if (CROSS) ++ld_phase;
+        // DETERMINISM: dQ = (((p0 + p1) + p2) + ...) * scale, as below.
+        for (int idx = tid; idx < S * C4 && ok; idx += NB) {
+          const int i = idx / C4, c4 = idx % C4;
+          const int last = CAUSAL ? min(nkb - 1, i / KB) : nkb - 1;
+          float4 v = reinterpret_cast<const float4*>(sp + i * HD)[c4];
+          for (int j = 1; j <= last; ++j) {
+            const float4 q = reinterpret_cast<const float4*>(sp + (j * S + i) * HD)[c4];
+            v = make_float4(v.x + q.x, v.y + q.y, v.z + q.z, v.w + q.w);
+          }
+          reinterpret_cast<float4*>(dq_out + i * row_stride)[c4] =
+              make_float4(v.x * a.scale, v.y * a.scale, v.z * a.scale, v.w * a.scale);
+        }
+        if (!ok && tid == 0) flag_timeout(a.err, a.sink);
+        continue;
       }
-      if (!ok && tid == 0) flag_timeout(a.err, a.sink);
-    } else if (s_int[0] == nkb - 1) {
-      const float* part = a.dq_part + static_cast<int64_t>(bh) * nkb * S * HD;
-      const int64_t row_stride = 3 * static_cast<int64_t>(a.H) * HD;
-      float* dq_base = a.dqkv + static_cast<int64_t>(b) * S * row_stride + h * HD;
       // DETERMINISM: dQ = (((p0 + p1) + p2) + ...) * scale over the key blocks holding a key <=
       // the row (causal) or all of them. Eight float4 items per thread at a time, each key
       // block's loads for the eight issued together.
@@ -852,7 +905,7 @@ __global__ void __launch_bounds__(NB, 1) bwd_tc_kernel(const BwdArgs a) {
         for (int u = 0; u < U; ++u) {
           const int idx = base + u * NB;
           if (last[u] >= 0)
-            reinterpret_cast<float4*>(dq_base + (idx / C4) * row_stride)[idx % C4] =
+            reinterpret_cast<float4*>(dq_out + (idx / C4) * row_stride)[idx % C4] =
                 make_float4(v[u].x * a.scale, v[u].y * a.scale, v[u].z * a.scale,
                             v[u].w * a.scale);
         }
@@ -922,6 +975,34 @@ cudaError_t launch_bwd_tc(const BwdArgs& args, int head_dim, int causal, cudaStr
   }
   if (causal) return launch_pdl(bwd_tc_kernel<true, 64>, grid, dim3(NB), SMEM_ALLOC, stream, a);
   return launch_pdl(bwd_tc_kernel<false, 64>, grid, dim3(NB), SMEM_ALLOC, stream, a);
+}
+
+cudaError_t setup_cross_bwd_tc_attributes() {
+  const cudaError_t e = cudaFuncSetAttribute(bwd_tc_kernel<false, 64, true>,
+                                             cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_ALLOC);
+  return e != cudaSuccess ? e
+                          : cudaFuncSetAttribute(bwd_tc_kernel<false, 32, true>,
+                                                 cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_ALLOC);
+}
+
+// The caller has laid out the workspace (cross_bwd_workspace_layout): the split tail's windows and
+// flags, when it planned one, are in a.tail_win, a.tail_flag with tail_units, tail_parts set for
+// CROSS_SMS blocks a wave.
+cudaError_t launch_cross_bwd_tc(const BwdArgs& args, int head_dim, cudaStream_t stream) {
+  BwdArgs a = args;
+  a.n_kblocks = (a.Sk + KB - 1) / KB;
+  int dev = 0, sms = 0;
+  a.wave_ctas = cudaGetDevice(&dev) == cudaSuccess &&
+                        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess
+                    ? sms
+                    : 0;
+  const int64_t units = static_cast<int64_t>(a.n_kblocks) * a.B * a.Hk;
+  const int64_t blocks = a.tail_parts > 1 ? units + static_cast<int64_t>(a.tail_units) * (a.tail_parts - 1)
+                                          : units;
+  const dim3 grid(static_cast<unsigned>(blocks));
+  if (head_dim == 32)
+    return launch_pdl(bwd_tc_kernel<false, 32, true>, grid, dim3(NB), SMEM_ALLOC, stream, a);
+  return launch_pdl(bwd_tc_kernel<false, 64, true>, grid, dim3(NB), SMEM_ALLOC, stream, a);
 }
 
 }  // namespace cfa

@@ -226,7 +226,7 @@ int* error_sink() { return g_sink.load(std::memory_order_relaxed); }
 
 extern "C" {
 
-int cfa_abi_version(void) { return (2 << 16) | 2; }
+int cfa_abi_version(void) { return (2 << 16) | 3; }
 
 const char* cfa_strerror(int status) {
   switch (status) {
@@ -241,6 +241,12 @@ const char* cfa_strerror(int status) {
     case CFA_ERR_LAUNCH: return "fused_attention: kernel launch failed";
     case CFA_ERR_TIMEOUT: return "fused_attention: a bounded device wait expired (results invalid)";
     case CFA_ERR_CUDA: return "fused_attention: CUDA runtime error";
+    case CFA_ERR_PAGE:
+      return "fused_attention: a page id outside the cache, or a length past its page table";
+    case CFA_ERR_TYPE: return "fused_attention: unsupported element types";
+    case CFA_ERR_HEADS: return "fused_attention: the query heads must be a multiple of the key heads";
+    case CFA_ERR_ROTARY:
+      return "fused_attention: the rotary dimension must be even and at most the head dim";
     default: return "fused_attention: unknown status";
   }
 }

@@ -215,6 +215,20 @@ __device__ __forceinline__ void flag_timeout(int* err, int* sink) {
   }
 }
 
+// The keys of batch element b that the CROSS kernels attend: key_lengths[b] held within 0 .. Sk.
+template <typename Args>
+__device__ __forceinline__ int cross_keys(const Args& a, int b) {
+  return a.key_lengths ? min(max(a.key_lengths[b], 0), a.Sk) : a.Sk;
+}
+
+// Another status into the host-visible flag (a page id outside the cache, found by a kernel).
+__device__ __forceinline__ void flag_error(int* sink, int status) {
+  if (sink != nullptr) {
+    asm volatile("st.relaxed.sys.global.b32 [%0], %1;" ::"l"(sink), "r"(status) : "memory");
+    __threadfence_system();
+  }
+}
+
 // Wait (one thread) until *turn == want, at most `timeout_ns` of GPU time. Returns true when the
 // turn came. On expiry it records CFA_ERR_TIMEOUT (flag_timeout) and returns false; it also
 // returns false as soon as any other waiter has recorded an error, so one expired wait ends every

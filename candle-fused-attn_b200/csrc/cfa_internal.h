@@ -48,6 +48,10 @@ struct FwdArgs {
   int n_qtiles;
   int wave_ctas;  // tensor-core forward: blocks resident at once (one per SM); 0: none
   int* sink;      // host-visible error flag (cfa_error_sink) or nullptr
+  // Cross attention (the CROSS kernels): H / Hk query heads share a key head, k and v have Sk rows,
+  // of which batch element b attends the first key_lengths[b] (nullptr: all).
+  int Hk, Sk;
+  const int* key_lengths;
 };
 
 struct BwdArgs {
@@ -82,6 +86,11 @@ struct BwdArgs {
   float* tail_win;  // [tail_units][query tiles][2][128][D] window sums
   int* tail_flag;   // [tail_units][tail_parts] flags, then the tail's ticket counter (cleared by the
                     // prep kernel)
+  // Cross attention (the CROSS kernels): as in FwdArgs; dQ and dK, dV go to buffers of their own.
+  int Hk, Sk;
+  const int* key_lengths;
+  float* dq;   // [B, S, H, D]
+  float* dkv;  // [B, Sk, 2, Hk, D] (dK, dV interleaved)
 };
 
 struct PrepArgs {
@@ -145,6 +154,16 @@ cudaError_t setup_hd_attributes();
 cudaError_t launch_hd_fwd(const FwdArgs& a, int head_dim, int causal, cudaStream_t stream);
 cudaError_t launch_hd_bwd_prep(const PrepArgs& a, int head_dim, cudaStream_t stream);
 cudaError_t launch_hd_bwd(const BwdArgs& a, int head_dim, int causal, cudaStream_t stream);
+
+// Cross attention: the same kernels with keys of another length (CROSS): head dims 64 and 32 on the
+// tensor-core pair, 128 on hd_ffma.cu. a.S is the query length, a.n_kblocks is set by the launcher.
+cudaError_t setup_cross_tc_attributes();
+cudaError_t setup_cross_bwd_tc_attributes();
+cudaError_t setup_cross_hd_attributes();
+cudaError_t launch_cross_fwd_tc(const FwdArgs& a, int head_dim, cudaStream_t stream);
+cudaError_t launch_cross_bwd_tc(const BwdArgs& a, int head_dim, cudaStream_t stream);
+cudaError_t launch_cross_hd_fwd(const FwdArgs& a, cudaStream_t stream);
+cudaError_t launch_cross_hd_bwd(const BwdArgs& a, cudaStream_t stream);
 
 // The projection GEMM (linear_tc.cu): C = A B over fp32 on the tensor cores (split bf16 parts).
 // A(m, k) = a[m a_sm + k a_sk], B(k, n) = b[k b_sk + n b_sn] (any strides), C(m, n) = c[m c_sm +

@@ -1,0 +1,403 @@
+// SPDX-License-Identifier: MIT OR Apache-2.0
+//
+// The C ABI of the operators beside the fused attention (include/cfa.h): cross attention, rotary
+// positions, the paged cache's append and its attention. Argument checks and launches, as
+// cfa_abi.cu does for the fused attention; everything on the caller's stream, no synchronisation.
+#include <algorithm>
+#include <mutex>
+
+#include "cfa_internal.h"
+#include "cfa_ops.h"
+
+namespace {
+
+constexpr int kMaxDevices = 64;
+struct DeviceOnce {
+  std::once_flag flag;
+  cudaError_t result = cudaSuccess;
+};
+DeviceOnce g_cross_once[kMaxDevices], g_split_once[kMaxDevices];
+
+int setup(DeviceOnce* table, cudaError_t (*fn)()) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return CFA_ERR_CUDA;
+  DeviceOnce& d = table[dev];
+  std::call_once(d.flag, [&] { d.result = fn(); });
+  return d.result == cudaSuccess ? CFA_OK : CFA_ERR_LAUNCH;
+}
+
+cudaError_t setup_cross() {
+  cudaError_t e = cfa::setup_cross_tc_attributes();
+  if (e == cudaSuccess) e = cfa::setup_cross_bwd_tc_attributes();
+  return e == cudaSuccess ? cfa::setup_cross_hd_attributes() : e;
+}
+
+constexpr int64_t kLim = (int64_t(1) << 31) - 1;
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+bool strides_ok(const int64_t* s, int64_t unit) {
+  return s[0] % unit == 0 && s[1] % unit == 0 && s[2] % unit == 0;
+}
+bool type_ok(int t) { return t == CFA_F32 || t == CFA_F16 || t == CFA_BF16; }
+// Input and cache types: the same, or an fp32 input over any cache.
+bool types_ok(int t, int cache) { return type_ok(t) && type_ok(cache) && (t == cache || t == CFA_F32); }
+int64_t type_size(int t) { return t == CFA_F32 ? 4 : 2; }
+bool head_dim_ok(int64_t d) { return d == 32 || d == 64 || d == 128; }
+int status(cudaError_t e) {
+  if (e == cudaSuccess) return CFA_OK;
+  return e == cudaErrorInvalidConfiguration ? CFA_ERR_OVERFLOW : CFA_ERR_LAUNCH;
+}
+
+// B, H, Hk, Sq, Sk of a cross attention.
+int check_cross(int64_t B, int64_t H, int64_t Hk, int64_t Sq, int64_t Sk, int64_t D) {
+  if (B < 0 || H < 0 || Hk < 0 || Sq < 0 || Sk < 0 || D < 0) return CFA_ERR_SHAPE;
+  if (!head_dim_ok(D)) return CFA_ERR_HEAD_DIM;
+  if (Hk == 0 ? H != 0 : H % Hk != 0) return CFA_ERR_HEADS;
+  if (B > kLim || H > kLim || Sq > kLim - 64 || Sk > kLim - 128) return CFA_ERR_OVERFLOW;
+  if (B == 0 || H == 0) return CFA_OK;
+  if (B * H > kLim / ((std::max(Sq, Sk) + 31) / 32 + 1)) return CFA_ERR_OVERFLOW;
+  if (B * H * Sq > kLim || B * Hk * Sk > kLim) return CFA_ERR_OVERFLOW;
+  return CFA_OK;
+}
+
+// The cross backward's workspace: ticket and error flag, turn counters and the split tail's flags
+// (one cleared range), D, then -- short key sequences -- the dQ partials and the tail's windows.
+constexpr int kCrossMaxKeyBlocks = 16;       // no-wait dQ up to as many key blocks
+constexpr int64_t kCrossWindowBytes = int64_t(512) << 20;  // most that a split tail's windows take
+struct CrossLayout {
+  int64_t n_zero;  // ints cleared before the backward
+  size_t turn_off, flag_off, dsum_off, part_off, win_off, total;
+  bool partials;
+  int tail_units, tail_parts;
+};
+CrossLayout cross_layout(int64_t B, int64_t H, int64_t Hk, int64_t Sq, int64_t Sk, int64_t D) {
+  CrossLayout w{};
+  const int64_t kb = D == 128 ? 64 : 128, nkb = (Sk + kb - 1) / kb, nqt = (Sq + 63) / 64;
+  const int64_t units = nkb * B * Hk, tiles = H / Hk * nqt;
+  w.partials = nkb <= kCrossMaxKeyBlocks;
+  // The key blocks of the partial last wave (all of them where they are fewer than the SMs) split by
+  // query tiles; the count of SMs is fixed, so that the workspace does not depend on the device.
+  if (w.partials && D != 128) {
+    const int64_t R = units % cfa::LIN_SMS;
+    const int64_t k = R > 0 ? std::min<int64_t>(tiles, cfa::LIN_SMS / R) : 0;
+    if (k >= 2 && R * tiles * 2 * 128 * D * 4 <= kCrossWindowBytes) {
+      w.tail_units = static_cast<int>(R);
+      w.tail_parts = static_cast<int>(k);
+    }
+  }
+  w.turn_off = 256;
+  const int64_t turns = std::max(B * H * nqt, B * Hk);
+  w.flag_off = w.turn_off + static_cast<size_t>(turns) * 4;
+  const int64_t flags = static_cast<int64_t>(w.tail_units) * w.tail_parts + 1;
+  w.n_zero = 64 + turns + flags;
+  w.dsum_off = cfa::align256(w.flag_off + static_cast<size_t>(flags) * 4);
+  w.part_off = w.dsum_off + cfa::align256(static_cast<size_t>(B * H * Sq) * 4);
+  w.win_off = w.part_off + (w.partials ? cfa::align256(static_cast<size_t>(nkb * B * H * Sq) * D * 4) : 0);
+  w.total = w.win_off + static_cast<size_t>(w.tail_units ? w.tail_units * tiles * 2 * 128 * D * 4 : 0);
+  return w;
+}
+
+}  // namespace
+
+extern "C" {
+
+int cfa_cross_fwd_f32(const float* q, const int64_t q_strides[3], const float* k,
+                      const int64_t k_strides[3], const float* v, const int64_t v_strides[3],
+                      const int32_t* key_lengths, float* o, float* lse, int64_t batch, int64_t heads,
+                      int64_t key_heads, int64_t seq, int64_t key_seq, int64_t head_dim, float scale,
+                      void* stream) {
+  int st = check_cross(batch, heads, key_heads, seq, key_seq, head_dim);
+  if (st != CFA_OK || batch == 0 || heads == 0 || seq == 0) return st;
+  if (!q || !o || !lse || !q_strides || !k_strides || !v_strides || (key_seq > 0 && (!k || !v)))
+    return CFA_ERR_NULL;
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o) || !strides_ok(q_strides, 4) ||
+      !strides_ok(k_strides, 4) || !strides_ok(v_strides, 4))
+    return CFA_ERR_ALIGNMENT;
+  st = setup(g_cross_once, setup_cross);
+  if (st != CFA_OK) return st;
+  cfa::FwdArgs a{};
+  a.q = q, a.k = k, a.v = v, a.o = o, a.lse = lse;
+  a.q_sb = q_strides[0], a.q_sh = q_strides[1], a.q_ss = q_strides[2];
+  a.k_sb = k_strides[0], a.k_sh = k_strides[1], a.k_ss = k_strides[2];
+  a.v_sb = v_strides[0], a.v_sh = v_strides[1], a.v_ss = v_strides[2];
+  a.B = static_cast<int>(batch), a.H = static_cast<int>(heads), a.S = static_cast<int>(seq);
+  a.Hk = static_cast<int>(key_heads), a.Sk = static_cast<int>(key_seq);
+  a.key_lengths = key_lengths;
+  a.scale = scale;
+  a.sink = cfa::error_sink();
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return status(head_dim == 128 ? cfa::launch_cross_hd_fwd(a, s)
+                                : cfa::launch_cross_fwd_tc(a, static_cast<int>(head_dim), s));
+}
+
+size_t cfa_cross_bwd_workspace_bytes(int64_t batch, int64_t heads, int64_t key_heads, int64_t seq,
+                                     int64_t key_seq, int64_t head_dim) {
+  if (check_cross(batch, heads, key_heads, seq, key_seq, head_dim) != CFA_OK || batch == 0 ||
+      heads == 0 || seq == 0 || key_seq == 0)
+    return 256;
+  return cross_layout(batch, heads, key_heads, seq, key_seq, head_dim).total;
+}
+
+int cfa_cross_bwd_f32(const float* q, const int64_t q_strides[3], const float* k,
+                      const int64_t k_strides[3], const float* v, const int64_t v_strides[3],
+                      const int32_t* key_lengths, const float* o, const float* lse, const float* d_o,
+                      const int64_t do_strides[3], float* dq, float* dkv, void* workspace,
+                      size_t workspace_bytes, int64_t batch, int64_t heads, int64_t key_heads,
+                      int64_t seq, int64_t key_seq, int64_t head_dim, float scale, void* stream) {
+  int st = check_cross(batch, heads, key_heads, seq, key_seq, head_dim);
+  if (st != CFA_OK || batch == 0 || heads == 0) return st;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (seq == 0 || key_seq == 0) {  // no score at all: the gradients that exist are zero
+    if (seq == 0 && key_seq == 0) return CFA_OK;
+    float* g = seq == 0 ? dkv : dq;
+    const int64_t n = seq == 0 ? 2 * batch * key_seq * key_heads : batch * seq * heads;
+    if (!g) return CFA_ERR_NULL;
+    return status(cudaMemsetAsync(g, 0, static_cast<size_t>(n * head_dim) * 4, s));
+  }
+  if (!q || !k || !v || !o || !lse || !d_o || !dq || !dkv || !workspace || !q_strides || !k_strides ||
+      !v_strides || !do_strides)
+    return CFA_ERR_NULL;
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o) || !aligned16(d_o) ||
+      !aligned16(dq) || !aligned16(dkv) || !strides_ok(q_strides, 4) || !strides_ok(k_strides, 4) ||
+      !strides_ok(v_strides, 4) || !strides_ok(do_strides, 4))
+    return CFA_ERR_ALIGNMENT;
+  const CrossLayout lay = cross_layout(batch, heads, key_heads, seq, key_seq, head_dim);
+  if (workspace_bytes < lay.total || (reinterpret_cast<uintptr_t>(workspace) & 255u) != 0)
+    return CFA_ERR_WORKSPACE;
+  st = setup(g_cross_once, setup_cross);
+  if (st != CFA_OK) return st;
+  char* ws = static_cast<char*>(workspace);
+  int* ticket = reinterpret_cast<int*>(ws);
+
+  cfa::PrepArgs p{};
+  p.o = o, p.d_o = d_o;
+  p.dsum = reinterpret_cast<float*>(ws + lay.dsum_off);
+  p.zero = ticket;
+  p.n_zero = lay.n_zero;
+  p.do_sb = do_strides[0], p.do_sh = do_strides[1], p.do_ss = do_strides[2];
+  p.B = static_cast<int>(batch), p.H = static_cast<int>(heads), p.S = static_cast<int>(seq);
+  cudaError_t e = head_dim == 64 ? cfa::launch_bwd_prep(p, s)
+                                 : cfa::launch_hd_bwd_prep(p, static_cast<int>(head_dim), s);
+  if (e != cudaSuccess) return status(e);
+
+  cfa::BwdArgs a{};
+  a.q = q, a.k = k, a.v = v, a.d_o = d_o, a.lse = lse, a.dsum = p.dsum;
+  a.dq = dq, a.dkv = dkv;
+  a.ticket = ticket;
+  a.err = ticket + 1;
+  a.turn = reinterpret_cast<int*>(ws + lay.turn_off);
+  a.q_sb = q_strides[0], a.q_sh = q_strides[1], a.q_ss = q_strides[2];
+  a.k_sb = k_strides[0], a.k_sh = k_strides[1], a.k_ss = k_strides[2];
+  a.v_sb = v_strides[0], a.v_sh = v_strides[1], a.v_ss = v_strides[2];
+  a.do_sb = do_strides[0], a.do_sh = do_strides[1], a.do_ss = do_strides[2];
+  a.B = static_cast<int>(batch), a.H = static_cast<int>(heads), a.S = static_cast<int>(seq);
+  a.Hk = static_cast<int>(key_heads), a.Sk = static_cast<int>(key_seq);
+  a.key_lengths = key_lengths;
+  a.scale = scale;
+  a.n_qtiles = static_cast<int>((seq + 63) / 64);
+  a.timeout_ns = cfa::WAIT_TIMEOUT_NS;
+  a.sink = cfa::error_sink();
+  a.dq_part = lay.partials ? reinterpret_cast<float*>(ws + lay.part_off) : nullptr;
+  if (lay.tail_parts > 1) {
+    const int64_t units = (key_seq + 127) / 128 * batch * key_heads;
+    a.tail_base = static_cast<int>(units - lay.tail_units);
+    a.tail_units = lay.tail_units;
+    a.tail_parts = lay.tail_parts;
+    a.tail_win = reinterpret_cast<float*>(ws + lay.win_off);
+    a.tail_flag = reinterpret_cast<int*>(ws + lay.flag_off);
+  }
+  return status(head_dim == 128 ? cfa::launch_cross_hd_bwd(a, s)
+                                : cfa::launch_cross_bwd_tc(a, static_cast<int>(head_dim), s));
+}
+
+size_t cfa_cross_few_workspace_bytes(int64_t batch, int64_t heads, int64_t seq, int64_t key_seq,
+                                     int64_t head_dim) {
+  if (batch <= 0 || heads <= 0 || seq <= 0 || key_seq <= 0 || !head_dim_ok(head_dim) ||
+      batch > kLim || heads > kLim || seq > kLim || key_seq > kLim || batch * heads > kLim / seq)
+    return 0;
+  return cfa::split_workspace_bytes(batch * heads * seq, key_seq, head_dim);
+}
+
+int cfa_cross_few_f32(const float* q, const int64_t q_strides[3], const float* k,
+                      const int64_t k_strides[3], const float* v, const int64_t v_strides[3],
+                      const int32_t* key_lengths, float* o, void* workspace, size_t workspace_bytes,
+                      int64_t batch, int64_t heads, int64_t key_heads, int64_t seq, int64_t key_seq,
+                      int64_t head_dim, float scale, void* stream) {
+  int st = check_cross(batch, heads, key_heads, seq, key_seq, head_dim);
+  if (st != CFA_OK || batch == 0 || heads == 0 || seq == 0) return st;
+  const size_t need = cfa_cross_few_workspace_bytes(batch, heads, seq, key_seq, head_dim);
+  if (!q || !o || !q_strides || !k_strides || !v_strides || (key_seq > 0 && (!k || !v)) ||
+      (need > 0 && !workspace))
+    return CFA_ERR_NULL;
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !strides_ok(q_strides, 4) ||
+      !strides_ok(k_strides, 4) || !strides_ok(v_strides, 4))
+    return CFA_ERR_ALIGNMENT;
+  if (workspace_bytes < need || (need && (reinterpret_cast<uintptr_t>(workspace) & 255u) != 0))
+    return CFA_ERR_WORKSPACE;
+  if (batch * cfa::split_max_chunks(key_seq) > kLim) return CFA_ERR_OVERFLOW;
+  st = setup(g_split_once, cfa::setup_split_attributes);
+  if (st != CFA_OK) return st;
+  cfa::SplitArgs a{};
+  a.q = q, a.k = k, a.v = v, a.o = o;
+  a.q_sb = q_strides[0], a.q_sh = q_strides[1], a.q_ss = q_strides[2];
+  a.k_sp = k_strides[0], a.k_sh = k_strides[1], a.k_sr = k_strides[2];
+  a.v_sp = v_strides[0], a.v_sh = v_strides[1], a.v_sr = v_strides[2];
+  a.lengths = key_lengths;
+  a.max_len = static_cast<int>(key_seq);
+  a.B = static_cast<int>(batch), a.H = static_cast<int>(heads), a.Hk = static_cast<int>(key_heads);
+  a.S = static_cast<int>(seq), a.D = static_cast<int>(head_dim);
+  a.scale = scale;
+  a.sink = cfa::error_sink();
+  return status(cfa::launch_split_attention(a, CFA_F32, CFA_F32, workspace,
+                                            static_cast<cudaStream_t>(stream)));
+}
+
+int cfa_rotary(const void* x, const int64_t x_strides[3], void* y, const int64_t y_strides[3],
+               int dtype, const void* positions, int position_bytes, const int64_t position_strides[2],
+               int64_t first_position, const double* freqs, float amplitude, int64_t batch,
+               int64_t heads, int64_t rotated_heads, int64_t seq, int64_t head_dim,
+               int64_t rotary_dim, int interleaved, int inverse, void* stream) {
+  if (batch < 0 || heads < 0 || seq < 0 || head_dim < 0 || rotated_heads < 0 || rotated_heads > heads)
+    return CFA_ERR_SHAPE;
+  if (rotary_dim < 0 || rotary_dim % 2 != 0 || rotary_dim > head_dim) return CFA_ERR_ROTARY;
+  if (head_dim > 1024) return CFA_ERR_HEAD_DIM;
+  if (!type_ok(dtype) || (positions && position_bytes != 4 && position_bytes != 8)) return CFA_ERR_TYPE;
+  if (batch == 0 || heads == 0 || seq == 0 || head_dim == 0) return CFA_OK;
+  if (batch > kLim || heads > kLim || seq > kLim || batch > kLim / seq) return CFA_ERR_OVERFLOW;
+  if (!x || !y || !x_strides || !y_strides || (positions && !position_strides) ||
+      (rotary_dim > 0 && !freqs))
+    return CFA_ERR_NULL;
+  cfa::RotaryArgs a{};
+  a.x = x, a.y = y;
+  a.x_sb = x_strides[0], a.x_sh = x_strides[1], a.x_ss = x_strides[2];
+  a.y_sb = y_strides[0], a.y_sh = y_strides[1], a.y_ss = y_strides[2];
+  a.freqs = freqs;
+  a.amplitude = amplitude;
+  a.interleaved = interleaved != 0, a.inverse = inverse != 0;
+  a.B = static_cast<int>(batch), a.H = static_cast<int>(heads), a.S = static_cast<int>(seq);
+  a.rot_heads = static_cast<int>(rotated_heads);
+  a.D = static_cast<int>(head_dim), a.rot = static_cast<int>(rotary_dim);
+  a.pos = positions;
+  a.pos64 = position_bytes == 8;
+  if (positions) a.pos_sb = position_strides[0], a.pos_ss = position_strides[1];
+  a.pos0 = first_position;
+  a.n_tokens = batch * seq;
+  return status(cfa::launch_rotary(a, dtype, static_cast<cudaStream_t>(stream)));
+}
+
+int cfa_paged_append(const void* q, const int64_t q_strides[3], void* q_out,
+                     const int64_t q_out_strides[3], const void* k, const int64_t k_strides[3],
+                     const void* v, const int64_t v_strides[3], int dtype, void* k_cache,
+                     const int64_t k_cache_strides[3], void* v_cache,
+                     const int64_t v_cache_strides[3], int cache_dtype, int64_t pages,
+                     int64_t page_size, const int32_t* page_table, int64_t table_stride,
+                     int64_t table_width, const int32_t* lengths, const int32_t* new_lengths,
+                     const double* freqs, float amplitude, int64_t batch, int64_t heads,
+                     int64_t key_heads, int64_t seq, int64_t head_dim, int64_t rotary_dim,
+                     int interleaved, void* stream) {
+  if (batch < 0 || heads < 0 || key_heads < 0 || seq < 0 || head_dim < 0 || pages < 0 ||
+      table_width < 0 || page_size < 1)
+    return CFA_ERR_SHAPE;
+  if (rotary_dim < 0 || rotary_dim % 2 != 0 || rotary_dim > head_dim) return CFA_ERR_ROTARY;
+  if (head_dim > 1024) return CFA_ERR_HEAD_DIM;
+  if (!types_ok(dtype, cache_dtype)) return CFA_ERR_TYPE;
+  if (!q) heads = 0;
+  if (batch == 0 || seq == 0 || head_dim == 0 || (heads == 0 && key_heads == 0)) return CFA_OK;
+  if (batch > kLim || seq > kLim || batch > kLim / seq || heads + 2 * key_heads > kLim ||
+      pages > kLim || page_size > kLim || table_width > kLim)
+    return CFA_ERR_OVERFLOW;
+  if ((q && (!q_out || !q_strides || !q_out_strides)) || !k || !v || !k_strides || !v_strides ||
+      !k_cache || !v_cache || !k_cache_strides || !v_cache_strides ||
+      (table_width > 0 && !page_table) || !lengths || (rotary_dim > 0 && !freqs))
+    return CFA_ERR_NULL;
+  cfa::RotaryArgs a{};
+  if (q) {
+    a.x = q, a.y = q_out;
+    a.x_sb = q_strides[0], a.x_sh = q_strides[1], a.x_ss = q_strides[2];
+    a.y_sb = q_out_strides[0], a.y_sh = q_out_strides[1], a.y_ss = q_out_strides[2];
+  }
+  a.k = k, a.v = v;
+  a.k_sb = k_strides[0], a.k_sh = k_strides[1], a.k_ss = k_strides[2];
+  a.v_sb = v_strides[0], a.v_sh = v_strides[1], a.v_ss = v_strides[2];
+  a.k_cache = k_cache, a.v_cache = v_cache;
+  a.kc_sp = k_cache_strides[0], a.kc_sr = k_cache_strides[1], a.kc_sh = k_cache_strides[2];
+  a.vc_sp = v_cache_strides[0], a.vc_sr = v_cache_strides[1], a.vc_sh = v_cache_strides[2];
+  a.table = page_table;
+  a.table_sb = table_stride;
+  a.table_width = static_cast<int>(table_width), a.n_pages = static_cast<int>(pages);
+  a.page = static_cast<int>(page_size);
+  a.lengths = lengths, a.new_lengths = new_lengths;
+  a.freqs = freqs;
+  a.amplitude = amplitude;
+  a.interleaved = interleaved != 0;
+  a.B = static_cast<int>(batch), a.H = static_cast<int>(heads), a.Hk = static_cast<int>(key_heads);
+  a.rot_heads = a.H;
+  a.S = static_cast<int>(seq), a.D = static_cast<int>(head_dim), a.rot = static_cast<int>(rotary_dim);
+  a.n_tokens = batch * seq;
+  a.sink = cfa::error_sink();
+  return status(cfa::launch_paged_append(a, dtype, cache_dtype, static_cast<cudaStream_t>(stream)));
+}
+
+size_t cfa_paged_attention_workspace_bytes(int64_t batch, int64_t heads, int64_t seq,
+                                           int64_t max_keys, int64_t head_dim) {
+  if (batch <= 0 || heads <= 0 || seq <= 0 || max_keys <= 0 || !head_dim_ok(head_dim) ||
+      batch > kLim || heads > kLim || seq > kLim || max_keys > kLim || batch * heads > kLim / seq)
+    return 0;
+  return cfa::split_workspace_bytes(batch * heads * seq, max_keys, head_dim);
+}
+
+int cfa_paged_attention(const void* q, const int64_t q_strides[3], int dtype, const void* k_cache,
+                        const int64_t k_cache_strides[3], const void* v_cache,
+                        const int64_t v_cache_strides[3], int cache_dtype, int64_t pages,
+                        int64_t page_size, const int32_t* page_table, int64_t table_stride,
+                        int64_t table_width, const int32_t* lengths, const int32_t* new_lengths,
+                        void* o, void* workspace, size_t workspace_bytes, int64_t batch,
+                        int64_t heads, int64_t key_heads, int64_t seq, int64_t head_dim,
+                        float scale, void* stream) {
+  if (batch < 0 || heads < 0 || key_heads < 0 || seq < 0 || head_dim < 0 || pages < 0 ||
+      table_width < 0 || page_size < 1)
+    return CFA_ERR_SHAPE;
+  if (!head_dim_ok(head_dim)) return CFA_ERR_HEAD_DIM;
+  if (key_heads == 0 ? heads != 0 : heads % key_heads != 0) return CFA_ERR_HEADS;
+  if (!types_ok(dtype, cache_dtype)) return CFA_ERR_TYPE;
+  if (batch == 0 || heads == 0 || seq == 0) return CFA_OK;
+  if (batch > kLim || heads > kLim || seq > kLim || batch * heads > kLim / seq || pages > kLim ||
+      page_size > kLim || table_width > kLim || table_width * page_size > kLim - 1024)
+    return CFA_ERR_OVERFLOW;
+  const int64_t max_keys = table_width * page_size;
+  const size_t need = cfa_paged_attention_workspace_bytes(batch, heads, seq, max_keys, head_dim);
+  if (!q || !o || !q_strides || !k_cache_strides || !v_cache_strides || !lengths ||
+      (max_keys > 0 && (!k_cache || !v_cache || !page_table)) || (need > 0 && !workspace))
+    return CFA_ERR_NULL;
+  const int64_t unit = 16 / type_size(cache_dtype);
+  if (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) ||
+      !strides_ok(q_strides, 16 / type_size(dtype)) || !strides_ok(k_cache_strides, unit) ||
+      !strides_ok(v_cache_strides, unit))
+    return CFA_ERR_ALIGNMENT;
+  if (workspace_bytes < need || (need && (reinterpret_cast<uintptr_t>(workspace) & 255u) != 0))
+    return CFA_ERR_WORKSPACE;
+  if (batch * cfa::split_max_chunks(max_keys) > kLim) return CFA_ERR_OVERFLOW;
+  const int st = setup(g_split_once, cfa::setup_split_attributes);
+  if (st != CFA_OK) return st;
+  cfa::SplitArgs a{};
+  a.q = q, a.k = k_cache, a.v = v_cache, a.o = o;
+  a.q_sb = q_strides[0], a.q_sh = q_strides[1], a.q_ss = q_strides[2];
+  a.k_sp = k_cache_strides[0], a.k_sr = k_cache_strides[1], a.k_sh = k_cache_strides[2];
+  a.v_sp = v_cache_strides[0], a.v_sr = v_cache_strides[1], a.v_sh = v_cache_strides[2];
+  // (A cache without a page has nothing to read: max_len 0 keeps every key away.)
+  a.table = page_table;
+  a.table_sb = table_stride;
+  a.table_width = static_cast<int>(table_width), a.n_pages = static_cast<int>(pages);
+  a.page = static_cast<int>(page_size);
+  a.lengths = lengths, a.new_lengths = new_lengths;
+  a.causal = 1;
+  a.max_len = static_cast<int>(max_keys);
+  a.B = static_cast<int>(batch), a.H = static_cast<int>(heads), a.Hk = static_cast<int>(key_heads);
+  a.S = static_cast<int>(seq), a.D = static_cast<int>(head_dim);
+  a.scale = scale;
+  a.sink = cfa::error_sink();
+  return status(cfa::launch_split_attention(a, dtype, cache_dtype, workspace,
+                                            static_cast<cudaStream_t>(stream)));
+}
+
+}  // extern "C"

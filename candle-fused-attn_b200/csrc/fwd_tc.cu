@@ -323,9 +323,12 @@ struct RowState {
   float m, lpart, alpha_prev;
 };
 
-template <bool CAUSAL, int HD>
+// CROSS: the keys have a length of their own (a.Sk rows, the first cross_keys(a, b) attended), and
+// H / Hk query heads share a key head; nothing else differs.
+template <bool CAUSAL, int HD, bool CROSS = false>
 __global__ void __launch_bounds__(NBLK, 1) fwd_tc_kernel(const FwdArgs a) {
   static_assert(HD == 64 || HD == 32, "head dims of the tensor-core forward");
+  static_assert(!(CAUSAL && CROSS), "cross attention has no causal mask");
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   const uint32_t raw = tc::smem_u32(smem_raw);
   unsigned char* sm = smem_raw + ((1024u - (raw & 1023u)) & 1023u);
@@ -359,15 +362,30 @@ __global__ void __launch_bounds__(NBLK, 1) fwd_tc_kernel(const FwdArgs a) {
   const int b = bh / a.H, h = bh % a.H;
   const int q0 = qb * BQ;
   const int S = a.S;
+  const int hk = CROSS ? h / (a.H / a.Hk) : h;
   const float* qp = a.q + b * a.q_sb + h * a.q_sh;
-  const float* kp = a.k + b * a.k_sb + h * a.k_sh;
-  const float* vp = a.v + b * a.v_sb + h * a.v_sh;
+  const float* kp = a.k + b * a.k_sb + hk * a.k_sh;
+  const float* vp = a.v + b * a.v_sb + hk * a.v_sh;
+  int SK = S;  // keys
+  if constexpr (CROSS) {
+    griddep_wait();  // the lengths may come from the previous kernel on the stream
+    SK = cross_keys(a, b);
+    if (SK == 0) {  // no key: O = 0, L = -inf (before any barrier or TMEM)
+      griddep_launch_dependents();
+      const int rows = min(BQ, S - q0);
+      for (int f = tid; f < rows * (HD / 4); f += NBLK)
+        reinterpret_cast<float4*>(a.o + ((static_cast<int64_t>(b) * S + q0 + f / (HD / 4)) * a.H + h) *
+                                            HD)[f % (HD / 4)] = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int r = tid; r < rows; r += NBLK) a.lse[static_cast<int64_t>(bh) * S + q0 + r] = -INFINITY;
+      return;
+    }
+  }
   // Key tiles of each query tile (0: the tile lies past the sequence), and of the block.
   int Tt[NTILE];
 #pragma unroll
   for (int t = 0; t < NTILE; ++t) {
     const int r0 = q0 + QT * t;
-    const int k_end = CAUSAL ? min(S, r0 + QT) : S;
+    const int k_end = CAUSAL ? min(SK, r0 + QT) : SK;
     Tt[t] = r0 < S ? (k_end + KT - 1) / KT : 0;
   }
   const int T0 = Tt[0], T1 = Tt[1];
@@ -397,9 +415,9 @@ __global__ void __launch_bounds__(NBLK, 1) fwd_tc_kernel(const FwdArgs a) {
   static_assert(PARTS + BQ * 256 <= OFF_V - OFF_K + PARTS, "the staged Q ends inside V part buffer 0");
   if (!mma_warp) {
     stage_q<HD>(qst, qp, a.q_ss, q0, S);
-    stage_item<HD>(Kst, kp, a.k_ss, 0, S);
-    if (T > 1) stage_item<HD>(Vp + PARTS, kp, a.k_ss, KT, S);
-    stage_item<HD>(Vst, vp, a.v_ss, 0, S);
+    stage_item<HD>(Kst, kp, a.k_ss, 0, SK);
+    if (T > 1) stage_item<HD>(Vp + PARTS, kp, a.k_ss, KT, SK);
+    stage_item<HD>(Vst, vp, a.v_ss, 0, SK);
     cp_async_commit();
   }
   tc::fence_before_sync();
@@ -443,9 +461,9 @@ __global__ void __launch_bounds__(NBLK, 1) fwd_tc_kernel(const FwdArgs a) {
     bar_sync(1, NSM);
     // In flight during key tile 0: K(2), then V(1) (two cp.async groups, in that order), issued
     // while the tensor core computes the first S (each thread reuses staging slots only it read).
-    if (T > 2) stage_item<HD>(Kst, kp, a.k_ss, 2 * KT, S);
+    if (T > 2) stage_item<HD>(Kst, kp, a.k_ss, 2 * KT, SK);
     cp_async_commit();
-    if (T > 1) stage_item<HD>(Vst, vp, a.v_ss, KT, S);
+    if (T > 1) stage_item<HD>(Vst, vp, a.v_ss, KT, SK);
     cp_async_commit();
   }
   bool err = false;
@@ -512,6 +530,8 @@ __global__ void __launch_bounds__(NBLK, 1) fwd_tc_kernel(const FwdArgs a) {
       nbh = nb / a.n_qtiles;
     }
     const int nb_b = nbh / a.H, nb_h = nbh % a.H;
+    const int nb_hk = CROSS ? nb_h / (a.H / a.Hk) : nb_h;
+    const int rows = CROSS && tid >= BQ ? a.Sk : S;
     const float* src;
     int r;
     if (tid < BQ) {
@@ -519,12 +539,12 @@ __global__ void __launch_bounds__(NBLK, 1) fwd_tc_kernel(const FwdArgs a) {
       src = a.q + nb_b * a.q_sb + nb_h * a.q_sh + static_cast<int64_t>(r) * a.q_ss;
     } else if (tid < BQ + 2 * KT) {
       r = tid - BQ;
-      src = a.k + nb_b * a.k_sb + nb_h * a.k_sh + static_cast<int64_t>(r) * a.k_ss;
+      src = a.k + nb_b * a.k_sb + nb_hk * a.k_sh + static_cast<int64_t>(r) * a.k_ss;
     } else {
       r = tid - BQ - 2 * KT;
-      src = a.v + nb_b * a.v_sb + nb_h * a.v_sh + static_cast<int64_t>(r) * a.v_ss;
+      src = a.v + nb_b * a.v_sb + nb_hk * a.v_sh + static_cast<int64_t>(r) * a.v_ss;
     }
-    if (r < S) asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src), "n"(4 * HD) : "memory");
+    if (r < rows) asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src), "n"(4 * HD) : "memory");
   };
 
   const uint64_t sc2 = tc::pack2(a.scale, a.scale);
@@ -574,12 +594,12 @@ __global__ void __launch_bounds__(NBLK, 1) fwd_tc_kernel(const FwdArgs a) {
       const uint64_t y = mul2(tc::pack2(sv[c], sv[c + 1]), sc2);
       tc::unpack2(y, sv[c], sv[c + 1]);
     }
-    const bool edge = (k0 + KT > S) || (CAUSAL && k0 + KT - 1 > q0 + QT * t);
+    const bool edge = (k0 + KT > SK) || (CAUSAL && k0 + KT - 1 > q0 + QT * t);
     if (edge) {
 #pragma unroll
       for (int c = 0; c < CW; ++c) {
         const int jj = k0 + CW * cq + c;
-        if (!(jj < S && !(CAUSAL && jj > qi))) sv[c] = -INFINITY;
+        if (!(jj < SK && !(CAUSAL && jj > qi))) sv[c] = -INFINITY;
       }
     }
     float tmax = max3f(sv[0], sv[1], sv[2]);
@@ -643,7 +663,7 @@ __global__ void __launch_bounds__(NBLK, 1) fwd_tc_kernel(const FwdArgs a) {
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(bar_k + (n & 1));
     }
-    if (n + 3 < T) stage_item<HD>(Kst, kp, a.k_ss, (n + 3) * KT, S);
+    if (n + 3 < T) stage_item<HD>(Kst, kp, a.k_ss, (n + 3) * KT, SK);
     cp_async_commit();
   };
   // V(n + 1) into V buffer (n + 1) % 2 (it held V(n - 1): both P V(t, n - 1) have completed --
@@ -656,7 +676,7 @@ __global__ void __launch_bounds__(NBLK, 1) fwd_tc_kernel(const FwdArgs a) {
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(bar_v + ((n + 1) & 1));
     }
-    if (n + 2 < T) stage_item<HD>(Vst, vp, a.v_ss, (n + 2) * KT, S);
+    if (n + 2 < T) stage_item<HD>(Vst, vp, a.v_ss, (n + 2) * KT, SK);
     cp_async_commit();
   };
 
@@ -754,6 +774,28 @@ cudaError_t launch_fwd_tc(const FwdArgs& args, int head_dim, int causal, cudaStr
   }
   if (causal) return launch_pdl(fwd_tc_kernel<true, 64>, grid, dim3(NBLK), SMEM_ALLOC, stream, a);
   return launch_pdl(fwd_tc_kernel<false, 64>, grid, dim3(NBLK), SMEM_ALLOC, stream, a);
+}
+
+cudaError_t setup_cross_tc_attributes() {
+  const cudaError_t e = cudaFuncSetAttribute(fwd_tc_kernel<false, 64, true>,
+                                             cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_ALLOC);
+  return e != cudaSuccess ? e
+                          : cudaFuncSetAttribute(fwd_tc_kernel<false, 32, true>,
+                                                 cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_ALLOC);
+}
+
+cudaError_t launch_cross_fwd_tc(const FwdArgs& args, int head_dim, cudaStream_t stream) {
+  FwdArgs a = args;
+  a.n_qtiles = (a.S + BQ - 1) / BQ;
+  int dev = 0, sms = 0;
+  a.wave_ctas = cudaGetDevice(&dev) == cudaSuccess &&
+                        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess
+                    ? sms
+                    : 0;
+  const dim3 grid(static_cast<unsigned>(static_cast<int64_t>(a.n_qtiles) * a.B * a.H));
+  if (head_dim == 32)
+    return launch_pdl(fwd_tc_kernel<false, 32, true>, grid, dim3(NBLK), SMEM_ALLOC, stream, a);
+  return launch_pdl(fwd_tc_kernel<false, 64, true>, grid, dim3(NBLK), SMEM_ALLOC, stream, a);
 }
 
 cudaError_t fwd_tc_status(int* flag) {

@@ -1,0 +1,902 @@
+// SPDX-License-Identifier: MIT OR Apache-2.0
+//
+// Attention of few query rows over many keys, split over the keys and joined: paged_attention (one
+// or a few new tokens over a paged cache) and cross_attention's few-row form (a dense operand).
+//
+//   o = sum_j e^(y_j - m) v_j / sum_j e^(y_j - m),  y_j = scale q k_j,  m = max_j y_j
+//
+// over the keys a row sees. A sequence's keys are cut into chunks (split_chunk: by its own length
+// alone); a block forms one chunk's (m_c, l_c, o_c) for the rows that share a key head, and a second
+// kernel joins the chunks in order: m = max m_c, l = sum e^(m_c - m) l_c, o = sum e^(m_c - m) o_c / l.
+// A sequence of one chunk is written by the first kernel.
+//
+// Bound by memory: every key and value is read once for all the query rows of its head (up to 8 a
+// block), at 4 rows D flops a key against 2 D elements. Each warp runs on its own: it takes every
+// fourth tile of 16 keys of the chunk through a ring of its own (cp.async, 16 bytes a lane, rows
+// padded by 16 bytes so that every later read is free of bank conflicts), and the four warps' sums
+// are joined through shared memory once a chunk.
+//   16-bit caches: S^T = K Q^T and O^T += V^T P^T by mma.m16n8k16, the keys (dims) as the 16 rows
+//     and up to 8 query rows as the 8 columns: a column's softmax state then lives in the lanes
+//     that hold the column's output. fp32 queries enter in parts that keep their 24 bits (three
+//     bf16, or two fp16 under a power of two a row), p as two or three parts (16 bits for a 16-bit
+//     output, 24 for fp32), every tile's product a fresh accumulator folded by an fp32 FMA -- the
+//     tensor core's truncating sums never run longer than a tile. tcgen05 has no shape below 64
+//     rows, and at a few rows the product is a small share of the tile's load time.
+//   fp32 caches: two lanes a key for the scores, a quarter of a row a lane for the output, FMAs.
+//
+// Order of summation: fixed by the sequence's length and the row alone (not by the batch, the grid
+// or the SM count): results are bit-identical across reruns and batches.
+//
+// Masked keys are excluded rather than weighted by zero, so what lies behind a sequence's end or a
+// row's last key -- infinities and NaN among it -- never reaches a result. A page id outside the
+// pool is reported through the error sink and its keys are left out.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <type_traits>
+
+#include "cfa_common.cuh"
+#include "cfa_ops.h"
+#include "cfa_split.cuh"
+#include "cfa_tc.cuh"
+
+namespace cfa {
+namespace {
+
+constexpr int WARPS = 4;
+constexpr int NT = 32 * WARPS;
+constexpr int TK = 16;     // keys per tile
+constexpr int MAXR = 8;    // query rows per block
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr int CHUNK_MIN = 64, CHUNK_MAX = 512, FEW_CHUNKS = 16, MOST_CHUNKS = 256;
+
+// Keys per chunk of a sequence of `len` keys: the smallest power of two from 64 that gives at most
+// 16 chunks, but 512 at most until that would make more than 256.
+__host__ __device__ inline int64_t split_chunk(int64_t len) {
+  int64_t c = CHUNK_MIN;
+  while (c < CHUNK_MAX && len > FEW_CHUNKS * c) c *= 2;
+  while (len > MOST_CHUNKS * c) c *= 2;
+  return c;
+}
+__host__ __device__ inline int chunks_of(int64_t len) {
+  if (len <= 0) return 1;  // one empty chunk: its block writes the zeros
+  const int64_t c = split_chunk(len);
+  return static_cast<int>((len + c - 1) / c);
+}
+
+template <typename T>
+__device__ __forceinline__ T from_f(float x);
+template <>
+__device__ __forceinline__ float from_f(float x) { return x; }
+template <>
+__device__ __forceinline__ __half from_f(float x) { return __float2half_rn(x); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f(float x) { return __float2bfloat16_rn(x); }
+
+__device__ __forceinline__ int seq_len(const SplitArgs& a, int b) {
+  return a.lengths ? min(max(a.lengths[b], 0), a.max_len) : a.max_len;
+}
+__device__ __forceinline__ int seq_new(const SplitArgs& a, int b) {
+  return a.new_lengths ? min(max(a.new_lengths[b], 0), a.S) : a.S;
+}
+
+// The chunks of the batch in order: each lane holds its share of the sequences (a contiguous range)
+// and the chunks before and in it.
+struct ChunkIndex {
+  int first, per, before, count, total;
+  __device__ __forceinline__ void init(const SplitArgs& a, int lane) {
+    per = (a.B + 31) / 32;
+    first = lane * per;
+    count = 0;
+    for (int i = first; i < min(first + per, a.B); ++i) {
+      count += chunks_of(seq_len(a, i));
+      if (a.table && blockIdx.x == 0 && a.lengths[i] > a.max_len) flag_error(a.sink, CFA_ERR_PAGE);
+    }
+    int incl = count;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += x;
+    }
+    before = incl - count;
+    total = __shfl_sync(0xffffffffu, incl, 31);
+  }
+  // Chunk g of the batch (g < total): its sequence, chunk in the sequence, chunks of it.
+  __device__ __forceinline__ void find(const SplitArgs& a, int g, int& b, int& c, int& nc) const {
+    const unsigned in = __ballot_sync(0xffffffffu, g >= before && g < before + count);
+    const int owner = __ffs(in) - 1;
+    b = __shfl_sync(0xffffffffu, first, owner);
+    c = g - __shfl_sync(0xffffffffu, before, owner);
+    nc = chunks_of(seq_len(a, b));
+    while (c >= nc) {
+      c -= nc;
+      nc = chunks_of(seq_len(a, ++b));
+    }
+  }
+};
+
+// One warp's ring of tiles: 16 rows of K, then of V, RB bytes apart.
+template <int D, int ES, int STAGES>
+struct Ring {
+  static constexpr int RB = D * ES + 16;
+  static constexpr int KV = TK * RB;          // bytes of a tile's K (or V)
+  static constexpr int STAGE = 2 * KV;
+  static constexpr int CPR = D * ES / 16;     // 16-byte pieces of a row
+  static constexpr int BYTES = STAGES * STAGE;
+
+  const SplitArgs& a;
+  unsigned char* base;
+  const char* kp;  // this (batch, key head)'s keys and values
+  const char* vp;
+  const int* table;
+  int lane, len;
+  bool bad = false;
+
+  __device__ __forceinline__ Ring(const SplitArgs& a_, unsigned char* base_, int lane_)
+      : a(a_), base(base_), lane(lane_) {}
+
+  __device__ __forceinline__ void start(int b, int hk, int len_) {
+    len = len_;
+    kp = static_cast<const char*>(a.k) + ES * (hk * a.k_sh + (a.table ? 0 : b * a.k_sp));
+    vp = static_cast<const char*>(a.v) + ES * (hk * a.v_sh + (a.table ? 0 : b * a.v_sp));
+    table = a.table ? a.table + b * a.table_sb : nullptr;
+  }
+  // The page of this lane's row of the tile at key k0 (0 where dense; -1 past the end).
+  __device__ __forceinline__ int page_of(int k0) const {
+    const int key = k0 + (lane & (TK - 1));
+    if (key >= len) return -1;
+    return table ? __ldg(table + key / a.page) : 0;
+  }
+  // Copies the tile at key k0 into `stage`; pg: page_of(k0). Returns the tile's live keys as bits.
+  __device__ __forceinline__ unsigned load(int k0, int stage, int pg) {
+    const int key = k0 + (lane & (TK - 1));
+    bool ok = key < len;
+    int64_t ko = 0, vo = 0;
+    if (table) {
+      if (ok && (pg < 0 || pg >= a.n_pages)) {
+        ok = false;
+        bad = true;
+      }
+      if (ok) {
+        const int row = key - key / a.page * a.page;
+        ko = pg * a.k_sp + row * a.k_sr;
+        vo = pg * a.v_sp + row * a.v_sr;
+      }
+    } else if (ok) {
+      ko = key * a.k_sr;
+      vo = key * a.v_sr;
+    }
+    const unsigned live = __ballot_sync(0xffffffffu, ok) & 0xffffu;
+    unsigned char* st = base + stage * STAGE;
+#pragma unroll
+    for (int j = 0; j < TK * CPR / 32; ++j) {
+      const int i = j * 32 + lane, r = i / CPR, c = i % CPR;
+      const int64_t kr = __shfl_sync(0xffffffffu, ko, r), vr = __shfl_sync(0xffffffffu, vo, r);
+      const int n = (live >> r) & 1u ? 16 : 0;
+      cp_async16(st + r * RB + 16 * c, kp + ES * kr + 16 * c, n);
+      cp_async16(st + KV + r * RB + 16 * c, vp + ES * vr + 16 * c, n);
+    }
+    return live;
+  }
+};
+
+template <int N>
+__device__ __forceinline__ void cp_async_wait_group() {
+  asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], const void* p) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(tc::smem_u32(p))
+               : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], const void* p) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(tc::smem_u32(p))
+               : "memory");
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+template <typename T>
+__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same_v<T, __half>)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+        "{%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+        "{%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// A pair of floats as the 16-bit type, the first low; and the pair it stands for.
+template <typename T>
+__device__ __forceinline__ uint32_t pack16(float lo, float hi) {
+  if constexpr (std::is_same_v<T, __half>) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+template <typename T>
+__device__ __forceinline__ float2 unpack16(uint32_t x) {
+  if constexpr (std::is_same_v<T, __half>) return __half22float2(*reinterpret_cast<__half2*>(&x));
+  else return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
+}
+
+// What a block knows of its unit.
+struct UnitInfo {
+  int b, hk, r0, chunk, nc, len, n_new, lo, hi;  // rows r0 .., keys lo .. hi - 1
+};
+__device__ __forceinline__ UnitInfo unit_info(const SplitArgs& a, const ChunkIndex& ix, int64_t u) {
+  UnitInfo n;
+  const int per = a.Hk * a.row_chunks;
+  const int g = static_cast<int>(u / per), rest = static_cast<int>(u - static_cast<int64_t>(g) * per);
+  n.hk = rest / a.row_chunks;
+  n.r0 = (rest - n.hk * a.row_chunks) * MAXR;
+  ix.find(a, g, n.b, n.chunk, n.nc);
+  n.len = seq_len(a, n.b);
+  n.n_new = seq_new(a, n.b);
+  const int64_t c = split_chunk(n.len);
+  n.lo = static_cast<int>(n.chunk * c);
+  n.hi = static_cast<int>(min(static_cast<int64_t>(n.len), n.lo + c));
+  return n;
+}
+// Row r of a key head's rows: query head r / S of the group, new token r % S. The keys it sees (a
+// row that is not there sees them all: its result is never written).
+__device__ __forceinline__ int row_limit(const SplitArgs& a, const UnitInfo& n, int r) {
+  const int i = r % a.S;
+  if (!a.causal || r >= a.rows || i >= n.n_new) return n.len;
+  return min(max(n.len - n.n_new + i + 1, 0), n.len);
+}
+
+// Joins the four warps' sums of rows r0 .. r0 + nr - 1 (red: [warp][row][D], ml: [warp][row]) and
+// writes the chunk's partial result, or, the sequence's only chunk, the output.
+template <typename QT, int D>
+__device__ __forceinline__ void write_chunk(const SplitArgs& a, const UnitInfo& n, const float* red,
+                                            const float2* ml, int nr) {
+  for (int idx = threadIdx.x; idx < nr * (D / 4); idx += NT) {
+    const int r = idx / (D / 4), c4 = idx % (D / 4);
+    const int row = n.r0 + r;
+    if (row >= a.rows) continue;
+    const int head = n.hk * a.group + row / a.S, i = row % a.S;
+    float m = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) m = fmaxf(m, ml[w * MAXR + r].x);
+    float l = 0.0f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    const float mu = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      const float2 x = ml[w * MAXR + r];
+      const float f = ex2((x.x - mu) * LOG2E);
+      const float4 v = *reinterpret_cast<const float4*>(red + (w * MAXR + r) * D + 4 * c4);
+      l = fmaf(x.y, f, l);
+      o.x = fmaf(v.x, f, o.x);
+      o.y = fmaf(v.y, f, o.y);
+      o.z = fmaf(v.z, f, o.z);
+      o.w = fmaf(v.w, f, o.w);
+    }
+    if (n.nc == 1) {
+      const bool live = i < n.n_new && l != 0.0f;  // no keys, or no such token: zeros
+      QT* dst = static_cast<QT*>(a.o) + ((static_cast<int64_t>(n.b) * a.S + i) * a.H + head) * D + 4 * c4;
+      dst[0] = from_f<QT>(live ? o.x / l : 0.0f);
+      dst[1] = from_f<QT>(live ? o.y / l : 0.0f);
+      dst[2] = from_f<QT>(live ? o.z / l : 0.0f);
+      dst[3] = from_f<QT>(live ? o.w / l : 0.0f);
+    } else if (i < n.n_new) {
+      const int64_t at = ((static_cast<int64_t>(n.b) * a.H + head) * a.S + i) * a.max_chunks + n.chunk;
+      *reinterpret_cast<float4*>(a.part_o + at * D + 4 * c4) = o;
+      if (c4 == 0) a.part_ml[at] = make_float2(m, l);
+    }
+  }
+}
+
+template <int D, int ES>
+__host__ __device__ constexpr int stages() {
+  // 24 KB a warp or so, at least two tiles in flight besides the one in use.
+  return D * ES >= 512 ? 3 : (D * ES >= 256 ? 3 : (D * ES >= 128 ? 4 : 6));
+}
+template <int D>
+__host__ __device__ constexpr int red_bytes() {
+  return WARPS * MAXR * D * 4;
+}
+template <int D, int ES>
+__host__ __device__ constexpr int split_smem() {
+  const int ring = WARPS * Ring<D, ES, stages<D, ES>()>::BYTES;
+  return (ring > red_bytes<D>() ? ring : red_bytes<D>()) + WARPS * MAXR * 8 + MAXR * D * 4;
+}
+
+// 16-bit caches.
+template <typename QT, typename T, int D>
+__global__ void __launch_bounds__(NT) split_mma_kernel(const SplitArgs a) {
+  constexpr int ST = stages<D, 2>();
+  using R = Ring<D, 2, ST>;
+  constexpr bool F32 = std::is_same_v<QT, float>;
+  constexpr bool HALF = std::is_same_v<T, __half>;
+  constexpr int QP = F32 ? (HALF ? 2 : 3) : 1;  // parts of q
+  constexpr int PP = F32 && !HALF ? 3 : 2;      // parts of p
+  constexpr int KS = D / 16;
+  extern __shared__ __align__(128) unsigned char smem[];
+  const int tid = threadIdx.x, w = tid >> 5, lane = tid & 31;
+  const int qr = lane >> 2, qc = lane & 3;  // a fragment's row (key, dim; B: column) and pair
+  float* red = reinterpret_cast<float*>(smem);
+  float2* ml = reinterpret_cast<float2*>(smem + split_smem<D, 2>() - WARPS * MAXR * 8 - MAXR * D * 4);
+  griddep_wait();
+  griddep_launch_dependents();
+  ChunkIndex ix;
+  ix.init(a, lane);
+  const int64_t units = static_cast<int64_t>(ix.total) * a.Hk * a.row_chunks;
+  R ring(a, smem + w * R::BYTES, lane);
+
+  for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
+    const UnitInfo n = unit_info(a, ix, u);
+    ring.start(n.b, n.hk, n.hi);
+    const int tiles = (n.hi - n.lo + TK - 1) / TK;
+    unsigned live[ST];
+    int t_load = w, pg = tiles > w ? ring.page_of(n.lo + TK * w) : -1;
+    auto issue = [&](int stage) -> unsigned {
+      unsigned x = 0;
+      if (t_load < tiles) {
+        x = ring.load(n.lo + TK * t_load, stage, pg);
+        t_load += WARPS;
+        if (t_load < tiles) pg = ring.page_of(n.lo + TK * t_load);
+      }
+      cp_async_commit();
+      return x;
+    };
+#pragma unroll
+    for (int s = 0; s < ST - 1; ++s) live[s] = issue(s);
+
+    // Q^T as B fragments: column qr, dims 16 ks + 2 qc, + 1 and + 8, + 9.
+    uint32_t qb[QP][KS][2];
+    float qscale0 = a.scale, qscale1 = a.scale;  // of columns 2 qc, 2 qc + 1
+    {
+      const int row = n.r0 + qr;
+      const bool ok = row < a.rows && row % a.S < n.n_new;
+      const QT* q = static_cast<const QT*>(a.q) + n.b * a.q_sb +
+                    (n.hk * a.group + (ok ? row / a.S : 0)) * a.q_sh + (ok ? row % a.S : 0) * a.q_ss;
+      if constexpr (!F32) {
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            qb[0][ks][h] = ok ? *reinterpret_cast<const uint32_t*>(q + 16 * ks + 8 * h + 2 * qc) : 0u;
+      } else {
+        float2 x[KS][2];
+        float top = 0.0f;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            x[ks][h] = ok ? *reinterpret_cast<const float2*>(q + 16 * ks + 8 * h + 2 * qc)
+                          : make_float2(0.f, 0.f);
+            top = fmaxf(top, fmaxf(fabsf(x[ks][h].x), fabsf(x[ks][h].y)));
+          }
+        if constexpr (HALF) {
+          // q = 2^e (h0 + 2^-11 h1), |h0| <= 2: what the two parts miss is below 2^-24 of q, or
+          // 2^-36 of the row's largest.
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+          int e = top > 0.0f && top < INFINITY ? ilogbf(top) : 0;
+          e = max(-120, min(120, e));
+          const float down = ldexpf(1.0f, -e), up = ldexpf(1.0f, e);
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const float lo = x[ks][h].x * down, hi = x[ks][h].y * down;
+              qb[0][ks][h] = pack16<T>(lo, hi);
+              const float2 z = unpack16<T>(qb[0][ks][h]);
+              qb[QP - 1][ks][h] = pack16<T>((lo - z.x) * 2048.0f, (hi - z.y) * 2048.0f);
+            }
+          qscale0 *= __shfl_sync(0xffffffffu, up, 8 * qc);
+          qscale1 *= __shfl_sync(0xffffffffu, up, 8 * qc + 4);
+        } else {
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              float2 y = x[ks][h];
+#pragma unroll
+              for (int p = 0; p < QP; ++p) {
+                qb[p][ks][h] = pack16<T>(y.x, y.y);
+                const float2 z = unpack16<T>(qb[p][ks][h]);
+                y = make_float2(y.x - z.x, y.y - z.y);
+              }
+            }
+        }
+      }
+    }
+    const int lim0 = row_limit(a, n, n.r0 + 2 * qc), lim1 = row_limit(a, n, n.r0 + 2 * qc + 1);
+    // The fewest keys that a row of the block sees: a tile that ends behind it masks row by row.
+    const int lim_min = a.causal ? max(n.len - n.n_new + 1, 0) : n.len;
+
+    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
+    float acc[KS][4];  // O^T: dims 16 mt + qr (+ 8), columns 2 qc, + 1
+#pragma unroll
+    for (int i = 0; i < KS; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[i][j] = 0.0f;
+
+    int stage = 0;
+    for (int t = w; t < tiles; t += WARPS) {
+      cp_async_wait_group<ST - 2>();
+      __syncwarp();  // the tile is in place for every lane, and the stage before it is free
+      unsigned now = live[0];
+#pragma unroll
+      for (int s = 0; s + 1 < ST - 1; ++s) live[s] = live[s + 1];
+      live[ST - 2] = issue(stage == 0 ? ST - 1 : stage - 1);
+      const unsigned char* kt = ring.base + stage * R::STAGE;
+      const unsigned char* vt = kt + R::KV;
+      const int k0 = n.lo + TK * t;
+
+      float s[4] = {0.f, 0.f, 0.f, 0.f};
+      if constexpr (F32) {  // the small parts first: their sums truncate at their own magnitude
+        float c[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          uint32_t ka[4];
+          ldsm4(ka, kt + (lane & 15) * R::RB + 32 * ks + 16 * (lane >> 4));
+#pragma unroll
+          for (int p = QP - 1; p > 0; --p) mma<T>(c, ka, qb[p][ks][0], qb[p][ks][1]);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[j] = HALF ? c[j] * (1.0f / 2048.0f) : c[j];
+      }
+      {
+        float c[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          uint32_t ka[4];
+          ldsm4(ka, kt + (lane & 15) * R::RB + 32 * ks + 16 * (lane >> 4));
+          mma<T>(c, ka, qb[0][ks][0], qb[0][ks][1]);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[j] = (s[j] + c[j]) * (j & 1 ? qscale1 : qscale0);
+      }
+      // s[0], s[1]: key qr, columns 2 qc, + 1; s[2], s[3]: key qr + 8.
+      const bool edge = lim_min < min(k0 + TK, n.hi);
+      if (now != 0xffffu || edge) {
+        const bool ka = (now >> qr) & 1u, kb = (now >> (qr + 8)) & 1u;
+        if (!ka || k0 + qr >= lim0) s[0] = -INFINITY;
+        if (!ka || k0 + qr >= lim1) s[1] = -INFINITY;
+        if (!kb || k0 + qr + 8 >= lim0) s[2] = -INFINITY;
+        if (!kb || k0 + qr + 8 >= lim1) s[3] = -INFINITY;
+      }
+      float t0 = fmaxf(s[0], s[2]), t1 = fmaxf(s[1], s[3]);
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) {
+        t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, o));
+        t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, o));
+      }
+      t0 = fmaxf(t0, m0);
+      t1 = fmaxf(t1, m1);
+      const float u0 = t0 == -INFINITY ? 0.0f : t0, u1 = t1 == -INFINITY ? 0.0f : t1;
+      const float a0 = ex2((m0 - u0) * LOG2E), a1 = ex2((m1 - u1) * LOG2E);
+      m0 = t0;
+      m1 = t1;
+      s[0] = ex2((s[0] - u0) * LOG2E);
+      s[1] = ex2((s[1] - u1) * LOG2E);
+      s[2] = ex2((s[2] - u0) * LOG2E);
+      s[3] = ex2((s[3] - u1) * LOG2E);
+      l0 = fmaf(l0, a0, s[0] + s[2]);
+      l1 = fmaf(l1, a1, s[1] + s[3]);
+      // P^T as B fragments (transposed 8 x 8 blocks), in parts.
+      uint32_t pb[PP][2];
+      float2 x = make_float2(s[0], s[1]), y = make_float2(s[2], s[3]);
+#pragma unroll
+      for (int p = 0; p < PP; ++p) {
+        const uint32_t hx = pack16<T>(x.x, x.y), hy = pack16<T>(y.x, y.y);
+        const float2 zx = unpack16<T>(hx), zy = unpack16<T>(hy);
+        x = make_float2(x.x - zx.x, x.y - zx.y);
+        y = make_float2(y.x - zy.x, y.y - zy.y);
+        pb[p][0] = transpose8(hx);
+        pb[p][1] = transpose8(hy);
+      }
+      // The V^T block of dims 16 mt ..: rows (keys) (lane % 8) + 8 (lane / 16), dims + 8 (lane / 8 % 2).
+      const unsigned char* va_at = vt + ((lane & 7) + 8 * (lane >> 4)) * R::RB + 16 * ((lane >> 3) & 1);
+      if (!edge) {
+#pragma unroll
+        for (int mt = 0; mt < KS; ++mt) {
+          uint32_t va[4];
+          ldsm4t(va, va_at + 32 * mt);
+          float c[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int p = PP - 1; p >= 0; --p) mma<T>(c, va, pb[p][0], pb[p][1]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[mt][j] = fmaf(acc[mt][j], j & 1 ? a1 : a0, c[j]);
+        }
+      } else {
+        // Keys that only some of the rows see: one row at a time, the values it does not see as
+        // zeros (0 times what they hold could be NaN).
+#pragma unroll
+        for (int mt = 0; mt < KS; ++mt)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[mt][j] *= j & 1 ? a1 : a0;
+        for (int r = 0; r < min(MAXR, a.rows - n.r0); ++r) {
+          const int lim = row_limit(a, n, n.r0 + r);
+          const int k = k0 + 2 * qc;  // this lane's keys of an A fragment: k, k + 1, k + 8, k + 9
+          const uint32_t mlo = (k < lim ? 0xffffu : 0u) | (k + 1 < lim ? 0xffff0000u : 0u);
+          const uint32_t mhi = (k + 8 < lim ? 0xffffu : 0u) | (k + 9 < lim ? 0xffff0000u : 0u);
+#pragma unroll
+          for (int mt = 0; mt < KS; ++mt) {
+            uint32_t va[4];
+            ldsm4t(va, va_at + 32 * mt);
+            va[0] &= mlo;
+            va[1] &= mlo;
+            va[2] &= mhi;
+            va[3] &= mhi;
+            float c[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int p = PP - 1; p >= 0; --p)
+              mma<T>(c, va, qr == r ? pb[p][0] : 0u, qr == r ? pb[p][1] : 0u);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (2 * qc + (j & 1) == r) acc[mt][j] += c[j];
+          }
+        }
+      }
+      stage = stage + 1 == ST ? 0 : stage + 1;
+    }
+    cp_async_wait_group<0>();
+#pragma unroll
+    for (int o = 4; o < 32; o <<= 1) {
+      l0 += __shfl_xor_sync(0xffffffffu, l0, o);
+      l1 += __shfl_xor_sync(0xffffffffu, l1, o);
+    }
+    __syncthreads();  // every warp's tiles are read: their space takes the sums
+    if (qr == 0) {
+      ml[w * MAXR + 2 * qc] = make_float2(m0, l0);
+      ml[w * MAXR + 2 * qc + 1] = make_float2(m1, l1);
+    }
+#pragma unroll
+    for (int mt = 0; mt < KS; ++mt)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        red[(w * MAXR + 2 * qc + (j & 1)) * D + 16 * mt + qr + 8 * (j >> 1)] = acc[mt][j];
+    __syncthreads();
+    write_chunk<QT, D>(a, n, red, ml, MAXR);
+    __syncthreads();  // the sums are read: the next unit's tiles may land
+  }
+  if (ring.bad) flag_error(a.sink, CFA_ERR_PAGE);
+}
+
+// fp32 caches: NR query rows (1, 2, 4 or 8).
+template <int D, int NR>
+__global__ void __launch_bounds__(NT) split_f32_kernel(const SplitArgs a) {
+  constexpr int ST = stages<D, 4>();
+  using R = Ring<D, 4, ST>;
+  constexpr int LPR = D / 4, KPI = 32 / LPR;  // lanes of a V row; keys at a time
+  extern __shared__ __align__(128) unsigned char smem[];
+  const int tid = threadIdx.x, w = tid >> 5, lane = tid & 31;
+  float* red = reinterpret_cast<float*>(smem);
+  float2* ml = reinterpret_cast<float2*>(smem + split_smem<D, 4>() - WARPS * MAXR * 8 - MAXR * D * 4);
+  float* qs = reinterpret_cast<float*>(smem + split_smem<D, 4>() - MAXR * D * 4);  // [NR][D]
+  griddep_wait();
+  griddep_launch_dependents();
+  ChunkIndex ix;
+  ix.init(a, lane);
+  const int64_t units = static_cast<int64_t>(ix.total) * a.Hk * a.row_chunks;
+  R ring(a, smem + w * R::BYTES, lane);
+
+  for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
+    const UnitInfo n = unit_info(a, ix, u);
+    ring.start(n.b, n.hk, n.hi);
+    const int tiles = (n.hi - n.lo + TK - 1) / TK;
+    unsigned live[ST];
+    int t_load = w, pg = tiles > w ? ring.page_of(n.lo + TK * w) : -1;
+    auto issue = [&](int stage) -> unsigned {
+      unsigned x = 0;
+      if (t_load < tiles) {
+        x = ring.load(n.lo + TK * t_load, stage, pg);
+        t_load += WARPS;
+        if (t_load < tiles) pg = ring.page_of(n.lo + TK * t_load);
+      }
+      cp_async_commit();
+      return x;
+    };
+#pragma unroll
+    for (int s = 0; s < ST - 1; ++s) live[s] = issue(s);
+    for (int i = tid; i < NR * LPR; i += NT) {
+      const int row = n.r0 + i / LPR, c = i % LPR;
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (row < a.rows && row % a.S < n.n_new)
+        x = *reinterpret_cast<const float4*>(static_cast<const float*>(a.q) + n.b * a.q_sb +
+                                             (n.hk * a.group + row / a.S) * a.q_sh +
+                                             (row % a.S) * a.q_ss + 4 * c);
+      reinterpret_cast<float4*>(qs)[i] = x;
+    }
+    __syncthreads();  // q in place
+    const int lim_min = a.causal ? max(n.len - n.n_new + 1, 0) : n.len;
+    float m[NR], l[NR], acc[NR][4];
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+      m[r] = -INFINITY;
+      l[r] = acc[r][0] = acc[r][1] = acc[r][2] = acc[r][3] = 0.0f;
+    }
+    int stage = 0;
+    for (int t = w; t < tiles; t += WARPS) {
+      cp_async_wait_group<ST - 2>();
+      __syncwarp();
+      const unsigned now = live[0];
+#pragma unroll
+      for (int s = 0; s + 1 < ST - 1; ++s) live[s] = live[s + 1];
+      live[ST - 2] = issue(stage == 0 ? ST - 1 : stage - 1);
+      const unsigned char* kt = ring.base + stage * R::STAGE;
+      const unsigned char* vt = kt + R::KV;
+      const int k0 = n.lo + TK * t;
+      const bool edge = lim_min < min(k0 + TK, n.hi);
+      // Scores: lanes 0-15 take the first half of their key's dims, lanes 16-31 the second.
+      float s[NR];
+#pragma unroll
+      for (int r = 0; r < NR; ++r) s[r] = 0.0f;
+      const float* kr = reinterpret_cast<const float*>(kt + (lane & 15) * R::RB) + (lane >> 4) * (D / 2);
+      const float* qh = qs + (lane >> 4) * (D / 2);
+#pragma unroll
+      for (int c = 0; c < D / 8; ++c) {
+        const float4 x = reinterpret_cast<const float4*>(kr)[c];
+#pragma unroll
+        for (int r = 0; r < NR; ++r) s[r] = dot4(x, ld4(qh + r * D + 4 * c), s[r]);
+      }
+      float p[NR], al[NR];
+#pragma unroll
+      for (int r = 0; r < NR; ++r) {
+        float y = (s[r] + __shfl_xor_sync(0xffffffffu, s[r], 16)) * a.scale;
+        const int key = k0 + (lane & 15);
+        if (!((now >> (lane & 15)) & 1u) || (edge && key >= row_limit(a, n, n.r0 + r))) y = -INFINITY;
+        float top = y;
+#pragma unroll
+        for (int o = 1; o < 16; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        top = fmaxf(top, m[r]);
+        const float mu = top == -INFINITY ? 0.0f : top;
+        al[r] = ex2((m[r] - mu) * LOG2E);
+        m[r] = top;
+        p[r] = ex2((y - mu) * LOG2E);
+        l[r] = fmaf(l[r], al[r], p[r]);  // this lane's keys (both halves hold the same)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) acc[r][c] *= al[r];
+      }
+#pragma unroll
+      for (int j = 0; j < TK / KPI; ++j) {
+        const int k = KPI * j + lane / LPR;
+        const float4 v = *reinterpret_cast<const float4*>(vt + k * R::RB + 16 * (lane % LPR));
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+          const float pk = __shfl_sync(0xffffffffu, p[r], k);
+          if (!edge || pk != 0.0f) {  // an unseen key's value may be NaN
+            acc[r][0] = fmaf(pk, v.x, acc[r][0]);
+            acc[r][1] = fmaf(pk, v.y, acc[r][1]);
+            acc[r][2] = fmaf(pk, v.z, acc[r][2]);
+            acc[r][3] = fmaf(pk, v.w, acc[r][3]);
+          }
+        }
+      }
+      stage = stage + 1 == ST ? 0 : stage + 1;
+    }
+    cp_async_wait_group<0>();
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+#pragma unroll
+      for (int o = 1; o < 16; o <<= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], o);
+#pragma unroll
+      for (int o = LPR; o < 32; o <<= 1)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) acc[r][c] += __shfl_xor_sync(0xffffffffu, acc[r][c], o);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+      if (lane == 0) ml[w * MAXR + r] = make_float2(m[r], l[r]);
+      if (lane < LPR)
+        *reinterpret_cast<float4*>(red + (w * MAXR + r) * D + 4 * lane) =
+            make_float4(acc[r][0], acc[r][1], acc[r][2], acc[r][3]);
+    }
+    __syncthreads();
+    write_chunk<float, D>(a, n, red, ml, NR);
+    __syncthreads();
+  }
+  if (ring.bad) flag_error(a.sink, CFA_ERR_PAGE);
+}
+
+// The chunks' join: a block per output row; its threads take the row's float4 columns and, side by
+// side, every G-th chunk, then add their sums in order.
+template <typename QT, int D>
+__global__ void __launch_bounds__(NT) split_join_kernel(const SplitArgs a) {
+  constexpr int C4 = D / 4, G = NT / C4;
+  __shared__ float wt[MOST_CHUNKS];
+  __shared__ float4 sums[G][C4];
+  __shared__ float red[2][WARPS];
+  griddep_wait();
+  griddep_launch_dependents();
+  const int tid = threadIdx.x, w = tid >> 5, lane = tid & 31;
+  const int64_t row = blockIdx.x;  // (b H + head) S + i
+  const int i = static_cast<int>(row % a.S);
+  const int64_t bh = row / a.S;
+  const int b = static_cast<int>(bh / a.H), head = static_cast<int>(bh % a.H);
+  const int nc = chunks_of(seq_len(a, b));
+  if (nc == 1) return;  // written by the first kernel
+  const bool live = i < seq_new(a, b);
+  const float2* ml = a.part_ml + row * a.max_chunks;
+  float m = -INFINITY;
+  float2 x[MOST_CHUNKS / NT];
+#pragma unroll
+  for (int j = 0; j < MOST_CHUNKS / NT; ++j) {
+    const int c = tid + j * NT;
+    x[j] = live && c < nc ? ml[c] : make_float2(-INFINITY, 0.0f);
+    m = fmaxf(m, x[j].x);
+  }
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if (lane == 0) red[0][w] = m;
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < WARPS; ++j) m = fmaxf(m, red[0][j]);
+  const float mu = m == -INFINITY ? 0.0f : m;
+  float l = 0.0f;
+#pragma unroll
+  for (int j = 0; j < MOST_CHUNKS / NT; ++j) {
+    const int c = tid + j * NT;
+    const float f = ex2((x[j].x - mu) * LOG2E);
+    if (c < nc) wt[c] = f;
+    l = fmaf(x[j].y, f, l);
+  }
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+  if (lane == 0) red[1][w] = l;
+  __syncthreads();
+  l = ((red[1][0] + red[1][1]) + red[1][2]) + red[1][3];
+  const int c4 = tid % C4, g = tid / C4;
+  const float4* po = reinterpret_cast<const float4*>(a.part_o + row * a.max_chunks * D) + c4;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (live) {
+#pragma unroll 8
+    for (int c = g; c < nc; c += G) {
+      const float4 v = po[static_cast<int64_t>(c) * C4];
+      const float f = wt[c];
+      o.x = fmaf(v.x, f, o.x);
+      o.y = fmaf(v.y, f, o.y);
+      o.z = fmaf(v.z, f, o.z);
+      o.w = fmaf(v.w, f, o.w);
+    }
+  }
+  sums[g][c4] = o;
+  __syncthreads();
+  if (g == 0) {
+#pragma unroll
+    for (int j = 1; j < G; ++j) {
+      const float4 v = sums[j][c4];
+      o = make_float4(o.x + v.x, o.y + v.y, o.z + v.z, o.w + v.w);
+    }
+    const bool some = live && l != 0.0f;
+    QT* dst = static_cast<QT*>(a.o) + ((static_cast<int64_t>(b) * a.S + i) * a.H + head) * D + 4 * c4;
+    dst[0] = from_f<QT>(some ? o.x / l : 0.0f);
+    dst[1] = from_f<QT>(some ? o.y / l : 0.0f);
+    dst[2] = from_f<QT>(some ? o.z / l : 0.0f);
+    dst[3] = from_f<QT>(some ? o.w / l : 0.0f);
+  }
+}
+
+// Resident blocks: the grid is persistent, as many as fit at once (or as there are units at most).
+template <typename F>
+int resident(F* kernel, int smem) {
+  int dev = 0, sms = 0, per = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess ||
+      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess ||
+      cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kernel, NT, smem) != cudaSuccess)
+    return 148;
+  return sms * (per > 0 ? per : 1);
+}
+
+template <typename F>
+cudaError_t launch_split(F* kernel, int smem, const SplitArgs& a, cudaStream_t stream) {
+  const int64_t units = static_cast<int64_t>(a.B) * a.max_chunks * a.Hk * a.row_chunks;
+  const int64_t fit = resident(kernel, smem);
+  return launch_pdl(kernel, dim3(static_cast<unsigned>(units < fit ? units : fit)), dim3(NT), smem,
+                    stream, a);
+}
+
+template <typename QT, int D>
+cudaError_t launch_join(const SplitArgs& a, cudaStream_t stream) {
+  if (a.max_chunks == 1) return cudaSuccess;
+  return launch_pdl(split_join_kernel<QT, D>, dim3(static_cast<unsigned>(a.B * a.H * a.S)), dim3(NT),
+                    0, stream, a);
+}
+
+template <int D>
+cudaError_t launch_d(const SplitArgs& a, int qd, int kd, cudaStream_t stream) {
+  cudaError_t e;
+  constexpr int S2 = split_smem<D, 2>(), S4 = split_smem<D, 4>();
+  if (qd == CFA_F32) {
+    if (kd == CFA_F32) {
+      e = a.rows == 1   ? launch_split(split_f32_kernel<D, 1>, S4, a, stream)
+          : a.rows == 2 ? launch_split(split_f32_kernel<D, 2>, S4, a, stream)
+          : a.rows <= 4 ? launch_split(split_f32_kernel<D, 4>, S4, a, stream)
+                        : launch_split(split_f32_kernel<D, 8>, S4, a, stream);
+    } else if (kd == CFA_F16) {
+      e = launch_split(split_mma_kernel<float, __half, D>, S2, a, stream);
+    } else {
+      e = launch_split(split_mma_kernel<float, __nv_bfloat16, D>, S2, a, stream);
+    }
+    return e == cudaSuccess ? launch_join<float, D>(a, stream) : e;
+  }
+  if (qd == CFA_F16) {
+    e = launch_split(split_mma_kernel<__half, __half, D>, S2, a, stream);
+    return e == cudaSuccess ? launch_join<__half, D>(a, stream) : e;
+  }
+  e = launch_split(split_mma_kernel<__nv_bfloat16, __nv_bfloat16, D>, S2, a, stream);
+  return e == cudaSuccess ? launch_join<__nv_bfloat16, D>(a, stream) : e;
+}
+
+template <int D>
+cudaError_t set_attrs() {
+  cudaError_t e = cudaSuccess;
+  auto set = [&](const void* fn, int bytes) {
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  };
+  constexpr int S2 = split_smem<D, 2>(), S4 = split_smem<D, 4>();
+  static_assert(S2 <= 232448 && S4 <= 232448, "shared memory per block");
+  set(reinterpret_cast<const void*>(split_f32_kernel<D, 1>), S4);
+  set(reinterpret_cast<const void*>(split_f32_kernel<D, 2>), S4);
+  set(reinterpret_cast<const void*>(split_f32_kernel<D, 4>), S4);
+  set(reinterpret_cast<const void*>(split_f32_kernel<D, 8>), S4);
+  set(reinterpret_cast<const void*>(split_mma_kernel<float, __half, D>), S2);
+  set(reinterpret_cast<const void*>(split_mma_kernel<float, __nv_bfloat16, D>), S2);
+  set(reinterpret_cast<const void*>(split_mma_kernel<__half, __half, D>), S2);
+  set(reinterpret_cast<const void*>(split_mma_kernel<__nv_bfloat16, __nv_bfloat16, D>), S2);
+  return e;
+}
+
+}  // namespace
+
+cudaError_t setup_split_attributes() {
+  cudaError_t e = set_attrs<32>();
+  if (e == cudaSuccess) e = set_attrs<64>();
+  return e == cudaSuccess ? set_attrs<128>() : e;
+}
+
+// Most chunks of a sequence of at most max_len keys.
+int split_max_chunks(int64_t max_len) {
+  if (max_len <= CHUNK_MIN) return 1;
+  int64_t n = (max_len + CHUNK_MAX - 1) / CHUNK_MAX;
+  if (n < FEW_CHUNKS) n = FEW_CHUNKS;
+  if (n > MOST_CHUNKS) n = MOST_CHUNKS;
+  const int64_t few = (max_len + CHUNK_MIN - 1) / CHUNK_MIN;
+  return static_cast<int>(n < few ? n : few);
+}
+
+size_t split_workspace_bytes(int64_t rows, int64_t max_len, int64_t head_dim) {
+  const int64_t n = split_max_chunks(max_len);
+  if (n == 1) return 0;
+  return static_cast<size_t>(rows * n) * (head_dim + 2) * sizeof(float);
+}
+
+cudaError_t launch_split_attention(const SplitArgs& args, int q_dtype, int kv_dtype, void* workspace,
+                                   cudaStream_t stream) {
+  SplitArgs a = args;
+  a.group = a.H / a.Hk;
+  a.rows = a.group * a.S;
+  a.row_chunks = (a.rows + MAXR - 1) / MAXR;
+  a.max_chunks = split_max_chunks(a.max_len);
+  a.part_o = static_cast<float*>(workspace);
+  a.part_ml = a.max_chunks == 1
+                  ? nullptr
+                  : reinterpret_cast<float2*>(a.part_o + static_cast<int64_t>(a.B) * a.H * a.S *
+                                                             a.max_chunks * a.D);
+  if (a.D == 32) return launch_d<32>(a, q_dtype, kv_dtype, stream);
+  if (a.D == 64) return launch_d<64>(a, q_dtype, kv_dtype, stream);
+  return launch_d<128>(a, q_dtype, kv_dtype, stream);
+}
+
+}  // namespace cfa

@@ -73,8 +73,15 @@ enum cfa_status {
   CFA_ERR_WORKSPACE = 6,  /* workspace smaller than cfa_bwd_workspace_bytes or misaligned */
   CFA_ERR_LAUNCH = 7,     /* the CUDA launch failed */
   CFA_ERR_TIMEOUT = 8,    /* a bounded device-side wait of a kernel expired */
-  CFA_ERR_CUDA = 9        /* another CUDA runtime error (device query, copy, sync) */
+  CFA_ERR_CUDA = 9,       /* another CUDA runtime error (device query, copy, sync) */
+  CFA_ERR_PAGE = 10,      /* a kernel met a page id outside the cache, or a length past its table */
+  CFA_ERR_TYPE = 11,      /* an element type, or pair of types, that the operator does not take */
+  CFA_ERR_HEADS = 12,     /* the query heads are no multiple of the key heads */
+  CFA_ERR_ROTARY = 13     /* the rotary dimension is odd or exceeds the head dim */
 };
+
+/* Element types of the operators that take more than fp32. */
+enum cfa_dtype { CFA_F32 = 0, CFA_F16 = 1, CFA_BF16 = 2 };
 
 /* Forward: O = softmax(q k^T * scale [+ causal mask]) v and L = rowwise log-sum-exp.
  * q, k, v: [batch, heads, seq, 64] through (batch, head, seq) strides `*_strides[3]`.
@@ -271,11 +278,113 @@ int cfa_matmul_f32(const float* a, int64_t a_row_stride, int64_t a_col_stride,
  * since the last call expired (its output is then invalid), else CFA_OK; clears the flag. */
 int cfa_matmul_status(void* stream);
 
+/* ------------------------------------------------------------------------------------------------
+ * Operators beside the fused attention (no counterpart in the reference): attention to another
+ * sequence, rotary positions, a paged key-value cache and its attention. The conventions above hold:
+ * device pointers, strides in elements with the head dim contiguous, asynchronous on `stream`, no
+ * allocation, results bit-identical across reruns and independent of how the batch is split. */
+
+/* Cross attention, fp32: O = softmax(q k^T * scale) v, q [batch, heads, seq, head_dim] over k, v
+ * [batch, key_heads, key_seq, head_dim], the (batch, head, seq) strides as for cfa_fwd_f32 (16-byte
+ * rows); head_dim 32, 64 or 128; heads a multiple of key_heads (query head h reads key head
+ * h / (heads / key_heads)). key_lengths: [batch] int32 on the device, the keys of each batch element
+ * (held within 0 .. key_seq), or NULL: all; what lies behind them is never read into a result. A
+ * row without a key: O = 0, L = -inf, no gradient. o: [batch, seq, heads, head_dim] dense; lse
+ * [batch, heads, seq] dense. Tensor-core kernels at head dims 32 and 64, CUDA-core ones at 128. */
+int cfa_cross_fwd_f32(const float* q, const int64_t q_strides[3],
+                      const float* k, const int64_t k_strides[3],
+                      const float* v, const int64_t v_strides[3],
+                      const int32_t* key_lengths, float* o, float* lse,
+                      int64_t batch, int64_t heads, int64_t key_heads, int64_t seq,
+                      int64_t key_seq, int64_t head_dim, float scale, void* stream);
+
+/* Its backward, from the forward's o and lse: dq [batch, seq, heads, head_dim] and dkv [batch,
+ * key_seq, 2, key_heads, head_dim] (dK, dV interleaved), dense, written whole (rows past a key
+ * length: zeros). Scratch (256-byte aligned, no initialisation) of the size the query gives;
+ * cfa_bwd_status reads its error flag. */
+size_t cfa_cross_bwd_workspace_bytes(int64_t batch, int64_t heads, int64_t key_heads, int64_t seq,
+                                     int64_t key_seq, int64_t head_dim);
+int cfa_cross_bwd_f32(const float* q, const int64_t q_strides[3],
+                      const float* k, const int64_t k_strides[3],
+                      const float* v, const int64_t v_strides[3],
+                      const int32_t* key_lengths, const float* o, const float* lse,
+                      const float* d_o, const int64_t do_strides[3], float* dq, float* dkv,
+                      void* workspace, size_t workspace_bytes,
+                      int64_t batch, int64_t heads, int64_t key_heads, int64_t seq,
+                      int64_t key_seq, int64_t head_dim, float scale, void* stream);
+
+/* The forward alone for few query rows a key head (single tokens): the same contract without the
+ * lse, split over the keys. Any seq is right; past 8 rows a key head (seq * heads / key_heads) the
+ * keys are read once for every 8. */
+size_t cfa_cross_few_workspace_bytes(int64_t batch, int64_t heads, int64_t seq, int64_t key_seq,
+                                     int64_t head_dim);
+int cfa_cross_few_f32(const float* q, const int64_t q_strides[3],
+                      const float* k, const int64_t k_strides[3],
+                      const float* v, const int64_t v_strides[3],
+                      const int32_t* key_lengths, float* o, void* workspace, size_t workspace_bytes,
+                      int64_t batch, int64_t heads, int64_t key_heads, int64_t seq,
+                      int64_t key_seq, int64_t head_dim, float scale, void* stream);
+
+/* Rotary positions: y = x with the first rotary_dim dims of each of the first rotated_heads heads
+ * turned by position * freqs[j] (radians; 64 bits on the device, rotary_dim / 2 of them) and scaled
+ * by amplitude; the pairs are (j, j + rotary_dim / 2), or with interleaved (2j, 2j + 1). The other
+ * dims and heads are copied. inverse: the transposed rotation (the backward). x, y [batch, heads,
+ * seq, head_dim] of `dtype` through (batch, head, seq) strides, any alignment (16-byte rows are
+ * fastest), y apart from x or x itself. positions: int32 or int64 (position_bytes) on the device
+ * through (batch, seq) strides, or NULL: first_position + index. head_dim <= 1024. */
+int cfa_rotary(const void* x, const int64_t x_strides[3], void* y, const int64_t y_strides[3],
+               int dtype, const void* positions, int position_bytes,
+               const int64_t position_strides[2], int64_t first_position, const double* freqs,
+               float amplitude, int64_t batch, int64_t heads, int64_t rotated_heads, int64_t seq,
+               int64_t head_dim, int64_t rotary_dim, int interleaved, int inverse, void* stream);
+
+/* A paged cache holds keys (and values) of key_heads heads in `pages` pages of page_size rows; its
+ * (page, row, head) strides describe any order of them. Row r of sequence b is row r % page_size of
+ * page page_table[b table_stride + r / page_size] (int32, table_width entries a sequence).
+ *
+ * cfa_paged_append writes the seq new tokens' k and v [batch, key_heads, seq, head_dim] (in a padded
+ * batch the first new_lengths[b] of them; NULL: all) behind what is there: lengths[b] counts the
+ * sequence's keys WITH the new ones, so token i of n sits at lengths[b] - n + i, and it is rotated by
+ * that position (rotary_dim 0: not at all). q, if given, is rotated into q_out (rows that are no
+ * token: zeros). `dtype`: q, k, v; the cache's type is the same or, for fp32 inputs, any. A token
+ * without a page (an id outside 0 .. pages - 1, past the table, a negative position) is not written;
+ * a bad page id is reported through cfa_error_sink (CFA_ERR_PAGE). Two tokens of a call must not
+ * share a slot. */
+int cfa_paged_append(const void* q, const int64_t q_strides[3], void* q_out,
+                     const int64_t q_out_strides[3], const void* k, const int64_t k_strides[3],
+                     const void* v, const int64_t v_strides[3], int dtype, void* k_cache,
+                     const int64_t k_cache_strides[3], void* v_cache,
+                     const int64_t v_cache_strides[3], int cache_dtype, int64_t pages,
+                     int64_t page_size, const int32_t* page_table, int64_t table_stride,
+                     int64_t table_width, const int32_t* lengths, const int32_t* new_lengths,
+                     const double* freqs, float amplitude, int64_t batch, int64_t heads,
+                     int64_t key_heads, int64_t seq, int64_t head_dim, int64_t rotary_dim,
+                     int interleaved, void* stream);
+
+/* Attention of the newest seq tokens (one, or a few; new_lengths as above) over a paged cache: query
+ * i of n sees the sequence's first lengths[b] - n + i + 1 keys. q [batch, heads, seq, head_dim] of
+ * `dtype`, 16-byte rows; o [batch, seq, heads, head_dim] dense, of `dtype`; rows that see nothing or
+ * are no token: zeros. head_dim 32, 64 or 128; the cache's rows 16-byte aligned; types and heads as
+ * above. Sums and softmax statistics are fp32. Keys on a bad page are left out and reported
+ * (CFA_ERR_PAGE), and so is a length past the table. Workspace (256-byte aligned, no initialisation)
+ * for max_keys = table_width * page_size. */
+size_t cfa_paged_attention_workspace_bytes(int64_t batch, int64_t heads, int64_t seq,
+                                           int64_t max_keys, int64_t head_dim);
+int cfa_paged_attention(const void* q, const int64_t q_strides[3], int dtype, const void* k_cache,
+                        const int64_t k_cache_strides[3], const void* v_cache,
+                        const int64_t v_cache_strides[3], int cache_dtype, int64_t pages,
+                        int64_t page_size, const int32_t* page_table, int64_t table_stride,
+                        int64_t table_width, const int32_t* lengths, const int32_t* new_lengths,
+                        void* o, void* workspace, size_t workspace_bytes, int64_t batch,
+                        int64_t heads, int64_t key_heads, int64_t seq, int64_t head_dim,
+                        float scale, void* stream);
+
 /* A static description of a status code. */
 const char* cfa_strerror(int status);
 
 /* ABI version: (major << 16) | minor (2.0: one kernel pair per entry point, the error sink;
- * 2.1: the projection GEMM; 2.2: head dim 32 on the tensor cores, the generic CUDA-core pair). */
+ * 2.1: the projection GEMM; 2.2: head dim 32 on the tensor cores, the generic CUDA-core pair;
+ * 2.3: cross attention, rotary positions, the paged cache). */
 int cfa_abi_version(void);
 
 #ifdef __cplusplus
