@@ -47,198 +47,14 @@
 //
 // Every mbarrier wait is bounded; an expired wait sets the workspace error flag
 // (cfa_bwd_status reads it) and the block writes nothing.
-#include <cuda_bf16.h>
-
-#include "cfa_common.cuh"
-#include "cfa_internal.h"
-#include "cfa_split.cuh"
-#include "cfa_tc.cuh"
+#include "bwd_tc.cuh"
 
 namespace cfa {
-using tc::kmaj_off;
-using tc::split16;
-using tc::split8;
-using tc::store_parts;
-using tc::tmem_ld8;
-using tc::tmem_st8;
 namespace {
 
-constexpr int KB = 128;   // keys per block: MMA M of S^T, dP^T, dV, dK
-constexpr int QT = 64;    // queries per tile: MMA N of S^T, dP^T; M of dQ
-constexpr int NT = 512;   // compute threads (16 warps)
-constexpr int NB = NT + 32;  // and the MMA warp
-constexpr int PART_K = KB * 64 * 2;  // one bf16 part of a [128][64] operand
-constexpr int PART_Q = QT * 64 * 2;  // one bf16 part of a [64][64] operand
-constexpr int OFF_K = 0;                      // K parts [128 keys][64 d]
-constexpr int OFF_Q = OFF_K + 3 * PART_K;     // Q parts [64 q][64 d], two tiles
-constexpr int OFF_DO = OFF_Q + 6 * PART_Q;    // dO parts [64 q][64 d], two tiles
-constexpr int OFF_DS = OFF_DO + 6 * PART_Q;   // dS^T parts [128 keys][64 q] (first: K staged)
-constexpr int OFF_ST = OFF_DS + 3 * PART_K;   // staging: the next tile's Q, dO (fp32)
-constexpr int OFF_LD = OFF_ST + 2 * QT * 64 * 4;  // L, D of two tiles: float [2][2][64]
-constexpr int OFF_BAR = OFF_LD + 2 * 2 * QT * 4;  // eight mbarriers, the TMEM base, four ints
-constexpr int SMEM = OFF_BAR + 96;
-constexpr int SMEM_ALLOC = SMEM + 1024;
-static_assert(SMEM_ALLOC <= 232448, "shared memory per block");
-// TMEM columns (lane = key row). V's parts, the A operand of dP^T: part i, K-step ks (16 dims) in
-// the 8 columns T_V + 32 i + 8 ks. S^T, dP^T of the current tile; P^T's parts (the A operand of
-// dV: pt_col) over the S^T columns each thread has read and in T_X; dV, dK; dQ's two 64-key
-// windows (M = 64).
-constexpr uint32_t T_V = 0, T_S = 96, T_DP = 160, T_DV = 224, T_DK = 288, T_DQ0 = 352,
-                   T_DQ1 = 416, T_X = 480;
-constexpr uint32_t TMEM_COLS = 512;
-
-// A split tail's window of one query tile (dV, dK sums of the tile as TMEM holds them, before the
-// fold): WIN floats as float4 items [which: dV, dK][c4][column group][key row], so a warp's 32
-// rows of one item are 512 contiguous bytes (coalesced stores, conflict-free shared-memory reads).
-template <int HD>
-struct TailWindow {
-  static constexpr int WIN = 2 * KB * HD;
-  static constexpr int CG = HD / 16;  // column groups of 16 floats
-  __host__ __device__ static constexpr int item(int which, int c4, int cg, int row) {
-    return ((which * 4 + c4) * CG + cg) * KB + row;
-  }
-};
-
-// P^T part i of K-step ks (queries 16 ks .. 16 ks + 15: the columns of group ks): parts 0, 1 over
-// that group's S^T columns, part 2 in T_X + 8 ks -- dP^T stays whole until dS^T is formed from
-// it, while dV already runs.
-__host__ __device__ constexpr uint32_t pt_col(int i, int ks) {
-  return i < 2 ? T_S + 16 * ks + 8 * i : T_X + 8 * ks;
-}
-static_assert(T_X + 32 == TMEM_COLS, "TMEM budget");
-
-// Row items (row r, elements 8 kc .. 8 kc + 7): item c takes row 8 (c / 64) + c % 8 and chunk
-// (c / 8) % 8 (a quarter-warp writes 8 rows of one chunk: 8 bank groups). Every thread copies
-// (cp.async) the fp32 chunks it splits into slots of its own: slot j of thread t at
-// (j * NT + t) * 16 bytes.
-__device__ __forceinline__ void row_item(int c, int& r, int& kc) {
-  r = 8 * (c >> 6) + (c & 7);
-  kc = (c >> 3) & 7;
-}
-
-// (Head dim 32: the row's chunks past the head dim are zero-filled, so the parts are those of a
-// 64-wide row whose upper half is zero.)
-template <int HD>
-__device__ __forceinline__ void stage_row_item(unsigned char* st, int slot, int c, const float* src,
-                                               int64_t stride, int r0, int seq) {
-  int r, kc;
-  row_item(c, r, kc);
-  const bool ok = r0 + r < seq && 8 * kc < HD;
-  const float* g = src + static_cast<int64_t>(ok ? r0 + r : 0) * stride + 8 * kc;
-  cp_async16(st + 16 * ((2 * slot) * NT + threadIdx.x), g, ok ? 16 : 0);
-  cp_async16(st + 16 * ((2 * slot + 1) * NT + threadIdx.x), g + 4, ok ? 16 : 0);
-}
-
-__device__ __forceinline__ void split_row_item(unsigned char* parts, int part_bytes,
-                                               const unsigned char* st, int slot, int c) {
-  int r, kc;
-  row_item(c, r, kc);
-  const float4 u = *reinterpret_cast<const float4*>(st + 16 * ((2 * slot) * NT + threadIdx.x));
-  const float4 v = *reinterpret_cast<const float4*>(st + 16 * ((2 * slot + 1) * NT + threadIdx.x));
-  const float x[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
-  store_parts(parts, part_bytes, kmaj_off(r, kc), x);
-}
-
-// Row item c of a row-major staging area with rows of 68 floats (rows >= valid and columns >= HD
-// read as zeros) into the K-major parts at part_bytes apart.
-template <int HD>
-__device__ __forceinline__ void split_staged_row(unsigned char* parts, int part_bytes,
-                                                 const float* rows, int c, int valid) {
-  int r, kc;
-  row_item(c, r, kc);
-  float x[8];
-  if (r < valid && 8 * kc < HD) {
-    const float4 u = reinterpret_cast<const float4*>(rows + r * 68 + 8 * kc)[0];
-    const float4 v = reinterpret_cast<const float4*>(rows + r * 68 + 8 * kc)[1];
-    x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w, x[4] = v.x, x[5] = v.y, x[6] = v.z, x[7] = v.w;
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = 0.0f;
-  }
-  store_parts(parts, part_bytes, kmaj_off(r, kc), x);
-}
-
-// One window: six split products over STEPS K-steps into the fresh accumulator `d`; descriptors
-// advance by A_STEP / B_STEP bytes per step and by A_PART / B_PART bytes per part. Part pairs
-// (P0(p), P1(p)) -- the small (0, 1), (1, 0), (0, 2), (1, 1), (2, 0) of every step, then the
-// (0, 0) of every step -- or, SWAP, (P1(p), P0(p)): the order in which the forward forms its
-// products when A and B trade places. Called by the whole MMA warp (tc::mma_bf16_warp).
-__host__ __device__ constexpr int P0(int p) { return p == 2 || p == 4 ? 1 : (p == 5 ? 2 : 0); }
-__host__ __device__ constexpr int P1(int p) { return p == 1 || p == 4 ? 1 : (p == 3 ? 2 : 0); }
-template <int STEPS, int A_PART, int B_PART, int A_STEP, int B_STEP, bool SWAP>
-__device__ __forceinline__ void issue6(uint32_t d, tc::Desc ad, tc::Desc bd, uint32_t idesc) {
-  const uint32_t alo = tc::opaque(ad.lo), blo = tc::opaque(bd.lo);
-#pragma unroll
-  for (int ks = 0; ks < STEPS; ++ks)
-#pragma unroll
-    for (int p = 1; p < 6; ++p) {
-      const int pa = SWAP ? P1(p) : P0(p), pb = SWAP ? P0(p) : P1(p);
-      tc::mma_bf16_warp(d, alo + ((pa * A_PART + A_STEP * ks) >> 4), ad.hi,
-                        blo + ((pb * B_PART + B_STEP * ks) >> 4), bd.hi, idesc, ks > 0 || p > 1);
-    }
-#pragma unroll
-  for (int ks = 0; ks < STEPS; ++ks)
-    tc::mma_bf16_warp(d, alo + ((A_STEP * ks) >> 4), ad.hi, blo + ((B_STEP * ks) >> 4), bd.hi,
-                      idesc, 1);
-}
-
-// The same window with the A operand in TMEM: part i of K-step ks at column acol(i, ks).
-template <int B_PART, int B_STEP, typename ACol, int STEPS = 4>
-__device__ __forceinline__ void issue6_tmem_a(uint32_t d, ACol acol, tc::Desc bd, uint32_t idesc) {
-  const uint32_t blo = tc::opaque(bd.lo);
-#pragma unroll
-  for (int ks = 0; ks < STEPS; ++ks)
-#pragma unroll
-    for (int p = 1; p < 6; ++p)
-      tc::mma_bf16_tmem_a_warp(d, acol(P0(p), ks), blo + ((P1(p) * B_PART + B_STEP * ks) >> 4),
-                               bd.hi, idesc, ks > 0 || p > 1);
-#pragma unroll
-  for (int ks = 0; ks < STEPS; ++ks)
-    tc::mma_bf16_tmem_a_warp(d, acol(0, ks), blo + ((B_STEP * ks) >> 4), bd.hi, idesc, 1);
-}
-
-constexpr float LOG2E = 1.4426950408889634f;  // log2(e), rounded to fp32
-
-// Packed fp32 pairs (tc::pack2 / unpack2), one instruction a pair.
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-__device__ __forceinline__ uint64_t fma2v(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-
-// Eight floats to global memory in one 32-byte store (address 32-byte aligned), cached in L2 only.
-__device__ __forceinline__ void st_cg_v8(float* p, const float (&v)[8]) {
-  asm volatile("st.global.cg.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "f"(v[0]),
-               "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
-               : "memory");
-}
-
-// atomicAdd with acquire-release semantics at GPU scope.
-__device__ __forceinline__ int atom_add_acq_rel(int* p, int v) {
-  int old;
-  asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], %2;" : "=r"(old) : "l"(p), "r"(v) : "memory");
-  return old;
-}
-
-// Named barrier 1: the 16 compute warps (the MMA warp never takes part).
-__device__ __forceinline__ void bar_sync(int id, int count) {
-  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(count) : "memory");
-}
-
-// CROSS (cross attention): the keys have a length of their own (a.Sk rows, the first
-// cross_keys(a, b) attended), and a key block belongs to a key head: it walks the query tiles of
-// every query head of the group, one head after the other, so dV and dK of a shared head are summed
-// in registers in that order. Key blocks past a batch element's length write zeros and take no part.
-// dQ and dK, dV go to buffers of their own (a.dq, a.dkv).
-template <bool CAUSAL, int HD, bool CROSS = false>
+template <bool CAUSAL, int HD>
 __global__ void __launch_bounds__(NB, 1) bwd_tc_kernel(const BwdArgs a) {
   static_assert(HD == 64 || HD == 32, "head dims of the tensor-core backward");
-  static_assert(!(CAUSAL && CROSS), "cross attention has no causal mask");
   constexpr int KSD = HD / 16;  // K-steps of the products that reduce over the head dim
   constexpr int WIN = TailWindow<HD>::WIN;
   constexpr auto win4 = TailWindow<HD>::item;
@@ -268,10 +84,8 @@ __global__ void __launch_bounds__(NB, 1) bwd_tc_kernel(const BwdArgs a) {
   const int row = 32 * (w & 3) + lane;  // key row: TMEM lane (compute warps)
   const int cg = (w >> 2) & 3;          // column group: 16 queries (S, dP) or dims (dV, dK, dQ)
   const int S = a.S;
-  const int HU = CROSS ? a.Hk : a.H;  // heads that own key blocks
-  const int BH = a.B * HU;
-  int nkb = a.n_kblocks;  // key blocks of this (batch, head) that take part
-  if constexpr (CROSS) griddep_wait();  // the lengths may come from the previous kernels
+  const int nkb = a.n_kblocks;
+  const int BH = a.B * a.H;
   // The work item. With the dQ partials (no-wait path): the block index, (b, h)-major, so a
   // (b, h)'s key blocks run side by side and its last one finishes early. With the turn chain: a
   // ticket drawn after the prep kernel's wait, key-block-major -- a block waits only on key block
@@ -307,61 +121,23 @@ __global__ void __launch_bounds__(NB, 1) bwd_tc_kernel(const BwdArgs a) {
     part = g + 1 < nparts ? g + 1 : 0;
     ticket = a.tail_base + tail_r;
   }
-  const int kb = chain ? ticket / BH : ticket % a.n_kblocks;
-  const int bh = chain ? ticket % BH : ticket / a.n_kblocks;
-  const int b = bh / HU, h = bh % HU;
+  const int kb = chain ? ticket / BH : ticket % nkb;
+  const int bh = chain ? ticket % BH : ticket / nkb;
+  const int b = bh / a.H, h = bh % a.H;
   const int k0 = kb * KB;
-  const int group = CROSS ? a.H / a.Hk : 1;  // query heads of the key block
-  const int h0 = h * group, nqt = (S + QT - 1) / QT;
-  int SK = S;  // keys
-  if constexpr (CROSS) {
-    SK = cross_keys(a, b);
-    nkb = (SK + KB - 1) / KB;
-    if (kb >= nkb) {  // no key of this block is attended: zeros, and no part in dQ's sums
-      griddep_launch_dependents();
-      if (part != 0) return;
-      constexpr int C4 = HD / 4;
-      const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
-      const int rows = min(KB, a.Sk - k0);
-      for (int f = tid; f < 2 * rows * C4; f += NB) {
-        const int which = f / (rows * C4), r = (f / C4) % rows;
-        reinterpret_cast<float4*>(
-            a.dkv + (((static_cast<int64_t>(b) * a.Sk + k0 + r) * 2 + which) * a.Hk + h) * HD)[f % C4] = zero;
-      }
-      if (kb == 0)  // no key at all: dQ = 0
-        for (int64_t f = tid; f < static_cast<int64_t>(S) * group * C4; f += NB)
-          reinterpret_cast<float4*>(a.dq + ((static_cast<int64_t>(b) * S + f / (group * C4)) * a.H + h0) *
-                                               HD)[f % (group * C4)] = zero;
-      return;
-    }
-  }
+  const float* qp = a.q + b * a.q_sb + h * a.q_sh;
   const float* kp = a.k + b * a.k_sb + h * a.k_sh;
   const float* vp = a.v + b * a.v_sb + h * a.v_sh;
-  const float* qp = a.q + b * a.q_sb + h * a.q_sh;
   const float* gp = a.d_o + b * a.do_sb + h * a.do_sh;
   const float* lp = a.lse + static_cast<int64_t>(bh) * S;
   const float* dp = a.dsum + static_cast<int64_t>(bh) * S;
-  // The query head and first query of the block's tile t, and that head's operands.
-  auto tile_head = [&](int t) { return CROSS ? h0 + t / nqt : h; };
-  auto tile_q0 = [&](int t) { return (CROSS ? t % nqt : t) * QT; };
-  auto q_rows = [&](int t) { return CROSS ? a.q + b * a.q_sb + tile_head(t) * a.q_sh : qp; };
-  auto g_rows = [&](int t) { return CROSS ? a.d_o + b * a.do_sb + tile_head(t) * a.do_sh : gp; };
-  auto query_bh = [&](int t) {
-    return CROSS ? static_cast<int64_t>(b) * a.H + tile_head(t) : static_cast<int64_t>(bh);
-  };
   const int t_first = CAUSAL ? k0 / QT : 0;  // queries before the block's first key see none
-  const int n_all = group * nqt - t_first;  // the key block's query tiles, >= 1 (k0 < SK)
+  const int n_all = (S + QT - 1) / QT - t_first;  // the key block's query tiles, >= 1 (k0 < S)
   const int n_lo = part * n_all / nparts, n_hi = (part + 1) * n_all / nparts;
   const int t_begin = t_first + n_lo;  // this block's first query tile
-  // Turn chain: counters per 64-query tile of a query head.
-  int* turn = a.turn + (CROSS ? (static_cast<int64_t>(b) * a.H + h0) * nqt
-                              : static_cast<int64_t>(bh) * a.n_qtiles);
-  // dqkv (CROSS: dq) floats per (b, s), and a query head's dQ rows.
-  const int64_t row_stride = (CROSS ? 1 : 3) * static_cast<int64_t>(a.H) * HD;
-  float* dq_base = (CROSS ? a.dq : a.dqkv) + static_cast<int64_t>(b) * S * row_stride + h * HD;
-  auto dq_rows = [&](int head) {
-    return CROSS ? a.dq + static_cast<int64_t>(b) * S * row_stride + head * HD : dq_base;
-  };
+  int* turn = a.turn + static_cast<int64_t>(bh) * a.n_qtiles;  // turn chain: per 64-query tile
+  const int64_t row_stride = 3 * static_cast<int64_t>(a.H) * HD;  // dqkv floats per (b, s)
+  float* dq_base = a.dqkv + static_cast<int64_t>(b) * S * row_stride + h * HD;
   const int N = n_hi - n_lo;  // this block's query tiles, >= 1 (a.tail_parts <= n_all)
   bool err0 = false;
 
@@ -375,7 +151,7 @@ __global__ void __launch_bounds__(NB, 1) bwd_tc_kernel(const BwdArgs a) {
     tc::mbar_init(bar_p, NT / 32);
     tc::mbar_init(bar_dv, 1);
     tc::fence_mbar_init();
-    tc::mbar_arrive_expect_tx(bar_ld, 4u * HD * (2 * min(KB, SK - k0) + 2 * min(QT, S - tile_q0(t_begin))));
+    tc::mbar_arrive_expect_tx(bar_ld, 4u * HD * (2 * min(KB, S - k0) + 2 * min(QT, S - t_begin * QT)));
   }
   griddep_launch_dependents();
 
@@ -383,17 +159,16 @@ __global__ void __launch_bounds__(NB, 1) bwd_tc_kernel(const BwdArgs a) {
   // L / D buffer n % 2 (threads 0-127).
   auto stage_ld = [&](int n) {
     if (tid < 2 * QT) {
-      const int r = tid & 63, i = tile_q0(t_begin + n) + r;
+      const int r = tid & 63, i = (t_begin + n) * QT + r;
       const bool ok = i < S;
-      const float* src = CROSS ? (tid < QT ? a.lse : a.dsum) + query_bh(t_begin + n) * S
-                               : (tid < QT ? lp : dp);
-      cp_async4(ld + (n & 1) * 128 + (tid < QT ? 0 : QT) + r, src + (ok ? i : 0), ok ? 4 : 0);
+      cp_async4(ld + (n & 1) * 128 + (tid < QT ? 0 : QT) + r, (tid < QT ? lp : dp) + (ok ? i : 0),
+                ok ? 4 : 0);
     }
   };
   auto stage_tile = [&](int n) {
-    const int q0 = tile_q0(t_begin + n);
-    stage_row_item<HD>(st, 0, tid, q_rows(t_begin + n), a.q_ss, q0, S);
-    stage_row_item<HD>(st, 1, tid, g_rows(t_begin + n), a.do_ss, q0, S);
+    const int q0 = (t_begin + n) * QT;
+    stage_row_item<HD>(st, 0, tid, qp, a.q_ss, q0, S);
+    stage_row_item<HD>(st, 1, tid, gp, a.do_ss, q0, S);
     stage_ld(n);
   };
   // The block one wave later (work item + a.wave_ctas) starts by reading its key block's K, V rows
@@ -401,13 +176,12 @@ __global__ void __launch_bounds__(NB, 1) bwd_tc_kernel(const BwdArgs a) {
   // this wave computes and HBM is otherwise idle (one 256-byte row per thread).
   auto prefetch_next_wave = [&]() {
     const int nb = ticket + a.wave_ctas;
-    const int n_kb = a.n_kblocks;
-    if (a.wave_ctas <= 0 || nparts > 1 || nb >= n_kb * BH || tid >= 2 * KB + 2 * QT) return;
-    const int nkb2 = chain ? nb / BH : nb % n_kb, nbh = chain ? nb % BH : nb / n_kb;
-    const int nb_b = nbh / HU, nb_h = tid < 2 * KB ? nbh % HU : nbh % HU * group;
+    if (a.wave_ctas <= 0 || nparts > 1 || nb >= nkb * BH || tid >= 2 * KB + 2 * QT) return;
+    const int nkb2 = chain ? nb / BH : nb % nkb, nbh = chain ? nb % BH : nb / nkb;
+    const int nb_b = nbh / a.H, nb_h = nbh % a.H;
     const int r = tid < 2 * KB ? (tid & (KB - 1)) : (tid & (QT - 1));
     const int row = tid < 2 * KB ? nkb2 * KB + r : (CAUSAL ? nkb2 * KB : 0) + r;
-    if (row >= (CROSS && tid < 2 * KB ? a.Sk : S)) return;
+    if (row >= S) return;
     const float* src;
     if (tid < KB) src = a.k + nb_b * a.k_sb + nb_h * a.k_sh + static_cast<int64_t>(row) * a.k_ss;
     else if (tid < 2 * KB) src = a.v + nb_b * a.v_sb + nb_h * a.v_sh + static_cast<int64_t>(row) * a.v_ss;
@@ -429,11 +203,11 @@ __global__ void __launch_bounds__(NB, 1) bwd_tc_kernel(const BwdArgs a) {
   constexpr int LDP = 68;
   float* k_rows = reinterpret_cast<float*>(dSp);
   float* v_rows = k_rows + KB * LDP;
-  float* q_st = reinterpret_cast<float*>(Qp + 3 * PART_Q);
-  float* o_st = reinterpret_cast<float*>(dOp + 3 * PART_Q);
+  float* q_rows = reinterpret_cast<float*>(Qp + 3 * PART_Q);
+  float* o_rows = reinterpret_cast<float*>(dOp + 3 * PART_Q);
   static_assert(2 * KB * LDP * 4 <= 3 * PART_K + 2 * QT * 64 * 4 && QT * LDP * 4 <= 3 * PART_Q,
                 "prologue staging");
-  const int nk = min(KB, SK - k0), nq = min(QT, S - tile_q0(t_begin));
+  const int nk = min(KB, S - k0), nq = min(QT, S - t_begin * QT);
   __syncthreads();  // the mbarriers' initialisation
   if (mma_warp) {  // TMEM, by the warp that is idle while the rows travel (it also frees it)
     tc::tmem_alloc(tbase_p, TMEM_COLS);
@@ -449,11 +223,9 @@ __global__ void __launch_bounds__(NB, 1) bwd_tc_kernel(const BwdArgs a) {
         if (r < nk) tc::bulk_load(v_rows + r * LDP, vp + static_cast<int64_t>(k0 + r) * a.v_ss, 4 * HD, bar_ld);
       } else if (tid < 2 * KB + QT) {
         if (r < nq)
-          tc::bulk_load(q_st + r * LDP, q_rows(t_begin) + static_cast<int64_t>(tile_q0(t_begin) + r) * a.q_ss,
-                        4 * HD, bar_ld);
+          tc::bulk_load(q_rows + r * LDP, qp + static_cast<int64_t>(t_begin * QT + r) * a.q_ss, 4 * HD, bar_ld);
       } else if (r < nq) {
-        tc::bulk_load(o_st + r * LDP, g_rows(t_begin) + static_cast<int64_t>(tile_q0(t_begin) + r) * a.do_ss,
-                      4 * HD, bar_ld);
+        tc::bulk_load(o_rows + r * LDP, gp + static_cast<int64_t>(t_begin * QT + r) * a.do_ss, 4 * HD, bar_ld);
       }
     }
     griddep_wait();  // L, D, the cleared counters: the prep kernel's writes
@@ -463,8 +235,8 @@ __global__ void __launch_bounds__(NB, 1) bwd_tc_kernel(const BwdArgs a) {
     cp_async_wait_all();
     split_staged_row<HD>(Kp, PART_K, k_rows, tid, nk);
     split_staged_row<HD>(Kp, PART_K, k_rows, tid + NT, nk);
-    split_staged_row<HD>(Qp, PART_Q, q_st, tid, nq);
-    split_staged_row<HD>(dOp, PART_Q, o_st, tid, nq);
+    split_staged_row<HD>(Qp, PART_Q, q_rows, tid, nq);
+    split_staged_row<HD>(dOp, PART_Q, o_rows, tid, nq);
 #pragma unroll
     for (int c4 = 0; c4 < 4; ++c4) {
       const float4 u = row < nk && 16 * cg < HD
@@ -565,14 +337,14 @@ __global__ void __launch_bounds__(NB, 1) bwd_tc_kernel(const BwdArgs a) {
     if (N > 1) stage_tile(1);  // while the MMA warp issues T1(0)
     cp_async_commit();
     for (int n = 0; n < N; ++n) {
-      const int q0 = tile_q0(t_begin + n);
+      const int q0 = (t_begin + n) * QT;
       // (C1a) P^T for this thread's 16 queries, its parts into TMEM (pt_col) for dV -- while the
       // tensor core computes dP^T.
       err |= !tc::mbar_wait(bar_s, n & 1, WAIT_TIMEOUT_NS);
       tc::fence_after_sync();
       const float* Lt = ld + (n & 1) * 128;
       const float* Dt = Lt + QT;
-      const bool edge = (q0 + QT > S) || (k0 + KB > SK) || (CAUSAL && k0 + KB - 1 > q0);
+      const bool edge = (q0 + QT > S) || (k0 + KB > S) || (CAUSAL && k0 + KB - 1 > q0);
       float pr[16];
       tc::tmem_ld16(tbase + lane_sel + T_S + 16 * cg, pr);
       tc::tmem_wait_ld();
@@ -591,8 +363,8 @@ __global__ void __launch_bounds__(NB, 1) bwd_tc_kernel(const BwdArgs a) {
           tc::unpack2(mul2(fma2v(tc::pack2(pr[u], pr[u + 1]), nsc2, l2), nl2e2), x0, x1);
           float p0 = ex2(x0), p1 = ex2(x1);
           if (edge) {
-            if (!(q0 + ql < S && key < SK && !(CAUSAL && key > q0 + ql))) p0 = 0.0f;
-            if (!(q0 + ql + 1 < S && key < SK && !(CAUSAL && key > q0 + ql + 1))) p1 = 0.0f;
+            if (!(q0 + ql < S && key < S && !(CAUSAL && key > q0 + ql))) p0 = 0.0f;
+            if (!(q0 + ql + 1 < S && key < S && !(CAUSAL && key > q0 + ql + 1))) p1 = 0.0f;
           }
           pr[u] = p0;
           pr[u + 1] = p1;
@@ -681,8 +453,7 @@ __global__ void __launch_bounds__(NB, 1) bwd_tc_kernel(const BwdArgs a) {
         if (lane < 16 && qi < S && 16 * cg < HD && !err) {
           // Two 32-byte stores: whole L2 sectors (16-byte stores 256 bytes apart across the warp
           // each wrote half of 16 sectors).
-          float* dst = a.dq_part +
-                       ((query_bh(t_begin + n) * (CROSS ? a.n_kblocks : nkb) + kb) * S + qi) * HD + 16 * cg;
+          float* dst = a.dq_part + ((static_cast<int64_t>(bh) * nkb + kb) * S + qi) * HD + 16 * cg;
 #pragma unroll
           for (int c8 = 0; c8 < 2; ++c8) {
             float v[8];
@@ -710,7 +481,7 @@ __global__ void __launch_bounds__(NB, 1) bwd_tc_kernel(const BwdArgs a) {
           go = s_int[2 + (n & 1)] != 0;
         }
         if (go && lane < 16 && qi < S && 16 * cg < HD) {
-          float4* dst = reinterpret_cast<float4*>(dq_rows(tile_head(t)) + qi * row_stride + 16 * cg);
+          float4* dst = reinterpret_cast<float4*>(dq_base + qi * row_stride + 16 * cg);
 #pragma unroll
           for (int c4 = 0; c4 < 4; ++c4) {
             float4 v = make_float4(xb[4 * c4] + xs[4 * c4], xb[4 * c4 + 1] + xs[4 * c4 + 1],
@@ -822,13 +593,12 @@ __global__ void __launch_bounds__(NB, 1) bwd_tc_kernel(const BwdArgs a) {
     if (tid == 0 && !chain) count = atom_add_acq_rel(a.turn + bh, 1);
     // dV, dK rows out of shared memory: every 16 threads store one whole row.
     {
+      const int64_t row_stride = 3 * static_cast<int64_t>(a.H) * HD;
       for (int f = tid; f < 2 * KB * C4; f += NB) {
         const int which = f / (KB * C4), r = (f / C4) % KB, c4 = f % C4;
-        if (k0 + r < (CROSS ? a.Sk : S)) {  // (CROSS: rows past the length hold zeros)
-          float* dst = CROSS ? a.dkv + (static_cast<int64_t>(b) * a.Sk + k0 + r) * 2 * a.Hk * HD +
-                                   (1 - which) * a.Hk * HD + h * HD
-                             : a.dqkv + (static_cast<int64_t>(b) * S + k0 + r) * row_stride +
-                                   (2 - which) * a.H * HD + h * HD;
+        if (k0 + r < S) {
+          float* dst = a.dqkv + (static_cast<int64_t>(b) * S + k0 + r) * row_stride +
+                       (2 - which) * a.H * HD + h * HD;
           reinterpret_cast<float4*>(dst)[c4] =
               reinterpret_cast<const float4*>((which ? sk : sv) + r * LDS)[c4];
         }
@@ -837,37 +607,36 @@ __global__ void __launch_bounds__(NB, 1) bwd_tc_kernel(const BwdArgs a) {
     if (tid == 0) s_int[0] = count;
     __syncthreads();
     const int64_t part_bytes = static_cast<int64_t>(nkb) * S * HD * 4;
-    // (CROSS: head by head of the group, the partials of a head a.n_kblocks apart.)
-    for (int hq = h0; s_int[0] == nkb - 1 && hq < h0 + group; ++hq) {
-      const float* part = a.dq_part + (static_cast<int64_t>(b) * a.H + hq) * a.n_kblocks * S * HD;
-      float* dq_out = dq_rows(hq);
-      if (part_bytes <= OFF_DS) {
-        // The (b, h)'s partials, contiguous [nkb][S][64], as one bulk copy into shared memory (the
-        // part buffers, free since the last T2; the dS^T buffer holds dV, dK), then summed there.
-        const float* sp = reinterpret_cast<const float*>(sm);
-        if (CROSS && hq > h0) __syncthreads();  // the previous head's sums are read
-        if (tid == 0) {
-          tc::fence_async_global();  // the partials the count made visible, for the copy engine
-          tc::mbar_arrive_expect_tx(bar_ld, static_cast<uint32_t>(part_bytes));
-          tc::bulk_load(sm, part, static_cast<uint32_t>(part_bytes), bar_ld);
-        }
-        const bool ok = tc::mbar_wait(bar_ld, ld_phase & 1, WAIT_TIMEOUT_NS);
-        if (CROSS) ++ld_phase;
-        // DETERMINISM: dQ = (((p0 + p1) + p2) + ...) * scale, as below.
-        for (int idx = tid; idx < S * C4 && ok; idx += NB) {
-          const int i = idx / C4, c4 = idx % C4;
-          const int last = CAUSAL ? min(nkb - 1, i / KB) : nkb - 1;
-          float4 v = reinterpret_cast<const float4*>(sp + i * HD)[c4];
-          for (int j = 1; j <= last; ++j) {
-            const float4 q = reinterpret_cast<const float4*>(sp + (j * S + i) * HD)[c4];
-            v = make_float4(v.x + q.x, v.y + q.y, v.z + q.z, v.w + q.w);
-          }
-          reinterpret_cast<float4*>(dq_out + i * row_stride)[c4] =
-              make_float4(v.x * a.scale, v.y * a.scale, v.z * a.scale, v.w * a.scale);
-        }
-        if (!ok && tid == 0) flag_timeout(a.err, a.sink);
-        continue;
+    if (s_int[0] == nkb - 1 && part_bytes <= OFF_DS) {
+      // The (b, h)'s partials, contiguous [nkb][S][64], as one bulk copy into shared memory (the
+      // part buffers, free since the last T2; the dS^T buffer holds dV, dK), then summed there.
+      const float* part = a.dq_part + static_cast<int64_t>(bh) * nkb * S * HD;
+      const float* sp = reinterpret_cast<const float*>(sm);
+      if (tid == 0) {
+        tc::fence_async_global();  // the partials the count made visible, for the copy engine
+        tc::mbar_arrive_expect_tx(bar_ld, static_cast<uint32_t>(part_bytes));
+        tc::bulk_load(sm, part, static_cast<uint32_t>(part_bytes), bar_ld);
       }
+      const bool ok = tc::mbar_wait(bar_ld, ld_phase & 1, WAIT_TIMEOUT_NS);
+      const int64_t row_stride = 3 * static_cast<int64_t>(a.H) * HD;
+      float* dq_base = a.dqkv + static_cast<int64_t>(b) * S * row_stride + h * HD;
+      // DETERMINISM: dQ = (((p0 + p1) + p2) + ...) * scale, as below.
+      for (int idx = tid; idx < S * C4 && ok; idx += NB) {
+        const int i = idx / C4, c4 = idx % C4;
+        const int last = CAUSAL ? min(nkb - 1, i / KB) : nkb - 1;
+        float4 v = reinterpret_cast<const float4*>(sp + i * HD)[c4];
+        for (int j = 1; j <= last; ++j) {
+          const float4 q = reinterpret_cast<const float4*>(sp + (j * S + i) * HD)[c4];
+          v = make_float4(v.x + q.x, v.y + q.y, v.z + q.z, v.w + q.w);
+        }
+        reinterpret_cast<float4*>(dq_base + i * row_stride)[c4] =
+            make_float4(v.x * a.scale, v.y * a.scale, v.z * a.scale, v.w * a.scale);
+      }
+      if (!ok && tid == 0) flag_timeout(a.err, a.sink);
+    } else if (s_int[0] == nkb - 1) {
+      const float* part = a.dq_part + static_cast<int64_t>(bh) * nkb * S * HD;
+      const int64_t row_stride = 3 * static_cast<int64_t>(a.H) * HD;
+      float* dq_base = a.dqkv + static_cast<int64_t>(b) * S * row_stride + h * HD;
       // DETERMINISM: dQ = (((p0 + p1) + p2) + ...) * scale over the key blocks holding a key <=
       // the row (causal) or all of them. Eight float4 items per thread at a time, each key
       // block's loads for the eight issued together.
@@ -905,7 +674,7 @@ __global__ void __launch_bounds__(NB, 1) bwd_tc_kernel(const BwdArgs a) {
         for (int u = 0; u < U; ++u) {
           const int idx = base + u * NB;
           if (last[u] >= 0)
-            reinterpret_cast<float4*>(dq_out + (idx / C4) * row_stride)[idx % C4] =
+            reinterpret_cast<float4*>(dq_base + (idx / C4) * row_stride)[idx % C4] =
                 make_float4(v[u].x * a.scale, v[u].y * a.scale, v[u].z * a.scale,
                             v[u].w * a.scale);
         }
@@ -975,34 +744,6 @@ cudaError_t launch_bwd_tc(const BwdArgs& args, int head_dim, int causal, cudaStr
   }
   if (causal) return launch_pdl(bwd_tc_kernel<true, 64>, grid, dim3(NB), SMEM_ALLOC, stream, a);
   return launch_pdl(bwd_tc_kernel<false, 64>, grid, dim3(NB), SMEM_ALLOC, stream, a);
-}
-
-cudaError_t setup_cross_bwd_tc_attributes() {
-  const cudaError_t e = cudaFuncSetAttribute(bwd_tc_kernel<false, 64, true>,
-                                             cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_ALLOC);
-  return e != cudaSuccess ? e
-                          : cudaFuncSetAttribute(bwd_tc_kernel<false, 32, true>,
-                                                 cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_ALLOC);
-}
-
-// The caller has laid out the workspace (cross_bwd_workspace_layout): the split tail's windows and
-// flags, when it planned one, are in a.tail_win, a.tail_flag with tail_units, tail_parts set for
-// CROSS_SMS blocks a wave.
-cudaError_t launch_cross_bwd_tc(const BwdArgs& args, int head_dim, cudaStream_t stream) {
-  BwdArgs a = args;
-  a.n_kblocks = (a.Sk + KB - 1) / KB;
-  int dev = 0, sms = 0;
-  a.wave_ctas = cudaGetDevice(&dev) == cudaSuccess &&
-                        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess
-                    ? sms
-                    : 0;
-  const int64_t units = static_cast<int64_t>(a.n_kblocks) * a.B * a.Hk;
-  const int64_t blocks = a.tail_parts > 1 ? units + static_cast<int64_t>(a.tail_units) * (a.tail_parts - 1)
-                                          : units;
-  const dim3 grid(static_cast<unsigned>(blocks));
-  if (head_dim == 32)
-    return launch_pdl(bwd_tc_kernel<false, 32, true>, grid, dim3(NB), SMEM_ALLOC, stream, a);
-  return launch_pdl(bwd_tc_kernel<false, 64, true>, grid, dim3(NB), SMEM_ALLOC, stream, a);
 }
 
 }  // namespace cfa

@@ -215,7 +215,7 @@ __device__ __forceinline__ void flag_timeout(int* err, int* sink) {
   }
 }
 
-// The keys of batch element b that the CROSS kernels attend: key_lengths[b] held within 0 .. Sk.
+// The keys of batch element b that cross attention sees: key_lengths[b] held within 0 .. Sk.
 template <typename Args>
 __device__ __forceinline__ int cross_keys(const Args& a, int b) {
   return a.key_lengths ? min(max(a.key_lengths[b], 0), a.Sk) : a.Sk;

@@ -48,7 +48,7 @@ struct FwdArgs {
   int n_qtiles;
   int wave_ctas;  // tensor-core forward: blocks resident at once (one per SM); 0: none
   int* sink;      // host-visible error flag (cfa_error_sink) or nullptr
-  // Cross attention (the CROSS kernels): H / Hk query heads share a key head, k and v have Sk rows,
+  // Cross attention: H / Hk query heads share a key head, k and v have Sk rows,
   // of which batch element b attends the first key_lengths[b] (nullptr: all).
   int Hk, Sk;
   const int* key_lengths;
@@ -86,7 +86,7 @@ struct BwdArgs {
   float* tail_win;  // [tail_units][query tiles][2][128][D] window sums
   int* tail_flag;   // [tail_units][tail_parts] flags, then the tail's ticket counter (cleared by the
                     // prep kernel)
-  // Cross attention (the CROSS kernels): as in FwdArgs; dQ and dK, dV go to buffers of their own.
+  // Cross attention: as in FwdArgs; dQ and dK, dV go to buffers of their own.
   int Hk, Sk;
   const int* key_lengths;
   float* dq;   // [B, S, H, D]
@@ -155,8 +155,8 @@ cudaError_t launch_hd_fwd(const FwdArgs& a, int head_dim, int causal, cudaStream
 cudaError_t launch_hd_bwd_prep(const PrepArgs& a, int head_dim, cudaStream_t stream);
 cudaError_t launch_hd_bwd(const BwdArgs& a, int head_dim, int causal, cudaStream_t stream);
 
-// Cross attention: the same kernels with keys of another length (CROSS): head dims 64 and 32 on the
-// tensor-core pair, 128 on hd_ffma.cu. a.S is the query length, a.n_kblocks is set by the launcher.
+// Cross attention: keys of another length, shared key heads. Head dims 64 and 32 run on the
+// tensor cores (fwd_tc.cu CROSS, cross_bwd_tc.cu), 128 on cross_hd_ffma.cu. a.S is the query length, a.n_kblocks is set by the launcher.
 cudaError_t setup_cross_tc_attributes();
 cudaError_t setup_cross_bwd_tc_attributes();
 cudaError_t setup_cross_hd_attributes();

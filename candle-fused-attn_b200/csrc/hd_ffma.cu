@@ -21,155 +21,14 @@
 // chain, the softmax butterflies, O and dK/dV over keys / queries in index order, D in fp64, dQ
 // over key blocks in key-block order (turn chain or no-wait partials, the same bits). Results are
 // bit-identical across reruns, batch splits and workspace sizes.
-//
-// The CROSS instantiations (head dim 128 of cross attention) take keys of another length and shared
-// key heads, as csrc/fwd_tc.cu's and csrc/bwd_tc.cu's do at 64 and 32: a key block walks the query
-// tiles of every query head of its group, and dQ and dK, dV have buffers of their own.
-#include "cfa_common.cuh"
+#include "hd_ffma.cuh"
 
 namespace cfa {
 namespace {
 
-template <int D>
-struct Hd;
-// The forward's rows per thread: two candidates per head dim (query tiles of 8 RPT rows), the one
-// that pads fewer rows at the sequence length taken (hd_fwd_rows; rows are independent, so the
-// choice changes no bit), and blocks per SM.
-template <>
-struct Hd<32> {
-  static constexpr int RPT_A = 8, RPT_B = 6;  // 64- or 48-query tiles
-  static constexpr int FWD_MINB = 3;          // forward blocks per SM (registers)
-};
-template <>
-struct Hd<128> {
-  // 48-query tiles at every length: against 32-query tiles (4 rows per thread) they measured
-  // faster at every shape tried (canvas-shaped 185 -> 158 us, s = 4096 causal 917 -> 820 us).
-  static constexpr int RPT_A = 6, RPT_B = 6;
-  static constexpr int FWD_MINB = 2;          // (shared memory: 107.3 KB per block)
-};
-
-template <int RPT>
-__host__ __device__ constexpr int fwd_bm() {
-  return 8 * RPT;  // 4 warps x 2 half-warps x RPT rows
-}
-
-// Row stride of the [rows][D] tiles: D + 4 floats, rows 16-byte aligned and 4 banks apart.
-template <int D>
-__host__ __device__ constexpr int ldh() {
-  return D + 4;
-}
-
-template <int D, int RPT>
-__host__ __device__ constexpr int hd_fwd_smem_floats() {
-  return (fwd_bm<RPT>() + 2 * 64) * ldh<D>() + fwd_bm<RPT>() * LDP;
-}
-
-template <int D>
-__host__ __device__ constexpr int hd_bwd_smem_floats() {
-  return 4 * 64 * ldh<D>() + 2 * 64 * LDP + 2 * 64 + 4;
-}
-
-// ROWS rows of a strided [seq, D] slice starting at row0 into a [ROWS][D + 4] tile (zero past seq;
-// the address given for such rows is row0's, which is < seq).
-template <int ROWS, int NT, int D>
-__device__ __forceinline__ void load_rows_async(float* dst, const float* __restrict__ src,
-                                                int64_t s_stride, int row0, int seq) {
-  constexpr int C = D / 4;
-#pragma unroll
-  for (int idx = threadIdx.x; idx < ROWS * C; idx += NT) {
-    const int r = idx / C, c4 = idx % C;
-    const int row = row0 + r;
-    const bool ok = row < seq;
-    const float* g = src + static_cast<int64_t>(ok ? row : row0) * s_stride + 4 * c4;
-    cp_async16(dst + r * ldh<D>() + 4 * c4, g, ok ? 16 : 0);
-  }
-}
-
-// S = A B^T for NR rows (rb + 2i) and the first JN of 4 key groups (keys tx + 16jj): an even-d
-// chain plus an odd-d chain per score, as the head-dim-64 kernels do. Groups >= JN are left at 0.
-template <int JN, int NR, int D>
-__device__ __forceinline__ void scores(const float* As, const float* Bs, int rb, int tx,
-                                       float (&s)[NR][4]) {
-  uint64_t s2[NR][JN];
-#pragma unroll
-  for (int i = 0; i < NR; ++i)
-#pragma unroll
-    for (int jj = 0; jj < JN; ++jj) s2[i][jj] = 0ull;
-#pragma unroll 2
-  for (int c = 0; c < D; c += 4) {
-    ulonglong2 bv[JN], av[NR];
-#pragma unroll
-    for (int jj = 0; jj < JN; ++jj) bv[jj] = ld2x2(Bs + (tx + 16 * jj) * ldh<D>() + c);
-#pragma unroll
-    for (int i = 0; i < NR; ++i) av[i] = ld2x2(As + (rb + 2 * i) * ldh<D>() + c);
-#pragma unroll
-    for (int i = 0; i < NR; ++i)
-#pragma unroll
-      for (int jj = 0; jj < JN; ++jj) s2[i][jj] = fma2(av[i].x, bv[jj].x, s2[i][jj]);
-#pragma unroll
-    for (int i = 0; i < NR; ++i)
-#pragma unroll
-      for (int jj = 0; jj < JN; ++jj) s2[i][jj] = fma2(av[i].y, bv[jj].y, s2[i][jj]);
-  }
-#pragma unroll
-  for (int i = 0; i < NR; ++i)
-#pragma unroll
-    for (int jj = 0; jj < 4; ++jj) s[i][jj] = jj < JN ? sum2(s2[i][jj < JN ? jj : 0]) : 0.0f;
-}
-
-// This thread's D / 16 output dims of a row, as register pairs: D = 32 -> dims 2tx, 2tx + 1 (one
-// pair); D = 128 -> dims 4tx .. 4tx + 3 and 64 + 4tx .. 64 + 4tx + 3 (four pairs).
-template <int D>
-struct Dims;
-template <>
-struct Dims<32> {
-  static constexpr int NP = 1;
-  __device__ __forceinline__ static void load(const float* row, int tx, uint64_t (&v)[1]) {
-    v[0] = *reinterpret_cast<const uint64_t*>(row + 2 * tx);
-  }
-  __device__ __forceinline__ static void load_f(const float* row, int tx, float (&v)[2]) {
-    const float2 x = *reinterpret_cast<const float2*>(row + 2 * tx);
-    v[0] = x.x;
-    v[1] = x.y;
-  }
-};
-template <>
-struct Dims<128> {
-  static constexpr int NP = 4;
-  __device__ __forceinline__ static void load(const float* row, int tx, uint64_t (&v)[4]) {
-    const ulonglong2 a = ld2x2(row + 4 * tx), b = ld2x2(row + 64 + 4 * tx);
-    v[0] = a.x;
-    v[1] = a.y;
-    v[2] = b.x;
-    v[3] = b.y;
-  }
-  __device__ __forceinline__ static void load_f(const float* row, int tx, float (&v)[8]) {
-    const float4 a = ld4(row + 4 * tx), b = ld4(row + 64 + 4 * tx);
-    v[0] = a.x;
-    v[1] = a.y;
-    v[2] = a.z;
-    v[3] = a.w;
-    v[4] = b.x;
-    v[5] = b.y;
-    v[6] = b.z;
-    v[7] = b.w;
-  }
-};
-
-// Store this thread's D / 16 dims of a row (the layout of Dims<D>) into row `dst`.
-template <int D>
-__device__ __forceinline__ void store_dims(float* dst, int tx, const float (&v)[D / 16]) {
-  if constexpr (D == 32) {
-    *reinterpret_cast<float2*>(dst + 2 * tx) = make_float2(v[0], v[1]);
-  } else {
-    *reinterpret_cast<float4*>(dst + 4 * tx) = make_float4(v[0], v[1], v[2], v[3]);
-    *reinterpret_cast<float4*>(dst + 64 + 4 * tx) = make_float4(v[4], v[5], v[6], v[7]);
-  }
-}
-
 // ---------------------------------------------------------------------------------------------
 // Forward: csrc/fwd_ffma.cu's kernel with D-sized tiles (see the header comment).
-template <int D, int RPT, bool CAUSAL, bool CROSS = false>
+template <int D, int RPT, bool CAUSAL>
 __global__ void __launch_bounds__(FWD_THREADS, Hd<D>::FWD_MINB) hd_fwd_kernel(const FwdArgs a) {
   constexpr int BM = fwd_bm<RPT>(), L = ldh<D>(), NP = Dims<D>::NP;
   extern __shared__ float4 smem4[];
@@ -194,23 +53,13 @@ __global__ void __launch_bounds__(FWD_THREADS, Hd<D>::FWD_MINB) hd_fwd_kernel(co
   const int b = bh / a.H, h = bh % a.H;
   const int q0 = qt * BM;
   const int S = a.S;
-  const int SK = CROSS ? cross_keys(a, b) : S;  // keys
-  const int hk = CROSS ? h / (a.H / a.Hk) : h;
-  if (CROSS && SK == 0) {  // no key: O = 0, L = -inf
-    const int rows = min(BM, S - q0);
-    for (int f = tid; f < rows * (D / 4); f += FWD_THREADS)
-      reinterpret_cast<float4*>(a.o + ((static_cast<int64_t>(b) * S + q0 + f / (D / 4)) * a.H + h) * D)[f % (D / 4)] =
-          make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int r = tid; r < rows; r += FWD_THREADS) a.lse[static_cast<int64_t>(bh) * S + q0 + r] = -INFINITY;
-    return;
-  }
   const float* qp = a.q + b * a.q_sb + h * a.q_sh;
-  const float* kp = a.k + b * a.k_sb + hk * a.k_sh;
-  const float* vp = a.v + b * a.v_sb + hk * a.v_sh;
-  const int k_end = CAUSAL ? min(SK, q0 + BM) : SK;
+  const float* kp = a.k + b * a.k_sb + h * a.k_sh;
+  const float* vp = a.v + b * a.v_sb + h * a.v_sh;
+  const int k_end = CAUSAL ? min(S, q0 + BM) : S;
 
   load_rows_async<BM, FWD_THREADS, D>(Qs, qp, a.q_ss, q0, S);
-  load_rows_async<64, FWD_THREADS, D>(Ks, kp, a.k_ss, 0, SK);
+  load_rows_async<64, FWD_THREADS, D>(Ks, kp, a.k_ss, 0, S);
   cp_async_commit();
 
   const int rb = 2 * RPT * w + ty;  // rows rb + 2i
@@ -227,17 +76,17 @@ __global__ void __launch_bounds__(FWD_THREADS, Hd<D>::FWD_MINB) hd_fwd_kernel(co
   for (int k0 = 0; k0 < k_end; k0 += 64) {
     cp_async_wait_all();
     __syncthreads();
-    load_rows_async<64, FWD_THREADS, D>(Vs, vp, a.v_ss, k0, SK);
+    load_rows_async<64, FWD_THREADS, D>(Vs, vp, a.v_ss, k0, S);
     cp_async_commit();
 
-    const int jn = min(4, (SK - k0 + 15) / 16);
+    const int jn = min(4, (S - k0 + 15) / 16);
     float s[RPT][4];
     if (jn == 3)
       scores<3, RPT, D>(Qs, Ks, rb, tx, s);
     else
       scores<4, RPT, D>(Qs, Ks, rb, tx, s);
 
-    const bool edge = (k0 + 64 > SK) || (CAUSAL && k0 + 63 > q0);
+    const bool edge = (k0 + 64 > S) || (CAUSAL && k0 + 63 > q0);
 #pragma unroll
     for (int i = 0; i < RPT; ++i) {
       float x[4];
@@ -248,7 +97,7 @@ __global__ void __launch_bounds__(FWD_THREADS, Hd<D>::FWD_MINB) hd_fwd_kernel(co
 #pragma unroll
         for (int jj = 0; jj < 4; ++jj) {
           const int j = k0 + tx + 16 * jj;
-          if (!(j < SK && !(CAUSAL && j > qi))) x[jj] = -INFINITY;
+          if (!(j < S && !(CAUSAL && j > qi))) x[jj] = -INFINITY;
         }
       }
       float tmax = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
@@ -272,7 +121,7 @@ __global__ void __launch_bounds__(FWD_THREADS, Hd<D>::FWD_MINB) hd_fwd_kernel(co
     cp_async_wait_all();
     __syncthreads();
     if (k0 + 64 < k_end) {
-      load_rows_async<64, FWD_THREADS, D>(Ks, kp, a.k_ss, k0 + 64, SK);
+      load_rows_async<64, FWD_THREADS, D>(Ks, kp, a.k_ss, k0 + 64, S);
       cp_async_commit();
     }
 
@@ -347,24 +196,7 @@ __global__ void __launch_bounds__(PREP_THREADS) hd_prep_kernel(const PrepArgs a)
 // ---------------------------------------------------------------------------------------------
 // Backward main kernel: csrc/bwd_ffma.cu's design (phases 1-3, dQ by turn chain or no-wait
 // partials, tickets, bounded waits) with the thread layout of the header comment.
-template <int D>
-struct Bwd;
-template <>
-struct Bwd<32> {
-  static constexpr int NT = 256, WG = 4;   // threads; warps per group
-  static constexpr int R1 = 8;             // phase 1 rows per thread (rows rb1 + 2i)
-  static constexpr int K2 = 8;             // phase 2 keys per thread
-  static constexpr int NP2 = 1;            // phase 2 dim pairs per key pair (dims 2tx, 2tx + 1)
-};
-template <>
-struct Bwd<128> {
-  static constexpr int NT = 512, WG = 8;
-  static constexpr int R1 = 4;
-  static constexpr int K2 = 4;
-  static constexpr int NP2 = 4;            // dims 4tx .. + 3 and 64 + 4tx .. + 3
-};
-
-template <int D, bool CAUSAL, bool CROSS = false>
+template <int D, bool CAUSAL>
 __global__ void __launch_bounds__(Bwd<D>::NT, 256 / (Bwd<D>::NT / 2)) hd_bwd_kernel(const BwdArgs a) {
   constexpr int NT = Bwd<D>::NT, WG = Bwd<D>::WG, R1 = Bwd<D>::R1, K2 = Bwd<D>::K2;
   constexpr int NP2 = Bwd<D>::NP2, L = ldh<D>();
@@ -399,51 +231,23 @@ __global__ void __launch_bounds__(Bwd<D>::NT, 256 / (Bwd<D>::NT / 2)) hd_bwd_ker
     __syncthreads();
     ticket = s_int[0];
   }
-  const int HU = CROSS ? a.Hk : a.H;  // heads that own key blocks
-  const int BH = a.B * HU;
+  const int BH = a.B * a.H;
   const bool bh_major = !CAUSAL && no_wait;
   const int kb = bh_major ? ticket % a.n_kblocks : ticket / BH;
   const int bh = bh_major ? ticket / a.n_kblocks : ticket % BH;
-  const int b = bh / HU, h = bh % HU;
+  const int b = bh / a.H, h = bh % a.H;
   const int k0 = kb * 64;
-  const int group = CROSS ? a.H / a.Hk : 1, h0 = h * group;  // the key block's query heads
-  const int nqt = a.n_qtiles;
-  int SK = S, nkb = a.n_kblocks;  // keys, and the key blocks that take part
-  if constexpr (CROSS) {
-    griddep_wait();  // the lengths may come from the previous kernels
-    SK = cross_keys(a, b);
-    nkb = (SK + 63) / 64;
-    if (kb >= nkb) {  // no key of this block is attended: zeros, and no part in dQ's sums
-      constexpr int C4 = D / 4;
-      const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
-      const int rows = min(64, a.Sk - k0);
-      for (int f = tid; f < 2 * rows * C4; f += NT) {
-        const int which = f / (rows * C4), r = (f / C4) % rows;
-        reinterpret_cast<float4*>(
-            a.dkv + (((static_cast<int64_t>(b) * a.Sk + k0 + r) * 2 + which) * a.Hk + h) * D)[f % C4] = zero;
-      }
-      if (kb == 0)  // no key at all: dQ = 0
-        for (int64_t f = tid; f < static_cast<int64_t>(S) * group * C4; f += NT)
-          reinterpret_cast<float4*>(a.dq + ((static_cast<int64_t>(b) * S + f / (group * C4)) * a.H + h0) *
-                                               D)[f % (group * C4)] = zero;
-      return;
-    }
-  }
+
   const float* qp = a.q + b * a.q_sb + h * a.q_sh;
   const float* gp = a.d_o + b * a.do_sb + h * a.do_sh;
   const float* lp = a.lse + static_cast<int64_t>(bh) * S;
   const float* dp = a.dsum + static_cast<int64_t>(bh) * S;
-  // The query head of the block's tile t and its first query.
-  auto tile_head = [&](int t) { return CROSS ? h0 + t / nqt : h; };
-  auto tile_q0 = [&](int t) { return (CROSS ? t % nqt : t) * 64; };
-  int* turn = a.turn + (static_cast<int64_t>(b) * a.H + h0) * nqt;
-  const int64_t row_stride = (CROSS ? 1 : 3) * static_cast<int64_t>(a.H) * D;
-  auto dq_rows = [&](int head) {
-    return (CROSS ? a.dq : a.dqkv) + static_cast<int64_t>(b) * S * row_stride + head * D;
-  };
+  int* turn = a.turn + static_cast<int64_t>(bh) * a.n_qtiles;
+  const int64_t row_stride = 3 * static_cast<int64_t>(a.H) * D;
+  float* dq_base = a.dqkv + static_cast<int64_t>(b) * S * row_stride + h * D;
 
-  load_rows_async<64, NT, D>(Ks, a.k + b * a.k_sb + h * a.k_sh, a.k_ss, k0, SK);
-  load_rows_async<64, NT, D>(Vs, a.v + b * a.v_sb + h * a.v_sh, a.v_ss, k0, SK);
+  load_rows_async<64, NT, D>(Ks, a.k + b * a.k_sb + h * a.k_sh, a.k_ss, k0, S);
+  load_rows_async<64, NT, D>(Vs, a.v + b * a.v_sb + h * a.v_sh, a.v_ss, k0, S);
 
   // grp 0: dV, grp 1: dK (unscaled). acc2[rp][e]: keys kb2 + 2rp, kb2 + 2rp + 1 (a pair), dim e
   // of this thread's phase 2 dims.
@@ -459,36 +263,34 @@ __global__ void __launch_bounds__(Bwd<D>::NT, 256 / (Bwd<D>::NT / 2)) hd_bwd_ker
   const int rb3 = D == 32 ? 8 * w + ty : 8 * wg + ty;
   const int d3 = D == 32 ? 2 * tx : 64 * grp + 4 * tx;
 
-  auto load_q_do = [&](int t) {
-    const int q0 = tile_q0(t), head = tile_head(t);
-    load_rows_async<64, NT, D>(Qs, CROSS ? a.q + b * a.q_sb + head * a.q_sh : qp, a.q_ss, q0, S);
-    load_rows_async<64, NT, D>(dOs, CROSS ? a.d_o + b * a.do_sb + head * a.do_sh : gp, a.do_ss, q0, S);
+  auto load_q_do = [&](int q0) {
+    load_rows_async<64, NT, D>(Qs, qp, a.q_ss, q0, S);
+    load_rows_async<64, NT, D>(dOs, gp, a.do_ss, q0, S);
   };
-  auto load_l_d = [&](int t) {
+  auto load_l_d = [&](int q0) {
     if (tid < 128) {
-      const int q0 = tile_q0(t), r = tid & 63, i = q0 + r;
+      const int r = tid & 63, i = q0 + r;
       const bool ok = i < S;
-      const int64_t rows = (static_cast<int64_t>(b) * a.H + tile_head(t)) * S;
-      const float* src = CROSS ? (tid < 64 ? a.lse : a.dsum) + rows : (tid < 64 ? lp : dp);
-      cp_async4((tid < 64 ? Lt : Dt) + r, src + (ok ? i : q0), ok ? 4 : 0);
+      const float* src = (tid < 64 ? lp : dp) + (ok ? i : q0);
+      cp_async4((tid < 64 ? Lt : Dt) + r, src, ok ? 4 : 0);
     }
   };
-  auto load_query_tile = [&](int t) {
-    load_q_do(t);
-    load_l_d(t);
+  auto load_query_tile = [&](int q0) {
+    load_q_do(q0);
+    load_l_d(q0);
   };
 
-  const int t_begin = CAUSAL ? k0 / 64 : 0, t_end = group * nqt;
-  load_q_do(t_begin);
+  const int t_begin = CAUSAL ? k0 / 64 : 0;
+  load_q_do(t_begin * 64);
   if (no_wait) griddep_wait();
-  load_l_d(t_begin);
+  load_l_d(t_begin * 64);
   cp_async_commit();
-  for (int t = t_begin; t < t_end; ++t) {
-    const int q0 = tile_q0(t);
+  for (int t = t_begin; t < a.n_qtiles; ++t) {
+    const int q0 = t * 64;
     cp_async_wait_all();
     __syncthreads();
 
-    const int jn = min(4, (SK - k0 + 15) / 16);
+    const int jn = min(4, (S - k0 + 15) / 16);
     const int iq = min(64, (S - q0 + 15) / 16 * 16);
 
     // Phase 1. grp 0: s = Q K^T; grp 1: s = dO V^T (dP).
@@ -511,7 +313,7 @@ __global__ void __launch_bounds__(Bwd<D>::NT, 256 / (Bwd<D>::NT / 2)) hd_bwd_ker
         scores<1, R1, D>(As, Bs, rb1, tx, s);
       }
       if (grp == 0) {
-        const bool edge = (q0 + 64 > S) || (k0 + 64 > SK) || (CAUSAL && k0 + 63 > q0);
+        const bool edge = (q0 + 64 > S) || (k0 + 64 > S) || (CAUSAL && k0 + 63 > q0);
 #pragma unroll
         for (int i = 0; i < R1; ++i) {
           const int il = rb1 + 2 * i, qi = q0 + il;
@@ -520,7 +322,7 @@ __global__ void __launch_bounds__(Bwd<D>::NT, 256 / (Bwd<D>::NT / 2)) hd_bwd_ker
           for (int jj = 0; jj < 4; ++jj) {
             const int jl = tx + 16 * jj, j = k0 + jl;
             float pr = expf(fmaf(s[i][jj], a.scale, -li));
-            if (edge && !(qi < S && j < SK && !(CAUSAL && j > qi))) pr = 0.0f;
+            if (edge && !(qi < S && j < S && !(CAUSAL && j > qi))) pr = 0.0f;
             Ps[il * LDP + jl] = pr;
           }
         }
@@ -546,7 +348,7 @@ __global__ void __launch_bounds__(Bwd<D>::NT, 256 / (Bwd<D>::NT / 2)) hd_bwd_ker
     {
       const float* Xs = grp ? dSs : Ps;
       const float* Ys = grp ? Qs : dOs;
-      const int iw = k0 + kb2 - K2 * ty >= SK ? 0 : iq;  // all this warp's keys past the end
+      const int iw = k0 + kb2 - K2 * ty >= S ? 0 : iq;  // all this warp's keys past the end
 #pragma unroll 8
       for (int i = 0; i < iw; ++i) {
         uint64_t xp[K2 / 2];
@@ -572,8 +374,8 @@ __global__ void __launch_bounds__(Bwd<D>::NT, 256 / (Bwd<D>::NT / 2)) hd_bwd_ker
       }
     }
     __syncthreads();
-    if (t + 1 < t_end) {
-      load_query_tile(t + 1);
+    if (t + 1 < a.n_qtiles) {
+      load_query_tile(q0 + 64);
       cp_async_commit();
     }
 
@@ -621,8 +423,7 @@ __global__ void __launch_bounds__(Bwd<D>::NT, 256 / (Bwd<D>::NT / 2)) hd_bwd_ker
       }
 
     if (a.dq_part != nullptr) {
-      float* part =
-          a.dq_part + ((static_cast<int64_t>(b) * a.H + tile_head(t)) * a.n_kblocks + kb) * S * D;
+      float* part = a.dq_part + (static_cast<int64_t>(bh) * a.n_kblocks + kb) * S * D;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int qi = q0 + rb3 + 2 * r;
@@ -636,7 +437,7 @@ __global__ void __launch_bounds__(Bwd<D>::NT, 256 / (Bwd<D>::NT / 2)) hd_bwd_ker
       continue;
     }
     // Turn chain (long sequences): key blocks add into dQ in index order, each on its turn.
-    const int last = CAUSAL ? min(nkb - 1, min(S - 1, q0 + 63) / 64) : nkb - 1;
+    const int last = CAUSAL ? min(a.n_kblocks - 1, min(S - 1, q0 + 63) / 64) : a.n_kblocks - 1;
     bool go = true;
     if (kb > 0) {
       if (tid == 0) {
@@ -651,7 +452,7 @@ __global__ void __launch_bounds__(Bwd<D>::NT, 256 / (Bwd<D>::NT / 2)) hd_bwd_ker
       for (int r = 0; r < 4; ++r) {
         const int qi = q0 + rb3 + 2 * r;
         if (qi >= S) continue;
-        float* dst = dq_rows(tile_head(t)) + qi * row_stride + d3;
+        float* dst = dq_base + qi * row_stride + d3;
 #pragma unroll
         for (int e = 0; e < E3; ++e) {
           float v = pq[r][e];
@@ -674,17 +475,16 @@ __global__ void __launch_bounds__(Bwd<D>::NT, 256 / (Bwd<D>::NT / 2)) hd_bwd_ker
     __syncthreads();
     if (tid == 0) s_int[1] = atomicAdd(a.turn + bh, 1);
     __syncthreads();
-    if (s_int[1] == nkb - 1) {
+    if (s_int[1] == a.n_kblocks - 1) {
       __threadfence();
+      const float* part = a.dq_part + static_cast<int64_t>(bh) * a.n_kblocks * S * D;
       constexpr int C = D / 4;  // float4 per row
       // DETERMINISM: (((p0 + p1) + p2) + ...) * scale over the contributing key blocks in order.
-      for (int hq = h0; hq < h0 + group; ++hq)
       for (int idx = tid; idx < S * C; idx += NT) {
-        const float* part = a.dq_part + (static_cast<int64_t>(b) * a.H + hq) * a.n_kblocks * S * D;
-        float* dq_base = dq_rows(hq);
         const int i = idx / C, c4 = idx % C;
         const int tq = i / 64;
-        const int last = CAUSAL ? min(nkb - 1, min(S - 1, tq * 64 + 63) / 64) : nkb - 1;
+        const int last = CAUSAL ? min(a.n_kblocks - 1, min(S - 1, tq * 64 + 63) / 64)
+                                : a.n_kblocks - 1;
         float4 v = __ldcg(reinterpret_cast<const float4*>(part + static_cast<int64_t>(i) * D + 4 * c4));
         for (int j = 1; j <= last; ++j) {
           const float4 p = __ldcg(reinterpret_cast<const float4*>(
@@ -698,11 +498,7 @@ __global__ void __launch_bounds__(Bwd<D>::NT, 256 / (Bwd<D>::NT / 2)) hd_bwd_ker
   }
 
   // grp 0 stores dV into slot 2, grp 1 stores dK * scale into slot 1.
-  // (CROSS: dkv [b, Sk, 2, Hk, D], dK first.)
-  const int64_t kv_stride = CROSS ? 2 * static_cast<int64_t>(a.Hk) * D : row_stride;
-  float* dst0 = CROSS ? a.dkv + static_cast<int64_t>(b) * a.Sk * kv_stride + (grp ? 0 : 1) * a.Hk * D + h * D
-                      : a.dqkv + static_cast<int64_t>(b) * S * row_stride + (grp ? 1 : 2) * a.H * D + h * D;
-  const int k_rows = CROSS ? a.Sk : S;  // (CROSS: rows past the length hold zeros)
+  float* dst0 = a.dqkv + static_cast<int64_t>(b) * S * row_stride + (grp ? 1 : 2) * a.H * D + h * D;
   const float f = grp ? a.scale : 1.0f;
 #pragma unroll
   for (int rp = 0; rp < K2 / 2; ++rp) {
@@ -714,8 +510,8 @@ __global__ void __launch_bounds__(Bwd<D>::NT, 256 / (Bwd<D>::NT / 2)) hd_bwd_ker
       hi[e] = v.y * f;
     }
     const int j = k0 + kb2 + 2 * rp;
-    if (j < k_rows) store_dims<D>(dst0 + j * kv_stride, tx, lo);
-    if (j + 1 < k_rows) store_dims<D>(dst0 + (j + 1) * kv_stride, tx, hi);
+    if (j < S) store_dims<D>(dst0 + j * row_stride, tx, lo);
+    if (j + 1 < S) store_dims<D>(dst0 + (j + 1) * row_stride, tx, hi);
   }
 }
 
@@ -801,35 +597,6 @@ cudaError_t launch_hd_bwd(const BwdArgs& a, int head_dim, int causal, cudaStream
   const size_t smem = hd_bwd_smem_floats<128>() * 4;
   return causal ? launch_pdl(hd_bwd_kernel<128, true>, grid, dim3(Bwd<128>::NT), smem, stream, a)
                 : launch_pdl(hd_bwd_kernel<128, false>, grid, dim3(Bwd<128>::NT), smem, stream, a);
-}
-
-// Cross attention at head dim 128.
-cudaError_t setup_cross_hd_attributes() {
-  constexpr int A = Hd<128>::RPT_A;
-  const cudaError_t e =
-      cudaFuncSetAttribute(hd_fwd_kernel<128, A, false, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           hd_fwd_smem_floats<128, A>() * 4);
-  return e != cudaSuccess ? e
-                          : cudaFuncSetAttribute(hd_bwd_kernel<128, false, true>,
-                                                 cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                 hd_bwd_smem_floats<128>() * 4);
-}
-
-cudaError_t launch_cross_hd_fwd(const FwdArgs& args, cudaStream_t stream) {
-  constexpr int A = Hd<128>::RPT_A, bm = fwd_bm<A>();
-  FwdArgs a = args;
-  a.n_qtiles = (a.S + bm - 1) / bm;
-  const dim3 grid(static_cast<unsigned>(static_cast<int64_t>(a.n_qtiles) * a.B * a.H));
-  return launch_pdl(hd_fwd_kernel<128, A, false, true>, grid, dim3(FWD_THREADS),
-                    static_cast<size_t>(hd_fwd_smem_floats<128, A>() * 4), stream, a);
-}
-
-cudaError_t launch_cross_hd_bwd(const BwdArgs& args, cudaStream_t stream) {
-  BwdArgs a = args;
-  a.n_kblocks = (a.Sk + 63) / 64;
-  const dim3 grid(static_cast<unsigned>(static_cast<int64_t>(a.n_kblocks) * a.B * a.Hk));
-  return launch_pdl(hd_bwd_kernel<128, false, true>, grid, dim3(Bwd<128>::NT),
-                    static_cast<size_t>(hd_bwd_smem_floats<128>() * 4), stream, a);
 }
 
 }  // namespace cfa
