@@ -173,7 +173,7 @@ def load() -> ctypes.CDLL:
                                      _p, _strides, _p, _strides, _d, _i64, _i64, _p, _i64, _i64,
                                      _p, _p, _p, _f, *[_i64] * 6, _d, _p]
     lib.cfa_paged_attention_workspace_bytes.restype = _n
-    lib.cfa_paged_attention_workspace_bytes.argtypes = [_i64] * 5
+    lib.cfa_paged_attention_workspace_bytes.argtypes = [*[_i64] * 5, _d]
     lib.cfa_paged_attention.restype = ctypes.c_int
     lib.cfa_paged_attention.argtypes = [_p, _strides, _d, _p, _strides, _p, _strides, _d, _i64,
                                         _i64, _p, _i64, _i64, _p, _p, _p, _p, _n, *[_i64] * 5, _f,
@@ -390,8 +390,8 @@ def paged_append(q_ptr, qs, qo_ptr, qos, k_ptr, ks, v_ptr, vs, dtype, kc_ptr, kc
         lengths_ptr, new_ptr, freqs_ptr, amplitude, b, h, hk, s, d, rot, int(interleaved), stream)
 
 
-def paged_attention_workspace_bytes(b, h, s, max_keys, d) -> int:
-    return int(load().cfa_paged_attention_workspace_bytes(b, h, s, max_keys, d))
+def paged_attention_workspace_bytes(b, h, s, max_keys, d, cache_dtype) -> int:
+    return int(load().cfa_paged_attention_workspace_bytes(b, h, s, max_keys, d, cache_dtype))
 
 
 def paged_attention(q_ptr, qs, dtype, kc_ptr, kcs, vc_ptr, vcs, cache_dtype, pages, page_size,

@@ -146,7 +146,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         q = q.clone(memory_format=torch.contiguous_format)
     o = torch.empty((b, s, h, d), dtype=q.dtype, device=dev)
     width, page = page_table.shape[1], k_cache.shape[1]
-    n = _abi.paged_attention_workspace_bytes(b, h, s, width * page, d)
+    n = _abi.paged_attention_workspace_bytes(b, h, s, width * page, d, DTYPES[k_cache.dtype])
     ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
     with on_device(dev):
         st = _abi.paged_attention(

@@ -69,11 +69,15 @@ struct SplitArgs {
   int* sink;
   // set by the launcher
   int group, rows, row_chunks, max_chunks;
+  uint32_t page_mul;  // key / page = key page_mul >> page_shift
+  int page_shift;
+  int one_page;       // every tile of keys lies on one page
+  int tile_log;       // log2 of the keys of a tile
   float* part_o;   // [B H S][max_chunks][D] unnormalised partial outputs
   float2* part_ml; // [B H S][max_chunks] running maximum (log2 units) and sum
 };
-int split_max_chunks(int64_t max_len);
-size_t split_workspace_bytes(int64_t rows, int64_t max_len, int64_t head_dim);
+int split_max_chunks(int64_t max_len, int64_t head_dim, int kv_dtype);
+size_t split_workspace_bytes(int64_t rows, int64_t max_len, int64_t head_dim, int kv_dtype);
 cudaError_t setup_split_attributes();
 cudaError_t launch_split_attention(const SplitArgs& a, int q_dtype, int kv_dtype, void* workspace,
                                    cudaStream_t stream);

@@ -48,12 +48,19 @@ int status(cudaError_t e) {
   return e == cudaErrorInvalidConfiguration ? CFA_ERR_OVERFLOW : CFA_ERR_LAUNCH;
 }
 
+// The split attention's units (chunks x key heads x rows of 8) fit 31 bits.
+bool split_units_ok(int64_t B, int64_t H, int64_t Hk, int64_t S, int64_t max_len, int64_t D, int kv) {
+  const int64_t chunks = B * cfa::split_max_chunks(max_len, D, kv);
+  const int64_t per = Hk * ((H / Hk * S + 7) / 8);
+  return chunks <= kLim && per <= kLim && chunks <= kLim / per;
+}
+
 // B, H, Hk, Sq, Sk of a cross attention.
 int check_cross(int64_t B, int64_t H, int64_t Hk, int64_t Sq, int64_t Sk, int64_t D) {
   if (B < 0 || H < 0 || Hk < 0 || Sq < 0 || Sk < 0 || D < 0) return CFA_ERR_SHAPE;
   if (!head_dim_ok(D)) return CFA_ERR_HEAD_DIM;
   if (Hk == 0 ? H != 0 : H % Hk != 0) return CFA_ERR_HEADS;
-  if (B > kLim || H > kLim || Sq > kLim - 64 || Sk > kLim - 128) return CFA_ERR_OVERFLOW;
+  if (B > kLim || H > kLim || Sq > kLim - 1024 || Sk > kLim - 1024) return CFA_ERR_OVERFLOW;
   if (B == 0 || H == 0) return CFA_OK;
   if (B * H > kLim / ((std::max(Sq, Sk) + 31) / 32 + 1)) return CFA_ERR_OVERFLOW;
   if (B * H * Sq > kLim || B * Hk * Sk > kLim) return CFA_ERR_OVERFLOW;
@@ -213,9 +220,9 @@ int cfa_cross_bwd_f32(const float* q, const int64_t q_strides[3], const float* k
 size_t cfa_cross_few_workspace_bytes(int64_t batch, int64_t heads, int64_t seq, int64_t key_seq,
                                      int64_t head_dim) {
   if (batch <= 0 || heads <= 0 || seq <= 0 || key_seq <= 0 || !head_dim_ok(head_dim) ||
-      batch > kLim || heads > kLim || seq > kLim || key_seq > kLim || batch * heads > kLim / seq)
+      batch > kLim || heads > kLim || seq > kLim || key_seq > kLim - 1024 || batch * heads > kLim / seq)
     return 0;
-  return cfa::split_workspace_bytes(batch * heads * seq, key_seq, head_dim);
+  return cfa::split_workspace_bytes(batch * heads * seq, key_seq, head_dim, CFA_F32);
 }
 
 int cfa_cross_few_f32(const float* q, const int64_t q_strides[3], const float* k,
@@ -234,7 +241,7 @@ int cfa_cross_few_f32(const float* q, const int64_t q_strides[3], const float* k
     return CFA_ERR_ALIGNMENT;
   if (workspace_bytes < need || (need && (reinterpret_cast<uintptr_t>(workspace) & 255u) != 0))
     return CFA_ERR_WORKSPACE;
-  if (batch * cfa::split_max_chunks(key_seq) > kLim) return CFA_ERR_OVERFLOW;
+  if (!split_units_ok(batch, heads, key_heads, seq, key_seq, head_dim, CFA_F32)) return CFA_ERR_OVERFLOW;
   st = setup(g_split_once, cfa::setup_split_attributes);
   if (st != CFA_OK) return st;
   cfa::SplitArgs a{};
@@ -339,11 +346,12 @@ int cfa_paged_append(const void* q, const int64_t q_strides[3], void* q_out,
 }
 
 size_t cfa_paged_attention_workspace_bytes(int64_t batch, int64_t heads, int64_t seq,
-                                           int64_t max_keys, int64_t head_dim) {
+                                           int64_t max_keys, int64_t head_dim, int cache_dtype) {
   if (batch <= 0 || heads <= 0 || seq <= 0 || max_keys <= 0 || !head_dim_ok(head_dim) ||
-      batch > kLim || heads > kLim || seq > kLim || max_keys > kLim || batch * heads > kLim / seq)
+      !type_ok(cache_dtype) || batch > kLim || heads > kLim || seq > kLim || max_keys > kLim - 1024 ||
+      batch * heads > kLim / seq)
     return 0;
-  return cfa::split_workspace_bytes(batch * heads * seq, max_keys, head_dim);
+  return cfa::split_workspace_bytes(batch * heads * seq, max_keys, head_dim, cache_dtype);
 }
 
 int cfa_paged_attention(const void* q, const int64_t q_strides[3], int dtype, const void* k_cache,
@@ -365,7 +373,7 @@ int cfa_paged_attention(const void* q, const int64_t q_strides[3], int dtype, co
       page_size > kLim || table_width > kLim || table_width * page_size > kLim - 1024)
     return CFA_ERR_OVERFLOW;
   const int64_t max_keys = table_width * page_size;
-  const size_t need = cfa_paged_attention_workspace_bytes(batch, heads, seq, max_keys, head_dim);
+  const size_t need = cfa_paged_attention_workspace_bytes(batch, heads, seq, max_keys, head_dim, cache_dtype);
   if (!q || !o || !q_strides || !k_cache_strides || !v_cache_strides || !lengths ||
       (max_keys > 0 && (!k_cache || !v_cache || !page_table)) || (need > 0 && !workspace))
     return CFA_ERR_NULL;
@@ -376,7 +384,8 @@ int cfa_paged_attention(const void* q, const int64_t q_strides[3], int dtype, co
     return CFA_ERR_ALIGNMENT;
   if (workspace_bytes < need || (need && (reinterpret_cast<uintptr_t>(workspace) & 255u) != 0))
     return CFA_ERR_WORKSPACE;
-  if (batch * cfa::split_max_chunks(max_keys) > kLim) return CFA_ERR_OVERFLOW;
+  if (!split_units_ok(batch, heads, key_heads, seq, max_keys, head_dim, cache_dtype))
+    return CFA_ERR_OVERFLOW;
   const int st = setup(g_split_once, cfa::setup_split_attributes);
   if (st != CFA_OK) return st;
   cfa::SplitArgs a{};

@@ -33,6 +33,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <atomic>
 #include <type_traits>
 
 #include "cfa_common.cuh"
@@ -45,23 +46,30 @@ namespace {
 
 constexpr int WARPS = 4;
 constexpr int NT = 32 * WARPS;
-constexpr int TK = 16;     // keys per tile
 constexpr int MAXR = 8;    // query rows per block
 constexpr float LOG2E = 1.4426950408889634f;
-constexpr int CHUNK_MIN = 64, CHUNK_MAX = 512, FEW_CHUNKS = 16, MOST_CHUNKS = 256;
 
-// Keys per chunk of a sequence of `len` keys: the smallest power of two from 64 that gives at most
-// 16 chunks, but 512 at most until that would make more than 256.
-__host__ __device__ inline int64_t split_chunk(int64_t len) {
-  int64_t c = CHUNK_MIN;
-  while (c < CHUNK_MAX && len > FEW_CHUNKS * c) c *= 2;
-  while (len > MOST_CHUNKS * c) c *= 2;
-  return c;
+// Keys per chunk, as a power of two, of a sequence of `len` keys in tiles of 2^tile_log keys: 16 tiles
+// (four a warp, 128 KB of keys and values) up to 16 chunks, then 32 tiles up to 256 chunks, then as many
+// as keep them 256.
+constexpr int FEW_CHUNKS_LOG = 4, MOST_CHUNKS_LOG = 8, MOST_CHUNKS = 1 << MOST_CHUNKS_LOG;
+__host__ __device__ __forceinline__ int bits_of(uint32_t x) {  // x < 2^bits
+#ifdef __CUDA_ARCH__
+  return 32 - __clz(x);
+#else
+  return x ? 32 - __builtin_clz(x) : 0;
+#endif
 }
-__host__ __device__ inline int chunks_of(int64_t len) {
+__host__ __device__ __forceinline__ int chunk_log(int len, int tile_log) {
+  const int few = tile_log + 4;
+  if (len <= 1 << (few + FEW_CHUNKS_LOG)) return few;
+  const int need = bits_of(static_cast<uint32_t>(len - 1)) - MOST_CHUNKS_LOG;
+  return need > few + 1 ? need : few + 1;
+}
+__host__ __device__ __forceinline__ int chunks_of(int len, int tile_log) {
   if (len <= 0) return 1;  // one empty chunk: its block writes the zeros
-  const int64_t c = split_chunk(len);
-  return static_cast<int>((len + c - 1) / c);
+  const int c = chunk_log(len, tile_log);
+  return static_cast<int>((static_cast<uint32_t>(len) + (1u << c) - 1) >> c);
 }
 
 template <typename T>
@@ -89,7 +97,7 @@ struct ChunkIndex {
     first = lane * per;
     count = 0;
     for (int i = first; i < min(first + per, a.B); ++i) {
-      count += chunks_of(seq_len(a, i));
+      count += chunks_of(seq_len(a, i), a.tile_log);
       if (a.table && blockIdx.x == 0 && a.lengths[i] > a.max_len) flag_error(a.sink, CFA_ERR_PAGE);
     }
     int incl = count;
@@ -107,76 +115,155 @@ struct ChunkIndex {
     const int owner = __ffs(in) - 1;
     b = __shfl_sync(0xffffffffu, first, owner);
     c = g - __shfl_sync(0xffffffffu, before, owner);
-    nc = chunks_of(seq_len(a, b));
+    nc = chunks_of(seq_len(a, b), a.tile_log);
     while (c >= nc) {
       c -= nc;
-      nc = chunks_of(seq_len(a, ++b));
+      nc = chunks_of(seq_len(a, ++b), a.tile_log);
     }
   }
 };
 
-// One warp's ring of tiles: 16 rows of K, then of V, RB bytes apart.
-template <int D, int ES, int STAGES>
+// A 16-byte asynchronous copy past L1 (the rows are read once).
+__device__ __forceinline__ void cp_async16_full(void* smem, const void* gmem) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(tc::smem_u32(smem)), "l"(gmem)
+               : "memory");
+}
+
+// One warp's ring of tiles: TK rows of K, then of V, RB bytes apart, a stage a tile. Each lane copies
+// the 16-byte piece `lane % CPR` of every RPI-th row.
+template <int D, int ES, int TK_, int ST_>
 struct Ring {
+  static constexpr int ST = ST_;   // stages
+  static constexpr int TK = TK_;   // keys per tile
   static constexpr int RB = D * ES + 16;
   static constexpr int KV = TK * RB;          // bytes of a tile's K (or V)
   static constexpr int STAGE = 2 * KV;
   static constexpr int CPR = D * ES / 16;     // 16-byte pieces of a row
-  static constexpr int BYTES = STAGES * STAGE;
+  static constexpr int RPI = 32 / CPR;        // rows that the warp copies at once
+  static constexpr int BYTES = ST * STAGE;
+  static constexpr unsigned ALL = 0xffffffffu >> (32 - TK);
 
   const SplitArgs& a;
   unsigned char* base;
-  const char* kp;  // this (batch, key head)'s keys and values
+  int lane;
+  int64_t k_lane, v_lane;  // this lane's first row and piece within a tile, in bytes
+  const char* kp;          // this (batch, key head)'s keys and values
   const char* vp;
   const int* table;
-  int lane, len;
+  int lo, tiles, len, next, pg;  // the unit's first key, its tiles and end; the next tile, its page
+  unsigned live[ST];             // the live keys of the tiles in flight, oldest first
   bool bad = false;
 
   __device__ __forceinline__ Ring(const SplitArgs& a_, unsigned char* base_, int lane_)
-      : a(a_), base(base_), lane(lane_) {}
-
-  __device__ __forceinline__ void start(int b, int hk, int len_) {
-    len = len_;
+      : a(a_), base(base_), lane(lane_) {
+    k_lane = (lane / CPR) * a.k_sr * ES + 16 * (lane % CPR);
+    v_lane = (lane / CPR) * a.v_sr * ES + 16 * (lane % CPR);
+  }
+  __device__ __forceinline__ int page_at(int key) const {  // key / a.page (key < 2^31)
+    return static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(key)) * a.page_mul) >> a.page_shift);
+  }
+  // The page of the next tile: of its first key, or (pages that end inside a tile) of this lane's
+  // row. 0 where dense, -1 where there is none.
+  __device__ __forceinline__ int page_of(int t) const {
+    const int key = lo + TK * t + (a.one_page ? 0 : (lane & (TK - 1)));
+    if (t >= tiles || key >= len) return -1;
+    return table ? __ldg(table + page_at(key)) : 0;
+  }
+  // Starts a unit: keys lo_ .. hi_ - 1 of (b, hk), the warp's tiles w, w + 4, ..: the first ST - 1 of
+  // them travel.
+  __device__ __forceinline__ void start(int b, int hk, int lo_, int hi_, int w) {
+    lo = lo_;
+    len = hi_;
+    tiles = (hi_ - lo_ + TK - 1) / TK;
+    next = w;
     kp = static_cast<const char*>(a.k) + ES * (hk * a.k_sh + (a.table ? 0 : b * a.k_sp));
     vp = static_cast<const char*>(a.v) + ES * (hk * a.v_sh + (a.table ? 0 : b * a.v_sp));
     table = a.table ? a.table + b * a.table_sb : nullptr;
+    pg = page_of(next);
+#pragma unroll
+    for (int s = 0; s < ST - 1; ++s) live[s] = issue(s);
   }
-  // The page of this lane's row of the tile at key k0 (0 where dense; -1 past the end).
-  __device__ __forceinline__ int page_of(int k0) const {
-    const int key = k0 + (lane & (TK - 1));
-    if (key >= len) return -1;
-    return table ? __ldg(table + key / a.page) : 0;
+  // The oldest tile's live keys as bits; the tile after those in flight goes into `stage`.
+  __device__ __forceinline__ unsigned advance(int stage) {
+    const unsigned now = live[0];
+#pragma unroll
+    for (int s = 0; s + 1 < ST - 1; ++s) live[s] = live[s + 1];
+    live[ST - 2] = issue(stage);
+    return now;
   }
-  // Copies the tile at key k0 into `stage`; pg: page_of(k0). Returns the tile's live keys as bits.
-  __device__ __forceinline__ unsigned load(int k0, int stage, int pg) {
+  __device__ __forceinline__ unsigned issue(int stage) {
+    unsigned x = 0;
+    if (next < tiles) {
+      const int now = pg;
+      const int k0 = lo + TK * next;
+      next += WARPS;
+      pg = page_of(next);
+      x = a.one_page ? load_page(k0, stage, now) : load_rows(k0, stage, now);
+    }
+    cp_async_commit();
+    return x;
+  }
+  // A tile whose rows lie on one page (page sizes that are multiples of TK; a dense operand).
+  __device__ __forceinline__ unsigned load_page(int k0, int stage, int p) {
+    int rows = min(TK, len - k0);
+    int64_t ko = 0, vo = 0;
+    if (!table) {
+      ko = k0 * a.k_sr;
+      vo = k0 * a.v_sr;
+    } else if (p < 0 || p >= a.n_pages) {
+      bad = true;
+      rows = 0;
+    } else {
+      const int row = k0 - page_at(k0) * a.page;
+      ko = p * a.k_sp + row * a.k_sr;
+      vo = p * a.v_sp + row * a.v_sr;
+    }
+    const char* kg = kp + ES * ko + k_lane;
+    const char* vg = vp + ES * vo + v_lane;
+    unsigned char* st = base + stage * STAGE + (lane / CPR) * RB + 16 * (lane % CPR);
+    const int64_t kj = RPI * ES * a.k_sr, vj = RPI * ES * a.v_sr;
+    if (rows == TK) {
+#pragma unroll
+      for (int j = 0; j < TK / RPI; ++j) {
+        cp_async16_full(st + j * RPI * RB, kg + j * kj);
+        cp_async16_full(st + KV + j * RPI * RB, vg + j * vj);
+      }
+      return ALL;
+    }
+#pragma unroll
+    for (int j = 0; j < TK / RPI; ++j) {  // rows past the end: zeros (from an address that exists)
+      const bool ok = j * RPI + lane / CPR < rows;
+      cp_async16(st + j * RPI * RB, ok ? kg + j * kj : kp, ok ? 16 : 0);
+      cp_async16(st + KV + j * RPI * RB, ok ? vg + j * vj : vp, ok ? 16 : 0);
+    }
+    return (1u << rows) - 1;
+  }
+  // Any page size: lane r % TK finds row r's address, the copying lanes ask it for theirs.
+  __device__ __forceinline__ unsigned load_rows(int k0, int stage, int p) {
     const int key = k0 + (lane & (TK - 1));
     bool ok = key < len;
     int64_t ko = 0, vo = 0;
-    if (table) {
-      if (ok && (pg < 0 || pg >= a.n_pages)) {
-        ok = false;
-        bad = true;
-      }
-      if (ok) {
-        const int row = key - key / a.page * a.page;
-        ko = pg * a.k_sp + row * a.k_sr;
-        vo = pg * a.v_sp + row * a.v_sr;
-      }
-    } else if (ok) {
-      ko = key * a.k_sr;
-      vo = key * a.v_sr;
+    if (ok && (p < 0 || p >= a.n_pages)) {
+      ok = false;
+      bad = true;
     }
-    const unsigned live = __ballot_sync(0xffffffffu, ok) & 0xffffu;
+    if (ok) {
+      const int row = key - page_at(key) * a.page;
+      ko = p * a.k_sp + row * a.k_sr;
+      vo = p * a.v_sp + row * a.v_sr;
+    }
+    const unsigned alive = __ballot_sync(0xffffffffu, ok) & ALL;
     unsigned char* st = base + stage * STAGE;
+    const int c = lane % CPR;
 #pragma unroll
-    for (int j = 0; j < TK * CPR / 32; ++j) {
-      const int i = j * 32 + lane, r = i / CPR, c = i % CPR;
+    for (int j = 0; j < TK / RPI; ++j) {
+      const int r = j * RPI + lane / CPR;
       const int64_t kr = __shfl_sync(0xffffffffu, ko, r), vr = __shfl_sync(0xffffffffu, vo, r);
-      const int n = (live >> r) & 1u ? 16 : 0;
+      const int n = (alive >> r) & 1u ? 16 : 0;
       cp_async16(st + r * RB + 16 * c, kp + ES * kr + 16 * c, n);
       cp_async16(st + KV + r * RB + 16 * c, vp + ES * vr + 16 * c, n);
     }
-    return live;
+    return alive;
   }
 };
 
@@ -199,19 +286,19 @@ __device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], const void* p) {
 }
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   uint32_t y;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
 template <typename T>
 __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   if constexpr (std::is_same_v<T, __half>)
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
         "{%8, %9}, {%0, %1, %2, %3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   else
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
         "{%8, %9}, {%0, %1, %2, %3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -239,38 +326,47 @@ __device__ __forceinline__ float2 unpack16(uint32_t x) {
 struct UnitInfo {
   int b, hk, r0, chunk, nc, len, n_new, lo, hi;  // rows r0 .., keys lo .. hi - 1
 };
-__device__ __forceinline__ UnitInfo unit_info(const SplitArgs& a, const ChunkIndex& ix, int64_t u) {
+__device__ __forceinline__ UnitInfo unit_info(const SplitArgs& a, const ChunkIndex& ix, uint32_t u) {
   UnitInfo n;
-  const int per = a.Hk * a.row_chunks;
-  const int g = static_cast<int>(u / per), rest = static_cast<int>(u - static_cast<int64_t>(g) * per);
+  const uint32_t per = a.Hk * a.row_chunks;
+  const int g = static_cast<int>(u / per), rest = static_cast<int>(u - g * per);
   n.hk = rest / a.row_chunks;
   n.r0 = (rest - n.hk * a.row_chunks) * MAXR;
   ix.find(a, g, n.b, n.chunk, n.nc);
   n.len = seq_len(a, n.b);
   n.n_new = seq_new(a, n.b);
-  const int64_t c = split_chunk(n.len);
-  n.lo = static_cast<int>(n.chunk * c);
-  n.hi = static_cast<int>(min(static_cast<int64_t>(n.len), n.lo + c));
+  const int c = chunk_log(n.len, a.tile_log);
+  n.lo = n.chunk << c;
+  n.hi = min(n.len, n.lo + (1 << c));  // (len <= 2^31 - 1025: no overflow)
   return n;
 }
-// Row r of a key head's rows: query head r / S of the group, new token r % S. The keys it sees (a
-// row that is not there sees them all: its result is never written).
+// Row r of a key head's rows: query head r / S of the group, new token r % S.
+__device__ __forceinline__ void row_of(const SplitArgs& a, int r, int& head, int& i) {
+  head = a.S == 1 ? r : r / a.S;
+  i = a.S == 1 ? 0 : r - head * a.S;
+}
+// The keys it sees (a row that is not there sees them all: its result is never written).
 __device__ __forceinline__ int row_limit(const SplitArgs& a, const UnitInfo& n, int r) {
-  const int i = r % a.S;
+  int head, i;
+  row_of(a, r, head, i);
   if (!a.causal || r >= a.rows || i >= n.n_new) return n.len;
   return min(max(n.len - n.n_new + i + 1, 0), n.len);
 }
 
-// Joins the four warps' sums of rows r0 .. r0 + nr - 1 (red: [warp][row][D], ml: [warp][row]) and
-// writes the chunk's partial result, or, the sequence's only chunk, the output.
+// Joins the four warps' sums of the block's first nr rows (a warp's: [row][D], red_step bytes from
+// warp to warp; ml: [warp][row]) and writes the chunk's partial result, or, the sequence's only chunk,
+// the output.
 template <typename QT, int D>
-__device__ __forceinline__ void write_chunk(const SplitArgs& a, const UnitInfo& n, const float* red,
-                                            const float2* ml, int nr) {
+__device__ __forceinline__ void write_chunk(const SplitArgs& a, const UnitInfo& n,
+                                            const unsigned char* red, int red_step, const float2* ml,
+                                            int nr) {
   for (int idx = threadIdx.x; idx < nr * (D / 4); idx += NT) {
     const int r = idx / (D / 4), c4 = idx % (D / 4);
     const int row = n.r0 + r;
     if (row >= a.rows) continue;
-    const int head = n.hk * a.group + row / a.S, i = row % a.S;
+    int head, i;
+    row_of(a, row, head, i);
+    head += n.hk * a.group;
     float m = -INFINITY;
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) m = fmaxf(m, ml[w * MAXR + r].x);
@@ -281,7 +377,7 @@ __device__ __forceinline__ void write_chunk(const SplitArgs& a, const UnitInfo& 
     for (int w = 0; w < WARPS; ++w) {
       const float2 x = ml[w * MAXR + r];
       const float f = ex2((x.x - mu) * LOG2E);
-      const float4 v = *reinterpret_cast<const float4*>(red + (w * MAXR + r) * D + 4 * c4);
+      const float4 v = *reinterpret_cast<const float4*>(red + w * red_step + (r * D + 4 * c4) * 4);
       l = fmaf(x.y, f, l);
       o.x = fmaf(v.x, f, o.x);
       o.y = fmaf(v.y, f, o.y);
@@ -303,121 +399,120 @@ __device__ __forceinline__ void write_chunk(const SplitArgs& a, const UnitInfo& 
   }
 }
 
+// Keys per tile (8 KB of keys and values for 16-bit caches at D = 64, 128 and for fp32) and the ring of
+// a kernel.
 template <int D, int ES>
-__host__ __device__ constexpr int stages() {
-  // 24 KB a warp or so, at least two tiles in flight besides the one in use.
-  return D * ES >= 512 ? 3 : (D * ES >= 256 ? 3 : (D * ES >= 128 ? 4 : 6));
-}
-template <int D>
-__host__ __device__ constexpr int red_bytes() {
-  return WARPS * MAXR * D * 4;
+__host__ __device__ constexpr int tile_keys() {
+  return ES == 2 ? (D == 128 ? 16 : 32) : 1024 / D;  // (tile_log_of says the same to the host)
 }
 template <int D, int ES>
-__host__ __device__ constexpr int split_smem() {
-  const int ring = WARPS * Ring<D, ES, stages<D, ES>()>::BYTES;
-  return (ring > red_bytes<D>() ? ring : red_bytes<D>()) + WARPS * MAXR * 8 + MAXR * D * 4;
+using RingOf = Ring<D, ES, tile_keys<D, ES>(), (ES == 2 ? 3 : 2)>;
+// Shared memory: the rings -- whose last stage also takes a warp's sums when a unit ends -- the (m, l)
+// of the warps' rows, and the fp32 kernel's two sets of query rows.
+template <int D, int ES>
+__host__ __device__ constexpr int off_ml() {
+  static_assert(RingOf<D, ES>::STAGE >= MAXR * D * 4, "a stage holds a warp's sums");
+  return WARPS * RingOf<D, ES>::BYTES;
+}
+template <int D, int ES>
+__host__ __device__ constexpr int off_q() {
+  return off_ml<D, ES>() + WARPS * MAXR * 8;
+}
+template <int D, int ES>
+__host__ __device__ constexpr int split_smem(int q_rows) {
+  return off_q<D, ES>() + 2 * q_rows * D * 4;
 }
 
 // 16-bit caches.
 template <typename QT, typename T, int D>
-__global__ void __launch_bounds__(NT) split_mma_kernel(const SplitArgs a) {
-  constexpr int ST = stages<D, 2>();
-  using R = Ring<D, 2, ST>;
+__global__ void __launch_bounds__(NT, 2)
+    split_mma_kernel(const SplitArgs a) {
+  using R = RingOf<D, 2>;
+  constexpr int ST = R::ST, TK = R::TK, MT = TK / 16;
   constexpr bool F32 = std::is_same_v<QT, float>;
   constexpr bool HALF = std::is_same_v<T, __half>;
   constexpr int QP = F32 ? (HALF ? 2 : 3) : 1;  // parts of q
   constexpr int PP = F32 && !HALF ? 3 : 2;      // parts of p
   constexpr int KS = D / 16;
+  using QPair = std::conditional_t<F32, float2, uint32_t>;
   extern __shared__ __align__(128) unsigned char smem[];
   const int tid = threadIdx.x, w = tid >> 5, lane = tid & 31;
   const int qr = lane >> 2, qc = lane & 3;  // a fragment's row (key, dim; B: column) and pair
-  float* red = reinterpret_cast<float*>(smem);
-  float2* ml = reinterpret_cast<float2*>(smem + split_smem<D, 2>() - WARPS * MAXR * 8 - MAXR * D * 4);
+  unsigned char* red = smem + (ST - 1) * R::STAGE;
+  float2* ml = reinterpret_cast<float2*>(smem + off_ml<D, 2>());
   griddep_wait();
   griddep_launch_dependents();
   ChunkIndex ix;
   ix.init(a, lane);
-  const int64_t units = static_cast<int64_t>(ix.total) * a.Hk * a.row_chunks;
+  const uint32_t units = static_cast<uint32_t>(ix.total) * a.Hk * a.row_chunks;
   R ring(a, smem + w * R::BYTES, lane);
 
-  for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
-    const UnitInfo n = unit_info(a, ix, u);
-    ring.start(n.b, n.hk, n.hi);
-    const int tiles = (n.hi - n.lo + TK - 1) / TK;
-    unsigned live[ST];
-    int t_load = w, pg = tiles > w ? ring.page_of(n.lo + TK * w) : -1;
-    auto issue = [&](int stage) -> unsigned {
-      unsigned x = 0;
-      if (t_load < tiles) {
-        x = ring.load(n.lo + TK * t_load, stage, pg);
-        t_load += WARPS;
-        if (t_load < tiles) pg = ring.page_of(n.lo + TK * t_load);
-      }
-      cp_async_commit();
-      return x;
-    };
+  // Q^T's pairs of column qr: dims 16 ks + 2 qc, + 1 and + 8, + 9 (zeros where there is no row).
+  QPair qx[KS][2];
+  auto load_q = [&](const UnitInfo& n) {
+    const int row = n.r0 + qr;
+    int head, i;
+    row_of(a, row, head, i);
+    const bool ok = row < a.rows && i < n.n_new;
+    const QT* q = static_cast<const QT*>(a.q) + n.b * a.q_sb +
+                  (n.hk * a.group + (ok ? head : 0)) * a.q_sh + (ok ? i : 0) * a.q_ss;
 #pragma unroll
-    for (int s = 0; s < ST - 1; ++s) live[s] = issue(s);
-
-    // Q^T as B fragments: column qr, dims 16 ks + 2 qc, + 1 and + 8, + 9.
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        qx[ks][h] = ok ? *reinterpret_cast<const QPair*>(q + 16 * ks + 8 * h + 2 * qc) : QPair{};
+  };
+  UnitInfo n;
+  if (blockIdx.x < units) {
+    n = unit_info(a, ix, blockIdx.x);
+    ring.start(n.b, n.hk, n.lo, n.hi, w);
+    load_q(n);
+  }
+  for (uint32_t u = blockIdx.x; u < units; u += gridDim.x) {
+    const int tiles = ring.tiles;
+    // Q^T as B fragments.
     uint32_t qb[QP][KS][2];
     float qscale0 = a.scale, qscale1 = a.scale;  // of columns 2 qc, 2 qc + 1
-    {
-      const int row = n.r0 + qr;
-      const bool ok = row < a.rows && row % a.S < n.n_new;
-      const QT* q = static_cast<const QT*>(a.q) + n.b * a.q_sb +
-                    (n.hk * a.group + (ok ? row / a.S : 0)) * a.q_sh + (ok ? row % a.S : 0) * a.q_ss;
-      if constexpr (!F32) {
+    if constexpr (!F32) {
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
+      for (int ks = 0; ks < KS; ++ks) qb[0][ks][0] = qx[ks][0], qb[0][ks][1] = qx[ks][1];
+    } else if constexpr (HALF) {
+      // q = 2^e (h0 + 2^-11 h1), |h0| <= 2: what the two parts miss is below 2^-24 of q, or
+      // 2^-36 of the row's largest.
+      float top = 0.0f;
 #pragma unroll
-          for (int h = 0; h < 2; ++h)
-            qb[0][ks][h] = ok ? *reinterpret_cast<const uint32_t*>(q + 16 * ks + 8 * h + 2 * qc) : 0u;
-      } else {
-        float2 x[KS][2];
-        float top = 0.0f;
+      for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
+        for (int h = 0; h < 2; ++h) top = fmaxf(top, fmaxf(fabsf(qx[ks][h].x), fabsf(qx[ks][h].y)));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      int e = top > 0.0f && top < INFINITY ? ilogbf(top) : 0;
+      e = max(-120, min(120, e));
+      const float down = ldexpf(1.0f, -e), up = ldexpf(1.0f, e);
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            x[ks][h] = ok ? *reinterpret_cast<const float2*>(q + 16 * ks + 8 * h + 2 * qc)
-                          : make_float2(0.f, 0.f);
-            top = fmaxf(top, fmaxf(fabsf(x[ks][h].x), fabsf(x[ks][h].y)));
-          }
-        if constexpr (HALF) {
-          // q = 2^e (h0 + 2^-11 h1), |h0| <= 2: what the two parts miss is below 2^-24 of q, or
-          // 2^-36 of the row's largest.
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-          int e = top > 0.0f && top < INFINITY ? ilogbf(top) : 0;
-          e = max(-120, min(120, e));
-          const float down = ldexpf(1.0f, -e), up = ldexpf(1.0f, e);
+      for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-          for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const float lo = x[ks][h].x * down, hi = x[ks][h].y * down;
-              qb[0][ks][h] = pack16<T>(lo, hi);
-              const float2 z = unpack16<T>(qb[0][ks][h]);
-              qb[QP - 1][ks][h] = pack16<T>((lo - z.x) * 2048.0f, (hi - z.y) * 2048.0f);
-            }
-          qscale0 *= __shfl_sync(0xffffffffu, up, 8 * qc);
-          qscale1 *= __shfl_sync(0xffffffffu, up, 8 * qc + 4);
-        } else {
-#pragma unroll
-          for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              float2 y = x[ks][h];
-#pragma unroll
-              for (int p = 0; p < QP; ++p) {
-                qb[p][ks][h] = pack16<T>(y.x, y.y);
-                const float2 z = unpack16<T>(qb[p][ks][h]);
-                y = make_float2(y.x - z.x, y.y - z.y);
-              }
-            }
+        for (int h = 0; h < 2; ++h) {
+          const float lo = qx[ks][h].x * down, hi = qx[ks][h].y * down;
+          qb[0][ks][h] = pack16<T>(lo, hi);
+          const float2 z = unpack16<T>(qb[0][ks][h]);
+          qb[QP - 1][ks][h] = pack16<T>((lo - z.x) * 2048.0f, (hi - z.y) * 2048.0f);
         }
-      }
+      qscale0 *= __shfl_sync(0xffffffffu, up, 8 * qc);
+      qscale1 *= __shfl_sync(0xffffffffu, up, 8 * qc + 4);
+    } else {
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float2 y = qx[ks][h];
+#pragma unroll
+          for (int p = 0; p < QP; ++p) {
+            qb[p][ks][h] = pack16<T>(y.x, y.y);
+            const float2 z = unpack16<T>(qb[p][ks][h]);
+            y = make_float2(y.x - z.x, y.y - z.y);
+          }
+        }
     }
     const int lim0 = row_limit(a, n, n.r0 + 2 * qc), lim1 = row_limit(a, n, n.r0 + 2 * qc + 1);
     // The fewest keys that a row of the block sees: a tile that ends behind it masks row by row.
@@ -434,48 +529,60 @@ __global__ void __launch_bounds__(NT) split_mma_kernel(const SplitArgs a) {
     for (int t = w; t < tiles; t += WARPS) {
       cp_async_wait_group<ST - 2>();
       __syncwarp();  // the tile is in place for every lane, and the stage before it is free
-      unsigned now = live[0];
-#pragma unroll
-      for (int s = 0; s + 1 < ST - 1; ++s) live[s] = live[s + 1];
-      live[ST - 2] = issue(stage == 0 ? ST - 1 : stage - 1);
       const unsigned char* kt = ring.base + stage * R::STAGE;
       const unsigned char* vt = kt + R::KV;
       const int k0 = n.lo + TK * t;
 
-      float s[4] = {0.f, 0.f, 0.f, 0.f};
-      if constexpr (F32) {  // the small parts first: their sums truncate at their own magnitude
-        float c[4] = {0.f, 0.f, 0.f, 0.f};
+      // Scores: s[i][0], [1]: key 16 i + qr, columns 2 qc, + 1; s[i][2], [3]: key 16 i + qr + 8.
+      float s[MT][4];
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-          uint32_t ka[4];
-          ldsm4(ka, kt + (lane & 15) * R::RB + 32 * ks + 16 * (lane >> 4));
+      for (int i = 0; i < MT; ++i) {
+        const unsigned char* ka_at = kt + (16 * i + (lane & 15)) * R::RB + 16 * (lane >> 4);
+        float c[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+        if constexpr (F32) {  // the small parts in a chain of their own, truncated at their magnitude
 #pragma unroll
-          for (int p = QP - 1; p > 0; --p) mma<T>(c, ka, qb[p][ks][0], qb[p][ks][1]);
+          for (int ks = 0; ks < KS; ++ks) {
+            uint32_t ka[4];
+            ldsm4(ka, ka_at + 32 * ks);
+#pragma unroll
+            for (int p = QP - 1; p > 0; --p) mma<T>(c[1], ka, qb[p][ks][0], qb[p][ks][1]);
+            mma<T>(c[0], ka, qb[0][ks][0], qb[0][ks][1]);
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            s[i][j] = (HALF ? fmaf(c[1][j], 1.0f / 2048.0f, c[0][j]) : c[1][j] + c[0][j]) *
+                      (j & 1 ? qscale1 : qscale0);
+        } else {  // two chains, half as long
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks) {
+            uint32_t ka[4];
+            ldsm4(ka, ka_at + 32 * ks);
+            mma<T>(c[ks & 1], ka, qb[0][ks][0], qb[0][ks][1]);
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) s[i][j] = (c[0][j] + c[1][j]) * (j & 1 ? qscale1 : qscale0);
         }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) s[j] = HALF ? c[j] * (1.0f / 2048.0f) : c[j];
       }
-      {
-        float c[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-          uint32_t ka[4];
-          ldsm4(ka, kt + (lane & 15) * R::RB + 32 * ks + 16 * (lane >> 4));
-          mma<T>(c, ka, qb[0][ks][0], qb[0][ks][1]);
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) s[j] = (s[j] + c[j]) * (j & 1 ? qscale1 : qscale0);
-      }
-      // s[0], s[1]: key qr, columns 2 qc, + 1; s[2], s[3]: key qr + 8.
+      // (behind the products: their latency hides the next loads' issue)
+      const unsigned now = ring.advance(stage == 0 ? ST - 1 : stage - 1);
       const bool edge = lim_min < min(k0 + TK, n.hi);
-      if (now != 0xffffu || edge) {
-        const bool ka = (now >> qr) & 1u, kb = (now >> (qr + 8)) & 1u;
-        if (!ka || k0 + qr >= lim0) s[0] = -INFINITY;
-        if (!ka || k0 + qr >= lim1) s[1] = -INFINITY;
-        if (!kb || k0 + qr + 8 >= lim0) s[2] = -INFINITY;
-        if (!kb || k0 + qr + 8 >= lim1) s[3] = -INFINITY;
+      if (now != R::ALL || edge) {
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          const int ka = 16 * i + qr, kb = ka + 8;
+          const bool la = (now >> ka) & 1u, lb = (now >> kb) & 1u;
+          if (!la || k0 + ka >= lim0) s[i][0] = -INFINITY;
+          if (!la || k0 + ka >= lim1) s[i][1] = -INFINITY;
+          if (!lb || k0 + kb >= lim0) s[i][2] = -INFINITY;
+          if (!lb || k0 + kb >= lim1) s[i][3] = -INFINITY;
+        }
       }
-      float t0 = fmaxf(s[0], s[2]), t1 = fmaxf(s[1], s[3]);
+      float t0 = fmaxf(s[0][0], s[0][2]), t1 = fmaxf(s[0][1], s[0][3]);
+#pragma unroll
+      for (int i = 1; i < MT; ++i) {
+        t0 = fmaxf(t0, fmaxf(s[i][0], s[i][2]));
+        t1 = fmaxf(t1, fmaxf(s[i][1], s[i][3]));
+      }
 #pragma unroll
       for (int o = 4; o < 32; o <<= 1) {
         t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, o));
@@ -487,34 +594,42 @@ __global__ void __launch_bounds__(NT) split_mma_kernel(const SplitArgs a) {
       const float a0 = ex2((m0 - u0) * LOG2E), a1 = ex2((m1 - u1) * LOG2E);
       m0 = t0;
       m1 = t1;
-      s[0] = ex2((s[0] - u0) * LOG2E);
-      s[1] = ex2((s[1] - u1) * LOG2E);
-      s[2] = ex2((s[2] - u0) * LOG2E);
-      s[3] = ex2((s[3] - u1) * LOG2E);
-      l0 = fmaf(l0, a0, s[0] + s[2]);
-      l1 = fmaf(l1, a1, s[1] + s[3]);
       // P^T as B fragments (transposed 8 x 8 blocks), in parts.
-      uint32_t pb[PP][2];
-      float2 x = make_float2(s[0], s[1]), y = make_float2(s[2], s[3]);
+      uint32_t pb[MT][PP][2];
+      float ps0 = 0.0f, ps1 = 0.0f;
 #pragma unroll
-      for (int p = 0; p < PP; ++p) {
-        const uint32_t hx = pack16<T>(x.x, x.y), hy = pack16<T>(y.x, y.y);
-        const float2 zx = unpack16<T>(hx), zy = unpack16<T>(hy);
-        x = make_float2(x.x - zx.x, x.y - zx.y);
-        y = make_float2(y.x - zy.x, y.y - zy.y);
-        pb[p][0] = transpose8(hx);
-        pb[p][1] = transpose8(hy);
+      for (int i = 0; i < MT; ++i) {
+        float2 x = make_float2(ex2((s[i][0] - u0) * LOG2E), ex2((s[i][1] - u1) * LOG2E));
+        float2 y = make_float2(ex2((s[i][2] - u0) * LOG2E), ex2((s[i][3] - u1) * LOG2E));
+        ps0 += x.x + y.x;
+        ps1 += x.y + y.y;
+#pragma unroll
+        for (int p = 0; p < PP; ++p) {
+          const uint32_t hx = pack16<T>(x.x, x.y), hy = pack16<T>(y.x, y.y);
+          if (p + 1 < PP) {
+            const float2 zx = unpack16<T>(hx), zy = unpack16<T>(hy);
+            x = make_float2(x.x - zx.x, x.y - zx.y);
+            y = make_float2(y.x - zy.x, y.y - zy.y);
+          }
+          pb[i][p][0] = transpose8(hx);
+          pb[i][p][1] = transpose8(hy);
+        }
       }
+      l0 = fmaf(l0, a0, ps0);
+      l1 = fmaf(l1, a1, ps1);
       // The V^T block of dims 16 mt ..: rows (keys) (lane % 8) + 8 (lane / 16), dims + 8 (lane / 8 % 2).
       const unsigned char* va_at = vt + ((lane & 7) + 8 * (lane >> 4)) * R::RB + 16 * ((lane >> 3) & 1);
       if (!edge) {
 #pragma unroll
         for (int mt = 0; mt < KS; ++mt) {
-          uint32_t va[4];
-          ldsm4t(va, va_at + 32 * mt);
           float c[4] = {0.f, 0.f, 0.f, 0.f};
+          uint32_t va[MT][4];
 #pragma unroll
-          for (int p = PP - 1; p >= 0; --p) mma<T>(c, va, pb[p][0], pb[p][1]);
+          for (int i = 0; i < MT; ++i) ldsm4t(va[i], va_at + 16 * i * R::RB + 32 * mt);
+#pragma unroll
+          for (int p = PP - 1; p >= 0; --p)
+#pragma unroll
+            for (int i = 0; i < MT; ++i) mma<T>(c, va[i], pb[i][p][0], pb[i][p][1]);
 #pragma unroll
           for (int j = 0; j < 4; ++j) acc[mt][j] = fmaf(acc[mt][j], j & 1 ? a1 : a0, c[j]);
         }
@@ -527,98 +642,104 @@ __global__ void __launch_bounds__(NT) split_mma_kernel(const SplitArgs a) {
           for (int j = 0; j < 4; ++j) acc[mt][j] *= j & 1 ? a1 : a0;
         for (int r = 0; r < min(MAXR, a.rows - n.r0); ++r) {
           const int lim = row_limit(a, n, n.r0 + r);
-          const int k = k0 + 2 * qc;  // this lane's keys of an A fragment: k, k + 1, k + 8, k + 9
-          const uint32_t mlo = (k < lim ? 0xffffu : 0u) | (k + 1 < lim ? 0xffff0000u : 0u);
-          const uint32_t mhi = (k + 8 < lim ? 0xffffu : 0u) | (k + 9 < lim ? 0xffff0000u : 0u);
 #pragma unroll
-          for (int mt = 0; mt < KS; ++mt) {
-            uint32_t va[4];
-            ldsm4t(va, va_at + 32 * mt);
-            va[0] &= mlo;
-            va[1] &= mlo;
-            va[2] &= mhi;
-            va[3] &= mhi;
-            float c[4] = {0.f, 0.f, 0.f, 0.f};
+          for (int i = 0; i < MT; ++i) {
+            const int k = k0 + 16 * i + 2 * qc;  // this lane's keys of an A fragment: k, + 1, + 8, + 9
+            const uint32_t mlo = (k < lim ? 0xffffu : 0u) | (k + 1 < lim ? 0xffff0000u : 0u);
+            const uint32_t mhi = (k + 8 < lim ? 0xffffu : 0u) | (k + 9 < lim ? 0xffff0000u : 0u);
 #pragma unroll
-            for (int p = PP - 1; p >= 0; --p)
-              mma<T>(c, va, qr == r ? pb[p][0] : 0u, qr == r ? pb[p][1] : 0u);
+            for (int mt = 0; mt < KS; ++mt) {
+              uint32_t va[4];
+              ldsm4t(va, va_at + 16 * i * R::RB + 32 * mt);
+              va[0] &= mlo;
+              va[1] &= mlo;
+              va[2] &= mhi;
+              va[3] &= mhi;
+              float c[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-              if (2 * qc + (j & 1) == r) acc[mt][j] += c[j];
+              for (int p = PP - 1; p >= 0; --p)
+                mma<T>(c, va, qr == r ? pb[i][p][0] : 0u, qr == r ? pb[i][p][1] : 0u);
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                if (2 * qc + (j & 1) == r) acc[mt][j] += c[j];
+            }
           }
         }
       }
       stage = stage + 1 == ST ? 0 : stage + 1;
     }
-    cp_async_wait_group<0>();
 #pragma unroll
     for (int o = 4; o < 32; o <<= 1) {
       l0 += __shfl_xor_sync(0xffffffffu, l0, o);
       l1 += __shfl_xor_sync(0xffffffffu, l1, o);
     }
-    __syncthreads();  // every warp's tiles are read: their space takes the sums
+    // The next unit's first tiles and queries travel while this one's sums are joined.
+    const UnitInfo done = n;
+    __syncwarp();  // every lane has read its last tile
+    if (u + gridDim.x < units) {
+      n = unit_info(a, ix, u + gridDim.x);
+      ring.start(n.b, n.hk, n.lo, n.hi, w);
+      load_q(n);
+    }
     if (qr == 0) {
       ml[w * MAXR + 2 * qc] = make_float2(m0, l0);
       ml[w * MAXR + 2 * qc + 1] = make_float2(m1, l1);
     }
+    float* sums = reinterpret_cast<float*>(red + w * R::BYTES);  // (this warp's last stage: free)
 #pragma unroll
     for (int mt = 0; mt < KS; ++mt)
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        red[(w * MAXR + 2 * qc + (j & 1)) * D + 16 * mt + qr + 8 * (j >> 1)] = acc[mt][j];
+        sums[(2 * qc + (j & 1)) * D + 16 * mt + qr + 8 * (j >> 1)] = acc[mt][j];
     __syncthreads();
-    write_chunk<QT, D>(a, n, red, ml, MAXR);
-    __syncthreads();  // the sums are read: the next unit's tiles may land
+    write_chunk<QT, D>(a, done, red, R::BYTES, ml, min(MAXR, a.rows - done.r0));
+    __syncthreads();  // the sums are read: the last stages take tiles again
   }
   if (ring.bad) flag_error(a.sink, CFA_ERR_PAGE);
 }
 
 // fp32 caches: NR query rows (1, 2, 4 or 8).
 template <int D, int NR>
-__global__ void __launch_bounds__(NT) split_f32_kernel(const SplitArgs a) {
-  constexpr int ST = stages<D, 4>();
-  using R = Ring<D, 4, ST>;
+__global__ void __launch_bounds__(NT, 3) split_f32_kernel(const SplitArgs a) {
+  using R = RingOf<D, 4>;
+  constexpr int ST = R::ST, TK = R::TK;
+  constexpr int LPK = 32 / TK, DL = D / LPK;  // lanes of a key's score, dims of each
   constexpr int LPR = D / 4, KPI = 32 / LPR;  // lanes of a V row; keys at a time
   extern __shared__ __align__(128) unsigned char smem[];
   const int tid = threadIdx.x, w = tid >> 5, lane = tid & 31;
-  float* red = reinterpret_cast<float*>(smem);
-  float2* ml = reinterpret_cast<float2*>(smem + split_smem<D, 4>() - WARPS * MAXR * 8 - MAXR * D * 4);
-  float* qs = reinterpret_cast<float*>(smem + split_smem<D, 4>() - MAXR * D * 4);  // [NR][D]
+  unsigned char* red = smem + (ST - 1) * R::STAGE;
+  float2* ml = reinterpret_cast<float2*>(smem + off_ml<D, 4>());
+  float* q_sets = reinterpret_cast<float*>(smem + off_q<D, 4>());  // two sets of [NR][D]
   griddep_wait();
   griddep_launch_dependents();
   ChunkIndex ix;
   ix.init(a, lane);
-  const int64_t units = static_cast<int64_t>(ix.total) * a.Hk * a.row_chunks;
+  const uint32_t units = static_cast<uint32_t>(ix.total) * a.Hk * a.row_chunks;
   R ring(a, smem + w * R::BYTES, lane);
 
-  for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
-    const UnitInfo n = unit_info(a, ix, u);
-    ring.start(n.b, n.hk, n.hi);
-    const int tiles = (n.hi - n.lo + TK - 1) / TK;
-    unsigned live[ST];
-    int t_load = w, pg = tiles > w ? ring.page_of(n.lo + TK * w) : -1;
-    auto issue = [&](int stage) -> unsigned {
-      unsigned x = 0;
-      if (t_load < tiles) {
-        x = ring.load(n.lo + TK * t_load, stage, pg);
-        t_load += WARPS;
-        if (t_load < tiles) pg = ring.page_of(n.lo + TK * t_load);
-      }
-      cp_async_commit();
-      return x;
-    };
-#pragma unroll
-    for (int s = 0; s < ST - 1; ++s) live[s] = issue(s);
+  auto load_q = [&](const UnitInfo& n, float* qs) {
     for (int i = tid; i < NR * LPR; i += NT) {
       const int row = n.r0 + i / LPR, c = i % LPR;
+      int head, t;
+      row_of(a, row, head, t);
       float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (row < a.rows && row % a.S < n.n_new)
+      if (row < a.rows && t < n.n_new)
         x = *reinterpret_cast<const float4*>(static_cast<const float*>(a.q) + n.b * a.q_sb +
-                                             (n.hk * a.group + row / a.S) * a.q_sh +
-                                             (row % a.S) * a.q_ss + 4 * c);
+                                             (n.hk * a.group + head) * a.q_sh + t * a.q_ss + 4 * c);
       reinterpret_cast<float4*>(qs)[i] = x;
     }
+  };
+  UnitInfo n;
+  if (blockIdx.x < units) {
+    n = unit_info(a, ix, blockIdx.x);
+    ring.start(n.b, n.hk, n.lo, n.hi, w);
+    load_q(n, q_sets);
     __syncthreads();  // q in place
+  }
+  int set = 0;
+  for (uint32_t u = blockIdx.x; u < units; u += gridDim.x, set ^= 1) {
+    const float* qs = q_sets + set * (NR * D);
+    const int tiles = ring.tiles;
     const int lim_min = a.causal ? max(n.len - n.n_new + 1, 0) : n.len;
     float m[NR], l[NR], acc[NR][4];
 #pragma unroll
@@ -630,43 +751,43 @@ __global__ void __launch_bounds__(NT) split_f32_kernel(const SplitArgs a) {
     for (int t = w; t < tiles; t += WARPS) {
       cp_async_wait_group<ST - 2>();
       __syncwarp();
-      const unsigned now = live[0];
-#pragma unroll
-      for (int s = 0; s + 1 < ST - 1; ++s) live[s] = live[s + 1];
-      live[ST - 2] = issue(stage == 0 ? ST - 1 : stage - 1);
+      const unsigned now = ring.advance(stage == 0 ? ST - 1 : stage - 1);
       const unsigned char* kt = ring.base + stage * R::STAGE;
       const unsigned char* vt = kt + R::KV;
       const int k0 = n.lo + TK * t;
       const bool edge = lim_min < min(k0 + TK, n.hi);
-      // Scores: lanes 0-15 take the first half of their key's dims, lanes 16-31 the second.
+      // Scores: lane x takes dims DL (x / TK) .. of key x % TK.
       float s[NR];
 #pragma unroll
       for (int r = 0; r < NR; ++r) s[r] = 0.0f;
-      const float* kr = reinterpret_cast<const float*>(kt + (lane & 15) * R::RB) + (lane >> 4) * (D / 2);
-      const float* qh = qs + (lane >> 4) * (D / 2);
+      const float* kr = reinterpret_cast<const float*>(kt + (lane % TK) * R::RB) + lane / TK * DL;
+      const float* qh = qs + lane / TK * DL;
 #pragma unroll
-      for (int c = 0; c < D / 8; ++c) {
+      for (int c = 0; c < DL / 4; ++c) {
         const float4 x = reinterpret_cast<const float4*>(kr)[c];
 #pragma unroll
         for (int r = 0; r < NR; ++r) s[r] = dot4(x, ld4(qh + r * D + 4 * c), s[r]);
       }
-      float p[NR], al[NR];
+      float p[NR];
 #pragma unroll
       for (int r = 0; r < NR; ++r) {
-        float y = (s[r] + __shfl_xor_sync(0xffffffffu, s[r], 16)) * a.scale;
-        const int key = k0 + (lane & 15);
-        if (!((now >> (lane & 15)) & 1u) || (edge && key >= row_limit(a, n, n.r0 + r))) y = -INFINITY;
+        float y = s[r];
+#pragma unroll
+        for (int o = TK; o < 32; o <<= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
+        y *= a.scale;
+        const int key = lane % TK;
+        if (!((now >> key) & 1u) || (edge && k0 + key >= row_limit(a, n, n.r0 + r))) y = -INFINITY;
         float top = y;
 #pragma unroll
-        for (int o = 1; o < 16; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        for (int o = 1; o < TK; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
         top = fmaxf(top, m[r]);
         const float mu = top == -INFINITY ? 0.0f : top;
-        al[r] = ex2((m[r] - mu) * LOG2E);
+        const float al = ex2((m[r] - mu) * LOG2E);
         m[r] = top;
         p[r] = ex2((y - mu) * LOG2E);
-        l[r] = fmaf(l[r], al[r], p[r]);  // this lane's keys (both halves hold the same)
+        l[r] = fmaf(l[r], al, p[r]);  // this lane's keys (the lanes of a key hold the same)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) acc[r][c] *= al[r];
+        for (int c = 0; c < 4; ++c) acc[r][c] *= al;
       }
 #pragma unroll
       for (int j = 0; j < TK / KPI; ++j) {
@@ -685,27 +806,34 @@ __global__ void __launch_bounds__(NT) split_f32_kernel(const SplitArgs a) {
       }
       stage = stage + 1 == ST ? 0 : stage + 1;
     }
-    cp_async_wait_group<0>();
 #pragma unroll
     for (int r = 0; r < NR; ++r) {
 #pragma unroll
-      for (int o = 1; o < 16; o <<= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], o);
+      for (int o = 1; o < TK; o <<= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], o);
 #pragma unroll
       for (int o = LPR; o < 32; o <<= 1)
 #pragma unroll
         for (int c = 0; c < 4; ++c) acc[r][c] += __shfl_xor_sync(0xffffffffu, acc[r][c], o);
     }
-    __syncthreads();
+    // The next unit's first tiles and queries travel while this one's sums are joined.
+    const UnitInfo done = n;
+    __syncwarp();  // every lane has read its last tile
+    if (u + gridDim.x < units) {
+      n = unit_info(a, ix, u + gridDim.x);
+      ring.start(n.b, n.hk, n.lo, n.hi, w);
+      load_q(n, q_sets + (set ^ 1) * (NR * D));
+    }
+    float* sums = reinterpret_cast<float*>(red + w * R::BYTES);  // (this warp's last stage: free)
 #pragma unroll
     for (int r = 0; r < NR; ++r) {
       if (lane == 0) ml[w * MAXR + r] = make_float2(m[r], l[r]);
       if (lane < LPR)
-        *reinterpret_cast<float4*>(red + (w * MAXR + r) * D + 4 * lane) =
+        *reinterpret_cast<float4*>(sums + r * D + 4 * lane) =
             make_float4(acc[r][0], acc[r][1], acc[r][2], acc[r][3]);
     }
-    __syncthreads();
-    write_chunk<float, D>(a, n, red, ml, NR);
-    __syncthreads();
+    __syncthreads();  // (the next unit's queries are in place too)
+    write_chunk<float, D>(a, done, red, R::BYTES, ml, min(NR, a.rows - done.r0));
+    __syncthreads();  // the sums are read: the last stages take tiles again
   }
   if (ring.bad) flag_error(a.sink, CFA_ERR_PAGE);
 }
@@ -725,7 +853,7 @@ __global__ void __launch_bounds__(NT) split_join_kernel(const SplitArgs a) {
   const int i = static_cast<int>(row % a.S);
   const int64_t bh = row / a.S;
   const int b = static_cast<int>(bh / a.H), head = static_cast<int>(bh % a.H);
-  const int nc = chunks_of(seq_len(a, b));
+  const int nc = chunks_of(seq_len(a, b), a.tile_log);
   if (nc == 1) return;  // written by the first kernel
   const bool live = i < seq_new(a, b);
   const float2* ml = a.part_ml + row * a.max_chunks;
@@ -788,22 +916,23 @@ __global__ void __launch_bounds__(NT) split_join_kernel(const SplitArgs a) {
   }
 }
 
-// Resident blocks: the grid is persistent, as many as fit at once (or as there are units at most).
-template <typename F>
-int resident(F* kernel, int smem) {
-  int dev = 0, sms = 0, per = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess ||
-      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess ||
-      cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kernel, NT, smem) != cudaSuccess)
-    return 148;
-  return sms * (per > 0 ? per : 1);
-}
-
-template <typename F>
-cudaError_t launch_split(F* kernel, int smem, const SplitArgs& a, cudaStream_t stream) {
+// A persistent grid: as many blocks as fit at once, or as there are units at most. The occupancy of a
+// kernel is asked for once (every device here is an sm_100a).
+template <auto Kernel>
+cudaError_t launch_split(int smem, const SplitArgs& a, cudaStream_t stream) {
+  static std::atomic<int> kept{0};
+  int dev = 0, sms = 0, per = kept.load(std::memory_order_relaxed);
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  if (e == cudaSuccess && per == 0) {
+    e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, Kernel, NT, smem);
+    if (e == cudaSuccess && per == 0) e = cudaErrorInvalidConfiguration;
+    kept.store(per, std::memory_order_relaxed);
+  }
+  if (e != cudaSuccess) return e;
   const int64_t units = static_cast<int64_t>(a.B) * a.max_chunks * a.Hk * a.row_chunks;
-  const int64_t fit = resident(kernel, smem);
-  return launch_pdl(kernel, dim3(static_cast<unsigned>(units < fit ? units : fit)), dim3(NT), smem,
+  const int64_t fit = static_cast<int64_t>(sms) * per;
+  return launch_pdl(Kernel, dim3(static_cast<unsigned>(units < fit ? units : fit)), dim3(NT), smem,
                     stream, a);
 }
 
@@ -817,25 +946,25 @@ cudaError_t launch_join(const SplitArgs& a, cudaStream_t stream) {
 template <int D>
 cudaError_t launch_d(const SplitArgs& a, int qd, int kd, cudaStream_t stream) {
   cudaError_t e;
-  constexpr int S2 = split_smem<D, 2>(), S4 = split_smem<D, 4>();
+  constexpr int S2 = split_smem<D, 2>(0);
   if (qd == CFA_F32) {
     if (kd == CFA_F32) {
-      e = a.rows == 1   ? launch_split(split_f32_kernel<D, 1>, S4, a, stream)
-          : a.rows == 2 ? launch_split(split_f32_kernel<D, 2>, S4, a, stream)
-          : a.rows <= 4 ? launch_split(split_f32_kernel<D, 4>, S4, a, stream)
-                        : launch_split(split_f32_kernel<D, 8>, S4, a, stream);
+      e = a.rows == 1   ? launch_split<split_f32_kernel<D, 1>>(split_smem<D, 4>(1), a, stream)
+          : a.rows == 2 ? launch_split<split_f32_kernel<D, 2>>(split_smem<D, 4>(2), a, stream)
+          : a.rows <= 4 ? launch_split<split_f32_kernel<D, 4>>(split_smem<D, 4>(4), a, stream)
+                        : launch_split<split_f32_kernel<D, 8>>(split_smem<D, 4>(8), a, stream);
     } else if (kd == CFA_F16) {
-      e = launch_split(split_mma_kernel<float, __half, D>, S2, a, stream);
+      e = launch_split<split_mma_kernel<float, __half, D>>(S2, a, stream);
     } else {
-      e = launch_split(split_mma_kernel<float, __nv_bfloat16, D>, S2, a, stream);
+      e = launch_split<split_mma_kernel<float, __nv_bfloat16, D>>(S2, a, stream);
     }
     return e == cudaSuccess ? launch_join<float, D>(a, stream) : e;
   }
   if (qd == CFA_F16) {
-    e = launch_split(split_mma_kernel<__half, __half, D>, S2, a, stream);
+    e = launch_split<split_mma_kernel<__half, __half, D>>(S2, a, stream);
     return e == cudaSuccess ? launch_join<__half, D>(a, stream) : e;
   }
-  e = launch_split(split_mma_kernel<__nv_bfloat16, __nv_bfloat16, D>, S2, a, stream);
+  e = launch_split<split_mma_kernel<__nv_bfloat16, __nv_bfloat16, D>>(S2, a, stream);
   return e == cudaSuccess ? launch_join<__nv_bfloat16, D>(a, stream) : e;
 }
 
@@ -845,12 +974,12 @@ cudaError_t set_attrs() {
   auto set = [&](const void* fn, int bytes) {
     if (e == cudaSuccess) e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   };
-  constexpr int S2 = split_smem<D, 2>(), S4 = split_smem<D, 4>();
-  static_assert(S2 <= 232448 && S4 <= 232448, "shared memory per block");
-  set(reinterpret_cast<const void*>(split_f32_kernel<D, 1>), S4);
-  set(reinterpret_cast<const void*>(split_f32_kernel<D, 2>), S4);
-  set(reinterpret_cast<const void*>(split_f32_kernel<D, 4>), S4);
-  set(reinterpret_cast<const void*>(split_f32_kernel<D, 8>), S4);
+  constexpr int S2 = split_smem<D, 2>(0);
+  static_assert(S2 <= 232448 && split_smem<D, 4>(MAXR) <= 232448, "shared memory per block");
+  set(reinterpret_cast<const void*>(split_f32_kernel<D, 1>), split_smem<D, 4>(1));
+  set(reinterpret_cast<const void*>(split_f32_kernel<D, 2>), split_smem<D, 4>(2));
+  set(reinterpret_cast<const void*>(split_f32_kernel<D, 4>), split_smem<D, 4>(4));
+  set(reinterpret_cast<const void*>(split_f32_kernel<D, 8>), split_smem<D, 4>(8));
   set(reinterpret_cast<const void*>(split_mma_kernel<float, __half, D>), S2);
   set(reinterpret_cast<const void*>(split_mma_kernel<float, __nv_bfloat16, D>), S2);
   set(reinterpret_cast<const void*>(split_mma_kernel<__half, __half, D>), S2);
@@ -866,18 +995,24 @@ cudaError_t setup_split_attributes() {
   return e == cudaSuccess ? set_attrs<128>() : e;
 }
 
-// Most chunks of a sequence of at most max_len keys.
-int split_max_chunks(int64_t max_len) {
-  if (max_len <= CHUNK_MIN) return 1;
-  int64_t n = (max_len + CHUNK_MAX - 1) / CHUNK_MAX;
-  if (n < FEW_CHUNKS) n = FEW_CHUNKS;
-  if (n > MOST_CHUNKS) n = MOST_CHUNKS;
-  const int64_t few = (max_len + CHUNK_MIN - 1) / CHUNK_MIN;
-  return static_cast<int>(n < few ? n : few);
+// log2 of tile_keys.
+static int tile_log_of(int64_t head_dim, int kv_dtype) {
+  if (kv_dtype == CFA_F32) return head_dim == 32 ? 5 : head_dim == 64 ? 4 : 3;
+  return head_dim == 128 ? 4 : 5;
 }
 
-size_t split_workspace_bytes(int64_t rows, int64_t max_len, int64_t head_dim) {
-  const int64_t n = split_max_chunks(max_len);
+// Most chunks of a sequence of at most max_len keys: its own, or 16 of a shorter one whose chunks are
+// half as long.
+int split_max_chunks(int64_t max_len, int64_t head_dim, int kv_dtype) {
+  const int t = tile_log_of(head_dim, kv_dtype), len = static_cast<int>(max_len);
+  const int own = chunks_of(len, t), few = 1 << (t + 4 + FEW_CHUNKS_LOG);
+  const int most = len > few && own < (1 << FEW_CHUNKS_LOG) ? 1 << FEW_CHUNKS_LOG : own;
+  // (past 256 chunks the count falls back to 129 at the next power of two)
+  return bits_of(static_cast<uint32_t>(len > 0 ? len - 1 : 0)) - MOST_CHUNKS_LOG > t + 5 ? MOST_CHUNKS : most;
+}
+
+size_t split_workspace_bytes(int64_t rows, int64_t max_len, int64_t head_dim, int kv_dtype) {
+  const int64_t n = split_max_chunks(max_len, head_dim, kv_dtype);
   if (n == 1) return 0;
   return static_cast<size_t>(rows * n) * (head_dim + 2) * sizeof(float);
 }
@@ -888,7 +1023,14 @@ cudaError_t launch_split_attention(const SplitArgs& args, int q_dtype, int kv_dt
   a.group = a.H / a.Hk;
   a.rows = a.group * a.S;
   a.row_chunks = (a.rows + MAXR - 1) / MAXR;
-  a.max_chunks = split_max_chunks(a.max_len);
+  a.max_chunks = split_max_chunks(a.max_len, a.D, kv_dtype);
+  a.tile_log = tile_log_of(a.D, kv_dtype);
+  // key / page for key < 2^31: key mul >> shift, mul = ceil(2^shift / page), 2^shift >= 2^31 page.
+  if (!a.table) a.page = 1;
+  a.page_shift = 31;
+  while ((int64_t(1) << (a.page_shift - 31)) < a.page) ++a.page_shift;
+  a.page_mul = static_cast<uint32_t>(((uint64_t(1) << a.page_shift) + a.page - 1) / a.page);
+  a.one_page = !a.table || a.page % (1 << a.tile_log) == 0;
   a.part_o = static_cast<float*>(workspace);
   a.part_ml = a.max_chunks == 1
                   ? nullptr

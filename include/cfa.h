@@ -369,7 +369,7 @@ int cfa_paged_append(const void* q, const int64_t q_strides[3], void* q_out,
  * (CFA_ERR_PAGE), and so is a length past the table. Workspace (256-byte aligned, no initialisation)
  * for max_keys = table_width * page_size. */
 size_t cfa_paged_attention_workspace_bytes(int64_t batch, int64_t heads, int64_t seq,
-                                           int64_t max_keys, int64_t head_dim);
+                                           int64_t max_keys, int64_t head_dim, int cache_dtype);
 int cfa_paged_attention(const void* q, const int64_t q_strides[3], int dtype, const void* k_cache,
                         const int64_t k_cache_strides[3], const void* v_cache,
                         const int64_t v_cache_strides[3], int cache_dtype, int64_t pages,

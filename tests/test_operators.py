@@ -74,8 +74,8 @@ def test_cross_backward_workspace():
 def test_few_rows_arguments():
     dims = (2, 4, 2, 1, 900, 64)
     need = _abi.cross_few_workspace_bytes(2, 4, 1, 900, 64)
-    assert need == 2 * 4 * 15 * 66 * 4
-    assert _abi.cross_few_workspace_bytes(2, 4, 1, 64, 64) == 0  # one chunk: nothing to join
+    assert need == 2 * 4 * 4 * 66 * 4  # four chunks of 256
+    assert _abi.cross_few_workspace_bytes(2, 4, 1, 256, 64) == 0  # one chunk: nothing to join
 
     def call(q=FAKE, ws=FAKE, nbytes=need, dims=dims):
         return _abi.cross_few(q, S3, FAKE, S3, FAKE, S3, None, FAKE, ws, nbytes, *dims, 0.1, None)
@@ -123,10 +123,10 @@ def test_append_arguments():
 
 
 def test_paged_attention_arguments():
-    need = _abi.paged_attention_workspace_bytes(2, 4, 1, 3 * 64, 64)
-    assert need == 2 * 4 * 3 * 66 * 4
+    need = _abi.paged_attention_workspace_bytes(2, 4, 1, 3 * 640, 64, _abi.CFA_BF16)
+    assert need == 2 * 4 * 4 * 66 * 4  # four chunks of 512
 
-    def call(q=FAKE, types=(_abi.CFA_F32, _abi.CFA_BF16), cache=FAKE, page=64, width=3, table=FAKE,
+    def call(q=FAKE, types=(_abi.CFA_F32, _abi.CFA_BF16), cache=FAKE, page=640, width=3, table=FAKE,
              lengths=FAKE, ws=FAKE, nbytes=need, dims=(2, 4, 2, 1, 64), st=S3):
         return _abi.paged_attention(q, S3, types[0], cache, st, cache, st, types[1], 9, page, table,
                                     width, width, lengths, None, FAKE, ws, nbytes, *dims, 0.1, None)
@@ -152,23 +152,28 @@ def test_statuses_have_words():
 
 # --- the chunks of a sequence, as csrc/split_attn.cu cuts them ---------------------------------------
 
-def chunk(n):
-    c = 64
-    while c < 512 and n > 16 * c:
-        c *= 2
+def chunk(n, tile):
+    """16 tiles up to 16 chunks, 32 up to 256, then powers of two that keep them 256."""
+    if n <= 256 * tile:
+        return 16 * tile
+    c = 32 * tile
     while n > 256 * c:
         c *= 2
     return c
 
 
-def test_workspace_holds_every_length_below_its_largest():
+@pytest.mark.parametrize("d,kv,tile", [(32, _abi.CFA_F32, 32), (64, _abi.CFA_F32, 16),
+                                       (128, _abi.CFA_F32, 8), (32, _abi.CFA_F16, 32),
+                                       (64, _abi.CFA_BF16, 32), (128, _abi.CFA_F16, 16)])
+def test_workspace_holds_every_length_below_its_largest(d, kv, tile):
     """The workspace is sized for the longest sequence; a shorter one can have more chunks than it
     (its chunks are smaller) and must fit all the same."""
     most, r = 0, random.Random(1)
-    lengths = sorted({*range(1, 9000), *(r.randint(9000, 2_000_000) for _ in range(3000))})
+    lengths = sorted({*range(1, 9000), *(r.randint(9000, 4_000_000) for _ in range(3000)),
+                      *(x + y for x in (1 << k for k in range(8, 31)) for y in (-1, 0, 1))})
     for n in lengths:
-        most = max(most, -(-n // chunk(n)))
-        got = _abi.paged_attention_workspace_bytes(1, 1, 1, n, 32) // (34 * 4) or 1
+        most = max(most, -(-n // chunk(n, tile)))
+        got = _abi.paged_attention_workspace_bytes(1, 1, 1, n, d, kv) // ((d + 2) * 4) or 1
         assert got >= most, n
     assert most <= 256
 
