@@ -41,7 +41,8 @@ struct RotaryArgs {
   int* sink;
   // set by the launcher
   int64_t n_tokens;  // (set by the caller: B S)
-  int tokens, units, head_chunk;
+  int tokens, units, head_step;
+  int pairs;  // rows aligned to two vectors: adjacent ones move as one access
   uint32_t div_units, div_heads;
 };
 cudaError_t launch_rotary(const RotaryArgs& p, int dtype, cudaStream_t stream);
