@@ -9,6 +9,7 @@ library is missing; there is no fallback of any kind.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 from pathlib import Path
 
@@ -186,9 +187,15 @@ def strerror(status: int) -> str:
     return load().cfa_strerror(int(status)).decode()
 
 
+@functools.lru_cache(maxsize=4096)
+def _int64s(s: tuple) -> ctypes.Array:
+    return (ctypes.c_int64 * len(s))(*(int(x) for x in s))
+
+
 def strides3(s) -> ctypes.Array:
-    """A (batch, head, seq) stride triple as the `const int64_t[3]` the ABI takes."""
-    return (ctypes.c_int64 * 3)(*(int(x) for x in s))
+    """A (batch, head, seq) stride triple as the `const int64_t[3]` the ABI takes (kept by value: the
+    ABI only reads it)."""
+    return _int64s(tuple(s))
 
 
 def check(status: int, where: str) -> None:
@@ -375,7 +382,7 @@ def rotary(x_ptr, xs, y_ptr, ys, dtype, pos_ptr, pos_bytes, pos_strides, first, 
     """cfa_rotary; returns the status. `pos_strides`: (batch, seq), or None without positions."""
     return load().cfa_rotary(
         x_ptr, strides3(xs), y_ptr, strides3(ys), dtype, pos_ptr, pos_bytes,
-        None if pos_strides is None else (ctypes.c_int64 * 2)(*pos_strides), first, freqs_ptr,
+        None if pos_strides is None else _int64s(pos_strides), first, freqs_ptr,
         amplitude, b, h, rotated, s, d, rot, int(interleaved), int(inverse), stream)
 
 

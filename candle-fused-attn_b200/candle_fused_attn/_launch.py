@@ -8,7 +8,7 @@ import contextlib
 
 import torch
 
-from . import FusedAttentionError, _abi, _raise_if_expired
+from . import FusedAttentionError, _abi, _raise_if_expired, _stream
 
 DTYPES = {torch.float32: _abi.CFA_F32, torch.float16: _abi.CFA_F16, torch.bfloat16: _abi.CFA_BF16}
 _nothing = contextlib.nullcontext()
@@ -21,15 +21,19 @@ def require(ok: bool, who: str, what: str) -> None:
 
 def one_device(who: str, *ts: torch.Tensor | None) -> torch.device:
     """The CUDA device that every given tensor is on."""
-    dev = ts[0].device
+    index = ts[0].get_device()
     for t in ts:
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise FusedAttentionError(f"{who}: CUDA tensors required")
-        if t.device != dev:
+        if t is not None and (t.get_device() != index or index < 0):
+            if not all(x is None or x.is_cuda for x in ts):
+                raise FusedAttentionError(f"{who}: CUDA tensors required")
             raise FusedAttentionError(f"{who}: tensors on different devices")
-    return dev
+    return ts[0].device
+
+
+def merged_heads(b: int, h: int, s: int, d: int, like: torch.Tensor) -> torch.Tensor:
+    """An empty [b, h, s, d] tensor laid out as [b, s, h, d] (merge-heads ready), of like's type."""
+    return torch.empty_strided((b, h, s, d), (s * h * d, d, h * d, 1), dtype=like.dtype,
+                               device=like.device)
 
 
 def int32_vector(who: str, name: str, t: torch.Tensor | None, n: int) -> None:
@@ -42,6 +46,15 @@ def int32_vector(who: str, name: str, t: torch.Tensor | None, n: int) -> None:
 def no_gradient(who: str, *ts: torch.Tensor | None) -> None:
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
         raise FusedAttentionError(f"{who}: has no backward (call it under torch.no_grad())")
+
+
+# (torch.cuda.current_stream builds a Stream object to read one integer of: 2 us of a 10 us call)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def current_stream(dev: torch.device) -> int:
+    """The current stream of `dev` as the handle that the ABI takes."""
+    return _stream(dev) if _raw_stream is None else _raw_stream(dev.index)
 
 
 def on_device(dev: torch.device):

@@ -6,9 +6,9 @@ from __future__ import annotations
 
 import torch
 
-from . import (FusedAttentionError, _abi, _aligned_grad, _bhs_strides, _check_head_dim,
-               _float4_rows, _stream)
-from ._launch import check_status, int32_vector, on_device, one_device, raise_if_expired, require
+from . import FusedAttentionError, _abi, _check_head_dim, _float4_rows
+from ._launch import (check_status, current_stream, int32_vector, merged_heads, on_device,
+                      one_device, raise_if_expired, require)
 
 __all__ = ["cross_attention"]
 
@@ -40,12 +40,12 @@ def _forward(q, k, v, key_lengths, scale, dims):
     b, h, hk, sq, sk, d = dims
     dev = q.device
     raise_if_expired()
-    o = torch.empty((b, sq, h, d), dtype=torch.float32, device=dev)
+    o = merged_heads(b, h, sq, d, q)
     lse = torch.empty((b, h, sq), dtype=torch.float32, device=dev)
     with on_device(dev):
-        st = _abi.cross_fwd(q.data_ptr(), _bhs_strides(q), k.data_ptr(), _bhs_strides(k),
-                            v.data_ptr(), _bhs_strides(v), _ptr(key_lengths), o.data_ptr(),
-                            lse.data_ptr(), b, h, hk, sq, sk, d, scale, _stream(dev))
+        st = _abi.cross_fwd(q.data_ptr(), q.stride()[:3], k.data_ptr(), k.stride()[:3],
+                            v.data_ptr(), v.stride()[:3], _ptr(key_lengths), o.data_ptr(),
+                            lse.data_ptr(), b, h, hk, sq, sk, d, scale, current_stream(dev))
     check_status(st, "cross_attention")
     return o, lse
 
@@ -54,19 +54,19 @@ def _few(q, k, v, key_lengths, scale, dims):
     b, h, hk, sq, sk, d = dims
     dev = q.device
     raise_if_expired()
-    o = torch.empty((b, sq, h, d), dtype=torch.float32, device=dev)
+    o = merged_heads(b, h, sq, d, q)
     n = _abi.cross_few_workspace_bytes(b, h, sq, sk, d)
     ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
     with on_device(dev):
-        st = _abi.cross_few(q.data_ptr(), _bhs_strides(q), k.data_ptr(), _bhs_strides(k),
-                            v.data_ptr(), _bhs_strides(v), _ptr(key_lengths), o.data_ptr(),
-                            _ptr(ws), n, b, h, hk, sq, sk, d, scale, _stream(dev))
+        st = _abi.cross_few(q.data_ptr(), q.stride()[:3], k.data_ptr(), k.stride()[:3],
+                            v.data_ptr(), v.stride()[:3], _ptr(key_lengths), o.data_ptr(),
+                            _ptr(ws), n, b, h, hk, sq, sk, d, scale, current_stream(dev))
     check_status(st, "cross_attention")
     return o
 
 
 class _CrossAttention(torch.autograd.Function):
-    """q [b, h, sq, d], k and v [b, hk, sk, d] -> [b, sq, h, d]."""
+    """q [b, h, sq, d], k and v [b, hk, sk, d] -> [b, h, sq, d]."""
 
     @staticmethod
     def forward(ctx, q, k, v, key_lengths, scale, dims):
@@ -81,21 +81,20 @@ class _CrossAttention(torch.autograd.Function):
         b, h, hk, sq, sk, d = ctx.dims
         dev = q.device
         raise_if_expired()
-        grad = _aligned_grad(grad)
-        gb, gs, gh, _ = grad.stride()
-        dq = torch.empty((b, sq, h, d), dtype=torch.float32, device=dev)
+        grad = _float4_rows(grad)
+        dq = merged_heads(b, h, sq, d, q)
         dkv = torch.empty((b, sk, 2, hk, d), dtype=torch.float32, device=dev)
         n = _abi.cross_bwd_workspace_bytes(b, h, hk, sq, sk, d)
         ws = torch.empty(n, dtype=torch.uint8, device=dev)
         with on_device(dev):
-            st = _abi.cross_bwd(q.data_ptr(), _bhs_strides(q), k.data_ptr(), _bhs_strides(k),
-                                v.data_ptr(), _bhs_strides(v), _ptr(key_lengths), o.data_ptr(),
-                                lse.data_ptr(), grad.data_ptr(), (gb, gh, gs), dq.data_ptr(),
+            st = _abi.cross_bwd(q.data_ptr(), q.stride()[:3], k.data_ptr(), k.stride()[:3],
+                                v.data_ptr(), v.stride()[:3], _ptr(key_lengths), o.data_ptr(),
+                                lse.data_ptr(), grad.data_ptr(), grad.stride()[:3], dq.data_ptr(),
                                 dkv.data_ptr(), ws.data_ptr(), n, b, h, hk, sq, sk, d, ctx.scale,
-                                _stream(dev))
+                                current_stream(dev))
         check_status(st, "cross_attention")
-        return (dq.transpose(1, 2), dkv[:, :, 0].transpose(1, 2), dkv[:, :, 1].transpose(1, 2),
-                None, None, None)
+        dk, dv = dkv.permute(2, 0, 3, 1, 4).unbind(0)
+        return dq, dk, dv, None, None, None
 
 
 def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float,
@@ -107,7 +106,7 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: fl
     query head i reads key head i // (heads // key_heads). `key_lengths`: int32 [batch] on the
     device, how many keys each batch element has (values are held within 0 .. sk); what lies behind
     them is not read into any result, and a query without a key gives zeros and no gradient.
-    -> [batch, heads, sq, d], a transposed view of a dense [batch, sq, heads, d] buffer.
+    -> [batch, heads, sq, d], laid out as a dense [batch, sq, heads, d].
 
     Differentiable in q, k and v (dk, dv of a shared head are summed over its query heads). Without
     gradients, few queries -- the single token of a decoding step -- take a kernel that splits the
@@ -121,9 +120,7 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: fl
     int32_vector("cross_attention", "key_lengths", key_lengths, dims[0])
     scale = float(scale)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        o = _CrossAttention.apply(q, k, v, key_lengths, scale, dims)
-    elif dims[2] and dims[1] // dims[2] * dims[3] <= FEW_ROWS:
-        o = _few(q, k, v, key_lengths, scale, dims)
-    else:
-        o = _forward(q, k, v, key_lengths, scale, dims)[0]
-    return o.transpose(1, 2)
+        return _CrossAttention.apply(q, k, v, key_lengths, scale, dims)
+    if dims[2] and dims[1] // dims[2] * dims[3] <= FEW_ROWS:
+        return _few(q, k, v, key_lengths, scale, dims)
+    return _forward(q, k, v, key_lengths, scale, dims)[0]

@@ -22,9 +22,9 @@ from __future__ import annotations
 
 import torch
 
-from . import FusedAttentionError, _abi, _check_head_dim, _stream
-from ._launch import (DTYPES, check_status, int32_vector, no_gradient, on_device, one_device,
-                      raise_if_expired, require)
+from . import FusedAttentionError, _abi, _check_head_dim
+from ._launch import (DTYPES, check_status, current_stream, int32_vector, merged_heads, no_gradient,
+                      on_device, one_device, raise_if_expired, require)
 from .positions import check_freqs
 
 __all__ = ["paged_append", "paged_attention"]
@@ -70,8 +70,8 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
     (as for `rotary`) k and q are turned by that position; v and, without freqs, k and q are not.
     Values are rounded once to the cache's type. Padded rows of q come back as zeros; tokens without
     a page, and every other row of the cache, leave the cache as it was. Two tokens of a call must
-    not have the same slot. -> q's rotation [batch, heads, s, d] (a transposed view of a dense
-    [batch, s, heads, d] buffer), or None without q. No gradients.
+    not have the same slot. -> q's rotation [batch, heads, s, d] (laid out as a dense [batch, s, heads,
+    d]), or None without q. No gradients.
     """
     who = "paged_append"
     if k.dim() != 4 or v.shape != k.shape:
@@ -93,7 +93,7 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
     out, h = None, 0
     if q is not None:
         q, h = _rows(q), q.shape[1]
-        out = torch.empty((b, s, h, d), dtype=q.dtype, device=dev)
+        out = merged_heads(b, h, s, d, q)
     with on_device(dev):
         st = _abi.paged_append(
             None if q is None else q.data_ptr(), None if q is None else q.stride()[:3],
@@ -104,9 +104,9 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
             page_table.stride(0), page_table.shape[1], lengths.data_ptr(),
             None if new_lengths is None else new_lengths.data_ptr(),
             None if freqs is None else freqs.data_ptr(), float(amplitude), b, h, hk, s, d,
-            0 if freqs is None else 2 * freqs.numel(), interleaved, _stream(dev))
+            0 if freqs is None else 2 * freqs.numel(), interleaved, current_stream(dev))
     check_status(st, who)
-    return None if out is None else out.transpose(1, 2)
+    return out
 
 
 def _aligned(t: torch.Tensor) -> bool:
@@ -124,8 +124,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     q [batch, heads, s, d], d in HEAD_DIMS, of the cache's type or f32; heads a multiple of the
     cache's key heads. Query i of a sequence's n (n = s, or new_lengths[b]) sees its first
     lengths[b] - n + i + 1 keys: all of them for a single token. The cache's rows must be 16-byte
-    aligned. -> [batch, heads, s, d], a transposed view of a dense [batch, s, heads, d] buffer, of
-    q's type; zeros where a query sees no key or a padded row is no query. The keys are split into
+    aligned. -> [batch, heads, s, d], laid out as a dense [batch, s, heads, d], of q's type; zeros where a query sees no key or a padded row is no query. The keys are split into
     chunks by the sequence's own length and joined in order: bit-identical across reruns and
     batches. Softmax statistics and sums are fp32. No gradients.
     """
@@ -144,7 +143,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     raise_if_expired()
     if not _aligned(q):
         q = q.clone(memory_format=torch.contiguous_format)
-    o = torch.empty((b, s, h, d), dtype=q.dtype, device=dev)
+    o = merged_heads(b, h, s, d, q)
     width, page = page_table.shape[1], k_cache.shape[1]
     n = _abi.paged_attention_workspace_bytes(b, h, s, width * page, d, DTYPES[k_cache.dtype])
     ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
@@ -154,6 +153,6 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
             v_cache.data_ptr(), v_cache.stride()[:3], DTYPES[k_cache.dtype], k_cache.shape[0], page,
             page_table.data_ptr(), page_table.stride(0), width, lengths.data_ptr(),
             None if new_lengths is None else new_lengths.data_ptr(), o.data_ptr(),
-            None if ws is None else ws.data_ptr(), n, b, h, hk, s, d, float(scale), _stream(dev))
+            None if ws is None else ws.data_ptr(), n, b, h, hk, s, d, float(scale), current_stream(dev))
     check_status(st, who)
-    return o.transpose(1, 2)
+    return o

@@ -7,8 +7,9 @@ import math
 
 import torch
 
-from . import FusedAttentionError, _abi, _stream, qkv_geometry
-from ._launch import DTYPES, check_status, on_device, one_device, raise_if_expired, require
+from . import FusedAttentionError, _abi, qkv_geometry
+from ._launch import (DTYPES, check_status, current_stream, merged_heads, on_device, one_device,
+                      raise_if_expired, require)
 
 __all__ = ["rotary", "rotary_qkv", "rotary_frequencies"]
 
@@ -71,18 +72,16 @@ def _launch(who, x_ptr, xs, dtype, dims, rotated, positions, freqs, amplitude, i
     with on_device(dev):
         st = _abi.rotary(x_ptr, xs, out.data_ptr(), outs, DTYPES[dtype], *at, freqs.data_ptr(),
                          amplitude, b, h, rotated, s, d, 2 * freqs.numel(), interleaved, inverse,
-                         _stream(dev))
+                         current_stream(dev))
     check_status(st, who)
 
 
 def _turn(x, positions, freqs, amplitude, interleaved, inverse):
-    """x [b, h, s, d] -> a dense [b, s, h, d] buffer."""
     b, h, s, d = x.shape
     if x.stride(3) != 1 and d > 1:
         x = x.contiguous()
-    y = torch.empty((b, s, h, d), dtype=x.dtype, device=x.device)
-    sb, sh, ss, _ = x.stride()
-    _launch("rotary", x.data_ptr(), (sb, sh, ss), x.dtype, (b, h, s, d), h, positions, freqs,
+    y = merged_heads(b, h, s, d, x)
+    _launch("rotary", x.data_ptr(), x.stride()[:3], x.dtype, (b, h, s, d), h, positions, freqs,
             amplitude, interleaved, inverse, y, (s * h * d, d, h * d), x.device)
     return y
 
@@ -101,8 +100,8 @@ class _Rotary(torch.autograd.Function):
     def backward(ctx, grad):
         freqs, *at = ctx.saved_tensors
         positions = at[0] if at else ctx.first
-        dx = _turn(grad.transpose(1, 2), positions, freqs, ctx.amplitude, ctx.interleaved, True)
-        return dx.transpose(1, 2), None, None, None, None
+        dx = _turn(grad, positions, freqs, ctx.amplitude, ctx.interleaved, True)
+        return dx, None, None, None, None
 
 
 def _turn_qkv(qkv, heads, positions, freqs, amplitude, interleaved, inverse):
@@ -142,7 +141,7 @@ def _check(who, x, positions, freqs, b, s, d):
         if positions.dim() > 2 or positions.shape not in ((s,), (b, s), (1, s), (b, 1)):
             raise FusedAttentionError(f"{who}: positions [{s}] or [{b}, {s}] expected, got "
                                       f"{list(positions.shape)}")
-        return positions.expand(b, s)
+        return positions if positions.shape == (b, s) else positions.expand(b, s)
     one_device(who, x, freqs)
     return int(positions)
 
@@ -156,17 +155,15 @@ def rotary(x: torch.Tensor, positions: torch.Tensor | int, freqs: torch.Tensor, 
     of consecutive ones. `freqs`: float64 radians a position (`rotary_frequencies`); pair j is
     (j, j + len(freqs)), or (2j, 2j + 1) with `interleaved`, and is turned by position * freqs[j] and
     scaled by `amplitude`; the dims past the pairs are copied. Angles are reduced in 64 bits, so far
-    positions lose nothing. -> [batch, heads, seq, d], a transposed view of a dense [batch, seq,
-    heads, d] buffer, of x's type. Differentiable in x.
+    positions lose nothing. -> [batch, heads, seq, d], laid out as a dense [batch, seq, heads, d], of
+    x's type. Differentiable in x.
     """
     require(x.dim() == 4, "rotary", f"[b, h, s, d] expected, shape {list(x.shape)}")
     b, _, s, d = x.shape
     at = _check("rotary", x, positions, freqs, b, s, d)
     if torch.is_grad_enabled() and x.requires_grad:
-        y = _Rotary.apply(x, at, freqs, float(amplitude), bool(interleaved))
-    else:
-        y = _turn(x, at, freqs, float(amplitude), bool(interleaved), False)
-    return y.transpose(1, 2)
+        return _Rotary.apply(x, at, freqs, float(amplitude), bool(interleaved))
+    return _turn(x, at, freqs, float(amplitude), bool(interleaved), False)
 
 
 def rotary_qkv(qkv: torch.Tensor, heads: int, positions: torch.Tensor | int, freqs: torch.Tensor, *,
