@@ -90,7 +90,12 @@ struct BwdArgs {
   int Hk, Sk;
   const int* key_lengths;
   float* dq;   // [B, S, H, D]
-  float* dkv;  // [B, Sk, 2, Hk, D] (dK, dV interleaved)
+  float* dkv;  // [B, Sk, 2, Hk, D] (dK, dV interleaved); n_parts > 1: as many of them, part_stride
+               // floats apart, in the workspace, summed into dkv_out
+  float* dkv_out;
+  int n_parts;          // blocks of a key block, each over consecutive query tiles
+  int64_t part_stride;
+  int join_dq;          // dQ's partials are summed by cross_join_kernel, not by the last key block
 };
 
 struct PrepArgs {
@@ -164,6 +169,7 @@ cudaError_t launch_cross_fwd_tc(const FwdArgs& a, int head_dim, cudaStream_t str
 cudaError_t launch_cross_bwd_tc(const BwdArgs& a, int head_dim, cudaStream_t stream);
 cudaError_t launch_cross_hd_fwd(const FwdArgs& a, cudaStream_t stream);
 cudaError_t launch_cross_hd_bwd(const BwdArgs& a, cudaStream_t stream);
+cudaError_t launch_cross_join(const BwdArgs& a, int head_dim, int key_block, cudaStream_t stream);
 
 // The projection GEMM (linear_tc.cu): C = A B over fp32 on the tensor cores (split bf16 parts).
 // A(m, k) = a[m a_sm + k a_sk], B(k, n) = b[k b_sk + n b_sn] (any strides), C(m, n) = c[m c_sm +

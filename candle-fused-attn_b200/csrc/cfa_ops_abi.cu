@@ -64,43 +64,39 @@ int check_cross(int64_t B, int64_t H, int64_t Hk, int64_t Sq, int64_t Sk, int64_
   if (B == 0 || H == 0) return CFA_OK;
   if (B * H > kLim / ((std::max(Sq, Sk) + 31) / 32 + 1)) return CFA_ERR_OVERFLOW;
   if (B * H * Sq > kLim || B * Hk * Sk > kLim) return CFA_ERR_OVERFLOW;
+  if (B * Hk * ((Sk + 63) / 64) > kLim / cfa::LIN_SMS) return CFA_ERR_OVERFLOW;  // key blocks x parts
   return CFA_OK;
 }
 
-// The cross backward's workspace: ticket and error flag, turn counters and the split tail's flags
-// (one cleared range), D, then -- short key sequences -- the dQ partials and the tail's windows.
-constexpr int kCrossMaxKeyBlocks = 16;       // no-wait dQ up to as many key blocks
-constexpr int64_t kCrossWindowBytes = int64_t(512) << 20;  // most that a split tail's windows take
+// The cross backward's workspace: ticket and error flag, turn counters (one cleared range), D, then --
+// short key sequences -- the dQ partials and, where the query tiles are cut into parts, theirs of dK, dV.
+// Everything below follows from the shapes of one batch element: no sum depends on the batch.
+constexpr int kCrossMaxKeyBlocks = 16;           // no-wait dQ up to as many key blocks
+constexpr int64_t kCrossJoinBytes = 512 << 10;   // dQ partials of a (batch, key head) one block may sum
+constexpr int kCrossPartTiles = 8;               // fewest query tiles of a part
 struct CrossLayout {
   int64_t n_zero;  // ints cleared before the backward
-  size_t turn_off, flag_off, dsum_off, part_off, win_off, total;
-  bool partials;
-  int tail_units, tail_parts;
+  size_t turn_off, dsum_off, part_off, kv_off, total;
+  bool partials, join_dq;
+  int n_parts;
 };
 CrossLayout cross_layout(int64_t B, int64_t H, int64_t Hk, int64_t Sq, int64_t Sk, int64_t D) {
   CrossLayout w{};
-  const int64_t kb = D == 128 ? 64 : 128, nkb = (Sk + kb - 1) / kb, nqt = (Sq + 63) / 64;
-  const int64_t units = nkb * B * Hk, tiles = H / Hk * nqt;
+  const int64_t kb = D == 128 ? 64 : 128, nkb = (Sk + kb - 1) / kb;
+  const int64_t group = H / Hk, tiles = (group * Sq + 63) / 64;
   w.partials = nkb <= kCrossMaxKeyBlocks;
-  // The key blocks of the partial last wave (all of them where they are fewer than the SMs) split by
-  // query tiles; the count of SMs is fixed, so that the workspace does not depend on the device.
-  if (w.partials && D != 128) {
-    const int64_t R = units % cfa::LIN_SMS;
-    const int64_t k = R > 0 ? std::min<int64_t>(tiles, cfa::LIN_SMS / R) : 0;
-    if (k >= 2 && R * tiles * 2 * 128 * D * 4 <= kCrossWindowBytes) {
-      w.tail_units = static_cast<int>(R);
-      w.tail_parts = static_cast<int>(k);
-    }
-  }
+  // A batch element with fewer key blocks than the GPU has SMs: parts of at least 8 tiles that give
+  // it as many blocks.
+  const int64_t want = (cfa::LIN_SMS + nkb * Hk - 1) / (nkb * Hk);
+  w.n_parts = static_cast<int>(std::max<int64_t>(1, std::min(want, tiles / kCrossPartTiles)));
+  w.join_dq = w.partials && (w.n_parts > 1 || group * Sq * D * 4 * nkb > kCrossJoinBytes);
   w.turn_off = 256;
-  const int64_t turns = std::max(B * H * nqt, B * Hk);
-  w.flag_off = w.turn_off + static_cast<size_t>(turns) * 4;
-  const int64_t flags = static_cast<int64_t>(w.tail_units) * w.tail_parts + 1;
-  w.n_zero = 64 + turns + flags;
-  w.dsum_off = cfa::align256(w.flag_off + static_cast<size_t>(flags) * 4);
+  const int64_t turns = B * Hk * tiles;
+  w.n_zero = 64 + turns;
+  w.dsum_off = w.turn_off + cfa::align256(static_cast<size_t>(turns) * 4);
   w.part_off = w.dsum_off + cfa::align256(static_cast<size_t>(B * H * Sq) * 4);
-  w.win_off = w.part_off + (w.partials ? cfa::align256(static_cast<size_t>(nkb * B * H * Sq) * D * 4) : 0);
-  w.total = w.win_off + static_cast<size_t>(w.tail_units ? w.tail_units * tiles * 2 * 128 * D * 4 : 0);
+  w.kv_off = w.part_off + (w.partials ? cfa::align256(static_cast<size_t>(nkb * B * H * Sq) * D * 4) : 0);
+  w.total = w.kv_off + (w.n_parts > 1 ? static_cast<size_t>(w.n_parts) * B * Sk * 2 * Hk * D * 4 : 0);
   return w;
 }
 
@@ -205,13 +201,12 @@ int cfa_cross_bwd_f32(const float* q, const int64_t q_strides[3], const float* k
   a.timeout_ns = cfa::WAIT_TIMEOUT_NS;
   a.sink = cfa::error_sink();
   a.dq_part = lay.partials ? reinterpret_cast<float*>(ws + lay.part_off) : nullptr;
-  if (lay.tail_parts > 1) {
-    const int64_t units = (key_seq + 127) / 128 * batch * key_heads;
-    a.tail_base = static_cast<int>(units - lay.tail_units);
-    a.tail_units = lay.tail_units;
-    a.tail_parts = lay.tail_parts;
-    a.tail_win = reinterpret_cast<float*>(ws + lay.win_off);
-    a.tail_flag = reinterpret_cast<int*>(ws + lay.flag_off);
+  a.n_parts = lay.n_parts;
+  a.join_dq = lay.join_dq;
+  a.dkv_out = dkv;
+  if (lay.n_parts > 1) {
+    a.dkv = reinterpret_cast<float*>(ws + lay.kv_off);
+    a.part_stride = batch * key_seq * 2 * key_heads * head_dim;
   }
   return status(head_dim == 128 ? cfa::launch_cross_hd_bwd(a, s)
                                 : cfa::launch_cross_bwd_tc(a, static_cast<int>(head_dim), s));

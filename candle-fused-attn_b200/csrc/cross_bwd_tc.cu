@@ -6,9 +6,15 @@
 // header states them; bwd_tc.cuh holds what both share); what differs:
 //  - a.Sk key rows, of which batch element b attends the first cross_keys(a, b). Key blocks past
 //    them write zeros and take no part;
-//  - a key block belongs to a key head and walks the query tiles of every query head of its group,
-//    head by head, so dV and dK of a shared head are summed in registers in that order and written
-//    once;
+//  - a key block belongs to a key head and walks the query rows of its whole group, head after head
+//    (row r: head r / S of the group, query r % S), in tiles of 64 rows, so dV and dK of a shared head
+//    are summed in registers in that order and a group of short query sequences fills the tiles;
+//  - with few key blocks a batch element (cross_layout's rule, by the shapes of one element alone) the
+//    tiles are cut into parts of consecutive ones, a block each, whose dV, dK sums cross_join_kernel
+//    adds in order. (bwd_tc.cu's split tail would have one block fold every tile of the others: at 16
+//    heads over one, [2, 16, 1024, 64], that and one block's sum of all dQ partials took 1.2 of 1.5
+//    ms.) Where the dQ partials of a (batch, key head) exceed half a MB, or with parts, that kernel
+//    sums them too, by all SMs;
 //  - dQ [B, S, H, HD] and dK, dV [B, Sk, 2, Hk, HD] go to buffers of their own.
 // It is a kernel of its own, because at 96 registers a thread the fused attention's backward keeps
 // its registers only as it stands: as one template, that instance spilled or slowed by 0.2 to 3 %.
@@ -24,8 +30,6 @@ template <int HD>
 __global__ void __launch_bounds__(NB, 1) cross_bwd_tc_kernel(const BwdArgs a) {
   static_assert(HD == 64 || HD == 32, "head dims of the tensor-core backward");
   constexpr int KSD = HD / 16;  // K-steps of the products that reduce over the head dim
-  constexpr int WIN = TailWindow<HD>::WIN;
-  constexpr auto win4 = TailWindow<HD>::item;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   const uint32_t raw = tc::smem_u32(smem_raw);
   unsigned char* sm = smem_raw + ((1024u - (raw & 1023u)) & 1023u);
@@ -57,7 +61,7 @@ __global__ void __launch_bounds__(NB, 1) cross_bwd_tc_kernel(const BwdArgs a) {
   // The work item. With the dQ partials (no-wait path): the block index, (b, h)-major, so a
   // (b, h)'s key blocks run side by side and its last one finishes early. With the turn chain: a
   // ticket drawn after the prep kernel's wait, key-block-major -- a block waits only on key block
-  // kb - 1 of its (b, h), which holds a smaller ticket, so it is running or done.
+  // kb - 1 of its (b, h) and part, which holds a smaller ticket, so it is running or done.
   const bool chain = a.dq_part == nullptr;
   int ticket = static_cast<int>(blockIdx.x);
   if (chain) {
@@ -65,66 +69,45 @@ __global__ void __launch_bounds__(NB, 1) cross_bwd_tc_kernel(const BwdArgs a) {
     __syncthreads();
     ticket = s_int[1];
   }
-  // Split tail (no-wait path): the key blocks from a.tail_base on -- the grid's last partial wave
-  // -- run as a.tail_parts blocks each, part p taking the p-th contiguous range of the query tiles.
-  // The helpers (parts >= 1) leave their tiles' dV, dK windows in a.tail_win; the first part adds
-  // them after its own, in tile order: the same sums as one block, bit for bit. Only the first
-  // part writes dV, dK and counts the key block in. The roles go by a ticket drawn at the start,
-  // helpers first, so a first part that runs finds every helper running or done (no assumption
-  // on the order in which the hardware starts blocks): its wait always ends.
-  int part = 0, nparts = 1, tail_r = 0;
-  if (!chain && a.tail_parts > 1 && ticket >= a.tail_base) {
-    if (tid == 0) s_int[1] = atomicAdd(a.tail_flag + a.tail_units * a.tail_parts, 1);
-    __syncthreads();
-    const int j = s_int[1];
-    const int g = j / a.tail_units;
-    tail_r = j - g * a.tail_units;
-    nparts = a.tail_parts;
-    part = g + 1 < nparts ? g + 1 : 0;
-    ticket = a.tail_base + tail_r;
-  }
-  const int kb = chain ? ticket / BH : ticket % a.n_kblocks;
-  const int bh = chain ? ticket % BH : ticket / a.n_kblocks;
+  const int nparts = a.n_parts, part = ticket % nparts, unit = ticket / nparts;
+  const int kb = chain ? unit / BH : unit % a.n_kblocks;
+  const int bh = chain ? unit % BH : unit / a.n_kblocks;
   const int b = bh / a.Hk, h = bh % a.Hk;  // the key head
   const int k0 = kb * KB;
   const int group = a.H / a.Hk, h0 = h * group;  // the key block's query heads
-  const int nqt = (S + QT - 1) / QT;
+  const int rows = group * S, nqt = (rows + QT - 1) / QT;  // and their rows, in tiles
   const int SK = cross_keys(a, b);
   const int nkb = (SK + KB - 1) / KB;  // key blocks of this (batch, head) that take part
+  float* dkv = a.dkv + static_cast<int64_t>(part) * a.part_stride;  // (parts: in the workspace)
   if (kb >= nkb) {  // no key of this block is attended: zeros, and no part in dQ's sums
     griddep_launch_dependents();
-    if (part != 0) return;
     constexpr int C4 = HD / 4;
     const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
-    const int rows = min(KB, a.Sk - k0);
-    for (int f = tid; f < 2 * rows * C4; f += NB) {
-      const int which = f / (rows * C4), r = (f / C4) % rows;
+    const int krows = min(KB, a.Sk - k0);
+    for (int f = tid; f < 2 * krows * C4; f += NB) {
+      const int which = f / (krows * C4), r = (f / C4) % krows;
       reinterpret_cast<float4*>(
-          a.dkv + (((static_cast<int64_t>(b) * a.Sk + k0 + r) * 2 + which) * a.Hk + h) * HD)[f % C4] = zero;
+          dkv + (((static_cast<int64_t>(b) * a.Sk + k0 + r) * 2 + which) * a.Hk + h) * HD)[f % C4] = zero;
     }
-    if (kb == 0)  // no key at all: dQ = 0
-      for (int64_t f = tid; f < static_cast<int64_t>(S) * group * C4; f += NB)
+    if (kb == 0 && part == 0)  // no key at all: dQ = 0
+      for (int64_t f = tid; f < static_cast<int64_t>(rows) * C4; f += NB)
         reinterpret_cast<float4*>(a.dq + ((static_cast<int64_t>(b) * S + f / (group * C4)) * a.H + h0) *
                                              HD)[f % (group * C4)] = zero;
     return;
   }
   const float* kp = a.k + b * a.k_sb + h * a.k_sh;
   const float* vp = a.v + b * a.v_sb + h * a.v_sh;
-  // The query head and first query of the block's tile t (0 .. n_all - 1), that head's operands, and
-  // its row in L, D, the counters and the partials.
-  auto tile_head = [&](int t) { return h0 + t / nqt; };
-  auto tile_q0 = [&](int t) { return t % nqt * QT; };
-  auto q_rows = [&](int t) { return a.q + b * a.q_sb + tile_head(t) * a.q_sh; };
-  auto g_rows = [&](int t) { return a.d_o + b * a.do_sb + tile_head(t) * a.do_sh; };
-  auto query_bh = [&](int t) { return static_cast<int64_t>(b) * a.H + tile_head(t); };
-  const int n_all = group * nqt;  // the key block's query tiles
-  const int n_lo = part * n_all / nparts, n_hi = (part + 1) * n_all / nparts;
+  // Row r of the group's rows as (query head, query).
+  auto query_of = [&](int r, int& head, int& i) {
+    const int g = group == 1 ? 0 : r / S;
+    head = h0 + g;
+    i = r - g * S;
+  };
+  const int n_lo = static_cast<int>(static_cast<int64_t>(part) * nqt / nparts);
+  const int n_hi = static_cast<int>((static_cast<int64_t>(part) + 1) * nqt / nparts);
   const int t_begin = n_lo;  // this block's first query tile
-  // Turn chain: counters per 64-query tile of a query head.
-  int* turn = a.turn + (static_cast<int64_t>(b) * a.H + h0) * nqt;
-  const int64_t row_stride = static_cast<int64_t>(a.H) * HD;  // dq floats per (b, s)
-  auto dq_rows = [&](int head) { return a.dq + static_cast<int64_t>(b) * S * row_stride + head * HD; };
-  const int N = n_hi - n_lo;  // this block's query tiles, >= 1 (a.tail_parts <= n_all)
+  int* turn = a.turn + static_cast<int64_t>(bh) * nqt;  // turn chain: counters per tile
+  const int N = n_hi - n_lo;  // this block's query tiles, >= 1 (n_parts <= nqt)
   bool err0 = false;
 
   if (tid == 0) {
@@ -137,7 +120,7 @@ __global__ void __launch_bounds__(NB, 1) cross_bwd_tc_kernel(const BwdArgs a) {
     tc::mbar_init(bar_p, NT / 32);
     tc::mbar_init(bar_dv, 1);
     tc::fence_mbar_init();
-    tc::mbar_arrive_expect_tx(bar_ld, 4u * HD * (2 * min(KB, SK - k0) + 2 * min(QT, S - tile_q0(t_begin))));
+    tc::mbar_arrive_expect_tx(bar_ld, 4u * HD * (2 * min(KB, SK - k0) + 2 * min(QT, rows - t_begin * QT)));
   }
   griddep_launch_dependents();
 
@@ -145,36 +128,29 @@ __global__ void __launch_bounds__(NB, 1) cross_bwd_tc_kernel(const BwdArgs a) {
   // L / D buffer n % 2 (threads 0-127).
   auto stage_ld = [&](int n) {
     if (tid < 2 * QT) {
-      const int r = tid & 63, i = tile_q0(t_begin + n) + r;
-      const bool ok = i < S;
-      const float* src = (tid < QT ? a.lse : a.dsum) + query_bh(t_begin + n) * S;
-      cp_async4(ld + (n & 1) * 128 + (tid < QT ? 0 : QT) + r, src + (ok ? i : 0), ok ? 4 : 0);
+      const int r = tid & 63, x = (t_begin + n) * QT + r;
+      const bool ok = x < rows;
+      int head, i;
+      query_of(ok ? x : 0, head, i);
+      const float* src = (tid < QT ? a.lse : a.dsum) + (static_cast<int64_t>(b) * a.H + head) * S + i;
+      cp_async4(ld + (n & 1) * 128 + (tid < QT ? 0 : QT) + r, src, ok ? 4 : 0);
     }
   };
   auto stage_tile = [&](int n) {
-    const int q0 = tile_q0(t_begin + n);
-    stage_row_item<HD>(st, 0, tid, q_rows(t_begin + n), a.q_ss, q0, S);
-    stage_row_item<HD>(st, 1, tid, g_rows(t_begin + n), a.do_ss, q0, S);
+    int r, kc;
+    row_item(tid, r, kc);
+    const int x = (t_begin + n) * QT + r;
+    const bool ok = x < rows && 8 * kc < HD;
+    int head, i;
+    query_of(ok ? x : 0, head, i);
+    const float* q = a.q + b * a.q_sb + head * a.q_sh + i * a.q_ss + (ok ? 8 * kc : 0);
+    const float* g = a.d_o + b * a.do_sb + head * a.do_sh + i * a.do_ss + (ok ? 8 * kc : 0);
+    const int n16 = ok ? 16 : 0;  // (slots 0-1: Q, 2-3: dO, as split_row_item reads them)
+    cp_async16(st + 16 * tid, q, n16);
+    cp_async16(st + 16 * (NT + tid), q + 4, n16);
+    cp_async16(st + 16 * (2 * NT + tid), g, n16);
+    cp_async16(st + 16 * (3 * NT + tid), g + 4, n16);
     stage_ld(n);
-  };
-  // The block one wave later (work item + a.wave_ctas) starts by reading its key block's K, V rows
-  // and its first query tile's Q, dO rows, all at once across the wave: pull them into L2 while
-  // this wave computes and HBM is otherwise idle (one 256-byte row per thread).
-  auto prefetch_next_wave = [&]() {
-    const int nb = ticket + a.wave_ctas;
-    const int n_kb = a.n_kblocks;
-    if (a.wave_ctas <= 0 || nparts > 1 || nb >= n_kb * BH || tid >= 2 * KB + 2 * QT) return;
-    const int nkb2 = chain ? nb / BH : nb % n_kb, nbh = chain ? nb % BH : nb / n_kb;
-    const int nb_b = nbh / a.Hk, nb_h = tid < 2 * KB ? nbh % a.Hk : nbh % a.Hk * group;
-    const int r = tid < 2 * KB ? (tid & (KB - 1)) : (tid & (QT - 1));
-    const int row = tid < 2 * KB ? nkb2 * KB + r : r;
-    if (row >= (tid < 2 * KB ? a.Sk : S)) return;
-    const float* src;
-    if (tid < KB) src = a.k + nb_b * a.k_sb + nb_h * a.k_sh + static_cast<int64_t>(row) * a.k_ss;
-    else if (tid < 2 * KB) src = a.v + nb_b * a.v_sb + nb_h * a.v_sh + static_cast<int64_t>(row) * a.v_ss;
-    else if (tid < 2 * KB + QT) src = a.q + nb_b * a.q_sb + nb_h * a.q_sh + static_cast<int64_t>(row) * a.q_ss;
-    else src = a.d_o + nb_b * a.do_sb + nb_h * a.do_sh + static_cast<int64_t>(row) * a.do_ss;
-    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src), "n"(4 * HD) : "memory");
   };
   auto split_tile = [&](int n) {
     split_row_item(Qp + (n & 1) * 3 * PART_Q, PART_Q, st, 0, tid);
@@ -194,7 +170,7 @@ __global__ void __launch_bounds__(NB, 1) cross_bwd_tc_kernel(const BwdArgs a) {
   float* o_st = reinterpret_cast<float*>(dOp + 3 * PART_Q);
   static_assert(2 * KB * LDP * 4 <= 3 * PART_K + 2 * QT * 64 * 4 && QT * LDP * 4 <= 3 * PART_Q,
                 "prologue staging");
-  const int nk = min(KB, SK - k0), nq = min(QT, S - tile_q0(t_begin));
+  const int nk = min(KB, SK - k0), nq = min(QT, rows - t_begin * QT);
   __syncthreads();  // the mbarriers' initialisation
   if (mma_warp) {  // TMEM, by the warp that is idle while the rows travel (it also frees it)
     tc::tmem_alloc(tbase_p, TMEM_COLS);
@@ -208,16 +184,15 @@ __global__ void __launch_bounds__(NB, 1) cross_bwd_tc_kernel(const BwdArgs a) {
         if (r < nk) tc::bulk_load(k_rows + r * LDP, kp + static_cast<int64_t>(k0 + r) * a.k_ss, 4 * HD, bar_ld);
       } else if (tid < 2 * KB) {
         if (r < nk) tc::bulk_load(v_rows + r * LDP, vp + static_cast<int64_t>(k0 + r) * a.v_ss, 4 * HD, bar_ld);
-      } else if (tid < 2 * KB + QT) {
-        if (r < nq)
-          tc::bulk_load(q_st + r * LDP, q_rows(t_begin) + static_cast<int64_t>(tile_q0(t_begin) + r) * a.q_ss,
-                        4 * HD, bar_ld);
       } else if (r < nq) {
-        tc::bulk_load(o_st + r * LDP, g_rows(t_begin) + static_cast<int64_t>(tile_q0(t_begin) + r) * a.do_ss,
-                      4 * HD, bar_ld);
+        int head, i;
+        query_of(t_begin * QT + r, head, i);
+        if (tid < 2 * KB + QT)
+          tc::bulk_load(q_st + r * LDP, a.q + b * a.q_sb + head * a.q_sh + i * a.q_ss, 4 * HD, bar_ld);
+        else
+          tc::bulk_load(o_st + r * LDP, a.d_o + b * a.do_sb + head * a.do_sh + i * a.do_ss, 4 * HD, bar_ld);
       }
     }
-    griddep_wait();  // L, D, the cleared counters: the prep kernel's writes
     stage_ld(0);
     cp_async_commit();
     err0 = !tc::mbar_wait(bar_ld, 0, WAIT_TIMEOUT_NS);
@@ -326,14 +301,14 @@ __global__ void __launch_bounds__(NB, 1) cross_bwd_tc_kernel(const BwdArgs a) {
     if (N > 1) stage_tile(1);  // while the MMA warp issues T1(0)
     cp_async_commit();
     for (int n = 0; n < N; ++n) {
-      const int q0 = tile_q0(t_begin + n);
+      const int q0 = (t_begin + n) * QT;
       // (C1a) P^T for this thread's 16 queries, its parts into TMEM (pt_col) for dV -- while the
       // tensor core computes dP^T.
       err |= !tc::mbar_wait(bar_s, n & 1, WAIT_TIMEOUT_NS);
       tc::fence_after_sync();
       const float* Lt = ld + (n & 1) * 128;
       const float* Dt = Lt + QT;
-      const bool edge = (q0 + QT > S) || (k0 + KB > SK);
+      const bool edge = (q0 + QT > rows) || (k0 + KB > SK);
       float pr[16];
       tc::tmem_ld16(tbase + lane_sel + T_S + 16 * cg, pr);
       tc::tmem_wait_ld();
@@ -352,8 +327,8 @@ __global__ void __launch_bounds__(NB, 1) cross_bwd_tc_kernel(const BwdArgs a) {
           tc::unpack2(mul2(fma2v(tc::pack2(pr[u], pr[u + 1]), nsc2, l2), nl2e2), x0, x1);
           float p0 = ex2(x0), p1 = ex2(x1);
           if (edge) {
-            if (!(q0 + ql < S && key < SK)) p0 = 0.0f;
-            if (!(q0 + ql + 1 < S && key < SK)) p1 = 0.0f;
+            if (!(q0 + ql < rows && key < SK)) p0 = 0.0f;
+            if (!(q0 + ql + 1 < rows && key < SK)) p1 = 0.0f;
           }
           pr[u] = p0;
           pr[u + 1] = p1;
@@ -394,7 +369,6 @@ __global__ void __launch_bounds__(NB, 1) cross_bwd_tc_kernel(const BwdArgs a) {
       tc::fence_before_sync();
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(bar_c1);
-      if (n == 0) prefetch_next_wave();
       // (C3) The next tile's Q, dO into their parts (its buffer was last read by T2(n - 1)), while
       // the tensor core computes dV, dK, dQ; the tile after it travels.
       if (n + 1 < N) {
@@ -415,35 +389,26 @@ __global__ void __launch_bounds__(NB, 1) cross_bwd_tc_kernel(const BwdArgs a) {
       tc::tmem_ld16(tbase + lane_sel + T_DK + 16 * cg, xs);
       tc::tmem_wait_ld();
       if (16 * cg < HD) {  // dV, dK have HD columns
-        if (part == 0) {
 #pragma unroll
-          for (int c = 0; c < 16; ++c) {
-            dv[c] += xb[c];
-            dk[c] += xs[c];
-          }
-        } else {  // a split tail's helper: the tile's windows for the first part (win4)
-          float4* wv = reinterpret_cast<float4*>(a.tail_win) +
-                       (static_cast<int64_t>(tail_r) * n_all + n_lo + n) * (WIN / 4);
-#pragma unroll
-          for (int c4 = 0; c4 < 4; ++c4) {
-            __stcg(wv + win4(0, c4, cg, row),
-                   make_float4(xb[4 * c4], xb[4 * c4 + 1], xb[4 * c4 + 2], xb[4 * c4 + 3]));
-            __stcg(wv + win4(1, c4, cg, row),
-                   make_float4(xs[4 * c4], xs[4 * c4 + 1], xs[4 * c4 + 2], xs[4 * c4 + 3]));
-          }
+        for (int c = 0; c < 16; ++c) {
+          dv[c] += xb[c];
+          dk[c] += xs[c];
         }
       }
       // dQ (M = 64): query row 16 (w % 4) + lane in lanes 0-15 of each quarter; the two windows.
       tc::tmem_ld16(tbase + lane_sel + T_DQ0 + 16 * cg, xb);
       tc::tmem_ld16(tbase + lane_sel + T_DQ1 + 16 * cg, xs);
       tc::tmem_wait_ld();
-      const int qi = q0 + 16 * (w & 3) + lane;
+      const int x = q0 + 16 * (w & 3) + lane;
+      const bool mine = lane < 16 && x < rows && 16 * cg < HD;
+      int head, qi;
+      query_of(mine ? x : 0, head, qi);
       if (!chain) {
-        if (lane < 16 && qi < S && 16 * cg < HD && !err) {
+        if (mine && !err) {
           // Two 32-byte stores: whole L2 sectors (16-byte stores 256 bytes apart across the warp
           // each wrote half of 16 sectors).
           float* dst = a.dq_part +
-                       ((query_bh(t_begin + n) * a.n_kblocks + kb) * S + qi) * HD + 16 * cg;
+                       (((static_cast<int64_t>(b) * a.H + head) * a.n_kblocks + kb) * S + qi) * HD + 16 * cg;
 #pragma unroll
           for (int c8 = 0; c8 < 2; ++c8) {
             float v[8];
@@ -470,8 +435,9 @@ __global__ void __launch_bounds__(NB, 1) cross_bwd_tc_kernel(const BwdArgs a) {
           bar_sync(1, NT);
           go = s_int[2 + (n & 1)] != 0;
         }
-        if (go && lane < 16 && qi < S && 16 * cg < HD) {
-          float4* dst = reinterpret_cast<float4*>(dq_rows(tile_head(t)) + qi * row_stride + 16 * cg);
+        if (go && mine) {
+          float4* dst = reinterpret_cast<float4*>(
+              a.dq + ((static_cast<int64_t>(b) * S + qi) * a.H + head) * HD + 16 * cg);
 #pragma unroll
           for (int c4 = 0; c4 < 4; ++c4) {
             float4 v = make_float4(xb[4 * c4] + xs[4 * c4], xb[4 * c4 + 1] + xs[4 * c4 + 1],
@@ -496,63 +462,10 @@ __global__ void __launch_bounds__(NB, 1) cross_bwd_tc_kernel(const BwdArgs a) {
     }
   }
   cp_async_wait_all();
-  if (part == 0 && nparts > 1) {
-    // The first part of a split key block: the helpers' tile windows, added after its own tiles'
-    // in tile order (dv = ((w0 + w1) + w2) + ..., as one block folds them).
-    if (tid == 0) {
-      bool ok = true;
-      for (int p = 1; p < nparts && ok; ++p)
-        ok = wait_turn_bounded(a.tail_flag + tail_r * nparts + p, 1, a.err, a.timeout_ns, a.sink);
-      s_int[2] = ok ? 1 : 0;
-      // ORDER: with the barrier below, extends thread 0's acquires to the block (the windows and
-      // the helpers' dQ partials; the count below passes the partials on to the summing block).
-      __threadfence();
-    }
-    __syncthreads();
-    const bool ok = s_int[2] != 0;
-    err |= !ok;
-    // The windows travel by bulk copy into shared memory (free since the last T2), up to WCH
-    // tiles at a time: loads a thread issued itself would each wait out the L2 round trip.
-    constexpr int WCH = OFF_BAR / (4 * WIN);
-    static_assert(WCH >= 1, "one tile's windows fit in shared memory");
-    const float4* wsm = reinterpret_cast<const float4*>(sm);
-    for (int t0 = n_hi; ok && t0 < n_all; t0 += WCH) {
-      const int nt = min(WCH, n_all - t0);
-      if (tid == 0) {
-        tc::fence_async_global();  // the windows the acquires made visible, for the copy engine
-        tc::mbar_arrive_expect_tx(bar_ld, static_cast<uint32_t>(4 * WIN * nt));
-        tc::bulk_load(sm, a.tail_win + (static_cast<int64_t>(tail_r) * n_all + t0) * WIN,
-                      static_cast<uint32_t>(4 * WIN * nt), bar_ld);
-      }
-      const bool got = tc::mbar_wait(bar_ld, ld_phase & 1, WAIT_TIMEOUT_NS);
-      ++ld_phase;
-      err |= !got;
-      if (got && !mma_warp && 16 * cg < HD) {
-        for (int t = 0; t < nt; ++t) {
-          const float4* wv = wsm + t * (WIN / 4);
-#pragma unroll
-          for (int c4 = 0; c4 < 4; ++c4) {
-            const float4 x = wv[win4(0, c4, cg, row)];
-            const float4 y = wv[win4(1, c4, cg, row)];
-            dv[4 * c4] += x.x, dv[4 * c4 + 1] += x.y, dv[4 * c4 + 2] += x.z, dv[4 * c4 + 3] += x.w;
-            dk[4 * c4] += y.x, dk[4 * c4 + 1] += y.y, dk[4 * c4 + 2] += y.z, dk[4 * c4 + 3] += y.w;
-          }
-        }
-      }
-      // Every read of the chunk done before the next copy lands (and every thread leaves together).
-      if (!__syncthreads_and(got)) break;
-    }
-  }
   err = __syncthreads_or(err);  // any expired wait in the block: nothing is written
   if (err) {
     if (tid == 0) flag_timeout(a.err, a.sink);
     tc::mbar_wait(bar_t2, (N - 1) & 1, WAIT_TIMEOUT_NS);  // no MMA left in flight
-  } else if (part != 0) {
-    // A helper of a split key block: its windows and dQ partials are written; hand them to the
-    // first part (ORDER: every thread's stores are visible GPU-wide before thread 0's release).
-    __threadfence();
-    __syncthreads();
-    if (tid == 0) st_release_gpu(a.tail_flag + tail_r * nparts + part, 1);
   } else {
     // The dQ partials' hand-off: after the barrier above, thread 0's acquire-release count
     // publishes every thread's partial stores (the barrier orders them before it) and, for the
@@ -580,13 +493,13 @@ __global__ void __launch_bounds__(NB, 1) cross_bwd_tc_kernel(const BwdArgs a) {
     // Thread 0's count -- an acquire-release round trip through L2 -- travels while the block
     // stores the dV, dK rows.
     int count = -1;
-    if (tid == 0 && !chain) count = atom_add_acq_rel(a.turn + bh, 1);
+    if (tid == 0 && !chain && !a.join_dq) count = atom_add_acq_rel(a.turn + bh, 1);
     // dV, dK rows out of shared memory: every 16 threads store one whole row.
     {
       for (int f = tid; f < 2 * KB * C4; f += NB) {
         const int which = f / (KB * C4), r = (f / C4) % KB, c4 = f % C4;
         if (k0 + r < a.Sk) {  // (rows past the length hold zeros)
-          float* dst = a.dkv + (static_cast<int64_t>(b) * a.Sk + k0 + r) * 2 * a.Hk * HD +
+          float* dst = dkv + (static_cast<int64_t>(b) * a.Sk + k0 + r) * 2 * a.Hk * HD +
                        (1 - which) * a.Hk * HD + h * HD;
           reinterpret_cast<float4*>(dst)[c4] =
               reinterpret_cast<const float4*>((which ? sk : sv) + r * LDS)[c4];
@@ -596,6 +509,7 @@ __global__ void __launch_bounds__(NB, 1) cross_bwd_tc_kernel(const BwdArgs a) {
     if (tid == 0) s_int[0] = count;
     __syncthreads();
     const int64_t part_bytes = static_cast<int64_t>(nkb) * S * HD * 4;
+    const int64_t row_stride = static_cast<int64_t>(a.H) * HD;  // dq floats per (b, s)
     auto sum_partials = [&](const float* part, float* dq_out) {
       if (part_bytes <= OFF_DS) {
         // The (b, h)'s partials, contiguous [nkb][S][64], as one bulk copy into shared memory (the
@@ -665,10 +579,10 @@ __global__ void __launch_bounds__(NB, 1) cross_bwd_tc_kernel(const BwdArgs a) {
         }
       }
     };
-    if (s_int[0] == nkb - 1) {
+    if (s_int[0] == nkb - 1) {  // (without join_dq there is one part)
       // Head by head of the group, the partials of a head a.n_kblocks apart.
       for (int hq = h0; hq < h0 + group; ++hq) {
-        sum_partials(a.dq_part + (static_cast<int64_t>(b) * a.H + hq) * a.n_kblocks * S * HD, dq_rows(hq));
+        sum_partials(a.dq_part + (static_cast<int64_t>(b) * a.H + hq) * a.n_kblocks * S * HD, a.dq + static_cast<int64_t>(b) * S * row_stride + hq * HD);
         ++ld_phase;
         __syncthreads();  // this head's sums are read: the next one's partials may land
       }
@@ -690,24 +604,15 @@ cudaError_t setup_cross_bwd_tc_attributes() {
                                                  cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_ALLOC);
 }
 
-// The caller has laid out the workspace (cross_bwd_workspace_layout): the split tail's windows and
-// flags, when it planned one, are in a.tail_win, a.tail_flag with tail_units, tail_parts set for
-// LIN_SMS blocks a wave.
 cudaError_t launch_cross_bwd_tc(const BwdArgs& args, int head_dim, cudaStream_t stream) {
   BwdArgs a = args;
   a.n_kblocks = (a.Sk + KB - 1) / KB;
-  int dev = 0, sms = 0;
-  a.wave_ctas = cudaGetDevice(&dev) == cudaSuccess &&
-                        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess
-                    ? sms
-                    : 0;
-  const int64_t units = static_cast<int64_t>(a.n_kblocks) * a.B * a.Hk;
-  const int64_t blocks = a.tail_parts > 1 ? units + static_cast<int64_t>(a.tail_units) * (a.tail_parts - 1)
-                                          : units;
+  const int64_t blocks = static_cast<int64_t>(a.n_kblocks) * a.B * a.Hk * a.n_parts;
   const dim3 grid(static_cast<unsigned>(blocks));
-  if (head_dim == 32)
-    return launch_pdl(cross_bwd_tc_kernel<32>, grid, dim3(NB), SMEM_ALLOC, stream, a);
-  return launch_pdl(cross_bwd_tc_kernel<64>, grid, dim3(NB), SMEM_ALLOC, stream, a);
+  const cudaError_t e =
+      head_dim == 32 ? launch_pdl(cross_bwd_tc_kernel<32>, grid, dim3(NB), SMEM_ALLOC, stream, a)
+                     : launch_pdl(cross_bwd_tc_kernel<64>, grid, dim3(NB), SMEM_ALLOC, stream, a);
+  return e == cudaSuccess ? launch_cross_join(a, head_dim, KB, stream) : e;
 }
 
 }  // namespace cfa

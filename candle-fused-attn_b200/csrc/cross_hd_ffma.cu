@@ -2,14 +2,41 @@
 //
 // Cross attention at head dim 128: the forward and the one-pass backward of hd_ffma.cu (whose header
 // states the tiles, the thread layout and the orders of summation; hd_ffma.cuh holds what both
-// share) with keys of another length and shared key heads: a.Sk key rows, of which batch element b
-// attends the first cross_keys(a, b); a key block belongs to a key head and walks the query tiles of
-// every query head of its group, head by head, so dV and dK of a shared head are summed in registers
-// in that order; dQ and dK, dV go to buffers of their own. Bound by fp32 FMA issue, as hd_ffma.cu is.
+// share) with keys of another length and shared key heads, as the tensor-core pair has them at 64 and
+// 32: a.Sk key rows, of which batch element b attends the first cross_keys(a, b); a block's query rows
+// are those of a key head's whole group (row r: head r / S of it, query r % S), dK, dV of a shared
+// head summed in that order; parts of the tiles and cross_join_kernel as in cross_bwd_tc.cu; dQ and
+// dK, dV go to buffers of their own. Bound by fp32 FMA issue, as hd_ffma.cu is.
 #include "hd_ffma.cuh"
 
 namespace cfa {
 namespace {
+
+// The query rows of a key head's group: row r is query r % S of head h0 + r / S.
+struct GroupRows {
+  int h0, S, n, group;
+  __device__ __forceinline__ GroupRows(int group_, int key_head, int S_)
+      : h0(key_head * group_), S(S_), n(group_ * S_), group(group_) {}
+  __device__ __forceinline__ void query_of(int r, int& head, int& i) const {
+    const int g = group == 1 ? 0 : r / S;
+    head = h0 + g;
+    i = r - g * S;
+  }
+  // Rows row0 .. of a [heads, S, D] operand into a [ROWS][D + 4] tile (zeros past the last row).
+  template <int ROWS, int NT, int D>
+  __device__ __forceinline__ void load(float* dst, const float* src, int64_t h_stride, int64_t s_stride,
+                                       int row0) const {
+    constexpr int C = D / 4;
+#pragma unroll
+    for (int idx = threadIdx.x; idx < ROWS * C; idx += NT) {
+      const int r = idx / C, c4 = idx % C;
+      const bool ok = row0 + r < n;
+      int head, i;
+      query_of(ok ? row0 + r : row0, head, i);
+      cp_async16(dst + r * ldh<D>() + 4 * c4, src + head * h_stride + i * s_stride + 4 * c4, ok ? 16 : 0);
+    }
+  }
+};
 
 template <int D, int RPT>
 __global__ void __launch_bounds__(FWD_THREADS, Hd<D>::FWD_MINB) cross_hd_fwd_kernel(const FwdArgs a) {
@@ -26,24 +53,24 @@ __global__ void __launch_bounds__(FWD_THREADS, Hd<D>::FWD_MINB) cross_hd_fwd_ker
   const int ty = lane >> 4, tx = lane & 15;
   const int qt = static_cast<int>(blockIdx.x % a.n_qtiles);
   const int bh = static_cast<int>(blockIdx.x / a.n_qtiles);
-  const int b = bh / a.H, h = bh % a.H;
+  const int b = bh / a.Hk, h = bh % a.Hk;  // the key head
   const int q0 = qt * BM;
-  const int S = a.S;
   const int SK = cross_keys(a, b);
-  const int hk = h / (a.H / a.Hk);
+  const GroupRows rows(a.H / a.Hk, h, a.S);
   if (SK == 0) {  // no key: O = 0, L = -inf
-    const int rows = min(BM, S - q0);
-    for (int f = tid; f < rows * (D / 4); f += FWD_THREADS)
-      reinterpret_cast<float4*>(a.o + ((static_cast<int64_t>(b) * S + q0 + f / (D / 4)) * a.H + h) * D)[f % (D / 4)] =
+    for (int f = tid; f < min(BM, rows.n - q0) * (D / 4); f += FWD_THREADS) {
+      int head, i;
+      rows.query_of(q0 + f / (D / 4), head, i);
+      reinterpret_cast<float4*>(a.o + ((static_cast<int64_t>(b) * a.S + i) * a.H + head) * D)[f % (D / 4)] =
           make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int r = tid; r < rows; r += FWD_THREADS) a.lse[static_cast<int64_t>(bh) * S + q0 + r] = -INFINITY;
+      if (f % (D / 4) == 0) a.lse[(static_cast<int64_t>(b) * a.H + head) * a.S + i] = -INFINITY;
+    }
     return;
   }
-  const float* qp = a.q + b * a.q_sb + h * a.q_sh;
-  const float* kp = a.k + b * a.k_sb + hk * a.k_sh;
-  const float* vp = a.v + b * a.v_sb + hk * a.v_sh;
+  const float* kp = a.k + b * a.k_sb + h * a.k_sh;
+  const float* vp = a.v + b * a.v_sb + h * a.v_sh;
 
-  load_rows_async<BM, FWD_THREADS, D>(Qs, qp, a.q_ss, q0, S);
+  rows.load<BM, FWD_THREADS, D>(Qs, a.q + b * a.q_sb, a.q_sh, a.q_ss, q0);
   load_rows_async<64, FWD_THREADS, D>(Ks, kp, a.k_ss, 0, SK);
   cp_async_commit();
 
@@ -131,8 +158,10 @@ __global__ void __launch_bounds__(FWD_THREADS, Hd<D>::FWD_MINB) cross_hd_fwd_ker
 #pragma unroll
   for (int i = 0; i < RPT; ++i) {
     const float l = half_warp_sum(lpart[i]);
-    const int qi = q0 + rb + 2 * i;
-    if (qi >= S) continue;
+    const int r = q0 + rb + 2 * i;
+    if (r >= rows.n) continue;
+    int head, qi;
+    rows.query_of(r, head, qi);
     float ov[D / 16];
 #pragma unroll
     for (int p = 0; p < NP; ++p) {
@@ -140,8 +169,8 @@ __global__ void __launch_bounds__(FWD_THREADS, Hd<D>::FWD_MINB) cross_hd_fwd_ker
       ov[2 * p] = __fdiv_rn(v.x, l);
       ov[2 * p + 1] = __fdiv_rn(v.y, l);
     }
-    store_dims<D>(a.o + ((static_cast<int64_t>(b) * S + qi) * a.H + h) * D, tx, ov);
-    if (tx == 0) a.lse[static_cast<int64_t>(bh) * S + qi] = m[i] + logf(l);
+    store_dims<D>(a.o + ((static_cast<int64_t>(b) * a.S + qi) * a.H + head) * D, tx, ov);
+    if (tx == 0) a.lse[(static_cast<int64_t>(b) * a.H + head) * a.S + qi] = m[i] + logf(l);
   }
 }
 
@@ -178,37 +207,34 @@ __global__ void __launch_bounds__(Bwd<D>::NT, 256 / (Bwd<D>::NT / 2)) cross_hd_b
     ticket = s_int[0];
   }
   const int BH = a.B * a.Hk;
-  const int kb = no_wait ? ticket % a.n_kblocks : ticket / BH;
-  const int bh = no_wait ? ticket / a.n_kblocks : ticket % BH;
+  const int nparts = a.n_parts, part = ticket % nparts, unit = ticket / nparts;
+  const int kb = no_wait ? unit % a.n_kblocks : unit / BH;
+  const int bh = no_wait ? unit / a.n_kblocks : unit % BH;
   const int b = bh / a.Hk, h = bh % a.Hk;  // the key head
   const int k0 = kb * 64;
-  const int group = a.H / a.Hk, h0 = h * group;  // the key block's query heads
-  const int nqt = a.n_qtiles;
+  const int group = a.H / a.Hk;
+  const GroupRows rows(group, h, S);  // the key block's query rows
+  const int nqt = (rows.n + 63) / 64;
   const int SK = cross_keys(a, b);
   const int nkb = (SK + 63) / 64;  // key blocks of this (batch, head) that take part
+  float* dkv = a.dkv + static_cast<int64_t>(part) * a.part_stride;  // (parts: in the workspace)
   if (kb >= nkb) {  // no key of this block is attended: zeros, and no part in dQ's sums
     constexpr int C4 = D / 4;
     const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
-    const int rows = min(64, a.Sk - k0);
-    for (int f = tid; f < 2 * rows * C4; f += NT) {
-      const int which = f / (rows * C4), r = (f / C4) % rows;
+    const int krows = min(64, a.Sk - k0);
+    for (int f = tid; f < 2 * krows * C4; f += NT) {
+      const int which = f / (krows * C4), r = (f / C4) % krows;
       reinterpret_cast<float4*>(
-          a.dkv + (((static_cast<int64_t>(b) * a.Sk + k0 + r) * 2 + which) * a.Hk + h) * D)[f % C4] = zero;
+          dkv + (((static_cast<int64_t>(b) * a.Sk + k0 + r) * 2 + which) * a.Hk + h) * D)[f % C4] = zero;
     }
-    if (kb == 0)  // no key at all: dQ = 0
-      for (int64_t f = tid; f < static_cast<int64_t>(S) * group * C4; f += NT)
-        reinterpret_cast<float4*>(a.dq + ((static_cast<int64_t>(b) * S + f / (group * C4)) * a.H + h0) *
+    if (kb == 0 && part == 0)  // no key at all: dQ = 0
+      for (int64_t f = tid; f < static_cast<int64_t>(rows.n) * C4; f += NT)
+        reinterpret_cast<float4*>(a.dq + ((static_cast<int64_t>(b) * S + f / (group * C4)) * a.H + rows.h0) *
                                              D)[f % (group * C4)] = zero;
     return;
   }
-  // The query head of the block's tile t, its first query, and its row in L, D, the counters and the
-  // partials.
-  auto tile_head = [&](int t) { return h0 + t / nqt; };
-  auto tile_q0 = [&](int t) { return t % nqt * 64; };
-  auto query_bh = [&](int t) { return static_cast<int64_t>(b) * a.H + tile_head(t); };
-  int* turn = a.turn + (static_cast<int64_t>(b) * a.H + h0) * nqt;
+  int* turn = a.turn + static_cast<int64_t>(bh) * nqt;  // turn chain: counters per tile
   const int64_t row_stride = static_cast<int64_t>(a.H) * D;  // dq floats per (b, s)
-  auto dq_rows = [&](int head) { return a.dq + static_cast<int64_t>(b) * S * row_stride + head * D; };
 
   load_rows_async<64, NT, D>(Ks, a.k + b * a.k_sb + h * a.k_sh, a.k_ss, k0, SK);
   load_rows_async<64, NT, D>(Vs, a.v + b * a.v_sb + h * a.v_sh, a.v_ss, k0, SK);
@@ -228,15 +254,16 @@ __global__ void __launch_bounds__(Bwd<D>::NT, 256 / (Bwd<D>::NT / 2)) cross_hd_b
   const int d3 = D == 32 ? 2 * tx : 64 * grp + 4 * tx;
 
   auto load_q_do = [&](int t) {
-    const int q0 = tile_q0(t), head = tile_head(t);
-    load_rows_async<64, NT, D>(Qs, a.q + b * a.q_sb + head * a.q_sh, a.q_ss, q0, S);
-    load_rows_async<64, NT, D>(dOs, a.d_o + b * a.do_sb + head * a.do_sh, a.do_ss, q0, S);
+    rows.load<64, NT, D>(Qs, a.q + b * a.q_sb, a.q_sh, a.q_ss, t * 64);
+    rows.load<64, NT, D>(dOs, a.d_o + b * a.do_sb, a.do_sh, a.do_ss, t * 64);
   };
   auto load_l_d = [&](int t) {
     if (tid < 128) {
-      const int q0 = tile_q0(t), r = tid & 63, i = q0 + r;
-      const bool ok = i < S;
-      const float* src = (tid < 64 ? a.lse : a.dsum) + query_bh(t) * S + (ok ? i : q0);
+      const int r = tid & 63, x = t * 64 + r;
+      const bool ok = x < rows.n;
+      int head, i;
+      rows.query_of(ok ? x : t * 64, head, i);
+      const float* src = (tid < 64 ? a.lse : a.dsum) + (static_cast<int64_t>(b) * a.H + head) * S + i;
       cp_async4((tid < 64 ? Lt : Dt) + r, src, ok ? 4 : 0);
     }
   };
@@ -245,23 +272,24 @@ __global__ void __launch_bounds__(Bwd<D>::NT, 256 / (Bwd<D>::NT / 2)) cross_hd_b
     load_l_d(t);
   };
 
-  const int t_end = group * nqt;
-  load_query_tile(0);
+  const int t_begin = static_cast<int>(static_cast<int64_t>(part) * nqt / nparts);
+  const int t_end = static_cast<int>((static_cast<int64_t>(part) + 1) * nqt / nparts);
+  load_query_tile(t_begin);
   cp_async_commit();
-  for (int t = 0; t < t_end; ++t) {
-    const int q0 = tile_q0(t);
+  for (int t = t_begin; t < t_end; ++t) {
+    const int q0 = t * 64;
     cp_async_wait_all();
     __syncthreads();
 
     const int jn = min(4, (SK - k0 + 15) / 16);
-    const int iq = min(64, (S - q0 + 15) / 16 * 16);
+    const int iq = min(64, (rows.n - q0 + 15) / 16 * 16);
 
     // Phase 1. grp 0: s = Q K^T; grp 1: s = dO V^T (dP).
     {
       const float* As = grp ? dOs : Qs;
       const float* Bs = grp ? Vs : Ks;
       float s[R1][4];
-      if (q0 + 2 * R1 * wg >= S) {
+      if (q0 + 2 * R1 * wg >= rows.n) {
 #pragma unroll
         for (int i = 0; i < R1; ++i)
 #pragma unroll
@@ -276,7 +304,7 @@ __global__ void __launch_bounds__(Bwd<D>::NT, 256 / (Bwd<D>::NT / 2)) cross_hd_b
         scores<1, R1, D>(As, Bs, rb1, tx, s);
       }
       if (grp == 0) {
-        const bool edge = (q0 + 64 > S) || (k0 + 64 > SK);
+        const bool edge = (q0 + 64 > rows.n) || (k0 + 64 > SK);
 #pragma unroll
         for (int i = 0; i < R1; ++i) {
           const int il = rb1 + 2 * i, qi = q0 + il;
@@ -285,7 +313,7 @@ __global__ void __launch_bounds__(Bwd<D>::NT, 256 / (Bwd<D>::NT / 2)) cross_hd_b
           for (int jj = 0; jj < 4; ++jj) {
             const int jl = tx + 16 * jj, j = k0 + jl;
             float pr = expf(fmaf(s[i][jj], a.scale, -li));
-            if (edge && !(qi < S && j < SK)) pr = 0.0f;
+            if (edge && !(qi < rows.n && j < SK)) pr = 0.0f;
             Ps[il * LDP + jl] = pr;
           }
         }
@@ -349,7 +377,7 @@ __global__ void __launch_bounds__(Bwd<D>::NT, 256 / (Bwd<D>::NT / 2)) cross_hd_b
     for (int r = 0; r < 4; ++r)
 #pragma unroll
       for (int p = 0; p < E3 / 2; ++p) pq2[r][p] = 0ull;
-    const int jlim = q0 + (rb3 - ty) >= S ? 0 : 16 * jn;
+    const int jlim = q0 + (rb3 - ty) >= rows.n ? 0 : 16 * jn;
 #pragma unroll 2
     for (int j = 0; j < jlim; j += 4) {
       uint64_t k2[4][E3 / 2];
@@ -386,12 +414,14 @@ __global__ void __launch_bounds__(Bwd<D>::NT, 256 / (Bwd<D>::NT / 2)) cross_hd_b
       }
 
     if (a.dq_part != nullptr) {
-      float* part = a.dq_part + (query_bh(t) * a.n_kblocks + kb) * S * D;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int qi = q0 + rb3 + 2 * r;
-        if (qi >= S) continue;
-        float* dst = part + static_cast<int64_t>(qi) * D + d3;
+        const int x = q0 + rb3 + 2 * r;
+        if (x >= rows.n) continue;
+        int head, qi;
+        rows.query_of(x, head, qi);
+        float* dst = a.dq_part +
+                     (((static_cast<int64_t>(b) * a.H + head) * a.n_kblocks + kb) * S + qi) * D + d3;
         if constexpr (E3 == 2)
           __stcg(reinterpret_cast<float2*>(dst), make_float2(pq[r][0], pq[r][1]));
         else
@@ -413,9 +443,11 @@ __global__ void __launch_bounds__(Bwd<D>::NT, 256 / (Bwd<D>::NT / 2)) cross_hd_b
     if (go) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int qi = q0 + rb3 + 2 * r;
-        if (qi >= S) continue;
-        float* dst = dq_rows(tile_head(t)) + qi * row_stride + d3;
+        const int x = q0 + rb3 + 2 * r;
+        if (x >= rows.n) continue;
+        int head, qi;
+        rows.query_of(x, head, qi);
+        float* dst = a.dq + ((static_cast<int64_t>(b) * S + qi) * a.H + head) * D + d3;
 #pragma unroll
         for (int e = 0; e < E3; ++e) {
           float v = pq[r][e];
@@ -432,7 +464,7 @@ __global__ void __launch_bounds__(Bwd<D>::NT, 256 / (Bwd<D>::NT / 2)) cross_hd_b
     }
   }
 
-  if (a.dq_part != nullptr) {
+  if (a.dq_part != nullptr && !a.join_dq) {  // (without join_dq there is one part)
     // ORDER: partials visible GPU-wide before counting in; the last to count sums them all.
     __threadfence();
     __syncthreads();
@@ -442,9 +474,9 @@ __global__ void __launch_bounds__(Bwd<D>::NT, 256 / (Bwd<D>::NT / 2)) cross_hd_b
       __threadfence();
       constexpr int C = D / 4;  // float4 per row
       // DETERMINISM: (((p0 + p1) + p2) + ...) * scale over the contributing key blocks in order.
-      for (int hq = h0; hq < h0 + group; ++hq) {
+      for (int hq = rows.h0; hq < rows.h0 + group; ++hq) {
         const float* part = a.dq_part + (static_cast<int64_t>(b) * a.H + hq) * a.n_kblocks * S * D;
-        float* dq_out = dq_rows(hq);
+        float* dq_out = a.dq + static_cast<int64_t>(b) * S * row_stride + hq * D;
         for (int idx = tid; idx < S * C; idx += NT) {
           const int i = idx / C, c4 = idx % C;
           float4 v = __ldcg(reinterpret_cast<const float4*>(part + static_cast<int64_t>(i) * D + 4 * c4));
@@ -463,7 +495,7 @@ __global__ void __launch_bounds__(Bwd<D>::NT, 256 / (Bwd<D>::NT / 2)) cross_hd_b
   // grp 0 stores dV, grp 1 stores dK * scale.
   // (dkv [b, Sk, 2, Hk, D], dK first; rows past the length hold zeros.)
   const int64_t kv_stride = 2 * static_cast<int64_t>(a.Hk) * D;
-  float* dst0 = a.dkv + static_cast<int64_t>(b) * a.Sk * kv_stride + (grp ? 0 : 1) * a.Hk * D + h * D;
+  float* dst0 = dkv + static_cast<int64_t>(b) * a.Sk * kv_stride + (grp ? 0 : 1) * a.Hk * D + h * D;
   const float f = grp ? a.scale : 1.0f;
 #pragma unroll
   for (int rp = 0; rp < K2 / 2; ++rp) {
@@ -497,8 +529,8 @@ cudaError_t setup_cross_hd_attributes() {
 cudaError_t launch_cross_hd_fwd(const FwdArgs& args, cudaStream_t stream) {
   constexpr int A = Hd<128>::RPT_A, bm = fwd_bm<A>();
   FwdArgs a = args;
-  a.n_qtiles = (a.S + bm - 1) / bm;
-  const dim3 grid(static_cast<unsigned>(static_cast<int64_t>(a.n_qtiles) * a.B * a.H));
+  a.n_qtiles = static_cast<int>((static_cast<int64_t>(a.H / a.Hk) * a.S + bm - 1) / bm);
+  const dim3 grid(static_cast<unsigned>(static_cast<int64_t>(a.n_qtiles) * a.B * a.Hk));
   return launch_pdl(cross_hd_fwd_kernel<128, A>, grid, dim3(FWD_THREADS),
                     static_cast<size_t>(hd_fwd_smem_floats<128, A>() * 4), stream, a);
 }
@@ -506,9 +538,10 @@ cudaError_t launch_cross_hd_fwd(const FwdArgs& args, cudaStream_t stream) {
 cudaError_t launch_cross_hd_bwd(const BwdArgs& args, cudaStream_t stream) {
   BwdArgs a = args;
   a.n_kblocks = (a.Sk + 63) / 64;
-  const dim3 grid(static_cast<unsigned>(static_cast<int64_t>(a.n_kblocks) * a.B * a.Hk));
-  return launch_pdl(cross_hd_bwd_kernel<128>, grid, dim3(Bwd<128>::NT),
-                    static_cast<size_t>(hd_bwd_smem_floats<128>() * 4), stream, a);
+  const dim3 grid(static_cast<unsigned>(static_cast<int64_t>(a.n_kblocks) * a.B * a.Hk * a.n_parts));
+  const cudaError_t e = launch_pdl(cross_hd_bwd_kernel<128>, grid, dim3(Bwd<128>::NT),
+                                   static_cast<size_t>(hd_bwd_smem_floats<128>() * 4), stream, a);
+  return e == cudaSuccess ? launch_cross_join(a, 128, 64, stream) : e;
 }
 
 }  // namespace cfa

@@ -98,12 +98,21 @@ def test_long_key_sequences(cuda, d, sq, sk, h, hk):
     check(cuda, 2, h, hk, sq, sk, d, [sk, sk // 2 + 3], seed=d)
 
 
-@pytest.mark.parametrize("b,h,hk,sq,sk", [(1, 8, 1, 500, 200), (1, 1, 1, 1000, 130), (5, 30, 30, 130, 130),
-                                          (2, 16, 4, 200, 1500)])
-def test_split_tail(cuda, b, h, hk, sq, sk):
-    """Few key blocks, or a partial last wave of them: a key block's query tiles run on several SMs."""
-    check(cuda, b, h, hk, sq, sk, 64, None, seed=sq)
-    check(cuda, b, h, hk, sq, sk, 32, [sk - 70] * b, seed=sq)
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("b,h,hk,sq,sk,lens", [
+    (1, 8, 1, 500, 200, None), (1, 1, 1, 1000, 130, [90]), (2, 6, 1, 700, 300, [300, 0]),
+    (3, 16, 2, 200, 1000, [1000, 64, 129]), (1, 2, 1, 2000, 2300, [2300]), (2, 4, 1, 1100, 64, [64, 1])])
+def test_few_key_blocks(cuda, d, b, h, hk, sq, sk, lens):
+    """Few key blocks a batch element: a key block's query tiles run in parts on several SMs, their dK,
+    dV summed in order by a kernel of its own, and dQ's partials too (or by the turn chain)."""
+    check(cuda, b, h, hk, sq, sk, d, lens, seed=sq)
+
+
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("sq", [1, 3, 10, 31, 63, 65])
+def test_short_groups_share_tiles(cuda, d, sq):
+    """The query rows of a group lie behind one another in the tiles: heads that begin inside one."""
+    check(cuda, 2, 15, 3, sq, 150, d, [150, 77], seed=sq)
 
 
 @pytest.mark.parametrize("d", [32, 64, 128])

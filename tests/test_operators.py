@@ -58,17 +58,19 @@ def test_cross_backward_arguments():
 
 def test_cross_backward_workspace():
     """D and the turn counters always; the dQ partials up to 16 key blocks (of 128; of 64 at head dim
-    128); the split tail's windows where a wave of key blocks is partial."""
+    128); a dK, dV a part where the query tiles are cut into parts."""
     size = _abi.cross_bwd_workspace_bytes
     assert size(0, 4, 2, 8, 9, 64) == 256 and size(2, 4, 3, 8, 9, 64) == 256
     for d, kb in ((32, 128), (64, 128), (128, 64)):
-        b, h, hk, sq = 4, 37, 37, 200  # 148 key heads: whole waves, no tail
+        b, h, hk, sq = 4, 37, 37, 200  # 37 key heads, 16 key blocks: one part
         plain = 256 + b * h * 4 * 4 + b * h * sq * 4
         short, long = size(b, h, hk, sq, 16 * kb, d), size(b, h, hk, sq, 16 * kb + 1, d)
         assert plain + 16 * b * h * sq * d * 4 <= short <= plain + 16 * b * h * sq * d * 4 + 1024
         assert plain <= long <= plain + 1024
-    # 2 key blocks over 64 query tiles: dV, dK windows of every tile
-    assert size(1, 8, 1, 500, 200, 64) > 2 * 64 * 2 * 128 * 64 * 4
+    # 2 key blocks of one key head over 63 query tiles: 7 parts, each with a dK and dV of its own
+    parts = 7 * 200 * 2 * 64 * 4
+    whole = size(1, 8, 8, 500, 200, 64)  # 16 key blocks over 8 tiles each: one part
+    assert size(1, 8, 1, 500, 200, 64) - parts == whole
 
 
 def test_few_rows_arguments():
