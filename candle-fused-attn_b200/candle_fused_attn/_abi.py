@@ -64,6 +64,7 @@ EXPORTS = (
     "cfa_bwd_f32_ffma",
     "cfa_cross_fwd_f32",
     "cfa_cross_bwd_workspace_bytes",
+    "cfa_cross_bwd_workspace_bytes_fast",
     "cfa_cross_bwd_f32",
     "cfa_cross_few_workspace_bytes",
     "cfa_cross_few_f32",
@@ -158,6 +159,8 @@ def load() -> ctypes.CDLL:
                                       *[_i64] * 6, _f, _p]
     lib.cfa_cross_bwd_workspace_bytes.restype = _n
     lib.cfa_cross_bwd_workspace_bytes.argtypes = [_i64] * 6
+    lib.cfa_cross_bwd_workspace_bytes_fast.restype = _n
+    lib.cfa_cross_bwd_workspace_bytes_fast.argtypes = [_i64] * 6
     lib.cfa_cross_bwd_f32.restype = ctypes.c_int
     lib.cfa_cross_bwd_f32.argtypes = [_p, _strides, _p, _strides, _p, _strides, _p, _p, _p, _p,
                                       _strides, _p, _p, _p, _n, *[_i64] * 6, _f, _p]
@@ -354,6 +357,10 @@ def cross_fwd(q_ptr, qs, k_ptr, ks, v_ptr, vs, lengths_ptr, o_ptr, lse_ptr, b, h
 
 def cross_bwd_workspace_bytes(b, h, hk, sq, sk, d) -> int:
     return int(load().cfa_cross_bwd_workspace_bytes(b, h, hk, sq, sk, d))
+
+
+def cross_bwd_workspace_bytes_fast(b, h, hk, sq, sk, d) -> int:
+    return int(load().cfa_cross_bwd_workspace_bytes_fast(b, h, hk, sq, sk, d))
 
 
 def cross_bwd(q_ptr, qs, k_ptr, ks, v_ptr, vs, lengths_ptr, o_ptr, lse_ptr, do_ptr, dos, dq_ptr,

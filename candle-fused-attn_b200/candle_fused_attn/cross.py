@@ -84,7 +84,7 @@ class _CrossAttention(torch.autograd.Function):
         grad = _float4_rows(grad)
         dq = merged_heads(b, h, sq, d, q)
         dkv = torch.empty((b, sk, 2, hk, d), dtype=torch.float32, device=dev)
-        n = _abi.cross_bwd_workspace_bytes(b, h, hk, sq, sk, d)
+        n = _abi.cross_bwd_workspace_bytes_fast(b, h, hk, sq, sk, d)
         ws = torch.empty(n, dtype=torch.uint8, device=dev)
         with on_device(dev):
             st = _abi.cross_bwd(q.data_ptr(), q.stride()[:3], k.data_ptr(), k.stride()[:3],

@@ -152,6 +152,29 @@ __global__ void __launch_bounds__(NB, 1) cross_bwd_tc_kernel(const BwdArgs a) {
     cp_async16(st + 16 * (3 * NT + tid), g + 4, n16);
     stage_ld(n);
   };
+  // The block one wave later starts by reading its key block's K, V rows and its first query tile's
+  // Q, dO rows: pull them into L2 while this one computes (one row a thread).
+  auto prefetch_next_wave = [&]() {
+    const int64_t nb = static_cast<int64_t>(ticket) + a.wave_ctas;
+    if (a.wave_ctas <= 0 || nb >= gridDim.x || tid >= 2 * KB + 2 * QT) return;
+    const int npart = static_cast<int>(nb % nparts), nu = static_cast<int>(nb / nparts);
+    const int nk = chain ? nu / BH : nu % a.n_kblocks, nbh = chain ? nu % BH : nu / a.n_kblocks;
+    const int nb_b = nbh / a.Hk, nb_h = nbh % a.Hk;
+    const float* src;
+    if (tid < 2 * KB) {
+      const int r = nk * KB + (tid & (KB - 1));
+      if (r >= cross_keys(a, nb_b)) return;
+      src = tid < KB ? a.k + nb_b * a.k_sb + nb_h * a.k_sh + r * a.k_ss
+                     : a.v + nb_b * a.v_sb + nb_h * a.v_sh + r * a.v_ss;
+    } else {
+      const int r = static_cast<int>(static_cast<int64_t>(npart) * nqt / nparts) * QT + (tid & (QT - 1));
+      if (r >= rows) return;
+      const int g = group == 1 ? 0 : r / S;
+      src = tid < 2 * KB + QT ? a.q + nb_b * a.q_sb + (nb_h * group + g) * a.q_sh + (r - g * S) * a.q_ss
+                              : a.d_o + nb_b * a.do_sb + (nb_h * group + g) * a.do_sh + (r - g * S) * a.do_ss;
+    }
+    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src), "n"(4 * HD) : "memory");
+  };
   auto split_tile = [&](int n) {
     split_row_item(Qp + (n & 1) * 3 * PART_Q, PART_Q, st, 0, tid);
     split_row_item(dOp + (n & 1) * 3 * PART_Q, PART_Q, st, 1, tid);
@@ -195,6 +218,7 @@ __global__ void __launch_bounds__(NB, 1) cross_bwd_tc_kernel(const BwdArgs a) {
     }
     stage_ld(0);
     cp_async_commit();
+    prefetch_next_wave();
     err0 = !tc::mbar_wait(bar_ld, 0, WAIT_TIMEOUT_NS);
     cp_async_wait_all();
     split_staged_row<HD>(Kp, PART_K, k_rows, tid, nk);
@@ -607,6 +631,11 @@ cudaError_t setup_cross_bwd_tc_attributes() {
 cudaError_t launch_cross_bwd_tc(const BwdArgs& args, int head_dim, cudaStream_t stream) {
   BwdArgs a = args;
   a.n_kblocks = (a.Sk + KB - 1) / KB;
+  int dev = 0, sms = 0;  // one block per SM: a wave is the SM count
+  a.wave_ctas = cudaGetDevice(&dev) == cudaSuccess &&
+                        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess
+                    ? sms
+                    : 0;
   const int64_t blocks = static_cast<int64_t>(a.n_kblocks) * a.B * a.Hk * a.n_parts;
   const dim3 grid(static_cast<unsigned>(blocks));
   const cudaError_t e =

@@ -300,10 +300,14 @@ int cfa_cross_fwd_f32(const float* q, const int64_t q_strides[3],
 
 /* Its backward, from the forward's o and lse: dq [batch, seq, heads, head_dim] and dkv [batch,
  * key_seq, 2, key_heads, head_dim] (dK, dV interleaved), dense, written whole (rows past a key
- * length: zeros). Scratch (256-byte aligned, no initialisation) of the size the query gives;
+ * length: zeros). Scratch (256-byte aligned, no initialisation): at least the first size; with the
+ * second (up to 4 GB more; the first where the partials would take more) dQ goes by partials instead of
+ * a chain of key blocks that wait for one another -- the same results, bit for bit, in less time.
  * cfa_bwd_status reads its error flag. */
 size_t cfa_cross_bwd_workspace_bytes(int64_t batch, int64_t heads, int64_t key_heads, int64_t seq,
                                      int64_t key_seq, int64_t head_dim);
+size_t cfa_cross_bwd_workspace_bytes_fast(int64_t batch, int64_t heads, int64_t key_heads,
+                                          int64_t seq, int64_t key_seq, int64_t head_dim);
 int cfa_cross_bwd_f32(const float* q, const int64_t q_strides[3],
                       const float* k, const int64_t k_strides[3],
                       const float* v, const int64_t v_strides[3],

@@ -14,6 +14,7 @@ import pytest
 import torch
 
 import candle_fused_attn as cfa
+from candle_fused_attn import _abi
 import formulas as ref
 
 pytestmark = pytest.mark.gpu
@@ -94,8 +95,23 @@ def test_key_lengths(cuda, d, h, hk, sq, sk, lens):
 @pytest.mark.parametrize("d,sq,sk,h,hk", [(64, 100, 2500, 4, 2), (32, 70, 2100, 2, 1), (128, 80, 1100, 4, 2),
                                           (64, 513, 2048, 2, 2), (128, 65, 1024, 2, 1)])
 def test_long_key_sequences(cuda, d, sq, sk, h, hk):
-    """Past 16 key blocks dQ goes by the turn chain, up to them by partials."""
+    """Many key blocks: their dQ partials summed by the last of them, or by a kernel of its own."""
     check(cuda, 2, h, hk, sq, sk, d, [sk, sk // 2 + 3], seed=d)
+
+
+@pytest.mark.parametrize("d,h,hk,sq,sk", [(64, 8, 4, 300, 900), (32, 3, 1, 130, 700), (128, 4, 2, 200, 400),
+                                          (64, 1, 1, 1500, 150)])
+def test_turn_chain_gives_the_same_bits(cuda, monkeypatch, d, h, hk, sq, sk):
+    """The workspace too small for the dQ partials (what more than 4 GB of them are): key blocks add to
+    dQ in turn, the same sums in the same order."""
+    lens = [sk, sk // 2, 0]
+    _, _, o, grads = run(cuda, 3, h, hk, sq, sk, d, lens)
+    fast = _abi.cross_bwd_workspace_bytes_fast(3, h, hk, sq, sk, d)
+    least = _abi.cross_bwd_workspace_bytes(3, h, hk, sq, sk, d)
+    assert least < fast
+    monkeypatch.setattr(_abi, "cross_bwd_workspace_bytes_fast", lambda *a: least)
+    _, _, o2, chain = run(cuda, 3, h, hk, sq, sk, d, lens)
+    assert torch.equal(o, o2) and all(torch.equal(x, y) for x, y in zip(grads, chain))
 
 
 @pytest.mark.parametrize("d", [32, 64, 128])

@@ -57,16 +57,20 @@ def test_cross_backward_arguments():
 
 
 def test_cross_backward_workspace():
-    """D and the turn counters always; the dQ partials up to 16 key blocks (of 128; of 64 at head dim
-    128); a dK, dV a part where the query tiles are cut into parts."""
-    size = _abi.cross_bwd_workspace_bytes
-    assert size(0, 4, 2, 8, 9, 64) == 256 and size(2, 4, 3, 8, 9, 64) == 256
+    """D and the turn counters always, and a dK, dV a part where the query tiles are cut into parts; the
+    fast size adds the dQ partials, one a key block (of 128; of 64 at head dim 128), up to 4 GB."""
+    size, fast = _abi.cross_bwd_workspace_bytes, _abi.cross_bwd_workspace_bytes_fast
+    for fn in (size, fast):
+        assert fn(0, 4, 2, 8, 9, 64) == 256 and fn(2, 4, 3, 8, 9, 64) == 256
     for d, kb in ((32, 128), (64, 128), (128, 64)):
-        b, h, hk, sq = 4, 37, 37, 200  # 37 key heads, 16 key blocks: one part
+        b, h, sq = 4, 37, 200  # 37 key heads, at least 16 key blocks: one part
         plain = 256 + b * h * 4 * 4 + b * h * sq * 4
-        short, long = size(b, h, hk, sq, 16 * kb, d), size(b, h, hk, sq, 16 * kb + 1, d)
-        assert plain + 16 * b * h * sq * d * 4 <= short <= plain + 16 * b * h * sq * d * 4 + 1024
-        assert plain <= long <= plain + 1024
+        most = (4 << 30) // (b * h * sq * d * 4)
+        for n in (16, 17, most):
+            least = size(b, h, h, sq, n * kb, d)
+            assert plain <= least <= plain + 1024
+            assert fast(b, h, h, sq, n * kb, d) - least == n * b * h * sq * d * 4
+        assert fast(b, h, h, sq, most * kb + 1, d) == size(b, h, h, sq, most * kb + 1, d)
     # 2 key blocks of one key head over 63 query tiles: 7 parts, each with a dK and dV of its own
     parts = 7 * 200 * 2 * 64 * 4
     whole = size(1, 8, 8, 500, 200, 64)  # 16 key blocks over 8 tiles each: one part
