@@ -123,6 +123,24 @@ struct ChunkIndex {
   }
 };
 
+// What a block knows of its unit.
+struct UnitInfo {
+  int b, hk, r0, chunk, nc, len, n_new, lo, hi;  // rows r0 .., keys lo .. hi - 1
+};
+__device__ __forceinline__ UnitInfo unit_info(const SplitArgs& a, const ChunkIndex& ix, uint32_t u) {
+  UnitInfo n;
+  const uint32_t per = a.Hk * a.row_chunks;
+  const int g = static_cast<int>(u / per), rest = static_cast<int>(u - g * per);
+  n.hk = rest / a.row_chunks;
+  n.r0 = (rest - n.hk * a.row_chunks) * MAXR;
+  ix.find(a, g, n.b, n.chunk, n.nc);
+  n.len = seq_len(a, n.b);
+  n.n_new = seq_new(a, n.b);
+  const int c = chunk_log(n.len, a.tile_log);
+  n.lo = n.chunk << c;
+  n.hi = min(n.len, n.lo + (1 << c));  // (len <= 2^31 - 1025: no overflow)
+  return n;
+}
 // A 16-byte asynchronous copy past L1 (the rows are read once).
 __device__ __forceinline__ void cp_async16_full(void* smem, const void* gmem) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(tc::smem_u32(smem)), "l"(gmem)
@@ -130,7 +148,10 @@ __device__ __forceinline__ void cp_async16_full(void* smem, const void* gmem) {
 }
 
 // One warp's ring of tiles: TK rows of K, then of V, RB bytes apart, a stage a tile. Each lane copies
-// the 16-byte piece `lane % CPR` of every RPI-th row.
+// the 16-byte piece `lane % CPR` of every RPI-th row. The ring runs through the block's units (u, u +
+// grid, ..) and, in each, the warp's tiles (w, w + 4, ..) without a pause: ST - 1 tiles are in flight
+// while one is in use, those of the next unit behind the last of this one, and a unit's index and
+// first page are looked up an iteration before they are needed.
 template <int D, int ES, int TK_, int ST_>
 struct Ring {
   static constexpr int ST = ST_;   // stages
@@ -144,20 +165,41 @@ struct Ring {
   static constexpr unsigned ALL = 0xffffffffu >> (32 - TK);
 
   const SplitArgs& a;
+  const ChunkIndex& ix;
   unsigned char* base;
-  int lane;
+  int lane, w;
+  uint32_t units, unit;    // all of them; the one being loaded
+  UnitInfo info;           // (of unit)
   int64_t k_lane, v_lane;  // this lane's first row and piece within a tile, in bytes
   const char* kp;          // this (batch, key head)'s keys and values
   const char* vp;
   const int* table;
-  int lo, tiles, len, next, pg;  // the unit's first key, its tiles and end; the next tile, its page
-  unsigned live[ST];             // the live keys of the tiles in flight, oldest first
+  int tiles, next, pg;  // of the unit: its tiles; the next one, its page
+  unsigned live[ST];    // the live keys of the tiles in flight, oldest first
   bool bad = false;
 
-  __device__ __forceinline__ Ring(const SplitArgs& a_, unsigned char* base_, int lane_)
-      : a(a_), base(base_), lane(lane_) {
+  __device__ __forceinline__ Ring(const SplitArgs& a_, const ChunkIndex& ix_, uint32_t units_,
+                                  unsigned char* base_, int lane_, int w_)
+      : a(a_), ix(ix_), base(base_), lane(lane_), w(w_), units(units_), unit(blockIdx.x) {
     k_lane = (lane / CPR) * a.k_sr * ES + 16 * (lane % CPR);
     v_lane = (lane / CPR) * a.v_sr * ES + 16 * (lane % CPR);
+    open();
+#pragma unroll
+    for (int s = 0; s < ST - 1; ++s) live[s] = issue(s);
+  }
+  // Looks up `unit`, or the first after it that has a tile for this warp.
+  __device__ __forceinline__ void open() {
+    for (; unit < units; unit += gridDim.x) {
+      info = unit_info(a, ix, unit);
+      tiles = (info.hi - info.lo + TK - 1) / TK;
+      next = w;
+      if (next < tiles) break;
+    }
+    if (unit >= units) return;
+    kp = static_cast<const char*>(a.k) + ES * (info.hk * a.k_sh + (a.table ? 0 : info.b * a.k_sp));
+    vp = static_cast<const char*>(a.v) + ES * (info.hk * a.v_sh + (a.table ? 0 : info.b * a.v_sp));
+    table = a.table ? a.table + info.b * a.table_sb : nullptr;
+    pg = page_of(next);
   }
   __device__ __forceinline__ int page_at(int key) const {  // key / a.page (key < 2^31)
     return static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(key)) * a.page_mul) >> a.page_shift);
@@ -165,23 +207,9 @@ struct Ring {
   // The page of the next tile: of its first key, or (pages that end inside a tile) of this lane's
   // row. 0 where dense, -1 where there is none.
   __device__ __forceinline__ int page_of(int t) const {
-    const int key = lo + TK * t + (a.one_page ? 0 : (lane & (TK - 1)));
-    if (t >= tiles || key >= len) return -1;
+    const int key = info.lo + TK * t + (a.one_page ? 0 : (lane & (TK - 1)));
+    if (key >= info.hi) return -1;
     return table ? __ldg(table + page_at(key)) : 0;
-  }
-  // Starts a unit: keys lo_ .. hi_ - 1 of (b, hk), the warp's tiles w, w + 4, ..: the first ST - 1 of
-  // them travel.
-  __device__ __forceinline__ void start(int b, int hk, int lo_, int hi_, int w) {
-    lo = lo_;
-    len = hi_;
-    tiles = (hi_ - lo_ + TK - 1) / TK;
-    next = w;
-    kp = static_cast<const char*>(a.k) + ES * (hk * a.k_sh + (a.table ? 0 : b * a.k_sp));
-    vp = static_cast<const char*>(a.v) + ES * (hk * a.v_sh + (a.table ? 0 : b * a.v_sp));
-    table = a.table ? a.table + b * a.table_sb : nullptr;
-    pg = page_of(next);
-#pragma unroll
-    for (int s = 0; s < ST - 1; ++s) live[s] = issue(s);
   }
   // The oldest tile's live keys as bits; the tile after those in flight goes into `stage`.
   __device__ __forceinline__ unsigned advance(int stage) {
@@ -193,19 +221,23 @@ struct Ring {
   }
   __device__ __forceinline__ unsigned issue(int stage) {
     unsigned x = 0;
-    if (next < tiles) {
-      const int now = pg;
-      const int k0 = lo + TK * next;
+    if (unit < units) {
+      const int k0 = info.lo + TK * next;
+      x = a.one_page ? load_page(k0, stage, pg) : load_rows(k0, stage, pg);
       next += WARPS;
-      pg = page_of(next);
-      x = a.one_page ? load_page(k0, stage, now) : load_rows(k0, stage, now);
+      if (next < tiles) {
+        pg = page_of(next);
+      } else {
+        unit += gridDim.x;
+        open();
+      }
     }
     cp_async_commit();
     return x;
   }
   // A tile whose rows lie on one page (page sizes that are multiples of TK; a dense operand).
   __device__ __forceinline__ unsigned load_page(int k0, int stage, int p) {
-    int rows = min(TK, len - k0);
+    int rows = min(TK, info.hi - k0);
     int64_t ko = 0, vo = 0;
     if (!table) {
       ko = k0 * a.k_sr;
@@ -241,7 +273,7 @@ struct Ring {
   // Any page size: lane r % TK finds row r's address, the copying lanes ask it for theirs.
   __device__ __forceinline__ unsigned load_rows(int k0, int stage, int p) {
     const int key = k0 + (lane & (TK - 1));
-    bool ok = key < len;
+    bool ok = key < info.hi;
     int64_t ko = 0, vo = 0;
     if (ok && (p < 0 || p >= a.n_pages)) {
       ok = false;
@@ -322,24 +354,6 @@ __device__ __forceinline__ float2 unpack16(uint32_t x) {
   else return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
 }
 
-// What a block knows of its unit.
-struct UnitInfo {
-  int b, hk, r0, chunk, nc, len, n_new, lo, hi;  // rows r0 .., keys lo .. hi - 1
-};
-__device__ __forceinline__ UnitInfo unit_info(const SplitArgs& a, const ChunkIndex& ix, uint32_t u) {
-  UnitInfo n;
-  const uint32_t per = a.Hk * a.row_chunks;
-  const int g = static_cast<int>(u / per), rest = static_cast<int>(u - g * per);
-  n.hk = rest / a.row_chunks;
-  n.r0 = (rest - n.hk * a.row_chunks) * MAXR;
-  ix.find(a, g, n.b, n.chunk, n.nc);
-  n.len = seq_len(a, n.b);
-  n.n_new = seq_new(a, n.b);
-  const int c = chunk_log(n.len, a.tile_log);
-  n.lo = n.chunk << c;
-  n.hi = min(n.len, n.lo + (1 << c));  // (len <= 2^31 - 1025: no overflow)
-  return n;
-}
 // Row r of a key head's rows: query head r / S of the group, new token r % S.
 __device__ __forceinline__ void row_of(const SplitArgs& a, int r, int& head, int& i) {
   head = a.S == 1 ? r : r / a.S;
@@ -353,12 +367,13 @@ __device__ __forceinline__ int row_limit(const SplitArgs& a, const UnitInfo& n, 
   return min(max(n.len - n.n_new + i + 1, 0), n.len);
 }
 
-// Joins the four warps' sums of the block's first nr rows (a warp's: [row][D], red_step bytes from
-// warp to warp; ml: [warp][row]) and writes the chunk's partial result, or, the sequence's only chunk,
+// Joins the four warps' sums of the block's first nr rows (warp w's: [row][D] at red + red_at[w]; ml:
+// [warp][row]) and writes the chunk's partial result, or, the sequence's only chunk,
 // the output.
 template <typename QT, int D>
 __device__ __forceinline__ void write_chunk(const SplitArgs& a, const UnitInfo& n,
-                                            const unsigned char* red, int red_step, const float2* ml,
+                                            const unsigned char* red, const int* red_at,
+                                            const float2* ml,
                                             int nr) {
   for (int idx = threadIdx.x; idx < nr * (D / 4); idx += NT) {
     const int r = idx / (D / 4), c4 = idx % (D / 4);
@@ -377,7 +392,7 @@ __device__ __forceinline__ void write_chunk(const SplitArgs& a, const UnitInfo& 
     for (int w = 0; w < WARPS; ++w) {
       const float2 x = ml[w * MAXR + r];
       const float f = ex2((x.x - mu) * LOG2E);
-      const float4 v = *reinterpret_cast<const float4*>(red + w * red_step + (r * D + 4 * c4) * 4);
+      const float4 v = *reinterpret_cast<const float4*>(red + red_at[w] + (r * D + 4 * c4) * 4);
       l = fmaf(x.y, f, l);
       o.x = fmaf(v.x, f, o.x);
       o.y = fmaf(v.y, f, o.y);
@@ -407,8 +422,8 @@ __host__ __device__ constexpr int tile_keys() {
 }
 template <int D, int ES>
 using RingOf = Ring<D, ES, tile_keys<D, ES>(), (ES == 2 ? 3 : 2)>;
-// Shared memory: the rings -- whose last stage also takes a warp's sums when a unit ends -- the (m, l)
-// of the warps' rows, and the fp32 kernel's two sets of query rows.
+// Shared memory: the rings -- whose free stage also takes a warp's sums when a unit ends -- the (m, l)
+// of the warps' rows and where their sums are, and the fp32 kernel's two sets of query rows.
 template <int D, int ES>
 __host__ __device__ constexpr int off_ml() {
   static_assert(RingOf<D, ES>::STAGE >= MAXR * D * 4, "a stage holds a warp's sums");
@@ -416,7 +431,7 @@ __host__ __device__ constexpr int off_ml() {
 }
 template <int D, int ES>
 __host__ __device__ constexpr int off_q() {
-  return off_ml<D, ES>() + WARPS * MAXR * 8;
+  return off_ml<D, ES>() + WARPS * MAXR * 8 + WARPS * 4;
 }
 template <int D, int ES>
 __host__ __device__ constexpr int split_smem(int q_rows) {
@@ -438,14 +453,14 @@ __global__ void __launch_bounds__(NT, 2)
   extern __shared__ __align__(128) unsigned char smem[];
   const int tid = threadIdx.x, w = tid >> 5, lane = tid & 31;
   const int qr = lane >> 2, qc = lane & 3;  // a fragment's row (key, dim; B: column) and pair
-  unsigned char* red = smem + (ST - 1) * R::STAGE;
   float2* ml = reinterpret_cast<float2*>(smem + off_ml<D, 2>());
+  int* red_at = reinterpret_cast<int*>(ml + WARPS * MAXR);
   griddep_wait();
   griddep_launch_dependents();
   ChunkIndex ix;
   ix.init(a, lane);
   const uint32_t units = static_cast<uint32_t>(ix.total) * a.Hk * a.row_chunks;
-  R ring(a, smem + w * R::BYTES, lane);
+  R ring(a, ix, units, smem + w * R::BYTES, lane, w);
 
   // Q^T's pairs of column qr: dims 16 ks + 2 qc, + 1 and + 8, + 9 (zeros where there is no row).
   QPair qx[KS][2];
@@ -465,11 +480,11 @@ __global__ void __launch_bounds__(NT, 2)
   UnitInfo n;
   if (blockIdx.x < units) {
     n = unit_info(a, ix, blockIdx.x);
-    ring.start(n.b, n.hk, n.lo, n.hi, w);
     load_q(n);
   }
+  int stage = 0;  // of the next tile; the stage before it is free
   for (uint32_t u = blockIdx.x; u < units; u += gridDim.x) {
-    const int tiles = ring.tiles;
+    const int tiles = (n.hi - n.lo + TK - 1) / TK;
     // Q^T as B fragments.
     uint32_t qb[QP][KS][2];
     float qscale0 = a.scale, qscale1 = a.scale;  // of columns 2 qc, 2 qc + 1
@@ -525,7 +540,6 @@ __global__ void __launch_bounds__(NT, 2)
 #pragma unroll
       for (int j = 0; j < 4; ++j) acc[i][j] = 0.0f;
 
-    int stage = 0;
     for (int t = w; t < tiles; t += WARPS) {
       cp_async_wait_group<ST - 2>();
       __syncwarp();  // the tile is in place for every lane, and the stage before it is free
@@ -673,27 +687,28 @@ __global__ void __launch_bounds__(NT, 2)
       l0 += __shfl_xor_sync(0xffffffffu, l0, o);
       l1 += __shfl_xor_sync(0xffffffffu, l1, o);
     }
-    // The next unit's first tiles and queries travel while this one's sums are joined.
+    // The next unit's queries travel while this one's sums are joined.
     const UnitInfo done = n;
+    const int free_at = w * R::BYTES + (stage == 0 ? ST - 1 : stage - 1) * R::STAGE;
     __syncwarp();  // every lane has read its last tile
     if (u + gridDim.x < units) {
-      n = unit_info(a, ix, u + gridDim.x);
-      ring.start(n.b, n.hk, n.lo, n.hi, w);
+      n = ring.unit == u + gridDim.x ? ring.info : unit_info(a, ix, u + gridDim.x);
       load_q(n);
     }
+    if (lane == 0) red_at[w] = free_at;
     if (qr == 0) {
       ml[w * MAXR + 2 * qc] = make_float2(m0, l0);
       ml[w * MAXR + 2 * qc + 1] = make_float2(m1, l1);
     }
-    float* sums = reinterpret_cast<float*>(red + w * R::BYTES);  // (this warp's last stage: free)
+    float* sums = reinterpret_cast<float*>(smem + free_at);
 #pragma unroll
     for (int mt = 0; mt < KS; ++mt)
 #pragma unroll
       for (int j = 0; j < 4; ++j)
         sums[(2 * qc + (j & 1)) * D + 16 * mt + qr + 8 * (j >> 1)] = acc[mt][j];
     __syncthreads();
-    write_chunk<QT, D>(a, done, red, R::BYTES, ml, min(MAXR, a.rows - done.r0));
-    __syncthreads();  // the sums are read: the last stages take tiles again
+    write_chunk<QT, D>(a, done, smem, red_at, ml, min(MAXR, a.rows - done.r0));
+    __syncthreads();  // the sums are read: their stages take tiles again
   }
   if (ring.bad) flag_error(a.sink, CFA_ERR_PAGE);
 }
@@ -707,15 +722,15 @@ __global__ void __launch_bounds__(NT, 3) split_f32_kernel(const SplitArgs a) {
   constexpr int LPR = D / 4, KPI = 32 / LPR;  // lanes of a V row; keys at a time
   extern __shared__ __align__(128) unsigned char smem[];
   const int tid = threadIdx.x, w = tid >> 5, lane = tid & 31;
-  unsigned char* red = smem + (ST - 1) * R::STAGE;
   float2* ml = reinterpret_cast<float2*>(smem + off_ml<D, 4>());
+  int* red_at = reinterpret_cast<int*>(ml + WARPS * MAXR);
   float* q_sets = reinterpret_cast<float*>(smem + off_q<D, 4>());  // two sets of [NR][D]
   griddep_wait();
   griddep_launch_dependents();
   ChunkIndex ix;
   ix.init(a, lane);
   const uint32_t units = static_cast<uint32_t>(ix.total) * a.Hk * a.row_chunks;
-  R ring(a, smem + w * R::BYTES, lane);
+  R ring(a, ix, units, smem + w * R::BYTES, lane, w);
 
   auto load_q = [&](const UnitInfo& n, float* qs) {
     for (int i = tid; i < NR * LPR; i += NT) {
@@ -732,14 +747,14 @@ __global__ void __launch_bounds__(NT, 3) split_f32_kernel(const SplitArgs a) {
   UnitInfo n;
   if (blockIdx.x < units) {
     n = unit_info(a, ix, blockIdx.x);
-    ring.start(n.b, n.hk, n.lo, n.hi, w);
     load_q(n, q_sets);
     __syncthreads();  // q in place
   }
+  int stage = 0;  // of the next tile; the stage before it is free
   int set = 0;
   for (uint32_t u = blockIdx.x; u < units; u += gridDim.x, set ^= 1) {
     const float* qs = q_sets + set * (NR * D);
-    const int tiles = ring.tiles;
+    const int tiles = (n.hi - n.lo + TK - 1) / TK;
     const int lim_min = a.causal ? max(n.len - n.n_new + 1, 0) : n.len;
     float m[NR], l[NR], acc[NR][4];
 #pragma unroll
@@ -747,7 +762,6 @@ __global__ void __launch_bounds__(NT, 3) split_f32_kernel(const SplitArgs a) {
       m[r] = -INFINITY;
       l[r] = acc[r][0] = acc[r][1] = acc[r][2] = acc[r][3] = 0.0f;
     }
-    int stage = 0;
     for (int t = w; t < tiles; t += WARPS) {
       cp_async_wait_group<ST - 2>();
       __syncwarp();
@@ -815,15 +829,16 @@ __global__ void __launch_bounds__(NT, 3) split_f32_kernel(const SplitArgs a) {
 #pragma unroll
         for (int c = 0; c < 4; ++c) acc[r][c] += __shfl_xor_sync(0xffffffffu, acc[r][c], o);
     }
-    // The next unit's first tiles and queries travel while this one's sums are joined.
+    // The next unit's queries travel while this one's sums are joined.
     const UnitInfo done = n;
+    const int free_at = w * R::BYTES + (stage == 0 ? ST - 1 : stage - 1) * R::STAGE;
     __syncwarp();  // every lane has read its last tile
     if (u + gridDim.x < units) {
-      n = unit_info(a, ix, u + gridDim.x);
-      ring.start(n.b, n.hk, n.lo, n.hi, w);
+      n = ring.unit == u + gridDim.x ? ring.info : unit_info(a, ix, u + gridDim.x);
       load_q(n, q_sets + (set ^ 1) * (NR * D));
     }
-    float* sums = reinterpret_cast<float*>(red + w * R::BYTES);  // (this warp's last stage: free)
+    if (lane == 0) red_at[w] = free_at;
+    float* sums = reinterpret_cast<float*>(smem + free_at);
 #pragma unroll
     for (int r = 0; r < NR; ++r) {
       if (lane == 0) ml[w * MAXR + r] = make_float2(m[r], l[r]);
@@ -832,37 +847,78 @@ __global__ void __launch_bounds__(NT, 3) split_f32_kernel(const SplitArgs a) {
             make_float4(acc[r][0], acc[r][1], acc[r][2], acc[r][3]);
     }
     __syncthreads();  // (the next unit's queries are in place too)
-    write_chunk<float, D>(a, done, red, R::BYTES, ml, min(NR, a.rows - done.r0));
-    __syncthreads();  // the sums are read: the last stages take tiles again
+    write_chunk<float, D>(a, done, smem, red_at, ml, min(NR, a.rows - done.r0));
+    __syncthreads();  // the sums are read: their stages take tiles again
   }
   if (ring.bad) flag_error(a.sink, CFA_ERR_PAGE);
 }
 
-// The chunks' join: a block per output row; its threads take the row's float4 columns and, side by
-// side, every G-th chunk, then add their sums in order.
+// The chunks' join, chunk c of a row in group c % G (G = 128 / (D / 4)): the groups' sums in chunk order,
+// then over the groups in order. Everything that does not come from the chunks' kernel is read before
+// waiting for it: that kernel has waited for its own predecessors when it lets this one start.
+template <int D>
+struct JoinRow {
+  static constexpr int C4 = D / 4, G = NT / C4;
+  int64_t row;  // (b H + head) S + i
+  int b, head, i, nc;
+  bool live;
+  __device__ __forceinline__ JoinRow(const SplitArgs& a, int64_t row_) : row(row_) {
+    i = a.S == 1 ? 0 : static_cast<int>(row % a.S);
+    const int64_t bh = a.S == 1 ? row : row / a.S;
+    b = static_cast<int>(bh / a.H);
+    head = static_cast<int>(bh - static_cast<int64_t>(b) * a.H);
+    nc = chunks_of(seq_len(a, b), a.tile_log);
+    live = i < seq_new(a, b);
+  }
+  template <typename QT>
+  __device__ __forceinline__ void store(const SplitArgs& a, int c4, float4 o, float l) const {
+    const bool some = live && l != 0.0f;
+    QT* dst = static_cast<QT*>(a.o) + ((static_cast<int64_t>(b) * a.S + i) * a.H + head) * D + 4 * c4;
+    dst[0] = from_f<QT>(some ? o.x / l : 0.0f);
+    dst[1] = from_f<QT>(some ? o.y / l : 0.0f);
+    dst[2] = from_f<QT>(some ? o.z / l : 0.0f);
+    dst[3] = from_f<QT>(some ? o.w / l : 0.0f);
+  }
+};
+__device__ __forceinline__ void fold(float4& o, float4 v, float f) {
+  o.x = fmaf(v.x, f, o.x);
+  o.y = fmaf(v.y, f, o.y);
+  o.z = fmaf(v.z, f, o.z);
+  o.w = fmaf(v.w, f, o.w);
+}
+__device__ __forceinline__ float4 plus(float4 o, float4 v) {
+  return make_float4(o.x + v.x, o.y + v.y, o.z + v.z, o.w + v.w);
+}
+
+// A block a row; its threads take the row's columns and, side by side, the groups. The first chunks of
+// each group travel while the weights are found.
 template <typename QT, int D>
 __global__ void __launch_bounds__(NT) split_join_kernel(const SplitArgs a) {
-  constexpr int C4 = D / 4, G = NT / C4;
+  using J = JoinRow<D>;
   __shared__ float wt[MOST_CHUNKS];
-  __shared__ float4 sums[G][C4];
+  __shared__ float4 sums[J::G][J::C4];
   __shared__ float red[2][WARPS];
+  const int tid = threadIdx.x, w = tid >> 5, lane = tid & 31;
+  const J r(a, blockIdx.x);
   griddep_wait();
   griddep_launch_dependents();
-  const int tid = threadIdx.x, w = tid >> 5, lane = tid & 31;
-  const int64_t row = blockIdx.x;  // (b H + head) S + i
-  const int i = static_cast<int>(row % a.S);
-  const int64_t bh = row / a.S;
-  const int b = static_cast<int>(bh / a.H), head = static_cast<int>(bh % a.H);
-  const int nc = chunks_of(seq_len(a, b), a.tile_log);
-  if (nc == 1) return;  // written by the first kernel
-  const bool live = i < seq_new(a, b);
-  const float2* ml = a.part_ml + row * a.max_chunks;
+  if (r.nc == 1) return;  // written by the first kernel
+  const float2* ml = a.part_ml + r.row * a.max_chunks;
+  const int c4 = tid % J::C4, g = tid / J::C4;
+  const float4* po = reinterpret_cast<const float4*>(a.part_o + r.row * a.max_chunks * D) + c4;
+  constexpr int EARLY = 4;
+  float4 early[EARLY];
+#pragma unroll
+  for (int j = 0; j < EARLY; ++j) {
+    const int c = g + J::G * j;
+    early[j] = r.live && c < r.nc ? po[static_cast<int64_t>(c) * J::C4] : make_float4(0.f, 0.f, 0.f, 0.f);
+  }
   float m = -INFINITY;
   float2 x[MOST_CHUNKS / NT];
 #pragma unroll
   for (int j = 0; j < MOST_CHUNKS / NT; ++j) {
     const int c = tid + j * NT;
-    x[j] = live && c < nc ? ml[c] : make_float2(-INFINITY, 0.0f);
+    x[j] = r.live && c < r.nc ? ml[c] : make_float2(-INFINITY, 0.0f);
     m = fmaxf(m, x[j].x);
   }
 #pragma unroll
@@ -877,42 +933,28 @@ __global__ void __launch_bounds__(NT) split_join_kernel(const SplitArgs a) {
   for (int j = 0; j < MOST_CHUNKS / NT; ++j) {
     const int c = tid + j * NT;
     const float f = ex2((x[j].x - mu) * LOG2E);
-    if (c < nc) wt[c] = f;
-    l = fmaf(x[j].y, f, l);
+    if (c < r.nc) wt[c] = f;
+    l = j == 0 ? x[j].y * f : fmaf(x[j].y, f, l);
   }
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
   if (lane == 0) red[1][w] = l;
   __syncthreads();
   l = ((red[1][0] + red[1][1]) + red[1][2]) + red[1][3];
-  const int c4 = tid % C4, g = tid / C4;
-  const float4* po = reinterpret_cast<const float4*>(a.part_o + row * a.max_chunks * D) + c4;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (live) {
+  if (r.live) {
+#pragma unroll
+    for (int j = 0; j < EARLY; ++j)
+      if (g + J::G * j < r.nc) fold(o, early[j], wt[g + J::G * j]);
 #pragma unroll 8
-    for (int c = g; c < nc; c += G) {
-      const float4 v = po[static_cast<int64_t>(c) * C4];
-      const float f = wt[c];
-      o.x = fmaf(v.x, f, o.x);
-      o.y = fmaf(v.y, f, o.y);
-      o.z = fmaf(v.z, f, o.z);
-      o.w = fmaf(v.w, f, o.w);
-    }
+    for (int c = g + J::G * EARLY; c < r.nc; c += J::G) fold(o, po[static_cast<int64_t>(c) * J::C4], wt[c]);
   }
   sums[g][c4] = o;
   __syncthreads();
   if (g == 0) {
 #pragma unroll
-    for (int j = 1; j < G; ++j) {
-      const float4 v = sums[j][c4];
-      o = make_float4(o.x + v.x, o.y + v.y, o.z + v.z, o.w + v.w);
-    }
-    const bool some = live && l != 0.0f;
-    QT* dst = static_cast<QT*>(a.o) + ((static_cast<int64_t>(b) * a.S + i) * a.H + head) * D + 4 * c4;
-    dst[0] = from_f<QT>(some ? o.x / l : 0.0f);
-    dst[1] = from_f<QT>(some ? o.y / l : 0.0f);
-    dst[2] = from_f<QT>(some ? o.z / l : 0.0f);
-    dst[3] = from_f<QT>(some ? o.w / l : 0.0f);
+    for (int j = 1; j < J::G; ++j) o = plus(o, sums[j][c4]);
+    r.template store<QT>(a, c4, o, l);
   }
 }
 
@@ -939,8 +981,8 @@ cudaError_t launch_split(int smem, const SplitArgs& a, cudaStream_t stream) {
 template <typename QT, int D>
 cudaError_t launch_join(const SplitArgs& a, cudaStream_t stream) {
   if (a.max_chunks == 1) return cudaSuccess;
-  return launch_pdl(split_join_kernel<QT, D>, dim3(static_cast<unsigned>(a.B * a.H * a.S)), dim3(NT),
-                    0, stream, a);
+  const int64_t rows = static_cast<int64_t>(a.B) * a.H * a.S;
+  return launch_pdl(split_join_kernel<QT, D>, dim3(static_cast<unsigned>(rows)), dim3(NT), 0, stream, a);
 }
 
 template <int D>

@@ -169,6 +169,20 @@ def test_bitwise_reruns_batches_and_shared_pages(cuda):
         assert torch.equal(o2[0], o[2]) and torch.equal(o2[1], o[2]) and torch.equal(o2[2], o[0])
 
 
+@pytest.mark.parametrize("qt,kt", TYPES)
+@pytest.mark.parametrize("d", [32, 64, 128])
+def test_a_wider_table_changes_nothing(cuda, qt, kt, d):
+    """Room for more pages (and with it another way of joining the chunks): the same bits."""
+    args, _ = check_attention(cuda, [5000, 31, 2000, 600], 4, 2, 1, d, 16, "token", qt, kt)
+    q, kc, vc, table, lengths = args
+    want = cfa.paged_attention(*args, 0.125)
+    for width in (2000, 20000):
+        wide = torch.full((4, width), -1, dtype=torch.int32, device=cuda)
+        wide[:, :table.shape[1]] = table
+        assert torch.equal(cfa.paged_attention(q, kc, vc, wide, lengths, 0.125), want)
+    cfa.check_status()
+
+
 def test_strided_and_unaligned_queries(cuda):
     args, _ = check_attention(cuda, [100, 40], 4, 2, 1, 64, 16, "token", F32, F32)
     q, rest = args[0], args[1:]
