@@ -423,7 +423,7 @@ __host__ __device__ constexpr int tile_keys() {
 template <int D, int ES>
 using RingOf = Ring<D, ES, tile_keys<D, ES>(), (ES == 2 ? 3 : 2)>;
 // Shared memory: the rings -- whose free stage also takes a warp's sums when a unit ends -- the (m, l)
-// of the warps' rows and where their sums are, and the fp32 kernel's two sets of query rows.
+// of the warps' rows and where their sums are, and the fp32 kernel's two sets of query rows and its p.
 template <int D, int ES>
 __host__ __device__ constexpr int off_ml() {
   static_assert(RingOf<D, ES>::STAGE >= MAXR * D * 4, "a stage holds a warp's sums");
@@ -435,7 +435,7 @@ __host__ __device__ constexpr int off_q() {
 }
 template <int D, int ES>
 __host__ __device__ constexpr int split_smem(int q_rows) {
-  return off_q<D, ES>() + 2 * q_rows * D * 4;
+  return off_q<D, ES>() + q_rows * (2 * D * 4 + WARPS * tile_keys<D, ES>() * 8);
 }
 
 // 16-bit caches.
@@ -725,6 +725,7 @@ __global__ void __launch_bounds__(NT, 3) split_f32_kernel(const SplitArgs a) {
   float2* ml = reinterpret_cast<float2*>(smem + off_ml<D, 4>());
   int* red_at = reinterpret_cast<int*>(ml + WARPS * MAXR);
   float* q_sets = reinterpret_cast<float*>(smem + off_q<D, 4>());  // two sets of [NR][D]
+  uint64_t* ps = reinterpret_cast<uint64_t*>(q_sets + 2 * NR * D) + w * TK * NR;  // p twice: [key][NR]
   griddep_wait();
   griddep_launch_dependents();
   ChunkIndex ix;
@@ -756,11 +757,13 @@ __global__ void __launch_bounds__(NT, 3) split_f32_kernel(const SplitArgs a) {
     const float* qs = q_sets + set * (NR * D);
     const int tiles = (n.hi - n.lo + TK - 1) / TK;
     const int lim_min = a.causal ? max(n.len - n.n_new + 1, 0) : n.len;
-    float m[NR], l[NR], acc[NR][4];
+    float m[NR], l[NR];
+    uint64_t acc[NR][2];  // this lane's four dims, packed
 #pragma unroll
     for (int r = 0; r < NR; ++r) {
       m[r] = -INFINITY;
-      l[r] = acc[r][0] = acc[r][1] = acc[r][2] = acc[r][3] = 0.0f;
+      l[r] = 0.0f;
+      acc[r][0] = acc[r][1] = 0ull;
     }
     for (int t = w; t < tiles; t += WARPS) {
       cp_async_wait_group<ST - 2>();
@@ -771,21 +774,25 @@ __global__ void __launch_bounds__(NT, 3) split_f32_kernel(const SplitArgs a) {
       const int k0 = n.lo + TK * t;
       const bool edge = lim_min < min(k0 + TK, n.hi);
       // Scores: lane x takes dims DL (x / TK) .. of key x % TK.
-      float s[NR];
+      // (packed fp32: dims 4 c, 4 c + 2, .. and the odd ones in two chains, added at the end)
+      uint64_t s2[NR];
 #pragma unroll
-      for (int r = 0; r < NR; ++r) s[r] = 0.0f;
+      for (int r = 0; r < NR; ++r) s2[r] = 0ull;
       const float* kr = reinterpret_cast<const float*>(kt + (lane % TK) * R::RB) + lane / TK * DL;
       const float* qh = qs + lane / TK * DL;
 #pragma unroll
       for (int c = 0; c < DL / 4; ++c) {
-        const float4 x = reinterpret_cast<const float4*>(kr)[c];
+        const ulonglong2 x = ld2x2(kr + 4 * c);
 #pragma unroll
-        for (int r = 0; r < NR; ++r) s[r] = dot4(x, ld4(qh + r * D + 4 * c), s[r]);
+        for (int r = 0; r < NR; ++r) {
+          const ulonglong2 y = ld2x2(qh + r * D + 4 * c);
+          s2[r] = fma2(x.y, y.y, fma2(x.x, y.x, s2[r]));
+        }
       }
       float p[NR];
 #pragma unroll
       for (int r = 0; r < NR; ++r) {
-        float y = s[r];
+        float y = sum2(s2[r]);
 #pragma unroll
         for (int o = TK; o < 32; o <<= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
         y *= a.scale;
@@ -800,34 +807,56 @@ __global__ void __launch_bounds__(NT, 3) split_f32_kernel(const SplitArgs a) {
         m[r] = top;
         p[r] = ex2((y - mu) * LOG2E);
         l[r] = fmaf(l[r], al, p[r]);  // this lane's keys (the lanes of a key hold the same)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) acc[r][c] *= al;
+        const uint64_t al2 = dup2(al);
+        acc[r][0] = mul2(acc[r][0], al2);
+        acc[r][1] = mul2(acc[r][1], al2);
+        if (lane < TK) ps[lane * NR + r] = dup2(p[r]);
       }
+      __syncwarp();  // every key's p in place
+      auto fold_keys = [&](auto masked) {
 #pragma unroll
-      for (int j = 0; j < TK / KPI; ++j) {
-        const int k = KPI * j + lane / LPR;
-        const float4 v = *reinterpret_cast<const float4*>(vt + k * R::RB + 16 * (lane % LPR));
+        for (int j = 0; j < TK / KPI; ++j) {
+          const int k = KPI * j + lane / LPR;
+          const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(vt + k * R::RB + 16 * (lane % LPR));
+          uint64_t pk[NR];
+          if constexpr (NR == 1) {
+            pk[0] = ps[k];
+          } else {
 #pragma unroll
-        for (int r = 0; r < NR; ++r) {
-          const float pk = __shfl_sync(0xffffffffu, p[r], k);
-          if (!edge || pk != 0.0f) {  // an unseen key's value may be NaN
-            acc[r][0] = fmaf(pk, v.x, acc[r][0]);
-            acc[r][1] = fmaf(pk, v.y, acc[r][1]);
-            acc[r][2] = fmaf(pk, v.z, acc[r][2]);
-            acc[r][3] = fmaf(pk, v.w, acc[r][3]);
+            for (int r = 0; r < NR; r += 2) {
+              const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(ps + k * NR + r);
+              pk[r] = x.x;
+              pk[r + 1] = x.y;
+            }
+          }
+#pragma unroll
+          for (int r = 0; r < NR; ++r) {
+            if (!decltype(masked)::value || pk[r] != 0ull) {
+              acc[r][0] = fma2(pk[r], v.x, acc[r][0]);
+              acc[r][1] = fma2(pk[r], v.y, acc[r][1]);
+            }
           }
         }
-      }
+      };
+      if (!edge) fold_keys(std::false_type{});
+      else fold_keys(std::true_type{});  // an unseen key's value may be NaN
+      __syncwarp();  // read: the next tile's p may land
       stage = stage + 1 == ST ? 0 : stage + 1;
     }
+    float4 o4[NR];
 #pragma unroll
     for (int r = 0; r < NR; ++r) {
 #pragma unroll
       for (int o = 1; o < TK; o <<= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], o);
+      const float2 lo = split2(acc[r][0]), hi = split2(acc[r][1]);
+      o4[r] = make_float4(lo.x, lo.y, hi.x, hi.y);
 #pragma unroll
-      for (int o = LPR; o < 32; o <<= 1)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) acc[r][c] += __shfl_xor_sync(0xffffffffu, acc[r][c], o);
+      for (int o = LPR; o < 32; o <<= 1) {
+        o4[r].x += __shfl_xor_sync(0xffffffffu, o4[r].x, o);
+        o4[r].y += __shfl_xor_sync(0xffffffffu, o4[r].y, o);
+        o4[r].z += __shfl_xor_sync(0xffffffffu, o4[r].z, o);
+        o4[r].w += __shfl_xor_sync(0xffffffffu, o4[r].w, o);
+      }
     }
     // The next unit's queries travel while this one's sums are joined.
     const UnitInfo done = n;
@@ -843,8 +872,7 @@ __global__ void __launch_bounds__(NT, 3) split_f32_kernel(const SplitArgs a) {
     for (int r = 0; r < NR; ++r) {
       if (lane == 0) ml[w * MAXR + r] = make_float2(m[r], l[r]);
       if (lane < LPR)
-        *reinterpret_cast<float4*>(sums + r * D + 4 * lane) =
-            make_float4(acc[r][0], acc[r][1], acc[r][2], acc[r][3]);
+        *reinterpret_cast<float4*>(sums + r * D + 4 * lane) = o4[r];
     }
     __syncthreads();  // (the next unit's queries are in place too)
     write_chunk<float, D>(a, done, smem, red_at, ml, min(NR, a.rows - done.r0));
