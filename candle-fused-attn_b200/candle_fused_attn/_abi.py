@@ -359,6 +359,7 @@ def cross_bwd_workspace_bytes(b, h, hk, sq, sk, d) -> int:
     return int(load().cfa_cross_bwd_workspace_bytes(b, h, hk, sq, sk, d))
 
 
+@functools.lru_cache(maxsize=1024)
 def cross_bwd_workspace_bytes_fast(b, h, hk, sq, sk, d) -> int:
     return int(load().cfa_cross_bwd_workspace_bytes_fast(b, h, hk, sq, sk, d))
 
@@ -372,6 +373,7 @@ def cross_bwd(q_ptr, qs, k_ptr, ks, v_ptr, vs, lengths_ptr, o_ptr, lse_ptr, do_p
         stream)
 
 
+@functools.lru_cache(maxsize=1024)
 def cross_few_workspace_bytes(b, h, sq, sk, d) -> int:
     return int(load().cfa_cross_few_workspace_bytes(b, h, sq, sk, d))
 
@@ -404,6 +406,7 @@ def paged_append(q_ptr, qs, qo_ptr, qos, k_ptr, ks, v_ptr, vs, dtype, kc_ptr, kc
         lengths_ptr, new_ptr, freqs_ptr, amplitude, b, h, hk, s, d, rot, int(interleaved), stream)
 
 
+@functools.lru_cache(maxsize=1024)
 def paged_attention_workspace_bytes(b, h, s, max_keys, d, cache_dtype) -> int:
     return int(load().cfa_paged_attention_workspace_bytes(b, h, s, max_keys, d, cache_dtype))
 

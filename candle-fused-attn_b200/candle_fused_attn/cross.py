@@ -5,6 +5,7 @@ padded batch of keys, key heads shared by groups of query heads; fp32, with grad
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import FusedAttentionError, _abi, _check_head_dim, _float4_rows
 from ._launch import (check_status, current_stream, int32_vector, merged_heads, on_device,
@@ -76,6 +77,7 @@ class _CrossAttention(torch.autograd.Function):
         return o
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad):
         q, k, v, key_lengths, o, lse = ctx.saved_tensors
         b, h, hk, sq, sk, d = ctx.dims

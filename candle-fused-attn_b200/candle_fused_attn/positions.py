@@ -6,6 +6,7 @@ from __future__ import annotations
 import math
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import FusedAttentionError, _abi, qkv_geometry
 from ._launch import (DTYPES, check_status, current_stream, merged_heads, on_device, one_device,
@@ -97,6 +98,7 @@ class _Rotary(torch.autograd.Function):
         return _turn(x, positions, freqs, amplitude, interleaved, False)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad):
         freqs, *at = ctx.saved_tensors
         positions = at[0] if at else ctx.first
@@ -123,6 +125,7 @@ class _RotaryQkv(torch.autograd.Function):
         return _turn_qkv(qkv, heads, positions, freqs, amplitude, interleaved, False)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad):
         freqs, *at = ctx.saved_tensors
         positions = at[0] if at else ctx.first

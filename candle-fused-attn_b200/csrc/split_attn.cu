@@ -138,7 +138,7 @@ __device__ __forceinline__ UnitInfo unit_info(const SplitArgs& a, const ChunkInd
   n.n_new = seq_new(a, n.b);
   const int c = chunk_log(n.len, a.tile_log);
   n.lo = n.chunk << c;
-  n.hi = min(n.len, n.lo + (1 << c));  // (len <= 2^31 - 1025: no overflow)
+  n.hi = n.len - n.lo > 1 << c ? n.lo + (1 << c) : n.len;
   return n;
 }
 // A 16-byte asynchronous copy past L1 (the rows are read once).

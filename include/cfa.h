@@ -27,6 +27,8 @@
  *   cfa_matmul_f32,            the projection next to the path: candle's broadcast_matmul of
  *   cfa_matmul_workspace_bytes           the training step (examples/tutorial.rs:103-118) as a
  *   cfa_matmul_status                    tensor-core kernel
+ *   cfa_cross_*, cfa_rotary,   operators beside the path (no counterpart): attention to another
+ *   cfa_paged_*                            sequence, rotary positions, a paged cache and its attention
  *
  * Head dim 64 runs one kernel pair, as the reference does (src/cuda.rs:140-260): the tensor-core
  * pair (csrc/fwd_tc.cu, csrc/bwd_tc.cu). A backward must run on the forward's L of the same pair
