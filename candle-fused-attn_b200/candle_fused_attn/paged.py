@@ -124,9 +124,10 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     q [batch, heads, s, d], d in HEAD_DIMS, of the cache's type or f32; heads a multiple of the
     cache's key heads. Query i of a sequence's n (n = s, or new_lengths[b]) sees its first
     lengths[b] - n + i + 1 keys: all of them for a single token. The cache's rows must be 16-byte
-    aligned. -> [batch, heads, s, d], laid out as a dense [batch, s, heads, d], of q's type; zeros where a query sees no key or a padded row is no query. The keys are split into
-    chunks by the sequence's own length and joined in order: bit-identical across reruns and
-    batches. Softmax statistics and sums are fp32. No gradients.
+    aligned. -> [batch, heads, s, d], laid out as a dense [batch, s, heads, d], of q's type; zeros
+    where a query sees no key or a padded row is no query. The keys are split into chunks by the
+    sequence's own length and joined in order: bit-identical across reruns and batches. Softmax
+    statistics and sums are fp32. No gradients.
     """
     who = "paged_attention"
     require(q.dim() == 4, who, f"q [b, h, s, d] expected, shape {list(q.shape)}")

@@ -9,8 +9,8 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import FusedAttentionError, _abi, qkv_geometry
-from ._launch import (DTYPES, check_status, current_stream, merged_heads, on_device, one_device,
-                      raise_if_expired, require)
+from ._launch import (DTYPES, check_status, current_stream, merged_heads, no_gradient, on_device,
+                      one_device, raise_if_expired, require)
 
 __all__ = ["rotary", "rotary_qkv", "rotary_frequencies"]
 
@@ -54,6 +54,7 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, *, scaling: str |
 
 
 def check_freqs(who: str, freqs: torch.Tensor, d: int) -> None:
+    no_gradient(f"{who}: freqs", freqs)
     if freqs.dtype != torch.float64 or freqs.dim() != 1 or (freqs.numel() > 1
                                                             and freqs.stride(0) != 1):
         raise FusedAttentionError(

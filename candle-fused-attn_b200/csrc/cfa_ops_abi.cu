@@ -60,8 +60,9 @@ int check_cross(int64_t B, int64_t H, int64_t Hk, int64_t Sq, int64_t Sk, int64_
   if (B < 0 || H < 0 || Hk < 0 || Sq < 0 || Sk < 0 || D < 0) return CFA_ERR_SHAPE;
   if (!head_dim_ok(D)) return CFA_ERR_HEAD_DIM;
   if (Hk == 0 ? H != 0 : H % Hk != 0) return CFA_ERR_HEADS;
-  if (B > kLim || H > kLim || Sq > kLim - 1024 || Sk > kLim - 1024) return CFA_ERR_OVERFLOW;
-  if (B == 0 || H == 0) return CFA_OK;
+  if (B > kLim || H > kLim || Hk > kLim || Sq > kLim - 1024 || Sk > kLim - 1024) return CFA_ERR_OVERFLOW;
+  if (B == 0 || Hk == 0) return CFA_OK;
+  if (B * Hk > kLim / ((Sk + 31) / 32 + 1)) return CFA_ERR_OVERFLOW;
   if (B * H > kLim / ((std::max(Sq, Sk) + 31) / 32 + 1)) return CFA_ERR_OVERFLOW;
   if (B * H * Sq > kLim || B * Hk * Sk > kLim) return CFA_ERR_OVERFLOW;
   if (B * Hk * ((Sk + 63) / 64) > kLim / cfa::LIN_SMS) return CFA_ERR_OVERFLOW;  // key blocks x parts
@@ -91,7 +92,8 @@ CrossLayout cross_layout(int64_t B, int64_t H, int64_t Hk, int64_t Sq, int64_t S
   // it as many blocks.
   const int64_t want = (cfa::LIN_SMS + nkb * Hk - 1) / (nkb * Hk);
   w.n_parts = static_cast<int>(std::max<int64_t>(1, std::min(want, tiles / kCrossPartTiles)));
-  w.join_dq = w.n_parts > 1 || group * Sq * D * 4 * nkb > kCrossJoinBytes;
+  const int64_t row_bytes = nkb * D * 4;  // of one query's dQ partials (below 2^34)
+  w.join_dq = w.n_parts > 1 || group * Sq > kCrossJoinBytes / row_bytes;
   w.turn_off = 256;
   const int64_t turns = B * Hk * tiles;
   w.n_zero = 64 + turns;
@@ -99,8 +101,8 @@ CrossLayout cross_layout(int64_t B, int64_t H, int64_t Hk, int64_t Sq, int64_t S
   w.kv_off = w.dsum_off + cfa::align256(static_cast<size_t>(B * H * Sq) * 4);
   w.total = w.kv_off + (w.n_parts > 1 ? static_cast<size_t>(w.n_parts) * B * Sk * 2 * Hk * D * 4 : 0);
   w.part_off = w.total;
-  const int64_t partials = nkb * B * H * Sq * D * 4;
-  w.total_fast = w.total + (partials <= kCrossPartialBytes ? static_cast<size_t>(partials) : 0);
+  const int64_t queries = B * H * Sq;
+  w.total_fast = w.total + (queries <= kCrossPartialBytes / row_bytes ? static_cast<size_t>(queries * row_bytes) : 0);
   return w;
 }
 
@@ -160,12 +162,13 @@ int cfa_cross_bwd_f32(const float* q, const int64_t q_strides[3], const float* k
                       size_t workspace_bytes, int64_t batch, int64_t heads, int64_t key_heads,
                       int64_t seq, int64_t key_seq, int64_t head_dim, float scale, void* stream) {
   int st = check_cross(batch, heads, key_heads, seq, key_seq, head_dim);
-  if (st != CFA_OK || batch == 0 || heads == 0) return st;
+  if (st != CFA_OK) return st;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (seq == 0 || key_seq == 0) {  // no score at all: the gradients that exist are zero
-    if (seq == 0 && key_seq == 0) return CFA_OK;
-    float* g = seq == 0 ? dkv : dq;
-    const int64_t n = seq == 0 ? 2 * batch * key_seq * key_heads : batch * seq * heads;
+  const int64_t queries = heads * seq, keys = key_heads * key_seq;
+  if (batch == 0 || queries == 0 || keys == 0) {  // no score at all: the gradients that exist are zero
+    if (batch == 0 || queries == keys) return CFA_OK;
+    float* g = queries == 0 ? dkv : dq;
+    const int64_t n = batch * (queries == 0 ? 2 * keys : queries);
     if (!g) return CFA_ERR_NULL;
     return status(cudaMemsetAsync(g, 0, static_cast<size_t>(n * head_dim) * 4, s));
   }
@@ -402,7 +405,6 @@ int cfa_paged_attention(const void* q, const int64_t q_strides[3], int dtype, co
   a.q_sb = q_strides[0], a.q_sh = q_strides[1], a.q_ss = q_strides[2];
   a.k_sp = k_cache_strides[0], a.k_sr = k_cache_strides[1], a.k_sh = k_cache_strides[2];
   a.v_sp = v_cache_strides[0], a.v_sr = v_cache_strides[1], a.v_sh = v_cache_strides[2];
-  // (A cache without a page has nothing to read: max_len 0 keeps every key away.)
   a.table = page_table;
   a.table_sb = table_stride;
   a.table_width = static_cast<int>(table_width), a.n_pages = static_cast<int>(pages);

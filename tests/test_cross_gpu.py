@@ -231,6 +231,19 @@ def test_empty(cuda):
     cfa.check_status()
 
 
+def test_no_query_heads(cuda):
+    """Key heads that no query reads: their gradients are zeros, whatever the memory held."""
+    for h, sq in ((0, 3), (2, 0), (0, 0)):
+        q = torch.ones(2, h, sq, 64, device=cuda, requires_grad=True)
+        k, v = (torch.ones(2, 2, 70, 64, device=cuda, requires_grad=True) for _ in range(2))
+        o = cfa.cross_attention(q, k, v, 0.125)
+        used = torch.full((2, 70, 2, 2, 64), 7.0, device=cuda)
+        del used
+        dq, dk, dv = torch.autograd.grad(o, (q, k, v), torch.empty_like(o))
+        assert dq.shape == q.shape and not dk.any() and not dv.any()
+    cfa.check_status()
+
+
 def test_graph_capture_and_streams(cuda):
     """A forward and backward captured once and replayed on new inputs; and on a side stream."""
     q, k, v, dout = (t.to(cuda) for t in make(2, 4, 2, 70, 300, 64, None))

@@ -71,6 +71,9 @@ def test_cross_backward_workspace():
             assert plain <= least <= plain + 1024
             assert fast(b, h, h, sq, n * kb, d) - least == n * b * h * sq * d * 4
         assert fast(b, h, h, sq, most * kb + 1, d) == size(b, h, h, sq, most * kb + 1, d)
+    # more queries x key blocks than 2^63 bytes of partials: none
+    huge = (1, 1, 1, 2**31 - 2000, 900_000_000, 128)
+    assert size(*huge) > 2**32 and fast(*huge) == size(*huge)
     # 2 key blocks of one key head over 63 query tiles: 7 parts, each with a dK and dV of its own
     parts = 7 * 200 * 2 * 64 * 4
     whole = size(1, 8, 8, 500, 200, 64)  # 16 key blocks over 8 tiles each: one part
@@ -244,6 +247,8 @@ def test_rotary_refuses():
         cfa.rotary(x[0], 0, f)
     with raises("not 3 x 5 heads"):
         cfa.rotary_qkv(torch.zeros(2, 4, 72), 5, 0, f)
+    with raises("freqs: has no backward"):
+        cfa.rotary(x, 0, f.clone().requires_grad_(True))
 
 
 def test_frequencies():
