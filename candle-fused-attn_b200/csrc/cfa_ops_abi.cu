@@ -77,7 +77,10 @@ int check_cross(int64_t B, int64_t H, int64_t Hk, int64_t Sq, int64_t Sk, int64_
 // 6990 keys 157 us against 311.
 constexpr int64_t kCrossPartialBytes = int64_t(4) << 30;
 constexpr int64_t kCrossJoinBytes = 512 << 10;   // dQ partials of a (batch, key head) one block may sum
-constexpr int kCrossPartTiles = 8;               // fewest query tiles of a part
+// Fewest query tiles of a part: each reads its keys again. With 4, 8, 16 and without parts: [1, 8 over 2,
+// 700 x 300, 64] 32, 51, 103 and 192 us; [8, 8, 512 x 512, 64] 122, 106, 106, 106; [2, 16 over 1, 1024 x
+// 1024, 64] 215, 215, 176, 1023.
+constexpr int kCrossPartTiles = 8;
 struct CrossLayout {
   int64_t n_zero;  // ints cleared before the backward
   size_t turn_off, dsum_off, kv_off, part_off, total, total_fast;

@@ -14,11 +14,15 @@
 //    adds in order. (bwd_tc.cu's split tail would have one block fold every tile of the others: at 16
 //    heads over one, [2, 16, 1024, 64], that and one block's sum of all dQ partials took 1.2 of 1.5
 //    ms.) Where the dQ partials of a (batch, key head) exceed half a MB, or with parts, that kernel
-//    sums them too, by all SMs;
+//    sums them too, by all SMs; below, the key head's last block does, behind which the others run on
+//    ([64, 6, 240, 64] over 100 to 600 keys: 272 us so, 279 by the join; [8, 8, 512 x 512, 64]: 106
+//    against 100);
 //  - dQ [B, S, H, HD] and dK, dV [B, Sk, 2, Hk, HD] go to buffers of their own.
 // It is a kernel of its own, because at 96 registers a thread the fused attention's backward keeps
 // its registers only as it stands: as one template, that instance spilled or slowed by 0.2 to 3 %.
-// Bound by the compute warps' work a tile, as bwd_tc.cu is.
+// Bound by the compute warps' work a tile, as bwd_tc.cu is: [4, 16 over 4, 2048 x 8192, 64] 4.4 to 4.7
+// ms, 147 to 155 TFLOP/s of fp32 products (six bf16 ones each); the training step's ragged [64, 6, 240,
+// 64] 272 us, 76 TFLOP/s: four tiles a block, whose first loads and last stores take 40 % of it.
 #include <algorithm>
 
 #include "bwd_tc.cuh"
@@ -44,7 +48,7 @@ __global__ void __launch_bounds__(NB, 1) cross_bwd_tc_kernel(const BwdArgs a) {
   uint64_t* bar_t2 = bar_s + 1;  // dK, dQ of a tile done: every MMA of the tile
   uint64_t* bar_c1 = bar_s + 2;  // dS^T of a tile in shared memory (arrivals)
   uint64_t* bar_q = bar_s + 3;   // Q, dO parts of the next tile in place (arrivals)
-  uint64_t* bar_ld = bar_s + 4;  // bulk copies: the prologue's rows, then the tail's windows
+  uint64_t* bar_ld = bar_s + 4;  // bulk copies: the prologue's rows, then the heads' dQ partials
   uint64_t* bar_dp = bar_s + 5;  // dP^T of a tile done
   uint64_t* bar_p = bar_s + 6;   // P^T's parts of a tile in TMEM (arrivals)
   uint64_t* bar_dv = bar_s + 7;  // dV of a tile done
@@ -58,8 +62,8 @@ __global__ void __launch_bounds__(NB, 1) cross_bwd_tc_kernel(const BwdArgs a) {
   const int S = a.S;
   const int BH = a.B * a.Hk;
   griddep_wait();  // the lengths, the cleared counters: the previous kernels' writes
-  // The work item. With the dQ partials (no-wait path): the block index, (b, h)-major, so a
-  // (b, h)'s key blocks run side by side and its last one finishes early. With the turn chain: a
+  // The work item. With the dQ partials (no block waits for another): the block index, (b, h)-major, so
+  // a (b, h)'s key blocks run side by side and its last one finishes early. With the turn chain: a
   // ticket drawn after the prep kernel's wait, key-block-major -- a block waits only on key block
   // kb - 1 of its (b, h) and part, which holds a smaller ticket, so it is running or done.
   const bool chain = a.dq_part == nullptr;
@@ -442,10 +446,9 @@ __global__ void __launch_bounds__(NB, 1) cross_bwd_tc_kernel(const BwdArgs a) {
           }
         }
       } else {
-        // Turn chain: query tile t's contributors are key blocks 0 .. last (causal: those holding
-        // a key <= the tile's last query); each adds its partial into dQ on its turn, through L2
-        // (__ldcg / __stcg), and the last multiplies by `scale`: dQ = ((p0 + p1) + ...) * scale,
-        // the no-wait path's sums bit for bit.
+        // Turn chain: key blocks 0 .. last each add their partial into dQ on their turn, through L2
+        // (__ldcg / __stcg), and the last multiplies by `scale`: dQ = ((p0 + p1) + ...) * scale, the
+        // partials' sums bit for bit.
         const int t = t_begin + n;
         const int last = nkb - 1;
         bool go = true;
@@ -495,8 +498,8 @@ __global__ void __launch_bounds__(NB, 1) cross_bwd_tc_kernel(const BwdArgs a) {
     // publishes every thread's partial stores (the barrier orders them before it) and, for the
     // last of the (b, h)'s key blocks, makes the other blocks' visible; that block sums them in
     // key-block order (the loads bypass L1).
-    // dV into slot 2, dK * scale into slot 1 of dqkv [b, s, 3, h, 64] go through shared memory (the
-    // dS^T and staging buffers, free since the last T2): rows of 68 floats (a 16-byte rotation per
+    // dV and dK * scale go through shared memory (the dS^T and staging buffers, free since the last
+    // T2): rows of 68 floats (a 16-byte rotation per
     // row keeps both passes conflict-free), stored as whole rows at the end.
     constexpr int LDS = 68;
     float* sv = reinterpret_cast<float*>(dSp);
@@ -560,8 +563,7 @@ __global__ void __launch_bounds__(NB, 1) cross_bwd_tc_kernel(const BwdArgs a) {
         if (!ok && tid == 0) flag_timeout(a.err, a.sink);
         return;
       }
-      // DETERMINISM: dQ = (((p0 + p1) + p2) + ...) * scale over the key blocks holding a key <=
-      // the row (causal) or all of them. Eight float4 items per thread at a time, each key
+      // DETERMINISM: dQ = (((p0 + p1) + p2) + ...) * scale over the key blocks. Eight float4 items per thread at a time, each key
       // block's loads for the eight issued together.
       constexpr int U = 8;
       const int items = S * C4;

@@ -12,17 +12,24 @@
 //
 // Bound by memory: every key and value is read once for all the query rows of its head (up to 8 a
 // block), at 4 rows D flops a key against 2 D elements. Each warp runs on its own: it takes every
-// fourth tile of 16 keys of the chunk through a ring of its own (cp.async, 16 bytes a lane, rows
-// padded by 16 bytes so that every later read is free of bank conflicts), and the four warps' sums
-// are joined through shared memory once a chunk.
+// fourth 8 KB tile of the chunk through a ring of its own (cp.async, 16 bytes a lane, rows padded by
+// 16 bytes so that every later read is free of bank conflicts), and the four warps' sums are joined
+// through shared memory once a chunk. The ring runs on through a block's chunks: a ring that drained
+// at the end of each took 204 us where this takes 199.
 //   16-bit caches: S^T = K Q^T and O^T += V^T P^T by mma.m16n8k16, the keys (dims) as the 16 rows
 //     and up to 8 query rows as the 8 columns: a column's softmax state then lives in the lanes
 //     that hold the column's output. fp32 queries enter in parts that keep their 24 bits (three
-//     bf16, or two fp16 under a power of two a row), p as two or three parts (16 bits for a 16-bit
-//     output, 24 for fp32), every tile's product a fresh accumulator folded by an fp32 FMA -- the
-//     tensor core's truncating sums never run longer than a tile. tcgen05 has no shape below 64
-//     rows, and at a few rows the product is a small share of the tile's load time.
-//   fp32 caches: two lanes a key for the scores, a quarter of a row a lane for the output, FMAs.
+//     bf16, or two fp16 under a power of two a row: 22 bits), p as two parts (16 bits of bf16, 22 of
+//     fp16) or, fp32 queries over bf16, three (24 bits), every tile's product a fresh accumulator
+//     folded by an fp32 FMA -- the tensor core's truncating sums never run longer than a tile.
+//     tcgen05 has no shape below 64 rows, and at a few rows the product is a small share of the
+//     tile's load time. Three stages of two blocks a SM (two of three blocks: 245 us for 204).
+//   fp32 caches: TK = 1024 / D keys a tile, 32 / TK lanes a key for the scores, four dims a lane for the
+//     output, p through shared memory; packed FMAs. Two stages of three blocks a SM.
+// On one B200, with the join: 64 sequences of up to 8192 keys, 32 heads over 8, [page 16] bf16, d = 128
+// 193 us (5.8 TB/s); 2 of 131071 keys, fp32 over bf16, d = 64 55 us; 16 of 1000 to 6000 keys, 16 heads,
+// fp32, d = 64 79 us (5.9 TB/s); fp32 with four or eight query heads a key head is bound by the FMAs and
+// their shared-memory reads instead: 78 and 120 us for 48 us of bytes. One sequence of 240 keys: 6.9 us.
 //
 // Order of summation: fixed by the sequence's length and the row alone (not by the batch, the grid
 // or the SM count): results are bit-identical across reruns and batches.
@@ -51,7 +58,8 @@ constexpr float LOG2E = 1.4426950408889634f;
 
 // Keys per chunk, as a power of two, of a sequence of `len` keys in tiles of 2^tile_log keys: 16 tiles
 // (four a warp, 128 KB of keys and values) up to 16 chunks, then 32 tiles up to 256 chunks, then as many
-// as keep them 256.
+// as keep them 256. (64 sequences of up to 8192 keys, at 204 us so: 279 and 256 us with chunks of 64 and
+// 128 keys throughout, 225 with the step at 32, 64 or 256 chunks.)
 constexpr int FEW_CHUNKS_LOG = 4, MOST_CHUNKS_LOG = 8, MOST_CHUNKS = 1 << MOST_CHUNKS_LOG;
 __host__ __device__ __forceinline__ int bits_of(uint32_t x) {  // x < 2^bits
 #ifdef __CUDA_ARCH__
