@@ -14,11 +14,11 @@ from ._launch import (check_status, current_stream, int32_vector, merged_heads, 
 __all__ = ["cross_attention"]
 
 # Up to as many query rows a key head (query heads of a group x queries) the forward without gradients
-# runs split over the keys, one block a chunk of keys and eight rows; above, the tensor-core kernels,
+# runs split over the keys, one block a chunk of keys and up to 16 rows; above, the tensor-core kernels,
 # which take 256 rows a block. The batch plays no part: the choice changes bits. Split and whole, in us,
-# [b, 6, rows, 64] over 1500 keys: 8 rows 14 and 55 (b 1), 32 and 58 (16), 113 and 169 (64); 16 rows 14
-# and 55, 58 and 58, 221 and 169; 24 rows 15 and 55, 86 and 58, 327 and 170.
-FEW_ROWS = 16
+# [b, 6, rows, 64] over 1500 keys: 16 rows 11 and 55 (b 1), 23 and 58 (16), 82 and 169 (64); 32 rows 11
+# and 55, 42 and 58, 156 and 169; 48 rows 11 and 55, 60 and 58, 226 and 170.
+FEW_ROWS = 32
 
 
 def _dims(q, k, v):

@@ -69,13 +69,13 @@ struct SplitArgs {
   float scale;
   int* sink;
   // set by the launcher
-  int group, rows, row_chunks, max_chunks;
+  int group, rows, block_rows, row_chunks, max_chunks;  // rows of a key head, of a block; blocks of them
   uint32_t page_mul;  // key / page = key page_mul >> page_shift
   int page_shift;
   int one_page;       // every tile of keys lies on one page
   int tile_log;       // log2 of the keys of a tile
   float* part_o;   // [B H S][max_chunks][D] unnormalised partial outputs
-  float2* part_ml; // [B H S][max_chunks] running maximum (log2 units) and sum
+  float2* part_ml; // [B H S][max_chunks] running maximum and sum
 };
 int split_max_chunks(int64_t max_len, int64_t head_dim, int kv_dtype);
 size_t split_workspace_bytes(int64_t rows, int64_t max_len, int64_t head_dim, int kv_dtype);

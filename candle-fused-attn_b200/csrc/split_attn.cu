@@ -11,7 +11,7 @@
 // A sequence of one chunk is written by the first kernel.
 //
 // Bound by memory: every key and value is read once for all the query rows of its head (up to 8 a
-// block), at 4 rows D flops a key against 2 D elements. Each warp runs on its own: it takes every
+// block, 16 of fp32), at 4 rows D flops a key against 2 D elements. Each warp runs on its own: it takes every
 // fourth 8 KB tile of the chunk through a ring of its own (cp.async, 16 bytes a lane, rows padded by
 // 16 bytes so that every later read is free of bank conflicts), and the four warps' sums are joined
 // through shared memory once a chunk. The ring runs on through a block's chunks: a ring that drained
@@ -24,15 +24,23 @@
 //     folded by an fp32 FMA -- the tensor core's truncating sums never run longer than a tile.
 //     tcgen05 has no shape below 64 rows, and at a few rows the product is a small share of the
 //     tile's load time. Three stages of two blocks a SM (two of three blocks: 245 us for 204).
-//   fp32 caches: TK = 1024 / D keys a tile, 32 / TK lanes a key for the scores, four dims a lane for the
+//   fp32 caches, three query rows and more: S = Q K^T and O += P V by mma.m16n8k8 on tf32 operands, 8 or
+//     16 query rows as the 16 rows. Every operand enters in two parts of 11 bits (x = hi + lo to 2^-22
+//     |x|; three or all four of the products of the parts), and dims and keys are numbered within a
+//     product so that a lane reads K and V 16 bytes at a time and P's fragment is S's. Three stages of
+//     two blocks a SM; bound by the issue of the splits and products at 16 rows.
+//   fp32 caches, one or two rows: 32 D / 1024 lanes a key for the scores, four dims a lane for the
 //     output, p through shared memory; packed FMAs. Two stages of three blocks a SM.
+//     By FMAs and by products, 32 sequences of 100 to 8000 keys, four key heads, in us: one row 61 and
+//     64 (d 64), 107 and 120 (d 128), two rows 63 and 65, 115 and 121, four rows 79 and 65, 148 and 122,
+//     eight rows 121 and 66, 241 and 125; 16 rows, in blocks of 8 and of 16: 222 and 92, 461 and 169; one
+//     row of 64 sequences over 240 keys 11.7 and 17.
 // On one B200, with the join: 64 sequences of up to 8192 keys, 32 heads over 8, [page 16] bf16, d = 128
 // 193 us (5.8 TB/s); 2 of 131071 keys, fp32 over bf16, d = 64 55 us; 16 of 1000 to 6000 keys, 16 heads,
-// fp32, d = 64 79 us (5.9 TB/s); fp32 with four or eight query heads a key head is bound by the FMAs and
-// their shared-memory reads instead: 78 and 120 us for 48 us of bytes. One sequence of 240 keys: 6.9 us.
+// fp32, d = 64 79 us (5.9 TB/s). One sequence of 240 keys: 6.9 us.
 //
-// Order of summation: fixed by the sequence's length and the row alone (not by the batch, the grid
-// or the SM count): results are bit-identical across reruns and batches.
+// Order of summation: fixed by the sequence's length, the number of rows and the row alone (not by the
+// batch, the grid or the SM count): results are bit-identical across reruns and batches.
 //
 // Masked keys are excluded rather than weighted by zero, so what lies behind a sequence's end or a
 // row's last key -- infinities and NaN among it -- never reaches a result. A page id outside the
@@ -53,7 +61,7 @@ namespace {
 
 constexpr int WARPS = 4;
 constexpr int NT = 32 * WARPS;
-constexpr int MAXR = 8;    // query rows per block
+constexpr int MAXR = 16;   // most query rows per block
 constexpr float LOG2E = 1.4426950408889634f;
 
 // Keys per chunk, as a power of two, of a sequence of `len` keys in tiles of 2^tile_log keys: 16 tiles
@@ -140,7 +148,7 @@ __device__ __forceinline__ UnitInfo unit_info(const SplitArgs& a, const ChunkInd
   const uint32_t per = a.Hk * a.row_chunks;
   const int g = static_cast<int>(u / per), rest = static_cast<int>(u - g * per);
   n.hk = rest / a.row_chunks;
-  n.r0 = (rest - n.hk * a.row_chunks) * MAXR;
+  n.r0 = (rest - n.hk * a.row_chunks) * a.block_rows;
   ix.find(a, g, n.b, n.chunk, n.nc);
   n.len = seq_len(a, n.b);
   n.n_new = seq_new(a, n.b);
@@ -160,17 +168,23 @@ __device__ __forceinline__ void cp_async16_full(void* smem, const void* gmem) {
 // grid, ..) and, in each, the warp's tiles (w, w + 4, ..) without a pause: ST - 1 tiles are in flight
 // while one is in use, those of the next unit behind the last of this one, and a unit's index and
 // first page are looked up an iteration before they are needed.
-template <int D, int ES, int TK_, int ST_>
+template <int D, int ES, int TK_, int ST_, bool SWIZZLE>
 struct Ring {
   static constexpr int ST = ST_;   // stages
   static constexpr int TK = TK_;   // keys per tile
-  static constexpr int RB = D * ES + 16;
+  static constexpr int RB = D * ES + (SWIZZLE ? 0 : 16);
   static constexpr int KV = TK * RB;          // bytes of a tile's K (or V)
   static constexpr int STAGE = 2 * KV;
   static constexpr int CPR = D * ES / 16;     // 16-byte pieces of a row
   static constexpr int RPI = 32 / CPR;        // rows that the warp copies at once
   static constexpr int BYTES = ST * STAGE;
   static constexpr unsigned ALL = 0xffffffffu >> (32 - TK);
+
+  // SWIZZLE (rows of 128 bytes and more): the piece c of row r of K, V is piece c ^ this of its row, by
+  // which the eight lanes of a 16-byte read (K: two rows, four pieces; V: every other row of eight, two
+  // pieces) meet eight banks of 16 bytes. Else rows are padded by 16 bytes.
+  static __device__ __forceinline__ int k_swizzle(int r) { return SWIZZLE ? 4 * (r & 1) : 0; }
+  static __device__ __forceinline__ int v_swizzle(int r) { return SWIZZLE ? 2 * ((r >> 1) & 3) : 0; }
 
   const SplitArgs& a;
   const ChunkIndex& ix;
@@ -260,21 +274,22 @@ struct Ring {
     }
     const char* kg = kp + ES * ko + k_lane;
     const char* vg = vp + ES * vo + v_lane;
-    unsigned char* st = base + stage * STAGE + (lane / CPR) * RB + 16 * (lane % CPR);
+    unsigned char* st = base + stage * STAGE + (lane / CPR) * RB;
+    const int ck = (lane % CPR) ^ k_swizzle(lane / CPR), cv = (lane % CPR) ^ v_swizzle(lane / CPR);
     const int64_t kj = RPI * ES * a.k_sr, vj = RPI * ES * a.v_sr;
     if (rows == TK) {
 #pragma unroll
       for (int j = 0; j < TK / RPI; ++j) {
-        cp_async16_full(st + j * RPI * RB, kg + j * kj);
-        cp_async16_full(st + KV + j * RPI * RB, vg + j * vj);
+        cp_async16_full(st + j * RPI * RB + 16 * (ck ^ k_swizzle(j * RPI)), kg + j * kj);
+        cp_async16_full(st + KV + j * RPI * RB + 16 * (cv ^ v_swizzle(j * RPI)), vg + j * vj);
       }
       return ALL;
     }
 #pragma unroll
     for (int j = 0; j < TK / RPI; ++j) {  // rows past the end: zeros (from an address that exists)
       const bool ok = j * RPI + lane / CPR < rows;
-      cp_async16(st + j * RPI * RB, ok ? kg + j * kj : kp, ok ? 16 : 0);
-      cp_async16(st + KV + j * RPI * RB, ok ? vg + j * vj : vp, ok ? 16 : 0);
+      cp_async16(st + j * RPI * RB + 16 * (ck ^ k_swizzle(j * RPI)), ok ? kg + j * kj : kp, ok ? 16 : 0);
+      cp_async16(st + KV + j * RPI * RB + 16 * (cv ^ v_swizzle(j * RPI)), ok ? vg + j * vj : vp, ok ? 16 : 0);
     }
     return (1u << rows) - 1;
   }
@@ -300,8 +315,8 @@ struct Ring {
       const int r = j * RPI + lane / CPR;
       const int64_t kr = __shfl_sync(0xffffffffu, ko, r), vr = __shfl_sync(0xffffffffu, vo, r);
       const int n = (alive >> r) & 1u ? 16 : 0;
-      cp_async16(st + r * RB + 16 * c, kp + ES * kr + 16 * c, n);
-      cp_async16(st + KV + r * RB + 16 * c, vp + ES * vr + 16 * c, n);
+      cp_async16(st + r * RB + 16 * (c ^ k_swizzle(r)), kp + ES * kr + 16 * c, n);
+      cp_async16(st + KV + r * RB + 16 * (c ^ v_swizzle(r)), vp + ES * vr + 16 * c, n);
     }
     return alive;
   }
@@ -428,29 +443,32 @@ template <int D, int ES>
 __host__ __device__ constexpr int tile_keys() {
   return ES == 2 ? (D == 128 ? 16 : 32) : 1024 / D;  // (tile_log_of says the same to the host)
 }
-template <int D, int ES>
-using RingOf = Ring<D, ES, tile_keys<D, ES>(), (ES == 2 ? 3 : 2)>;
+// ROWS: query rows of a block (fp32 caches: up to two by FMAs, else 8 or 16 by matrix products).
+template <int D, int ES, int ROWS>
+using RingOf = Ring<D, ES, tile_keys<D, ES>(), (ROWS <= 2 ? 2 : 3), (ES == 4 && ROWS > 2)>;
 // Shared memory: the rings -- whose free stage also takes a warp's sums when a unit ends -- the (m, l)
-// of the warps' rows and where their sums are, and the fp32 kernel's two sets of query rows and its p.
-template <int D, int ES>
+// of the warps' rows and where their sums are, and, fp32, two sets of query rows and p (FMAs) or the
+// fragments of 16 rows.
+template <int D, int ES, int ROWS>
 __host__ __device__ constexpr int off_ml() {
-  static_assert(RingOf<D, ES>::STAGE >= MAXR * D * 4, "a stage holds a warp's sums");
-  return WARPS * RingOf<D, ES>::BYTES;
+  static_assert(RingOf<D, ES, ROWS>::STAGE >= ROWS * D * 4, "a stage holds a warp's sums");
+  return WARPS * RingOf<D, ES, ROWS>::BYTES;
 }
-template <int D, int ES>
+template <int D, int ES, int ROWS>
 __host__ __device__ constexpr int off_q() {
-  return off_ml<D, ES>() + WARPS * MAXR * 8 + WARPS * 4;
+  return off_ml<D, ES, ROWS>() + WARPS * MAXR * 8 + WARPS * 4;
 }
-template <int D, int ES>
-__host__ __device__ constexpr int split_smem(int q_rows) {
-  return off_q<D, ES>() + q_rows * (2 * D * 4 + WARPS * tile_keys<D, ES>() * 8);
+template <int D, int ES, int ROWS>
+__host__ __device__ constexpr int split_smem() {
+  return off_q<D, ES, ROWS>() +
+         (ROWS <= 2 ? ROWS * (2 * D * 4 + WARPS * tile_keys<D, ES>() * 8) : ROWS == 16 ? 128 * D : 0);
 }
 
 // 16-bit caches.
 template <typename QT, typename T, int D>
 __global__ void __launch_bounds__(NT, 2)
     split_mma_kernel(const SplitArgs a) {
-  using R = RingOf<D, 2>;
+  using R = RingOf<D, 2, 8>;
   constexpr int ST = R::ST, TK = R::TK, MT = TK / 16;
   constexpr bool F32 = std::is_same_v<QT, float>;
   constexpr bool HALF = std::is_same_v<T, __half>;
@@ -461,7 +479,7 @@ __global__ void __launch_bounds__(NT, 2)
   extern __shared__ __align__(128) unsigned char smem[];
   const int tid = threadIdx.x, w = tid >> 5, lane = tid & 31;
   const int qr = lane >> 2, qc = lane & 3;  // a fragment's row (key, dim; B: column) and pair
-  float2* ml = reinterpret_cast<float2*>(smem + off_ml<D, 2>());
+  float2* ml = reinterpret_cast<float2*>(smem + off_ml<D, 2, 8>());
   int* red_at = reinterpret_cast<int*>(ml + WARPS * MAXR);
   griddep_wait();
   griddep_launch_dependents();
@@ -662,7 +680,7 @@ __global__ void __launch_bounds__(NT, 2)
         for (int mt = 0; mt < KS; ++mt)
 #pragma unroll
           for (int j = 0; j < 4; ++j) acc[mt][j] *= j & 1 ? a1 : a0;
-        for (int r = 0; r < min(MAXR, a.rows - n.r0); ++r) {
+        for (int r = 0; r < min(8, a.rows - n.r0); ++r) {
           const int lim = row_limit(a, n, n.r0 + r);
 #pragma unroll
           for (int i = 0; i < MT; ++i) {
@@ -715,24 +733,24 @@ __global__ void __launch_bounds__(NT, 2)
       for (int j = 0; j < 4; ++j)
         sums[(2 * qc + (j & 1)) * D + 16 * mt + qr + 8 * (j >> 1)] = acc[mt][j];
     __syncthreads();
-    write_chunk<QT, D>(a, done, smem, red_at, ml, min(MAXR, a.rows - done.r0));
+    write_chunk<QT, D>(a, done, smem, red_at, ml, min(8, a.rows - done.r0));
     __syncthreads();  // the sums are read: their stages take tiles again
   }
   if (ring.bad) flag_error(a.sink, CFA_ERR_PAGE);
 }
 
-// fp32 caches: NR query rows (1, 2, 4 or 8).
+// fp32 caches, one or two query rows (NR): FMAs.
 template <int D, int NR>
-__global__ void __launch_bounds__(NT, 3) split_f32_kernel(const SplitArgs a) {
-  using R = RingOf<D, 4>;
+__global__ void __launch_bounds__(NT, 3) split_fma_kernel(const SplitArgs a) {
+  using R = RingOf<D, 4, NR>;
   constexpr int ST = R::ST, TK = R::TK;
   constexpr int LPK = 32 / TK, DL = D / LPK;  // lanes of a key's score, dims of each
   constexpr int LPR = D / 4, KPI = 32 / LPR;  // lanes of a V row; keys at a time
   extern __shared__ __align__(128) unsigned char smem[];
   const int tid = threadIdx.x, w = tid >> 5, lane = tid & 31;
-  float2* ml = reinterpret_cast<float2*>(smem + off_ml<D, 4>());
+  float2* ml = reinterpret_cast<float2*>(smem + off_ml<D, 4, NR>());
   int* red_at = reinterpret_cast<int*>(ml + WARPS * MAXR);
-  float* q_sets = reinterpret_cast<float*>(smem + off_q<D, 4>());  // two sets of [NR][D]
+  float* q_sets = reinterpret_cast<float*>(smem + off_q<D, 4, NR>());  // two sets of [NR][D]
   uint64_t* ps = reinterpret_cast<uint64_t*>(q_sets + 2 * NR * D) + w * TK * NR;  // p twice: [key][NR]
   griddep_wait();
   griddep_launch_dependents();
@@ -889,6 +907,323 @@ __global__ void __launch_bounds__(NT, 3) split_f32_kernel(const SplitArgs a) {
   if (ring.bad) flag_error(a.sink, CFA_ERR_PAGE);
 }
 
+// x in two parts of 11 bits each, x = hi + lo to 2^-22 |x|: hi rounded to the nearest, lo what is left (the
+// tensor core drops its last bits).
+__device__ __forceinline__ void split_tf32(const float4 x, uint32_t (&hi)[4], uint32_t (&lo)[4]) {
+  const float v[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    hi[e] = (__float_as_uint(v[e]) + 0x1000u) & 0xffffe000u;
+    lo[e] = __float_as_uint(v[e] - __uint_as_float(hi[e]));
+  }
+}
+__device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+      "{%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// fp32 caches: up to 8 HALVES query rows a block. One half: rows g of m16n8k8 are a query row's large
+// part, rows g + 8 its small one, so two products take all four parts of it and a key; two halves: the
+// parts are products of their own, and the one of both small parts is left out.
+template <int D, int HALVES>
+__global__ void __launch_bounds__(NT, 2) split_f32_kernel(const SplitArgs a) {
+  using R = RingOf<D, 4, 8 * HALVES>;
+  constexpr int ST = R::ST, TK = R::TK;
+  constexpr int NK = TK / 8, J = D / 16, JV = D / 32;
+  constexpr int CH = NK == 1 ? 2 : 1;          // chains of a score's large products (and of its small ones)
+  constexpr int JQ = HALVES == 1 ? J : (J + WARPS - 1) / WARPS;  // this warp's share of q's columns
+  extern __shared__ __align__(128) unsigned char smem[];
+  const int tid = threadIdx.x, w = tid >> 5, lane = tid & 31;
+  const int g = lane >> 2, t4 = lane & 3;  // a fragment's row (B: column), and k
+  float2* ml = reinterpret_cast<float2*>(smem + off_ml<D, 4, 8 * HALVES>());
+  int* red_at = reinterpret_cast<int*>(ml + WARPS * MAXR);
+  uint4* qs = reinterpret_cast<uint4*>(smem + off_q<D, 4, 8 * HALVES>());  // [J][k-step][hi, lo][lane]
+  griddep_wait();
+  griddep_launch_dependents();
+  ChunkIndex ix;
+  ix.init(a, lane);
+  const uint32_t units = static_cast<uint32_t>(ix.total) * a.Hk * a.row_chunks;
+  R ring(a, ix, units, smem + w * R::BYTES, lane, w);
+
+  // Dims 16 j + 4 t4 .. + 3 of rows g (and g + 8): k-steps 2 j, 2 j + 1 with k = t4, t4 + 4 for each
+  // adjacent pair of dims.
+  float4 qx[JQ][HALVES];
+  auto load_q = [&](const UnitInfo& n) {
+#pragma unroll
+    for (int h = 0; h < HALVES; ++h) {
+      const int row = n.r0 + g + 8 * h;
+      int head, i;
+      row_of(a, row, head, i);
+      const bool ok = row < a.rows && i < n.n_new;
+      const float* q = static_cast<const float*>(a.q) + n.b * a.q_sb +
+                       (n.hk * a.group + (ok ? head : 0)) * a.q_sh + (ok ? i : 0) * a.q_ss;
+#pragma unroll
+      for (int x = 0; x < JQ; ++x) {
+        const int j = HALVES == 1 ? x : w + WARPS * x;
+        qx[x][h] = ok && j < J ? ld4(q + 16 * j + 4 * t4) : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+    }
+  };
+  // (two halves: the fragments in shared memory, shared by the warps)
+  auto store_q = [&]() {
+    if constexpr (HALVES == 2) {
+#pragma unroll
+      for (int x = 0; x < JQ; ++x) {
+        const int j = w + WARPS * x;
+        uint32_t hi[2][4], lo[2][4];
+        split_tf32(qx[x][0], hi[0], lo[0]);
+        split_tf32(qx[x][1], hi[1], lo[1]);
+        if (j < J) {
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            qs[(j * 4 + 2 * k) * 32 + lane] = make_uint4(hi[0][2 * k], hi[1][2 * k], hi[0][2 * k + 1], hi[1][2 * k + 1]);
+            qs[(j * 4 + 2 * k + 1) * 32 + lane] = make_uint4(lo[0][2 * k], lo[1][2 * k], lo[0][2 * k + 1], lo[1][2 * k + 1]);
+          }
+        }
+      }
+    }
+  };
+  UnitInfo n;
+  if (blockIdx.x < units) {
+    n = unit_info(a, ix, blockIdx.x);
+    load_q(n);
+    if constexpr (HALVES == 2) {
+      store_q();
+      __syncthreads();  // q in place
+    }
+  }
+  int stage = 0;  // of the next tile; the stage before it is free
+  for (uint32_t u = blockIdx.x; u < units; u += gridDim.x) {
+    const int tiles = (n.hi - n.lo + TK - 1) / TK;
+    uint32_t qa[HALVES == 1 ? J : 1][2][4];
+    if constexpr (HALVES == 1) {
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        uint32_t hi[4], lo[4];
+        split_tf32(qx[j][0], hi, lo);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) qa[j][x >> 1][2 * (x & 1)] = hi[x], qa[j][x >> 1][2 * (x & 1) + 1] = lo[x];
+      }
+    }
+    int lim[HALVES];
+#pragma unroll
+    for (int h = 0; h < HALVES; ++h) lim[h] = row_limit(a, n, n.r0 + g + 8 * h);
+    // The fewest keys that a row of the block sees: a tile that ends behind it masks row by row.
+    const int lim_min = a.causal ? max(n.len - n.n_new + 1, 0) : n.len;
+    float m[HALVES], l[HALVES];
+    float acc[JV][4][2 * HALVES];  // rows g (, g + 8): dims 32 j + 8 t4 + e (, + 4)
+#pragma unroll
+    for (int h = 0; h < HALVES; ++h) m[h] = -INFINITY, l[h] = 0.0f;
+#pragma unroll
+    for (int j = 0; j < JV; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int x = 0; x < 2 * HALVES; ++x) acc[j][e][x] = 0.0f;
+
+    for (int t = w; t < tiles; t += WARPS) {
+      cp_async_wait_group<ST - 2>();
+      __syncwarp();  // the tile is in place for every lane, and the stage before it is free
+      const unsigned char* kt = ring.base + stage * R::STAGE;
+      const unsigned char* vt = kt + R::KV;
+      const int k0 = n.lo + TK * t;
+
+      // Scores: rows g, g + 8; keys 8 i + 2 t4, + 1. The small products in chains of their own,
+      // truncated at their magnitude.
+      float ch[NK][CH][4], cl[NK][CH][4];
+#pragma unroll
+      for (int i = 0; i < NK; ++i)
+#pragma unroll
+        for (int x = 0; x < CH; ++x)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) ch[i][x][e] = cl[i][x][e] = 0.0f;
+      const unsigned char* ka = kt + g * R::RB + 16 * (t4 ^ (4 * (g & 1)));
+      const unsigned char* kb = kt + g * R::RB + 16 * (t4 ^ (4 * (~g & 1)));
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        uint32_t ah[2][4], al[2][4];  // (one half: both parts in ah)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          if constexpr (HALVES == 1) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) ah[x][e] = qa[j][x][e];
+          } else {
+            const uint4 h = qs[(j * 4 + 2 * x) * 32 + lane], y = qs[(j * 4 + 2 * x + 1) * 32 + lane];
+            ah[x][0] = h.x, ah[x][1] = h.y, ah[x][2] = h.z, ah[x][3] = h.w;
+            al[x][0] = y.x, al[x][1] = y.y, al[x][2] = y.z, al[x][3] = y.w;
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < NK; ++i) {
+          uint32_t kh[4], kl[4];
+          split_tf32(*reinterpret_cast<const float4*>((j & 1 ? kb : ka) + 8 * i * R::RB + 128 * (j >> 1)),
+                     kh, kl);
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            if constexpr (HALVES == 2) mma_tf32(cl[i][x % CH], al[x], kh[2 * x], kh[2 * x + 1]);
+            mma_tf32(cl[i][x % CH], ah[x], kl[2 * x], kl[2 * x + 1]);
+            mma_tf32(ch[i][x % CH], ah[x], kh[2 * x], kh[2 * x + 1]);
+          }
+        }
+      }
+      float s[NK][2 * HALVES];
+#pragma unroll
+      for (int i = 0; i < NK; ++i)
+#pragma unroll
+        for (int x = 0; x < 2 * HALVES; ++x) {
+          float small = cl[i][0][x], large = ch[i][0][x];
+          if constexpr (CH == 2) small += cl[i][CH - 1][x], large += ch[i][CH - 1][x];
+          if constexpr (HALVES == 1) {
+            small += ch[i][0][2 + x] + cl[i][0][2 + x];
+            if constexpr (CH == 2) small += ch[i][CH - 1][2 + x] + cl[i][CH - 1][2 + x];
+          }
+          s[i][x] = (small + large) * a.scale;
+        }
+      // (behind the products: their latency hides the next loads' issue)
+      const unsigned now = ring.advance(stage == 0 ? ST - 1 : stage - 1);
+      const bool edge = lim_min < min(k0 + TK, n.hi);
+      if (now != R::ALL || edge) {
+#pragma unroll
+        for (int i = 0; i < NK; ++i)
+#pragma unroll
+          for (int x = 0; x < 2 * HALVES; ++x) {
+            const int k = 8 * i + 2 * t4 + (x & 1);
+            if (!((now >> k) & 1u) || k0 + k >= lim[x >> 1]) s[i][x] = -INFINITY;
+          }
+      }
+      // P as A fragments: k = t4 is key 8 i + 2 t4, t4 + 4 the one after (one half: both parts in ph).
+      uint32_t ph[NK][4], pl[NK][4];
+      float alpha[HALVES];
+#pragma unroll
+      for (int h = 0; h < HALVES; ++h) {
+        float top = fmaxf(s[0][2 * h], s[0][2 * h + 1]);
+#pragma unroll
+        for (int i = 1; i < NK; ++i) top = fmaxf(top, fmaxf(s[i][2 * h], s[i][2 * h + 1]));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        top = fmaxf(top, m[h]);
+        const float mu = top == -INFINITY ? 0.0f : top;
+        alpha[h] = ex2((m[h] - mu) * LOG2E);
+        m[h] = top;
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NK; ++i) {
+          const float p0 = ex2((s[i][2 * h] - mu) * LOG2E), p1 = ex2((s[i][2 * h + 1] - mu) * LOG2E);
+          sum += p0 + p1;
+          uint32_t hi[4], lo[4];
+          split_tf32(make_float4(p0, p1, 0.f, 0.f), hi, lo);
+          ph[i][h] = hi[0], ph[i][2 + h] = hi[1];
+          if constexpr (HALVES == 1) ph[i][1] = lo[0], ph[i][3] = lo[1];
+          else pl[i][h] = lo[0], pl[i][2 + h] = lo[1];
+        }
+        l[h] = fmaf(l[h], alpha[h], sum);
+      }
+      // Values of keys 8 i + 2 t4, + 1; columns g of the four products e: dims 32 j + 4 g + e.
+      const unsigned char* va = vt + 2 * t4 * R::RB + 16 * (g ^ (2 * t4));
+      if (!edge) {
+#pragma unroll
+        for (int j = 0; j < JV; ++j) {
+          float c[4][4] = {};
+#pragma unroll
+          for (int i = 0; i < NK; ++i) {
+            uint32_t xh[4], xl[4], yh[4], yl[4];
+            const unsigned char* at = va + 8 * i * R::RB + 128 * j;
+            split_tf32(*reinterpret_cast<const float4*>(at), xh, xl);
+            split_tf32(*reinterpret_cast<const float4*>(at + R::RB), yh, yl);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if constexpr (HALVES == 2) mma_tf32(c[e], pl[i], xh[e], yh[e]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) mma_tf32(c[e], ph[i], xl[e], yl[e]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) mma_tf32(c[e], ph[i], xh[e], yh[e]);
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int x = 0; x < 2 * HALVES; ++x)
+              acc[j][e][x] = fmaf(acc[j][e][x], alpha[x >> 1], HALVES == 1 ? c[e][x] + c[e][2 + x] : c[e][x]);
+        }
+      } else {
+        // Keys that only some of the rows see: one row at a time, the values it does not see as
+        // zeros (0 times what they hold could be NaN).
+#pragma unroll
+        for (int j = 0; j < JV; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int x = 0; x < 2 * HALVES; ++x) acc[j][e][x] *= alpha[x >> 1];
+        for (int r = 0; r < min(8 * HALVES, a.rows - n.r0); ++r) {
+          const int end = row_limit(a, n, n.r0 + r);
+#pragma unroll
+          for (int i = 0; i < NK; ++i) {
+            const int k = k0 + 8 * i + 2 * t4;
+            uint32_t rh[4], rl[4];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              const bool mine = g + (HALVES == 1 ? 0 : 8 * (x & 1)) == r;
+              rh[x] = mine ? ph[i][x] : 0u;
+              if constexpr (HALVES == 2) rl[x] = mine ? pl[i][x] : 0u;
+            }
+#pragma unroll
+            for (int j = 0; j < JV; ++j) {
+              const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
+              const unsigned char* at = va + 8 * i * R::RB + 128 * j;
+              uint32_t xh[4], xl[4], yh[4], yl[4];
+              split_tf32(k < end ? *reinterpret_cast<const float4*>(at) : zero, xh, xl);
+              split_tf32(k + 1 < end ? *reinterpret_cast<const float4*>(at + R::RB) : zero, yh, yl);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                float c[4] = {0.f, 0.f, 0.f, 0.f};
+                if constexpr (HALVES == 2) mma_tf32(c, rl, xh[e], yh[e]);
+                mma_tf32(c, rh, xl[e], yl[e]);
+                mma_tf32(c, rh, xh[e], yh[e]);
+#pragma unroll
+                for (int x = 0; x < 2 * HALVES; ++x)
+                  if (g + 8 * (x >> 1) == r) acc[j][e][x] += HALVES == 1 ? c[x] + c[2 + x] : c[x];
+              }
+            }
+          }
+        }
+      }
+      stage = stage + 1 == ST ? 0 : stage + 1;
+    }
+    const UnitInfo done = n;
+    const int free_at = w * R::BYTES + (stage == 0 ? ST - 1 : stage - 1) * R::STAGE;
+    __syncwarp();  // every lane has read its last tile
+    if (lane == 0) red_at[w] = free_at;
+    float* sums = reinterpret_cast<float*>(smem + free_at);
+#pragma unroll
+    for (int h = 0; h < HALVES; ++h) {
+      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+      if (t4 == 0) ml[w * MAXR + g + 8 * h] = make_float2(m[h], l[h]);
+#pragma unroll
+      for (int j = 0; j < JV; ++j)
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+          *reinterpret_cast<float4*>(sums + (g + 8 * h) * D + 32 * j + 8 * t4 + 4 * x) =
+              make_float4(acc[j][0][2 * h + x], acc[j][1][2 * h + x], acc[j][2][2 * h + x],
+                          acc[j][3][2 * h + x]);
+    }
+    // The next unit's queries travel while this one's sums are joined.
+    const bool more = u + gridDim.x < units;
+    if (more) {
+      n = ring.unit == u + gridDim.x ? ring.info : unit_info(a, ix, u + gridDim.x);
+      load_q(n);
+    }
+    __syncthreads();
+    write_chunk<float, D>(a, done, smem, red_at, ml, min(8 * HALVES, a.rows - done.r0));
+    if constexpr (HALVES == 2) {
+      if (more) store_q();
+    }
+    __syncthreads();  // the sums are read: their stages take tiles again (and q is in place)
+  }
+  if (ring.bad) flag_error(a.sink, CFA_ERR_PAGE);
+}
+
 // The chunks' join, chunk c of a row in group c % G (G = 128 / (D / 4)): the groups' sums in chunk order,
 // then over the groups in order. Everything that does not come from the chunks' kernel is read before
 // waiting for it: that kernel has waited for its own predecessors when it lets this one start.
@@ -1024,13 +1359,13 @@ cudaError_t launch_join(const SplitArgs& a, cudaStream_t stream) {
 template <int D>
 cudaError_t launch_d(const SplitArgs& a, int qd, int kd, cudaStream_t stream) {
   cudaError_t e;
-  constexpr int S2 = split_smem<D, 2>(0);
+  constexpr int S2 = split_smem<D, 2, 8>();
   if (qd == CFA_F32) {
     if (kd == CFA_F32) {
-      e = a.rows == 1   ? launch_split<split_f32_kernel<D, 1>>(split_smem<D, 4>(1), a, stream)
-          : a.rows == 2 ? launch_split<split_f32_kernel<D, 2>>(split_smem<D, 4>(2), a, stream)
-          : a.rows <= 4 ? launch_split<split_f32_kernel<D, 4>>(split_smem<D, 4>(4), a, stream)
-                        : launch_split<split_f32_kernel<D, 8>>(split_smem<D, 4>(8), a, stream);
+      e = a.rows == 1         ? launch_split<split_fma_kernel<D, 1>>(split_smem<D, 4, 1>(), a, stream)
+          : a.rows == 2       ? launch_split<split_fma_kernel<D, 2>>(split_smem<D, 4, 2>(), a, stream)
+          : a.block_rows == 8 ? launch_split<split_f32_kernel<D, 1>>(split_smem<D, 4, 8>(), a, stream)
+                              : launch_split<split_f32_kernel<D, 2>>(split_smem<D, 4, 16>(), a, stream);
     } else if (kd == CFA_F16) {
       e = launch_split<split_mma_kernel<float, __half, D>>(S2, a, stream);
     } else {
@@ -1052,12 +1387,12 @@ cudaError_t set_attrs() {
   auto set = [&](const void* fn, int bytes) {
     if (e == cudaSuccess) e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   };
-  constexpr int S2 = split_smem<D, 2>(0);
-  static_assert(S2 <= 232448 && split_smem<D, 4>(MAXR) <= 232448, "shared memory per block");
-  set(reinterpret_cast<const void*>(split_f32_kernel<D, 1>), split_smem<D, 4>(1));
-  set(reinterpret_cast<const void*>(split_f32_kernel<D, 2>), split_smem<D, 4>(2));
-  set(reinterpret_cast<const void*>(split_f32_kernel<D, 4>), split_smem<D, 4>(4));
-  set(reinterpret_cast<const void*>(split_f32_kernel<D, 8>), split_smem<D, 4>(8));
+  constexpr int S2 = split_smem<D, 2, 8>();
+  static_assert(S2 <= 232448 && split_smem<D, 4, 16>() <= 232448, "shared memory per block");
+  set(reinterpret_cast<const void*>(split_fma_kernel<D, 1>), split_smem<D, 4, 1>());
+  set(reinterpret_cast<const void*>(split_fma_kernel<D, 2>), split_smem<D, 4, 2>());
+  set(reinterpret_cast<const void*>(split_f32_kernel<D, 1>), split_smem<D, 4, 8>());
+  set(reinterpret_cast<const void*>(split_f32_kernel<D, 2>), split_smem<D, 4, 16>());
   set(reinterpret_cast<const void*>(split_mma_kernel<float, __half, D>), S2);
   set(reinterpret_cast<const void*>(split_mma_kernel<float, __nv_bfloat16, D>), S2);
   set(reinterpret_cast<const void*>(split_mma_kernel<__half, __half, D>), S2);
@@ -1100,7 +1435,8 @@ cudaError_t launch_split_attention(const SplitArgs& args, int q_dtype, int kv_dt
   SplitArgs a = args;
   a.group = a.H / a.Hk;
   a.rows = a.group * a.S;
-  a.row_chunks = (a.rows + MAXR - 1) / MAXR;
+  a.block_rows = kv_dtype == CFA_F32 && a.rows > 8 ? 16 : 8;
+  a.row_chunks = (a.rows + a.block_rows - 1) / a.block_rows;
   a.max_chunks = split_max_chunks(a.max_len, a.D, kv_dtype);
   a.tile_log = tile_log_of(a.D, kv_dtype);
   // key / page for key < 2^31: key mul >> shift, mul = ceil(2^shift / page), 2^shift >= 2^31 page.
