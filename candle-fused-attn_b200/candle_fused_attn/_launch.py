@@ -7,8 +7,9 @@ from __future__ import annotations
 import contextlib
 
 import torch
+from torch.autograd.function import once_differentiable
 
-from . import FusedAttentionError, _abi, _raise_if_expired, _stream
+from . import FusedAttentionError, _abi, _raise_if_expired, _sink_flag, _stream
 
 DTYPES = {torch.float32: _abi.CFA_F32, torch.float16: _abi.CFA_F16, torch.bfloat16: _abi.CFA_BF16}
 _nothing = contextlib.nullcontext()
@@ -67,4 +68,24 @@ def check_status(status: int, who: str) -> None:
         raise FusedAttentionError(f"{who}: {_abi.strerror(status)}")
 
 
-raise_if_expired = _raise_if_expired
+def first_order(backward):
+    """A Function's backward whose result cannot be differentiated again: an error then. (The wrapper that
+    watches for it costs 10 us, and only `create_graph` needs it.)"""
+    watched = once_differentiable(backward)
+
+    def call(ctx, grad):
+        return (watched if torch.is_grad_enabled() else backward)(ctx, grad)
+
+    return call
+
+
+_flag = None
+
+
+def raise_if_expired() -> None:
+    """As the fused attention does before a launch (its check, without looking the flag up each time)."""
+    global _flag
+    if _flag is None:
+        _flag = _sink_flag()
+    if _flag.value:
+        _raise_if_expired()

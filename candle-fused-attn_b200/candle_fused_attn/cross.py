@@ -5,11 +5,10 @@ padded batch of keys, key heads shared by groups of query heads; fp32, with grad
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import FusedAttentionError, _abi, _check_head_dim, _float4_rows
-from ._launch import (check_status, current_stream, int32_vector, merged_heads, on_device,
-                      one_device, raise_if_expired, require)
+from ._launch import (check_status, current_stream, first_order, int32_vector, merged_heads,
+                      on_device, one_device, raise_if_expired, require)
 
 __all__ = ["cross_attention"]
 
@@ -79,7 +78,7 @@ class _CrossAttention(torch.autograd.Function):
         return o
 
     @staticmethod
-    @once_differentiable
+    @first_order
     def backward(ctx, grad):
         q, k, v, key_lengths, o, lse = ctx.saved_tensors
         b, h, hk, sq, sk, d = ctx.dims
@@ -97,8 +96,9 @@ class _CrossAttention(torch.autograd.Function):
                                 dkv.data_ptr(), ws.data_ptr(), n, b, h, hk, sq, sk, d, ctx.scale,
                                 current_stream(dev))
         check_status(st, "cross_attention")
-        dk, dv = dkv.permute(2, 0, 3, 1, 4).unbind(0)
-        return dq, dk, dv, None, None, None
+        shape, strides = (b, hk, sk, d), (2 * sk * hk * d, d, 2 * hk * d, 1)
+        return (dq, dkv.as_strided(shape, strides), dkv.as_strided(shape, strides, hk * d),
+                None, None, None)
 
 
 def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float,

@@ -6,11 +6,10 @@ from __future__ import annotations
 import math
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import FusedAttentionError, _abi, qkv_geometry
-from ._launch import (DTYPES, check_status, current_stream, merged_heads, no_gradient, on_device,
-                      one_device, raise_if_expired, require)
+from ._launch import (DTYPES, check_status, current_stream, first_order, merged_heads, no_gradient,
+                      on_device, one_device, raise_if_expired, require)
 
 __all__ = ["rotary", "rotary_qkv", "rotary_frequencies"]
 
@@ -99,7 +98,7 @@ class _Rotary(torch.autograd.Function):
         return _turn(x, positions, freqs, amplitude, interleaved, False)
 
     @staticmethod
-    @once_differentiable
+    @first_order
     def backward(ctx, grad):
         freqs, *at = ctx.saved_tensors
         positions = at[0] if at else ctx.first
@@ -126,7 +125,7 @@ class _RotaryQkv(torch.autograd.Function):
         return _turn_qkv(qkv, heads, positions, freqs, amplitude, interleaved, False)
 
     @staticmethod
-    @once_differentiable
+    @first_order
     def backward(ctx, grad):
         freqs, *at = ctx.saved_tensors
         positions = at[0] if at else ctx.first

@@ -178,3 +178,15 @@ def test_other_stream_and_graph(cuda):
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(out, cfa.rotary(x, pos, freqs)) and not torch.equal(out, want)
+
+
+def test_second_derivative_is_refused(cuda):
+    """Not dropped: an error where the gradient itself is differentiated, none where it only could be."""
+    freqs, _ = cfa.rotary_frequencies(64, device=cuda)
+    x = torch.randn(1, 2, 5, 64, device=cuda, requires_grad=True)
+    for y in (cfa.rotary(x, 3, freqs), cfa.cross_attention(x, x, x, 0.125)):
+        dx, = torch.autograd.grad((y * y).sum(), x, create_graph=True, retain_graph=True)
+        want, = torch.autograd.grad((y * y).sum(), x)
+        assert torch.equal(dx, want)
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            dx.sum().backward()
