@@ -1,6 +1,7 @@
 # SPDX-License-Identifier: MIT OR Apache-2.0
 """Builds libcfa.so in-tree: the sm_100a kernels and the C ABI of include/cfa.h; and
-libcfa_host.so, the C++ host layer above it (host/: src/lib.rs's API for compiled callers).
+libcfa_host.so, the C++ host layer above it (host/: src/lib.rs's API for compiled callers); and
+_ops.so, the Python extension of the operators beside it (binding/, against torch's headers).
 
     python candle-fused-attn_b200/build.py
 
@@ -15,6 +16,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -27,6 +29,8 @@ SOURCES = ["fwd_ffma.cu", "fwd_tc.cu", "bwd_ffma.cu", "bwd_tc.cu", "hd_ffma.cu",
 HOST_DIR = PKG / "host"
 HOST_OUT = PKG / "candle_fused_attn" / "libcfa_host.so"
 HOST_SOURCES = ["tensor.cu", "candle_fused_attn.cpp"]
+OPS_SOURCE = PKG / "binding" / "torch_ops.cpp"
+OPS_OUT = PKG / "candle_fused_attn" / "_ops.so"
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -88,6 +92,33 @@ def build_host(force: bool = False, verbose: bool = False) -> Path:
     return HOST_OUT
 
 
+def build_ops(force: bool = False, verbose: bool = False) -> Path:
+    """_ops.so: binding/torch_ops.cpp against the headers and libraries of the installed torch (which is
+    loaded before it, so no path to them is kept; a torch newer than the extension rebuilds it)."""
+    import torch
+
+    base = Path(torch.__file__).resolve().parent
+    deps = [OPS_SOURCE, ROOT / "include" / "cfa.h", base / "version.py"]
+    if not force and OPS_OUT.exists() and all(
+            p.stat().st_mtime <= OPS_OUT.stat().st_mtime for p in deps):
+        return OPS_OUT
+    cuda = Path(nvcc()).resolve().parent.parent
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           "-I", str(ROOT / "include"), "-isystem", str(base / "include"),
+           "-isystem", str(base / "include" / "torch" / "csrc" / "api" / "include"),
+           "-isystem", str(cuda / "include"), "-isystem", sysconfig.get_paths()["include"],
+           "-o", str(OPS_OUT), str(OPS_SOURCE), "-L", str(base / "lib"), "-ltorch_python", "-ltorch",
+           "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if verbose or r.returncode != 0:
+        sys.stderr.write(r.stdout + r.stderr)
+    if r.returncode != 0:
+        raise RuntimeError(f"{cmd[0]} failed on the extension ({r.returncode})")
+    return OPS_OUT
+
+
 if __name__ == "__main__":
     print(build(force="--force" in sys.argv, verbose=True))
     print(build_host(force="--force" in sys.argv, verbose=True))
+    print(build_ops(force="--force" in sys.argv, verbose=True))

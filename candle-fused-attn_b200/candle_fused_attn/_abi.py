@@ -9,9 +9,7 @@ library is missing; there is no fallback of any kind.
 from __future__ import annotations
 
 import ctypes
-import functools
 import os
-import struct
 from pathlib import Path
 
 LIB_NAME = "libcfa.so"
@@ -73,7 +71,6 @@ EXPORTS = (
     "cfa_paged_append",
     "cfa_paged_attention_workspace_bytes",
     "cfa_paged_attention",
-    "cfa_call",
 )
 
 # Head dims the generic entry points (cfa_fwd_f32, cfa_bwd_f32) take; the _d64 ones take 64 only,
@@ -155,17 +152,35 @@ def load() -> ctypes.CDLL:
         fn = getattr(lib, name)
         fn.restype = ctypes.c_size_t
         fn.argtypes = [_i64, _i64, _i64, _i64]
-    _n = ctypes.c_size_t
+    _f, _d, _n = ctypes.c_float, ctypes.c_int, ctypes.c_size_t
+    lib.cfa_cross_fwd_f32.restype = ctypes.c_int
+    lib.cfa_cross_fwd_f32.argtypes = [_p, _strides, _p, _strides, _p, _strides, _p, _p, _p,
+                                      *[_i64] * 6, _f, _p]
     lib.cfa_cross_bwd_workspace_bytes.restype = _n
     lib.cfa_cross_bwd_workspace_bytes.argtypes = [_i64] * 6
     lib.cfa_cross_bwd_workspace_bytes_fast.restype = _n
     lib.cfa_cross_bwd_workspace_bytes_fast.argtypes = [_i64] * 6
+    lib.cfa_cross_bwd_f32.restype = ctypes.c_int
+    lib.cfa_cross_bwd_f32.argtypes = [_p, _strides, _p, _strides, _p, _strides, _p, _p, _p, _p,
+                                      _strides, _p, _p, _p, _n, *[_i64] * 6, _f, _p]
     lib.cfa_cross_few_workspace_bytes.restype = _n
     lib.cfa_cross_few_workspace_bytes.argtypes = [_i64] * 5
+    lib.cfa_cross_few_f32.restype = ctypes.c_int
+    lib.cfa_cross_few_f32.argtypes = [_p, _strides, _p, _strides, _p, _strides, _p, _p, _p, _n,
+                                      *[_i64] * 6, _f, _p]
+    lib.cfa_rotary.restype = ctypes.c_int
+    lib.cfa_rotary.argtypes = [_p, _strides, _p, _strides, _d, _p, _d, _strides, _i64, _p, _f,
+                               *[_i64] * 6, _d, _d, _p]
+    lib.cfa_paged_append.restype = ctypes.c_int
+    lib.cfa_paged_append.argtypes = [_p, _strides, _p, _strides, _p, _strides, _p, _strides, _d,
+                                     _p, _strides, _p, _strides, _d, _i64, _i64, _p, _i64, _i64,
+                                     _p, _p, _p, _f, *[_i64] * 6, _d, _p]
     lib.cfa_paged_attention_workspace_bytes.restype = _n
-    lib.cfa_paged_attention_workspace_bytes.argtypes = [*[_i64] * 5, ctypes.c_int]
-    lib.cfa_call.restype = ctypes.c_int
-    lib.cfa_call.argtypes = [ctypes.c_int, ctypes.c_char_p]
+    lib.cfa_paged_attention_workspace_bytes.argtypes = [*[_i64] * 5, _d]
+    lib.cfa_paged_attention.restype = ctypes.c_int
+    lib.cfa_paged_attention.argtypes = [_p, _strides, _d, _p, _strides, _p, _strides, _d, _i64,
+                                        _i64, _p, _i64, _i64, _p, _p, _p, _p, _n, *[_i64] * 5, _f,
+                                        _p]
     _lib = lib
     return lib
 
@@ -174,15 +189,9 @@ def strerror(status: int) -> str:
     return load().cfa_strerror(int(status)).decode()
 
 
-@functools.lru_cache(maxsize=4096)
-def _int64s(s: tuple) -> ctypes.Array:
-    return (ctypes.c_int64 * len(s))(*(int(x) for x in s))
-
-
 def strides3(s) -> ctypes.Array:
-    """A (batch, head, seq) stride triple as the `const int64_t[3]` the ABI takes (kept by value: the
-    ABI only reads it)."""
-    return _int64s(tuple(s))
+    """A (batch, head, seq) stride triple as the `const int64_t[3]` the ABI takes."""
+    return (ctypes.c_int64 * 3)(*(int(x) for x in s))
 
 
 def check(status: int, where: str) -> None:
@@ -331,35 +340,18 @@ def matmul_status(stream) -> int:
     return load().cfa_matmul_status(stream)
 
 
-# The operators go through cfa_call, their arguments packed into words (20 to 40 arguments cost ctypes
-# 4 us and more a call, two cost it 0.6): a letter a word, q an integer or a pointer, d a float.
-_TENSOR = "qqqq"  # a pointer and its strides
-_CROSS_FWD = (0, struct.Struct(3 * _TENSOR + "qqq" + "qqqqqqdq"))
-_CROSS_BWD = (1, struct.Struct(3 * _TENSOR + "qqq" + _TENSOR + "qqqq" + "qqqqqqdq"))
-_CROSS_FEW = (2, struct.Struct(3 * _TENSOR + "qqqq" + "qqqqqqdq"))
-_ROTARY = (3, struct.Struct(2 * _TENSOR + "qqqqqqqqd" + "qqqqqqqqq"))
-_PAGED_APPEND = (4, struct.Struct(4 * _TENSOR + "q" + 2 * _TENSOR + "qqqqqqqqqd" + "qqqqqqqq"))
-_PAGED_ATTENTION = (5, struct.Struct(_TENSOR + "q" + 2 * _TENSOR + "qqqqqqqqqqq" + "qqqqqdq"))
-_NONE3 = (0, 0, 0)
-
-
-def _call(op, *words) -> int:
-    number, packing = op
-    return load().cfa_call(number, packing.pack(*words))
-
-
 def cross_fwd(q_ptr, qs, k_ptr, ks, v_ptr, vs, lengths_ptr, o_ptr, lse_ptr, b, h, hk, sq, sk, d,
               scale, stream) -> int:
     """cfa_cross_fwd_f32; returns the status."""
-    return _call(_CROSS_FWD, q_ptr or 0, *qs, k_ptr or 0, *ks, v_ptr or 0, *vs, lengths_ptr or 0,
-                 o_ptr or 0, lse_ptr or 0, b, h, hk, sq, sk, d, scale, stream or 0)
+    return load().cfa_cross_fwd_f32(
+        q_ptr, strides3(qs), k_ptr, strides3(ks), v_ptr, strides3(vs), lengths_ptr, o_ptr, lse_ptr,
+        b, h, hk, sq, sk, d, scale, stream)
 
 
 def cross_bwd_workspace_bytes(b, h, hk, sq, sk, d) -> int:
     return int(load().cfa_cross_bwd_workspace_bytes(b, h, hk, sq, sk, d))
 
 
-@functools.lru_cache(maxsize=1024)
 def cross_bwd_workspace_bytes_fast(b, h, hk, sq, sk, d) -> int:
     return int(load().cfa_cross_bwd_workspace_bytes_fast(b, h, hk, sq, sk, d))
 
@@ -367,12 +359,12 @@ def cross_bwd_workspace_bytes_fast(b, h, hk, sq, sk, d) -> int:
 def cross_bwd(q_ptr, qs, k_ptr, ks, v_ptr, vs, lengths_ptr, o_ptr, lse_ptr, do_ptr, dos, dq_ptr,
               dkv_ptr, ws_ptr, ws_bytes, b, h, hk, sq, sk, d, scale, stream) -> int:
     """cfa_cross_bwd_f32; returns the status."""
-    return _call(_CROSS_BWD, q_ptr or 0, *qs, k_ptr or 0, *ks, v_ptr or 0, *vs, lengths_ptr or 0,
-                 o_ptr or 0, lse_ptr or 0, do_ptr or 0, *dos, dq_ptr or 0, dkv_ptr or 0,
-                 ws_ptr or 0, ws_bytes, b, h, hk, sq, sk, d, scale, stream or 0)
+    return load().cfa_cross_bwd_f32(
+        q_ptr, strides3(qs), k_ptr, strides3(ks), v_ptr, strides3(vs), lengths_ptr, o_ptr, lse_ptr,
+        do_ptr, strides3(dos), dq_ptr, dkv_ptr, ws_ptr, ws_bytes, b, h, hk, sq, sk, d, scale,
+        stream)
 
 
-@functools.lru_cache(maxsize=1024)
 def cross_few_workspace_bytes(b, h, sq, sk, d) -> int:
     return int(load().cfa_cross_few_workspace_bytes(b, h, sq, sk, d))
 
@@ -380,30 +372,31 @@ def cross_few_workspace_bytes(b, h, sq, sk, d) -> int:
 def cross_few(q_ptr, qs, k_ptr, ks, v_ptr, vs, lengths_ptr, o_ptr, ws_ptr, ws_bytes, b, h, hk, sq,
               sk, d, scale, stream) -> int:
     """cfa_cross_few_f32 (the forward for few query rows a key head); returns the status."""
-    return _call(_CROSS_FEW, q_ptr or 0, *qs, k_ptr or 0, *ks, v_ptr or 0, *vs, lengths_ptr or 0,
-                 o_ptr or 0, ws_ptr or 0, ws_bytes, b, h, hk, sq, sk, d, scale, stream or 0)
+    return load().cfa_cross_few_f32(
+        q_ptr, strides3(qs), k_ptr, strides3(ks), v_ptr, strides3(vs), lengths_ptr, o_ptr, ws_ptr,
+        ws_bytes, b, h, hk, sq, sk, d, scale, stream)
 
 
 def rotary(x_ptr, xs, y_ptr, ys, dtype, pos_ptr, pos_bytes, pos_strides, first, freqs_ptr,
            amplitude, b, h, rotated, s, d, rot, interleaved, inverse, stream) -> int:
     """cfa_rotary; returns the status. `pos_strides`: (batch, seq), or None without positions."""
-    return _call(_ROTARY, x_ptr or 0, *xs, y_ptr or 0, *ys, dtype, pos_ptr or 0, pos_bytes,
-                 *(pos_strides or (0, 0)), 0, first, freqs_ptr or 0, amplitude, b, h, rotated, s,
-                 d, rot, interleaved, inverse, stream or 0)
+    return load().cfa_rotary(
+        x_ptr, strides3(xs), y_ptr, strides3(ys), dtype, pos_ptr, pos_bytes,
+        None if pos_strides is None else (ctypes.c_int64 * 2)(*pos_strides), first, freqs_ptr,
+        amplitude, b, h, rotated, s, d, rot, int(interleaved), int(inverse), stream)
 
 
 def paged_append(q_ptr, qs, qo_ptr, qos, k_ptr, ks, v_ptr, vs, dtype, kc_ptr, kcs, vc_ptr, vcs,
                  cache_dtype, pages, page_size, table_ptr, table_stride, table_width, lengths_ptr,
                  new_ptr, freqs_ptr, amplitude, b, h, hk, s, d, rot, interleaved, stream) -> int:
     """cfa_paged_append; returns the status. `qs`, `qos`: None without q."""
-    return _call(_PAGED_APPEND, q_ptr or 0, *(qs or _NONE3), qo_ptr or 0, *(qos or _NONE3),
-                 k_ptr or 0, *ks, v_ptr or 0, *vs, dtype, kc_ptr or 0, *kcs, vc_ptr or 0, *vcs,
-                 cache_dtype, pages, page_size, table_ptr or 0, table_stride, table_width,
-                 lengths_ptr or 0, new_ptr or 0, freqs_ptr or 0, amplitude, b, h, hk, s, d, rot,
-                 interleaved, stream or 0)
+    return load().cfa_paged_append(
+        q_ptr, None if qs is None else strides3(qs), qo_ptr, None if qos is None else strides3(qos),
+        k_ptr, strides3(ks), v_ptr, strides3(vs), dtype, kc_ptr, strides3(kcs), vc_ptr,
+        strides3(vcs), cache_dtype, pages, page_size, table_ptr, table_stride, table_width,
+        lengths_ptr, new_ptr, freqs_ptr, amplitude, b, h, hk, s, d, rot, int(interleaved), stream)
 
 
-@functools.lru_cache(maxsize=1024)
 def paged_attention_workspace_bytes(b, h, s, max_keys, d, cache_dtype) -> int:
     return int(load().cfa_paged_attention_workspace_bytes(b, h, s, max_keys, d, cache_dtype))
 
@@ -412,7 +405,7 @@ def paged_attention(q_ptr, qs, dtype, kc_ptr, kcs, vc_ptr, vcs, cache_dtype, pag
                     table_ptr, table_stride, table_width, lengths_ptr, new_ptr, o_ptr, ws_ptr,
                     ws_bytes, b, h, hk, s, d, scale, stream) -> int:
     """cfa_paged_attention; returns the status."""
-    return _call(_PAGED_ATTENTION, q_ptr or 0, *qs, dtype, kc_ptr or 0, *kcs, vc_ptr or 0, *vcs,
-                 cache_dtype, pages, page_size, table_ptr or 0, table_stride, table_width,
-                 lengths_ptr or 0, new_ptr or 0, o_ptr or 0, ws_ptr or 0, ws_bytes, b, h, hk, s, d,
-                 scale, stream or 0)
+    return load().cfa_paged_attention(
+        q_ptr, strides3(qs), dtype, kc_ptr, strides3(kcs), vc_ptr, strides3(vcs), cache_dtype,
+        pages, page_size, table_ptr, table_stride, table_width, lengths_ptr, new_ptr, o_ptr,
+        ws_ptr, ws_bytes, b, h, hk, s, d, scale, stream)

@@ -226,7 +226,7 @@ int* error_sink() { return g_sink.load(std::memory_order_relaxed); }
 
 extern "C" {
 
-int cfa_abi_version(void) { return (2 << 16) | 4; }
+int cfa_abi_version(void) { return (2 << 16) | 3; }
 
 const char* cfa_strerror(int status) {
   switch (status) {

@@ -4,10 +4,7 @@
 // positions, the paged cache's append and its attention. Argument checks and launches, as
 // cfa_abi.cu does for the fused attention; everything on the caller's stream, no synchronisation.
 #include <algorithm>
-#include <cstring>
 #include <mutex>
-#include <tuple>
-#include <type_traits>
 
 #include "cfa_internal.h"
 #include "cfa_ops.h"
@@ -56,28 +53,6 @@ bool split_units_ok(int64_t B, int64_t H, int64_t Hk, int64_t S, int64_t max_len
   const int64_t chunks = B * cfa::split_max_chunks(max_len, D, kv);
   const int64_t per = Hk * ((H / Hk * S + 7) / 8);
   return chunks <= kLim && per <= kLim && chunks <= kLim / per;
-}
-
-// The next argument of cfa_call's words. (const int64_t* is a strides array: no data is of that type.)
-template <typename T>
-T take(const int64_t*& w) {
-  if constexpr (std::is_same_v<T, const int64_t*>) {
-    w += 3;
-    return w - 3;
-  } else if constexpr (std::is_pointer_v<T>) {
-    return reinterpret_cast<T>(static_cast<uintptr_t>(*w++));
-  } else if constexpr (std::is_same_v<T, float>) {
-    double x;
-    std::memcpy(&x, w++, sizeof x);
-    return static_cast<float>(x);
-  } else {
-    return static_cast<T>(*w++);
-  }
-}
-template <typename... A>
-int call_words(int (*fn)(A...), const int64_t* w) {
-  const std::tuple<A...> args{take<A>(w)...};  // (in order: a braced list)
-  return std::apply(fn, args);
 }
 
 // B, H, Hk, Sq, Sk of a cross attention.
@@ -446,19 +421,6 @@ int cfa_paged_attention(const void* q, const int64_t q_strides[3], int dtype, co
   a.sink = cfa::error_sink();
   return status(cfa::launch_split_attention(a, dtype, cache_dtype, workspace,
                                             static_cast<cudaStream_t>(stream)));
-}
-
-int cfa_call(int op, const int64_t* words) {
-  if (!words) return CFA_ERR_NULL;
-  switch (op) {
-    case CFA_OP_CROSS_FWD: return call_words(cfa_cross_fwd_f32, words);
-    case CFA_OP_CROSS_BWD: return call_words(cfa_cross_bwd_f32, words);
-    case CFA_OP_CROSS_FEW: return call_words(cfa_cross_few_f32, words);
-    case CFA_OP_ROTARY: return call_words(cfa_rotary, words);
-    case CFA_OP_PAGED_APPEND: return call_words(cfa_paged_append, words);
-    case CFA_OP_PAGED_ATTENTION: return call_words(cfa_paged_attention, words);
-    default: return CFA_ERR_SHAPE;
-  }
 }
 
 }  // extern "C"

@@ -385,26 +385,12 @@ int cfa_paged_attention(const void* q, const int64_t q_strides[3], int dtype, co
                         int64_t heads, int64_t key_heads, int64_t seq, int64_t head_dim,
                         float scale, void* stream);
 
-/* One of the operators' entry points by its number, its arguments as 64-bit words in their order:
- * pointers (NULL: 0) and integers as they are, a float as a double, a strides array as its three words
- * (position_strides: two and one that is not read; of an operand that is not there: not read). For
- * bindings whose calls cost by the argument. CFA_ERR_SHAPE for a number that is none of these. */
-enum cfa_op {
-  CFA_OP_CROSS_FWD = 0,
-  CFA_OP_CROSS_BWD = 1,
-  CFA_OP_CROSS_FEW = 2,
-  CFA_OP_ROTARY = 3,
-  CFA_OP_PAGED_APPEND = 4,
-  CFA_OP_PAGED_ATTENTION = 5
-};
-int cfa_call(int op, const int64_t* words);
-
 /* A static description of a status code. */
 const char* cfa_strerror(int status);
 
 /* ABI version: (major << 16) | minor (2.0: one kernel pair per entry point, the error sink;
  * 2.1: the projection GEMM; 2.2: head dim 32 on the tensor cores, the generic CUDA-core pair;
- * 2.3: cross attention, rotary positions, the paged cache; 2.4: cfa_call). */
+ * 2.3: cross attention, rotary positions, the paged cache). */
 int cfa_abi_version(void);
 
 #ifdef __cplusplus

@@ -101,17 +101,28 @@ def test_long_key_sequences(cuda, d, sq, sk, h, hk):
 
 @pytest.mark.parametrize("d,h,hk,sq,sk", [(64, 8, 4, 300, 900), (32, 3, 1, 130, 700), (128, 4, 2, 200, 400),
                                           (64, 1, 1, 1500, 150)])
-def test_turn_chain_gives_the_same_bits(cuda, monkeypatch, d, h, hk, sq, sk):
+def test_turn_chain_gives_the_same_bits(cuda, d, h, hk, sq, sk):
     """The workspace too small for the dQ partials (what more than 4 GB of them are): key blocks add to
     dQ in turn, the same sums in the same order."""
-    lens = [sk, sk // 2, 0]
-    _, _, o, grads = run(cuda, 3, h, hk, sq, sk, d, lens)
-    fast = _abi.cross_bwd_workspace_bytes_fast(3, h, hk, sq, sk, d)
-    least = _abi.cross_bwd_workspace_bytes(3, h, hk, sq, sk, d)
-    assert least < fast
-    monkeypatch.setattr(_abi, "cross_bwd_workspace_bytes_fast", lambda *a: least)
-    _, _, o2, chain = run(cuda, 3, h, hk, sq, sk, d, lens)
-    assert torch.equal(o, o2) and all(torch.equal(x, y) for x, y in zip(grads, chain))
+    b, lens = 3, [sk, sk // 2, 0]
+    (_, _, _, dout, scale, lengths), x, o, grads = run(cuda, b, h, hk, sq, sk, d, lens)
+    q, k, v = (t.detach() for t in x)
+    dout = dout.to(cuda)
+    n = _abi.cross_bwd_workspace_bytes(b, h, hk, sq, sk, d)
+    assert n < _abi.cross_bwd_workspace_bytes_fast(b, h, hk, sq, sk, d)
+    ws = torch.empty(n, dtype=torch.uint8, device=cuda)
+    o2, dq = (torch.empty(b, sq, h, d, device=cuda) for _ in range(2))
+    lse, dkv = torch.empty(b, h, sq, device=cuda), torch.empty(b, sk, 2, hk, d, device=cuda)
+    operands = [a for t in (q, k, v) for a in (t.data_ptr(), t.stride()[:3])]
+    shape, stream = (b, h, hk, sq, sk, d, scale), torch.cuda.current_stream().cuda_stream
+    assert _abi.cross_fwd(*operands, lengths.data_ptr(), o2.data_ptr(), lse.data_ptr(), *shape,
+                          stream) == _abi.CFA_OK
+    assert _abi.cross_bwd(*operands, lengths.data_ptr(), o2.data_ptr(), lse.data_ptr(), dout.data_ptr(),
+                          dout.stride()[:3], dq.data_ptr(), dkv.data_ptr(), ws.data_ptr(), n, *shape,
+                          stream) == _abi.CFA_OK
+    cfa.check_status()
+    chain = (dq.transpose(1, 2), *(dkv[:, :, i].transpose(1, 2) for i in (0, 1)))
+    assert torch.equal(o, o2.transpose(1, 2)) and all(torch.equal(y, z) for y, z in zip(grads, chain))
 
 
 @pytest.mark.parametrize("d", [32, 64, 128])

@@ -5,8 +5,6 @@ arithmetic (a page id outside the pool never becomes an address)."""
 
 import math
 import random
-import re
-from pathlib import Path
 
 import pytest
 import torch
@@ -153,25 +151,6 @@ def test_paged_attention_arguments():
     assert call(st=(4096, 64, 60)) == _abi.CFA_ERR_ALIGNMENT  # 16-bit rows: multiples of 8
     assert call(nbytes=need - 1) == _abi.CFA_ERR_WORKSPACE
     assert call(dims=(0, 4, 2, 1, 64), q=None) == _abi.CFA_OK
-
-
-def test_packed_arguments_are_the_headers():
-    """The words that a packed call sends, against the declarations: a strides array three of them, a
-    float a double, everything else one."""
-    header = (Path(__file__).resolve().parent.parent / "include" / "cfa.h").read_text()
-    numbers = dict(re.findall(r"CFA_OP_(\w+) = (\d)", header))
-    ops = {"cross_fwd_f32": _abi._CROSS_FWD, "cross_bwd_f32": _abi._CROSS_BWD,
-           "cross_few_f32": _abi._CROSS_FEW, "rotary": _abi._ROTARY,
-           "paged_append": _abi._PAGED_APPEND, "paged_attention": _abi._PAGED_ATTENTION}
-    assert len(numbers) == len(ops)
-    for name, (number, packing) in ops.items():
-        arguments = re.search(rf"\bint cfa_{name}\((.*?)\);", header, re.S).group(1).split(",")
-        words = "".join("qqq" if "]" in a else "d" if re.match(r"\s*float \w+$", a) else "q"
-                        for a in arguments)
-        assert packing.format == words and packing.size == 8 * len(words), name
-        assert int(numbers[name.removesuffix("_f32").upper()]) == number
-    assert _abi.load().cfa_call(99, bytes(400)) == _abi.CFA_ERR_SHAPE
-    assert _abi.load().cfa_call(3, None) == _abi.CFA_ERR_NULL
 
 
 def test_statuses_have_words():
