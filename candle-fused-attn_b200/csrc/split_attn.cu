@@ -10,20 +10,24 @@
 // kernel joins the chunks in order: m = max m_c, l = sum e^(m_c - m) l_c, o = sum e^(m_c - m) o_c / l.
 // A sequence of one chunk is written by the first kernel.
 //
-// Bound by memory: every key and value is read once for all the query rows of its head (up to 8 a
-// block, 16 of fp32), at 4 rows D flops a key against 2 D elements. Each warp runs on its own: it takes every
+// Bound by memory: every key and value is read once for all the query rows of its head (up to 8 or 16
+// a block), at 4 rows D flops a key against 2 D elements. Each warp runs on its own: it takes every
 // fourth 8 KB tile of the chunk through a ring of its own (cp.async, 16 bytes a lane, rows padded by
-// 16 bytes so that every later read is free of bank conflicts), and the four warps' sums are joined
-// through shared memory once a chunk. The ring runs on through a block's chunks: a ring that drained
+// 16 bytes or their pieces exchanged, so that every later read is free of bank conflicts), and the four
+// warps' sums are joined through shared memory once a chunk. The ring runs on through a block's chunks: a ring that drained
 // at the end of each took 204 us where this takes 199.
-//   16-bit caches: S^T = K Q^T and O^T += V^T P^T by mma.m16n8k16, the keys (dims) as the 16 rows
-//     and up to 8 query rows as the 8 columns: a column's softmax state then lives in the lanes
+//   16-bit caches, up to 8 query rows: S^T = K Q^T and O^T += V^T P^T by mma.m16n8k16, the keys (dims)
+//     as the 16 rows and the query rows as the 8 columns: a column's softmax state then lives in the lanes
 //     that hold the column's output. fp32 queries enter in parts that keep their 24 bits (three
 //     bf16, or two fp16 under a power of two a row: 22 bits), p as two parts (16 bits of bf16, 22 of
 //     fp16) or, fp32 queries over bf16, three (24 bits), every tile's product a fresh accumulator
 //     folded by an fp32 FMA -- the tensor core's truncating sums never run longer than a tile.
 //     tcgen05 has no shape below 64 rows, and at a few rows the product is a small share of the
 //     tile's load time. Three stages of two blocks a SM (two of three blocks: 245 us for 204).
+//   16-bit caches, more rows: S = Q K^T and O += P V, 16 query rows as the 16 rows; the same parts. In
+//     blocks of 8 and of 16, 32 sequences of 100 to 8000 keys, four key heads, in us: 16 rows bf16 69
+//     and 56 (d 64), 113 and 81 (d 128), fp32 over bf16 75 and 68, 131 and 98; 40 rows bf16 d 128 270
+//     and 209. Bound by the issue of the products and the softmax, two warps a scheduler.
 //   fp32 caches, three query rows and more: S = Q K^T and O += P V by mma.m16n8k8 on tf32 operands, 8 or
 //     16 query rows as the 16 rows. Every operand enters in two parts of 11 bits (x = hi + lo to 2^-22
 //     |x|; three or all four of the products of the parts), and dims and keys are numbered within a
@@ -180,11 +184,15 @@ struct Ring {
   static constexpr int BYTES = ST * STAGE;
   static constexpr unsigned ALL = 0xffffffffu >> (32 - TK);
 
-  // SWIZZLE (rows of 128 bytes and more): the piece c of row r of K, V is piece c ^ this of its row, by
-  // which the eight lanes of a 16-byte read (K: two rows, four pieces; V: every other row of eight, two
-  // pieces) meet eight banks of 16 bytes. Else rows are padded by 16 bytes.
-  static __device__ __forceinline__ int k_swizzle(int r) { return SWIZZLE ? 4 * (r & 1) : 0; }
-  static __device__ __forceinline__ int v_swizzle(int r) { return SWIZZLE ? 2 * ((r >> 1) & 3) : 0; }
+  // SWIZZLE: the piece c of row r of K, V is piece c ^ this of its row, by which the eight lanes of a
+  // 16-byte read meet eight banks of 16 bytes (fp32: two rows of K, four pieces; every other row of eight
+  // of V, two pieces; 16-bit: one piece of eight rows). Else rows are padded by 16 bytes.
+  static __device__ __forceinline__ int k_swizzle(int r) {
+    return !SWIZZLE ? 0 : ES == 4 ? 4 * (r & 1) : CPR == 4 ? (r >> 1) & 3 : r & 7;
+  }
+  static __device__ __forceinline__ int v_swizzle(int r) {
+    return SWIZZLE && ES == 4 ? 2 * ((r >> 1) & 3) : k_swizzle(r);
+  }
 
   const SplitArgs& a;
   const ChunkIndex& ix;
@@ -443,12 +451,12 @@ template <int D, int ES>
 __host__ __device__ constexpr int tile_keys() {
   return ES == 2 ? (D == 128 ? 16 : 32) : 1024 / D;  // (tile_log_of says the same to the host)
 }
-// ROWS: query rows of a block (fp32 caches: up to two by FMAs, else 8 or 16 by matrix products).
+// ROWS: query rows of a block, 8 or 16 (fp32 caches: one or two by FMAs).
 template <int D, int ES, int ROWS>
-using RingOf = Ring<D, ES, tile_keys<D, ES>(), (ROWS <= 2 ? 2 : 3), (ES == 4 && ROWS > 2)>;
+using RingOf = Ring<D, ES, tile_keys<D, ES>(), (ROWS <= 2 ? 2 : 3), (ES == 4 ? ROWS > 2 : ROWS == 16)>;
 // Shared memory: the rings -- whose free stage also takes a warp's sums when a unit ends -- the (m, l)
-// of the warps' rows and where their sums are, and, fp32, two sets of query rows and p (FMAs) or the
-// fragments of 16 rows.
+// of the warps' rows and where their sums are, and two sets of query rows and p (FMAs) or the fragments
+// of 16 rows (two parts of fp32, up to three of 16 bits).
 template <int D, int ES, int ROWS>
 __host__ __device__ constexpr int off_ml() {
   static_assert(RingOf<D, ES, ROWS>::STAGE >= ROWS * D * 4, "a stage holds a warp's sums");
@@ -461,7 +469,7 @@ __host__ __device__ constexpr int off_q() {
 template <int D, int ES, int ROWS>
 __host__ __device__ constexpr int split_smem() {
   return off_q<D, ES, ROWS>() +
-         (ROWS <= 2 ? ROWS * (2 * D * 4 + WARPS * tile_keys<D, ES>() * 8) : ROWS == 16 ? 128 * D : 0);
+         (ROWS <= 2 ? ROWS * (2 * D * 4 + WARPS * tile_keys<D, ES>() * 8) : ROWS == 16 ? 16 * D * (ES == 4 ? 8 : 6) : 0);
 }
 
 // 16-bit caches.
@@ -735,6 +743,312 @@ __global__ void __launch_bounds__(NT, 2)
     __syncthreads();
     write_chunk<QT, D>(a, done, smem, red_at, ml, min(8, a.rows - done.r0));
     __syncthreads();  // the sums are read: their stages take tiles again
+  }
+  if (ring.bad) flag_error(a.sink, CFA_ERR_PAGE);
+}
+
+// 16-bit caches, up to 16 query rows a block as the 16 rows of the products: S = Q K^T, O += P V, the
+// queries' fragments in shared memory, P's those of S.
+template <typename QT, typename T, int D>
+__global__ void __launch_bounds__(NT, 2) split_rows_kernel(const SplitArgs a) {
+  using R = RingOf<D, 2, 16>;
+  constexpr int ST = R::ST, TK = R::TK, MT = TK / 16, KS = D / 16;
+  constexpr bool F32 = std::is_same_v<QT, float>;
+  constexpr bool HALF = std::is_same_v<T, __half>;
+  constexpr int QP = F32 ? (HALF ? 2 : 3) : 1;  // parts of q
+  constexpr int PP = F32 && !HALF ? 3 : 2;      // parts of p
+  constexpr int JQ = (KS + WARPS - 1) / WARPS;  // this warp's share of q's columns
+  using QPair = std::conditional_t<F32, float2, uint32_t>;
+  extern __shared__ __align__(128) unsigned char smem[];
+  const int tid = threadIdx.x, w = tid >> 5, lane = tid & 31;
+  const int g = lane >> 2, t4 = lane & 3;  // a fragment's row (B: column) and pair
+  float2* ml = reinterpret_cast<float2*>(smem + off_ml<D, 2, 16>());
+  int* red_at = reinterpret_cast<int*>(ml + WARPS * MAXR);
+  uint4* qs = reinterpret_cast<uint4*>(smem + off_q<D, 2, 16>());  // [KS][part][lane]
+  griddep_wait();
+  griddep_launch_dependents();
+  ChunkIndex ix;
+  ix.init(a, lane);
+  const uint32_t units = static_cast<uint32_t>(ix.total) * a.Hk * a.row_chunks;
+  R ring(a, ix, units, smem + w * R::BYTES, lane, w);
+
+  // Dims 16 ks + 2 t4, + 1 and + 8, + 9 of rows g and g + 8 (zeros where there is no row).
+  QPair qx[JQ][2][2];
+  float up[2];  // fp32 queries over fp16: a row's power of two
+  auto load_q = [&](const UnitInfo& n) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int row = n.r0 + g + 8 * h;
+      int head, i;
+      row_of(a, row, head, i);
+      const bool ok = row < a.rows && i < n.n_new;
+      const QT* q = static_cast<const QT*>(a.q) + n.b * a.q_sb +
+                    (n.hk * a.group + (ok ? head : 0)) * a.q_sh + (ok ? i : 0) * a.q_ss + 2 * t4;
+#pragma unroll
+      for (int x = 0; x < JQ; ++x)
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          const int ks = w + WARPS * x;
+          qx[x][h][y] = ok && ks < KS ? *reinterpret_cast<const QPair*>(q + 16 * ks + 8 * y) : QPair{};
+        }
+      up[h] = 1.0f;
+      if constexpr (F32 && HALF) {  // (as split_mma_kernel: q = 2^e (h0 + 2^-11 h1), |h0| <= 2)
+        float top = 0.0f;
+        if (ok) {
+#pragma unroll
+          for (int x = 0; x < D / 8; ++x) {
+            const float2 z = *reinterpret_cast<const float2*>(q + 8 * x);
+            top = fmaxf(top, fmaxf(fabsf(z.x), fabsf(z.y)));
+          }
+        }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const int e = top > 0.0f && top < INFINITY ? ilogbf(top) : 0;
+        up[h] = ldexpf(1.0f, max(-120, min(120, e)));
+      }
+    }
+  };
+  auto store_q = [&]() {
+#pragma unroll
+    for (int x = 0; x < JQ; ++x) {
+      const int ks = w + WARPS * x;
+      uint32_t parts[QP][4];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          if constexpr (!F32) {
+            parts[0][h + 2 * y] = qx[x][h][y];
+          } else if constexpr (HALF) {
+            const float down = 1.0f / up[h], lo = qx[x][h][y].x * down, hi = qx[x][h][y].y * down;
+            parts[0][h + 2 * y] = pack16<T>(lo, hi);
+            const float2 z = unpack16<T>(parts[0][h + 2 * y]);
+            parts[QP - 1][h + 2 * y] = pack16<T>((lo - z.x) * 2048.0f, (hi - z.y) * 2048.0f);
+          } else {
+            float2 v = qx[x][h][y];
+#pragma unroll
+            for (int p = 0; p < QP; ++p) {
+              parts[p][h + 2 * y] = pack16<T>(v.x, v.y);
+              const float2 z = unpack16<T>(parts[p][h + 2 * y]);
+              v = make_float2(v.x - z.x, v.y - z.y);
+            }
+          }
+        }
+      if (ks < KS) {
+#pragma unroll
+        for (int p = 0; p < QP; ++p)
+          qs[(ks * QP + p) * 32 + lane] = make_uint4(parts[p][0], parts[p][1], parts[p][2], parts[p][3]);
+      }
+    }
+  };
+  UnitInfo n;
+  if (blockIdx.x < units) {
+    n = unit_info(a, ix, blockIdx.x);
+    load_q(n);
+    store_q();
+    __syncthreads();  // q in place
+  }
+  // Addresses within a tile: K's rows (lane % 8) + 8 (lane / 16), pieces 2 ks + lane / 8 % 2; V's rows
+  // (lane % 8) + 8 (lane / 8 % 2), pieces 2 mt + lane / 16.
+  const int k_row = (lane & 7) + 8 * (lane >> 4), k_piece = (lane >> 3) & 1;
+  const int v_row = (lane & 7) + 8 * ((lane >> 3) & 1), v_piece = lane >> 4;
+  int stage = 0;  // of the next tile; the stage before it is free
+  for (uint32_t u = blockIdx.x; u < units; u += gridDim.x) {
+    const int tiles = (n.hi - n.lo + TK - 1) / TK;
+    const float qscale[2] = {a.scale * up[0], a.scale * up[1]};
+    const int lim[2] = {row_limit(a, n, n.r0 + g), row_limit(a, n, n.r0 + g + 8)};
+    // The fewest keys that a row of the block sees: a tile that ends behind it masks row by row.
+    const int lim_min = a.causal ? max(n.len - n.n_new + 1, 0) : n.len;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+    float acc[KS][2][4];  // rows g, g + 8: dims 16 mt + 8 y + 2 t4, + 1
+#pragma unroll
+    for (int mt = 0; mt < KS; ++mt)
+#pragma unroll
+      for (int y = 0; y < 2; ++y)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) acc[mt][y][x] = 0.0f;
+
+    for (int t = w; t < tiles; t += WARPS) {
+      cp_async_wait_group<ST - 2>();
+      __syncwarp();  // the tile is in place for every lane, and the stage before it is free
+      const unsigned char* kt = ring.base + stage * R::STAGE;
+      const unsigned char* vt = kt + R::KV;
+      const int k0 = n.lo + TK * t;
+
+      // Scores of rows g, g + 8 and keys 16 i + 8 y + 2 t4, + 1. fp32: the small parts in a chain of
+      // their own, truncated at their magnitude; else two chains, half as long.
+      float c[MT][2][2][4];
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int y = 0; y < 2; ++y)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) c[i][y][0][x] = c[i][y][1][x] = 0.0f;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        uint32_t qa[QP][4];
+#pragma unroll
+        for (int p = 0; p < QP; ++p) {
+          const uint4 z = qs[(ks * QP + p) * 32 + lane];
+          qa[p][0] = z.x, qa[p][1] = z.y, qa[p][2] = z.z, qa[p][3] = z.w;
+        }
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          uint32_t kf[4];
+          ldsm4(kf, kt + (16 * i + k_row) * R::RB + 16 * ((2 * ks + k_piece) ^ R::k_swizzle(k_row)));
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            if constexpr (F32) {
+#pragma unroll
+              for (int p = QP - 1; p > 0; --p) mma<T>(c[i][y][1], qa[p], kf[2 * y], kf[2 * y + 1]);
+              mma<T>(c[i][y][0], qa[0], kf[2 * y], kf[2 * y + 1]);
+            } else {
+              mma<T>(c[i][y][ks & 1], qa[0], kf[2 * y], kf[2 * y + 1]);
+            }
+          }
+        }
+      }
+      float s[MT][2][4];
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int y = 0; y < 2; ++y)
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+            s[i][y][x] = (F32 && HALF ? fmaf(c[i][y][1][x], 1.0f / 2048.0f, c[i][y][0][x])
+                                      : c[i][y][1][x] + c[i][y][0][x]) * qscale[x >> 1];
+      // (behind the products: their latency hides the next loads' issue)
+      const unsigned now = ring.advance(stage == 0 ? ST - 1 : stage - 1);
+      const bool edge = lim_min < min(k0 + TK, n.hi);
+      if (now != R::ALL || edge) {
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int y = 0; y < 2; ++y)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              const int k = 16 * i + 8 * y + 2 * t4 + (x & 1);
+              if (!((now >> k) & 1u) || k0 + k >= lim[x >> 1]) s[i][y][x] = -INFINITY;
+            }
+      }
+      uint32_t pa[MT][PP][4];  // P as A fragments, in parts
+      float alpha[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float top = m[h];
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int y = 0; y < 2; ++y) top = fmaxf(top, fmaxf(s[i][y][2 * h], s[i][y][2 * h + 1]));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const float mu = top == -INFINITY ? 0.0f : top;
+        alpha[h] = ex2((m[h] - mu) * LOG2E);
+        m[h] = top;
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            float2 v = make_float2(ex2((s[i][y][2 * h] - mu) * LOG2E), ex2((s[i][y][2 * h + 1] - mu) * LOG2E));
+            sum += v.x + v.y;
+#pragma unroll
+            for (int p = 0; p < PP; ++p) {
+              pa[i][p][h + 2 * y] = pack16<T>(v.x, v.y);
+              const float2 z = unpack16<T>(pa[i][p][h + 2 * y]);
+              v = make_float2(v.x - z.x, v.y - z.y);
+            }
+          }
+        l[h] = fmaf(l[h], alpha[h], sum);
+      }
+      auto v_at = [&](int i, int mt) {
+        return vt + (16 * i + v_row) * R::RB + 16 * ((2 * mt + v_piece) ^ R::v_swizzle(v_row));
+      };
+      if (!edge) {
+#pragma unroll
+        for (int mt = 0; mt < KS; ++mt) {
+          float o[2][4] = {};
+          uint32_t vf[MT][4];
+#pragma unroll
+          for (int i = 0; i < MT; ++i) ldsm4t(vf[i], v_at(i, mt));
+#pragma unroll
+          for (int p = PP - 1; p >= 0; --p)
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+              for (int y = 0; y < 2; ++y) mma<T>(o[y], pa[i][p], vf[i][2 * y], vf[i][2 * y + 1]);
+#pragma unroll
+          for (int y = 0; y < 2; ++y)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) acc[mt][y][x] = fmaf(acc[mt][y][x], alpha[x >> 1], o[y][x]);
+        }
+      } else {
+        // Keys that only some of the rows see: one row at a time, the values it does not see as
+        // zeros (0 times what they hold could be NaN).
+#pragma unroll
+        for (int mt = 0; mt < KS; ++mt)
+#pragma unroll
+          for (int y = 0; y < 2; ++y)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) acc[mt][y][x] *= alpha[x >> 1];
+        for (int r = 0; r < min(16, a.rows - n.r0); ++r) {
+          const int end = row_limit(a, n, n.r0 + r);
+#pragma unroll
+          for (int i = 0; i < MT; ++i) {
+            const int k = k0 + 16 * i + 2 * t4;  // this lane's keys of a B fragment: k, + 1, + 8, + 9
+            const uint32_t mlo = (k < end ? 0xffffu : 0u) | (k + 1 < end ? 0xffff0000u : 0u);
+            const uint32_t mhi = (k + 8 < end ? 0xffffu : 0u) | (k + 9 < end ? 0xffff0000u : 0u);
+            uint32_t mine[PP][4];
+#pragma unroll
+            for (int p = 0; p < PP; ++p)
+#pragma unroll
+              for (int x = 0; x < 4; ++x) mine[p][x] = g + 8 * (x & 1) == r ? pa[i][p][x] : 0u;
+#pragma unroll
+            for (int mt = 0; mt < KS; ++mt) {
+              uint32_t vf[4];
+              ldsm4t(vf, v_at(i, mt));
+#pragma unroll
+              for (int y = 0; y < 2; ++y) {
+                float o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int p = PP - 1; p >= 0; --p) mma<T>(o, mine[p], vf[2 * y] & mlo, vf[2 * y + 1] & mhi);
+#pragma unroll
+                for (int x = 0; x < 4; ++x)
+                  if (g + 8 * (x >> 1) == r) acc[mt][y][x] += o[x];
+              }
+            }
+          }
+        }
+      }
+      stage = stage + 1 == ST ? 0 : stage + 1;
+    }
+    const UnitInfo done = n;
+    const int free_at = w * R::BYTES + (stage == 0 ? ST - 1 : stage - 1) * R::STAGE;
+    __syncwarp();  // every lane has read its last tile
+    if (lane == 0) red_at[w] = free_at;
+    float* sums = reinterpret_cast<float*>(smem + free_at);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+      if (t4 == 0) ml[w * MAXR + g + 8 * h] = make_float2(m[h], l[h]);
+#pragma unroll
+      for (int mt = 0; mt < KS; ++mt)
+#pragma unroll
+        for (int y = 0; y < 2; ++y)
+          *reinterpret_cast<float2*>(sums + (g + 8 * h) * D + 16 * mt + 8 * y + 2 * t4) =
+              make_float2(acc[mt][y][2 * h], acc[mt][y][2 * h + 1]);
+    }
+    // The next unit's queries travel while this one's sums are joined.
+    const bool more = u + gridDim.x < units;
+    if (more) {
+      n = ring.unit == u + gridDim.x ? ring.info : unit_info(a, ix, u + gridDim.x);
+      load_q(n);
+    }
+    __syncthreads();
+    write_chunk<QT, D>(a, done, smem, red_at, ml, min(16, a.rows - done.r0));
+    if (more) store_q();
+    __syncthreads();  // the sums are read: their stages take tiles again, and q is in place
   }
   if (ring.bad) flag_error(a.sink, CFA_ERR_PAGE);
 }
@@ -1356,10 +1670,16 @@ cudaError_t launch_join(const SplitArgs& a, cudaStream_t stream) {
   return launch_pdl(split_join_kernel<QT, D>, dim3(static_cast<unsigned>(rows)), dim3(NT), 0, stream, a);
 }
 
+// A 16-bit cache.
+template <typename QT, typename T, int D>
+cudaError_t launch_16(const SplitArgs& a, cudaStream_t stream) {
+  return a.block_rows == 8 ? launch_split<split_mma_kernel<QT, T, D>>(split_smem<D, 2, 8>(), a, stream)
+                           : launch_split<split_rows_kernel<QT, T, D>>(split_smem<D, 2, 16>(), a, stream);
+}
+
 template <int D>
 cudaError_t launch_d(const SplitArgs& a, int qd, int kd, cudaStream_t stream) {
   cudaError_t e;
-  constexpr int S2 = split_smem<D, 2, 8>();
   if (qd == CFA_F32) {
     if (kd == CFA_F32) {
       e = a.rows == 1         ? launch_split<split_fma_kernel<D, 1>>(split_smem<D, 4, 1>(), a, stream)
@@ -1367,17 +1687,17 @@ cudaError_t launch_d(const SplitArgs& a, int qd, int kd, cudaStream_t stream) {
           : a.block_rows == 8 ? launch_split<split_f32_kernel<D, 1>>(split_smem<D, 4, 8>(), a, stream)
                               : launch_split<split_f32_kernel<D, 2>>(split_smem<D, 4, 16>(), a, stream);
     } else if (kd == CFA_F16) {
-      e = launch_split<split_mma_kernel<float, __half, D>>(S2, a, stream);
+      e = launch_16<float, __half, D>(a, stream);
     } else {
-      e = launch_split<split_mma_kernel<float, __nv_bfloat16, D>>(S2, a, stream);
+      e = launch_16<float, __nv_bfloat16, D>(a, stream);
     }
     return e == cudaSuccess ? launch_join<float, D>(a, stream) : e;
   }
   if (qd == CFA_F16) {
-    e = launch_split<split_mma_kernel<__half, __half, D>>(S2, a, stream);
+    e = launch_16<__half, __half, D>(a, stream);
     return e == cudaSuccess ? launch_join<__half, D>(a, stream) : e;
   }
-  e = launch_split<split_mma_kernel<__nv_bfloat16, __nv_bfloat16, D>>(S2, a, stream);
+  e = launch_16<__nv_bfloat16, __nv_bfloat16, D>(a, stream);
   return e == cudaSuccess ? launch_join<__nv_bfloat16, D>(a, stream) : e;
 }
 
@@ -1397,6 +1717,12 @@ cudaError_t set_attrs() {
   set(reinterpret_cast<const void*>(split_mma_kernel<float, __nv_bfloat16, D>), S2);
   set(reinterpret_cast<const void*>(split_mma_kernel<__half, __half, D>), S2);
   set(reinterpret_cast<const void*>(split_mma_kernel<__nv_bfloat16, __nv_bfloat16, D>), S2);
+  constexpr int S16 = split_smem<D, 2, 16>();
+  static_assert(S16 <= 232448, "shared memory per block");
+  set(reinterpret_cast<const void*>(split_rows_kernel<float, __half, D>), S16);
+  set(reinterpret_cast<const void*>(split_rows_kernel<float, __nv_bfloat16, D>), S16);
+  set(reinterpret_cast<const void*>(split_rows_kernel<__half, __half, D>), S16);
+  set(reinterpret_cast<const void*>(split_rows_kernel<__nv_bfloat16, __nv_bfloat16, D>), S16);
   return e;
 }
 
@@ -1435,7 +1761,7 @@ cudaError_t launch_split_attention(const SplitArgs& args, int q_dtype, int kv_dt
   SplitArgs a = args;
   a.group = a.H / a.Hk;
   a.rows = a.group * a.S;
-  a.block_rows = kv_dtype == CFA_F32 && a.rows > 8 ? 16 : 8;
+  a.block_rows = a.rows > 8 ? 16 : 8;
   a.row_chunks = (a.rows + a.block_rows - 1) / a.block_rows;
   a.max_chunks = split_max_chunks(a.max_len, a.D, kv_dtype);
   a.tile_log = tile_log_of(a.D, kv_dtype);

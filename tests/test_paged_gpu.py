@@ -98,6 +98,32 @@ def test_several_new_tokens(cuda, qt, kt, s, h, hk):
     check_attention(cuda, [s, 1, 0, s + 1, 16, 90, 300], h, hk, s, 64, 16, "token", qt, kt, seed=s)
 
 
+@pytest.mark.parametrize("qt,kt", TYPES)
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("s,h,hk", [(1, 3, 1), (1, 16, 2), (3, 3, 1), (2, 16, 2), (17, 1, 1), (4, 10, 1)])
+def test_rows_of_a_key_head(cuda, qt, kt, d, s, h, hk):
+    """3, 8, 9, 16, 17 and 40 query rows a key head: each kernel's first and last, and one row over."""
+    check_attention(cuda, [333, 0, 1, 40, 1500, 16], h, hk, s, d, 24, "head", qt, kt, seed=s + h)
+    check_attention(cuda, [64, 700], h, hk, s, d, 32, "token", qt, kt, seed=s)
+
+
+@pytest.mark.parametrize("qt,kt", TYPES)
+@pytest.mark.parametrize("d", [32, 64, 128])
+def test_unseen_keys_of_many_rows_may_hold_anything(cuda, qt, kt, d):
+    """As above for 24 rows a key head: the last token's key is infinite, its value NaN."""
+    n, s, h = 45, 3, 8
+    q, k, v, _ = make([n], h, 1, s, d, 16, "token", qt, kt, seed=19)
+    k[0][:, n - 1] = math.inf
+    v[0][:, n - 1] = math.nan
+    kc, vc, table, lengths = ref.paged(k, v, 16, torch.Generator().manual_seed(1), kt)
+    o = cfa.paged_attention(*(t.to(cuda) for t in (q, kc, vc, table, lengths)), 0.125)
+    cfa.check_status()
+    k0, v0 = (t[0][:, :n - 1].double() for t in (k, v))
+    want = ref.attend(q[0].double(), k0, v0, 0.125, [n - 2, n - 1, 0])[:, :2]
+    lim = band(q[0].double(), k0, v0, 0.125, want, qt)
+    assert bool(((o[0].cpu().double()[:, :2] - want).abs() <= lim).all())
+
+
 @pytest.mark.parametrize("qt,kt", [(F32, F32), (BF16, BF16)])
 def test_padded_new_tokens(cuda, qt, kt):
     check_attention(cuda, [10, 70, 3, 64, 5], 4, 2, 4, 64, 16, "token", qt, kt,
@@ -153,11 +179,26 @@ def test_wide_range_fp32_queries_over_fp16(cuda):
         assert bool(((o[0].cpu().double() - want).abs() <= lim).all())
 
 
+def test_wide_range_of_many_rows(cuda):
+    """The same for 12 rows, each of a size of its own."""
+    g = torch.Generator().manual_seed(14)
+    size = 10.0 ** torch.linspace(-25, 25, 12)[None, :, None, None]
+    q = torch.randn(1, 12, 1, 64, generator=g) * size
+    k, v = [torch.randn(1, 40, 64, generator=g).half()], [torch.randn(1, 40, 64, generator=g).half()]
+    kc, vc, table, lengths = ref.paged(k, v, 16, g, F16)
+    for i, scale in ((0, 1e24), (6, 0.01), (11, 1e-26)):
+        o = cfa.paged_attention(*(t.to(cuda) for t in (q, kc, vc, table, lengths)), scale)
+        row = q[0, i:i + 1].double()
+        want = ref.attend(row, k[0].double(), v[0].double(), scale, [40])
+        lim = band(row, k[0].double(), v[0].double(), scale, want, F32)
+        assert bool(((o[0, i].cpu().double() - want[0]).abs() <= lim).all())
+
+
 def test_bitwise_reruns_batches_and_shared_pages(cuda):
     """A sequence's result is its own: alone, in a batch, with its pages shared with another (the same
     prefix twice), and again."""
-    for qt, kt in TYPES:
-        args, _ = check_attention(cuda, [900, 31, 5000, 1], 8, 2, 1, 64, 16, "token", qt, kt)
+    for (qt, kt), h in ((t, h) for t in TYPES for h in (8, 24)):
+        args, _ = check_attention(cuda, [900, 31, 5000, 1], h, 2, 1, 64, 16, "token", qt, kt)
         q, kc, vc, table, lengths = args
         o = cfa.paged_attention(*args, 0.125)
         assert torch.equal(o, cfa.paged_attention(*args, 0.125))
