@@ -247,6 +247,14 @@ def test_rotary_refuses():
         cfa.rotary(x[0], 0, f)
     with raises("not 3 x 5 heads"):
         cfa.rotary_qkv(torch.zeros(2, 4, 72), 5, 0, f)
+    with raises("x must be a tensor"):
+        cfa.rotary([1.0], 0, f)
+    with pytest.raises(TypeError):
+        cfa.rotary(x, 0.5, f)
+    with pytest.raises(OverflowError):
+        cfa.rotary(x, 1 << 63, f)
+    with pytest.raises(TypeError):
+        cfa.rotary(x, 0, f, amplitude="1")
     with raises("freqs: has no backward"):
         cfa.rotary(x, 0, f.clone().requires_grad_(True))
 
