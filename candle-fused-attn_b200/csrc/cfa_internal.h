@@ -161,7 +161,8 @@ cudaError_t launch_hd_bwd_prep(const PrepArgs& a, int head_dim, cudaStream_t str
 cudaError_t launch_hd_bwd(const BwdArgs& a, int head_dim, int causal, cudaStream_t stream);
 
 // Cross attention: keys of another length, shared key heads. Head dims 64 and 32 run on the
-// tensor cores (fwd_tc.cu CROSS, cross_bwd_tc.cu), 128 on cross_hd_ffma.cu. a.S is the query length, a.n_kblocks is set by the launcher.
+// tensor cores (fwd_tc.cu CROSS, cross_bwd_tc.cu), 128 on cross_hd_tf32.cu (mma.sync).
+// a.S is the query length, a.n_kblocks is set by the launcher.
 cudaError_t setup_cross_tc_attributes();
 cudaError_t setup_cross_bwd_tc_attributes();
 cudaError_t setup_cross_hd_attributes();

@@ -292,7 +292,7 @@ int cfa_matmul_status(void* stream);
  * h / (heads / key_heads)). key_lengths: [batch] int32 on the device, the keys of each batch element
  * (held within 0 .. key_seq), or NULL: all; what lies behind them is never read into a result. A
  * row without a key: O = 0, L = -inf, no gradient. o: [batch, seq, heads, head_dim] dense; lse
- * [batch, heads, seq] dense. Tensor-core kernels at head dims 32 and 64, CUDA-core ones at 128. */
+ * [batch, heads, seq] dense. Tensor-core kernels. */
 int cfa_cross_fwd_f32(const float* q, const int64_t q_strides[3],
                       const float* k, const int64_t k_strides[3],
                       const float* v, const int64_t v_strides[3],

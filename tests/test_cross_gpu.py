@@ -4,7 +4,7 @@
 The band is the fused attention's, 1e-5 relative, normwise, here of every (batch, head) slice: it
 follows from the split products' error model (tests/test_linear_gpu.py), by which scores are off by
 26 2^-24 sum |q| |k| scale, 8e-6 at d = 64 and unit inputs, p by that factor and 2^-22, both averaged
-down in the sums. To it come 26 2^-24 of the same sums over absolute values: dP - D cancels (for a
+down in the sums. (d = 128: two tf32 parts an operand leave out at most 3 2^-22 |q| |k| of a product.) To it come 26 2^-24 of the same sums over absolute values: dP - D cancels (for a
 single key to nothing), and what dP and D are off by stays.
 """
 
@@ -157,8 +157,9 @@ def test_bitwise_reruns_and_batches(cuda, d):
 
 
 def test_equal_lengths_match_the_fused_attention(cuda):
-    """Keys as long as the queries, a head each: fused_attention's own result, bit for bit."""
-    for d in (32, 64, 128):
+    """Keys as long as the queries, a head each: fused_attention's own result, bit for bit (at 128 the two
+    run on different units)."""
+    for d in (32, 64):
         q, k, v, dout = make(2, 3, 3, 200, 200, d, None)
         res = []
         for fn in (lambda *x: cfa.cross_attention(*x, 0.2), lambda *x: cfa.fused_attention(*x, 0.2, False)):
