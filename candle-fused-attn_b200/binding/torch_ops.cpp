@@ -282,26 +282,31 @@ Tensor rotate(const Tensor& x, const Turn& t) {
 struct Dims {
   int64_t b, h, hk, sq, sk, d;
 };
+// Up to as many query rows a key head (query heads of a group x queries) the forward runs split over the
+// keys, one block a chunk of keys and up to 16 rows; above, kernels that take 256 rows a block (64 at head
+// dim 128). The batch plays no part: the choice changes bits. Split and whole, in us, [b, 6, rows, 64] over
+// 1500 keys: 16 rows 11 and 55 (b 1), 23 and 58 (16), 82 and 169 (64); 32 rows 11 and 55, 42 and 58, 156 and
+// 169; 48 rows 11 and 55, 60 and 58, 226 and 170.
+constexpr int64_t kFewRows = 32;
+
 Tensor cross_forward(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& lengths, float scale,
-                     const Dims& m, Tensor& lse) {
+                     const Dims& m, bool gradients, Tensor& lse) {
   const Launch on(q);
   const Tensor o = merged_heads(m.b, m.h, m.sq, m.d, q);
-  lse = empty({m.b, m.h, m.sq}, {m.h * m.sq, m.sq, 1}, q, at::kFloat);
+  const bool few = m.hk && m.h / m.hk * m.sq <= kFewRows;
+  if (gradients || !few) lse = empty({m.b, m.h, m.sq}, {m.h * m.sq, m.sq, 1}, q, at::kFloat);
+  float *const op = o.mutable_data_ptr<float>(), *const lp = lse.defined() ? lse.mutable_data_ptr<float>() : nullptr;
+  if (few) {
+    const size_t n = abi.cross_few_workspace(m.b, m.h, m.sq, m.sk, m.d);
+    const Tensor ws = workspace(n, q);
+    check_status(abi.cross_few(ptr<float>(q), Strides3(q), ptr<float>(k), Strides3(k), ptr<float>(v),
+                               Strides3(v), ptr<int32_t>(lengths), op, lp, n ? ws.mutable_data_ptr() : nullptr,
+                               n, m.b, m.h, m.hk, m.sq, m.sk, m.d, scale, on.stream),
+                 "cross_attention");
+    return o;
+  }
   check_status(abi.cross_fwd(ptr<float>(q), Strides3(q), ptr<float>(k), Strides3(k), ptr<float>(v),
-                             Strides3(v), ptr<int32_t>(lengths), o.mutable_data_ptr<float>(),
-                             lse.mutable_data_ptr<float>(), m.b, m.h, m.hk, m.sq, m.sk, m.d, scale, on.stream),
-               "cross_attention");
-  return o;
-}
-Tensor cross_few(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& lengths, float scale,
-                 const Dims& m) {
-  const Launch on(q);
-  const Tensor o = merged_heads(m.b, m.h, m.sq, m.d, q);
-  const size_t n = abi.cross_few_workspace(m.b, m.h, m.sq, m.sk, m.d);
-  const Tensor ws = workspace(n, q);
-  check_status(abi.cross_few(ptr<float>(q), Strides3(q), ptr<float>(k), Strides3(k), ptr<float>(v),
-                             Strides3(v), ptr<int32_t>(lengths), o.mutable_data_ptr<float>(),
-                             n ? ws.mutable_data_ptr() : nullptr, n, m.b, m.h, m.hk, m.sq, m.sk, m.d, scale,
+                             Strides3(v), ptr<int32_t>(lengths), op, lp, m.b, m.h, m.hk, m.sq, m.sk, m.d, scale,
                              on.stream),
                "cross_attention");
   return o;
@@ -313,7 +318,7 @@ struct Cross : torch::autograd::Function<Cross> {
   static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v,
                         const Keys& keys, double scale, const Dims& m) {
     Tensor lse;
-    const Tensor o = cross_forward(q, k, v, keys.lengths, static_cast<float>(scale), m, lse);
+    const Tensor o = cross_forward(q, k, v, keys.lengths, static_cast<float>(scale), m, true, lse);
     ctx->save_for_backward({q, k, v, keys.lengths, o, lse});
     ctx->saved_data["scale"] = scale;
     return o;
@@ -412,13 +417,6 @@ PyObject* rotary_qkv(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// Up to as many query rows a key head (query heads of a group x queries) the forward without gradients
-// runs split over the keys, one block a chunk of keys and up to 16 rows; above, the tensor-core kernels,
-// which take 256 rows a block. The batch plays no part: the choice changes bits. Split and whole, in us,
-// [b, 6, rows, 64] over 1500 keys: 16 rows 11 and 55 (b 1), 23 and 58 (16), 82 and 169 (64); 32 rows 11
-// and 55, 42 and 58, 156 and 169; 48 rows 11 and 55, 60 and 58, 226 and 170.
-constexpr int64_t kFewRows = 32;
-
 PyObject* cross_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   const char* who = "cross_attention";
@@ -440,10 +438,8 @@ PyObject* cross_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   q = aligned_rows(q), k = aligned_rows(k), v = aligned_rows(v);
   if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad()))
     return THPVariable_Wrap(Cross::apply(q, k, v, Keys{lengths}, scale, m));
-  const float f = static_cast<float>(scale);
-  if (m.hk && m.h / m.hk * m.sq <= kFewRows) return THPVariable_Wrap(cross_few(q, k, v, lengths, f, m));
   Tensor lse;
-  return THPVariable_Wrap(cross_forward(q, k, v, lengths, f, m, lse));
+  return THPVariable_Wrap(cross_forward(q, k, v, lengths, static_cast<float>(scale), m, false, lse));
   END_HANDLE_TH_ERRORS
 }
 

@@ -166,7 +166,7 @@ def load() -> ctypes.CDLL:
     lib.cfa_cross_few_workspace_bytes.restype = _n
     lib.cfa_cross_few_workspace_bytes.argtypes = [_i64] * 5
     lib.cfa_cross_few_f32.restype = ctypes.c_int
-    lib.cfa_cross_few_f32.argtypes = [_p, _strides, _p, _strides, _p, _strides, _p, _p, _p, _n,
+    lib.cfa_cross_few_f32.argtypes = [_p, _strides, _p, _strides, _p, _strides, _p, _p, _p, _p, _n,
                                       *[_i64] * 6, _f, _p]
     lib.cfa_rotary.restype = ctypes.c_int
     lib.cfa_rotary.argtypes = [_p, _strides, _p, _strides, _d, _p, _d, _strides, _i64, _p, _f,
@@ -369,12 +369,12 @@ def cross_few_workspace_bytes(b, h, sq, sk, d) -> int:
     return int(load().cfa_cross_few_workspace_bytes(b, h, sq, sk, d))
 
 
-def cross_few(q_ptr, qs, k_ptr, ks, v_ptr, vs, lengths_ptr, o_ptr, ws_ptr, ws_bytes, b, h, hk, sq,
-              sk, d, scale, stream) -> int:
+def cross_few(q_ptr, qs, k_ptr, ks, v_ptr, vs, lengths_ptr, o_ptr, lse_ptr, ws_ptr, ws_bytes, b, h,
+              hk, sq, sk, d, scale, stream) -> int:
     """cfa_cross_few_f32 (the forward for few query rows a key head); returns the status."""
     return load().cfa_cross_few_f32(
-        q_ptr, strides3(qs), k_ptr, strides3(ks), v_ptr, strides3(vs), lengths_ptr, o_ptr, ws_ptr,
-        ws_bytes, b, h, hk, sq, sk, d, scale, stream)
+        q_ptr, strides3(qs), k_ptr, strides3(ks), v_ptr, strides3(vs), lengths_ptr, o_ptr,
+        lse_ptr, ws_ptr, ws_bytes, b, h, hk, sq, sk, d, scale, stream)
 
 
 def rotary(x_ptr, xs, y_ptr, ys, dtype, pos_ptr, pos_bytes, pos_strides, first, freqs_ptr,

@@ -22,8 +22,8 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: fl
     them is not read into any result, and a query without a key gives zeros and no gradient.
     -> [batch, heads, sq, d], laid out as a dense [batch, sq, heads, d].
 
-    Differentiable in q, k and v (dk, dv of a shared head are summed over its query heads). Without
-    gradients, few queries -- the single token of a decoding step -- take a kernel that splits the
-    keys instead. Bit-identical across reruns and batch splits.
+    Differentiable in q, k and v (dk, dv of a shared head are summed over its query heads). Few
+    queries -- the single token of a decoding step -- take a kernel that splits the keys.
+    Bit-identical across reruns and batch splits.
     """
     return _ops.cross_attention(q, k, v, scale, key_lengths)

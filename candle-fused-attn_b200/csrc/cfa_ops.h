@@ -65,6 +65,7 @@ struct SplitArgs {
   int causal;              // query i of n sees lengths - n + i + 1 keys, else all of them
   int max_len;             // most keys of a sequence (lengths beyond are cut)
   void* o;                 // [B, S, H, D] dense
+  float* lse;              // [B, H, S] or nullptr: the rows' log-sum-exp
   int B, H, Hk, S, D;
   float scale;
   int* sink;

@@ -242,9 +242,9 @@ size_t cfa_cross_few_workspace_bytes(int64_t batch, int64_t heads, int64_t seq, 
 
 int cfa_cross_few_f32(const float* q, const int64_t q_strides[3], const float* k,
                       const int64_t k_strides[3], const float* v, const int64_t v_strides[3],
-                      const int32_t* key_lengths, float* o, void* workspace, size_t workspace_bytes,
-                      int64_t batch, int64_t heads, int64_t key_heads, int64_t seq, int64_t key_seq,
-                      int64_t head_dim, float scale, void* stream) {
+                      const int32_t* key_lengths, float* o, float* lse, void* workspace,
+                      size_t workspace_bytes, int64_t batch, int64_t heads, int64_t key_heads, int64_t seq,
+                      int64_t key_seq, int64_t head_dim, float scale, void* stream) {
   int st = check_cross(batch, heads, key_heads, seq, key_seq, head_dim);
   if (st != CFA_OK || batch == 0 || heads == 0 || seq == 0) return st;
   const size_t need = cfa_cross_few_workspace_bytes(batch, heads, seq, key_seq, head_dim);
@@ -260,7 +260,7 @@ int cfa_cross_few_f32(const float* q, const int64_t q_strides[3], const float* k
   st = setup(g_split_once, cfa::setup_split_attributes);
   if (st != CFA_OK) return st;
   cfa::SplitArgs a{};
-  a.q = q, a.k = k, a.v = v, a.o = o;
+  a.q = q, a.k = k, a.v = v, a.o = o, a.lse = lse;
   a.q_sb = q_strides[0], a.q_sh = q_strides[1], a.q_ss = q_strides[2];
   a.k_sp = k_strides[0], a.k_sh = k_strides[1], a.k_sr = k_strides[2];
   a.v_sp = v_strides[0], a.v_sh = v_strides[1], a.v_sr = v_strides[2];

@@ -438,6 +438,7 @@ __device__ __forceinline__ void write_chunk(const SplitArgs& a, const UnitInfo& 
       dst[1] = from_f<QT>(live ? o.y / l : 0.0f);
       dst[2] = from_f<QT>(live ? o.z / l : 0.0f);
       dst[3] = from_f<QT>(live ? o.w / l : 0.0f);
+      if (a.lse && c4 == 0) a.lse[(static_cast<int64_t>(n.b) * a.H + head) * a.S + i] = m + logf(l);
     } else if (i < n.n_new) {
       const int64_t at = ((static_cast<int64_t>(n.b) * a.H + head) * a.S + i) * a.max_chunks + n.chunk;
       *reinterpret_cast<float4*>(a.part_o + at * D + 4 * c4) = o;
@@ -1624,6 +1625,7 @@ __global__ void __launch_bounds__(NT) split_join_kernel(const SplitArgs a) {
 #pragma unroll
     for (int j = 1; j < J::G; ++j) o = plus(o, sums[j][c4]);
     r.template store<QT>(a, c4, o, l);
+    if (a.lse && c4 == 0) a.lse[r.row] = m + logf(l);  // (no key: -inf)
   }
 }
 

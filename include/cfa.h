@@ -319,17 +319,17 @@ int cfa_cross_bwd_f32(const float* q, const int64_t q_strides[3],
                       int64_t batch, int64_t heads, int64_t key_heads, int64_t seq,
                       int64_t key_seq, int64_t head_dim, float scale, void* stream);
 
-/* The forward alone for few query rows a key head (single tokens): the same contract without the
- * lse, split over the keys. Any seq is right; past 8 rows a key head (seq * heads / key_heads) the
- * keys are read once for every 8. */
+/* The forward for few query rows a key head (single tokens): the same contract, split over the keys;
+ * lse may be NULL. Any seq is right; past 16 rows a key head (seq * heads / key_heads) the keys are
+ * read once for every 16. */
 size_t cfa_cross_few_workspace_bytes(int64_t batch, int64_t heads, int64_t seq, int64_t key_seq,
                                      int64_t head_dim);
 int cfa_cross_few_f32(const float* q, const int64_t q_strides[3],
                       const float* k, const int64_t k_strides[3],
                       const float* v, const int64_t v_strides[3],
-                      const int32_t* key_lengths, float* o, void* workspace, size_t workspace_bytes,
-                      int64_t batch, int64_t heads, int64_t key_heads, int64_t seq,
-                      int64_t key_seq, int64_t head_dim, float scale, void* stream);
+                      const int32_t* key_lengths, float* o, float* lse, void* workspace,
+                      size_t workspace_bytes, int64_t batch, int64_t heads, int64_t key_heads,
+                      int64_t seq, int64_t key_seq, int64_t head_dim, float scale, void* stream);
 
 /* Rotary positions: y = x with the first rotary_dim dims of each of the first rotated_heads heads
  * turned by position * freqs[j] (radians; 64 bits on the device, rotary_dim / 2 of them) and scaled

@@ -87,7 +87,8 @@ def test_few_rows_arguments():
     assert _abi.cross_few_workspace_bytes(2, 4, 1, 256, 64) == 0  # one chunk: nothing to join
 
     def call(q=FAKE, ws=FAKE, nbytes=need, dims=dims):
-        return _abi.cross_few(q, S3, FAKE, S3, FAKE, S3, None, FAKE, ws, nbytes, *dims, 0.1, None)
+        return _abi.cross_few(q, S3, FAKE, S3, FAKE, S3, None, FAKE, None, ws, nbytes, *dims, 0.1,
+                              None)
 
     assert call(nbytes=need - 1) == _abi.CFA_ERR_WORKSPACE
     assert call(ws=FAKE + 4) == _abi.CFA_ERR_WORKSPACE and call(ws=None) == _abi.CFA_ERR_NULL
