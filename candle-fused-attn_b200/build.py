@@ -24,8 +24,8 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 OUT = PKG / "candle_fused_attn" / "libcfa.so"
 SOURCES = ["fwd_ffma.cu", "fwd_tc.cu", "bwd_ffma.cu", "bwd_tc.cu", "hd_ffma.cu", "linear_tc.cu",
-           "cross_bwd_tc.cu", "cross_hd_tf32.cu", "cross_join.cu", "rotary.cu", "split_attn.cu",
-           "cfa_abi.cu", "cfa_ops_abi.cu", "cfa_noalloc.cu"]
+           "cross_bwd_tc.cu", "cross_hd_tf32.cu", "cross_few_bwd.cu", "cross_join.cu", "rotary.cu",
+           "split_attn.cu", "cfa_abi.cu", "cfa_ops_abi.cu", "cfa_noalloc.cu"]
 HOST_DIR = PKG / "host"
 HOST_OUT = PKG / "candle_fused_attn" / "libcfa_host.so"
 HOST_SOURCES = ["tensor.cu", "candle_fused_attn.cpp"]

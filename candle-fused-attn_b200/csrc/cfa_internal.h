@@ -166,10 +166,14 @@ cudaError_t launch_hd_bwd(const BwdArgs& a, int head_dim, int causal, cudaStream
 cudaError_t setup_cross_tc_attributes();
 cudaError_t setup_cross_bwd_tc_attributes();
 cudaError_t setup_cross_hd_attributes();
+cudaError_t setup_cross_few_bwd_attributes();
 cudaError_t launch_cross_fwd_tc(const FwdArgs& a, int head_dim, cudaStream_t stream);
 cudaError_t launch_cross_bwd_tc(const BwdArgs& a, int head_dim, cudaStream_t stream);
 cudaError_t launch_cross_hd_fwd(const FwdArgs& a, cudaStream_t stream);
 cudaError_t launch_cross_hd_bwd(const BwdArgs& a, cudaStream_t stream);
+// Up to CROSS_FEW_ROWS query rows a key head, one batch element's or a thousand's (dq_part is set).
+constexpr int CROSS_FEW_ROWS = 32;
+cudaError_t launch_cross_few_bwd(const BwdArgs& a, int head_dim, cudaStream_t stream);
 cudaError_t launch_cross_join(const BwdArgs& a, int head_dim, int key_block, cudaStream_t stream);
 
 // The projection GEMM (linear_tc.cu): C = A B over fp32 on the tensor cores (split bf16 parts).

@@ -29,7 +29,8 @@ int setup(DeviceOnce* table, cudaError_t (*fn)()) {
 cudaError_t setup_cross() {
   cudaError_t e = cfa::setup_cross_tc_attributes();
   if (e == cudaSuccess) e = cfa::setup_cross_bwd_tc_attributes();
-  return e == cudaSuccess ? cfa::setup_cross_hd_attributes() : e;
+  if (e == cudaSuccess) e = cfa::setup_cross_hd_attributes();
+  return e == cudaSuccess ? cfa::setup_cross_few_bwd_attributes() : e;
 }
 
 constexpr int64_t kLim = (int64_t(1) << 31) - 1;
@@ -86,6 +87,7 @@ struct CrossLayout {
   size_t turn_off, dsum_off, kv_off, part_off, total, total_fast;
   bool join_dq;    // (with the partials)
   int n_parts;
+  bool few;
 };
 CrossLayout cross_layout(int64_t B, int64_t H, int64_t Hk, int64_t Sq, int64_t Sk, int64_t D) {
   CrossLayout w{};
@@ -106,6 +108,9 @@ CrossLayout cross_layout(int64_t B, int64_t H, int64_t Hk, int64_t Sq, int64_t S
   w.part_off = w.total;
   const int64_t queries = B * H * Sq;
   w.total_fast = w.total + (queries <= kCrossPartialBytes / row_bytes ? static_cast<size_t>(queries * row_bytes) : 0);
+  // Few query rows: by partials alone (at most a quarter of what the key blocks' keys and values take).
+  w.few = group * Sq <= cfa::CROSS_FEW_ROWS;
+  if (w.few) w.total = w.total_fast = w.part_off + static_cast<size_t>(queries * row_bytes);
   return w;
 }
 
@@ -219,15 +224,16 @@ int cfa_cross_bwd_f32(const float* q, const int64_t q_strides[3], const float* k
   a.timeout_ns = cfa::WAIT_TIMEOUT_NS;
   a.sink = cfa::error_sink();
   // The dQ partials when the workspace holds them (the same results, bit for bit).
-  const bool partials = lay.total_fast > lay.total && workspace_bytes >= lay.total_fast;
+  const bool partials = lay.few || (lay.total_fast > lay.total && workspace_bytes >= lay.total_fast);
   a.dq_part = partials ? reinterpret_cast<float*>(ws + lay.part_off) : nullptr;
   a.n_parts = lay.n_parts;
-  a.join_dq = partials && lay.join_dq;
+  a.join_dq = lay.few || (partials && lay.join_dq);
   a.dkv_out = dkv;
   if (lay.n_parts > 1) {
     a.dkv = reinterpret_cast<float*>(ws + lay.kv_off);
     a.part_stride = batch * key_seq * 2 * key_heads * head_dim;
   }
+  if (lay.few) return status(cfa::launch_cross_few_bwd(a, static_cast<int>(head_dim), s));
   return status(head_dim == 128 ? cfa::launch_cross_hd_bwd(a, s)
                                 : cfa::launch_cross_bwd_tc(a, static_cast<int>(head_dim), s));
 }

@@ -126,6 +126,16 @@ def test_turn_chain_gives_the_same_bits(cuda, d, h, hk, sq, sk):
 
 
 @pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("h,hk,sq", [(2, 2, 1), (8, 1, 1), (3, 1, 3), (4, 2, 8), (17, 1, 1), (2, 2, 32), (3, 1, 11)])
+def test_few_query_rows(cuda, d, h, hk, sq):
+    """1, 8, 9, 16, 17, 32 and 33 query rows a key head: the kernels of few rows, and one row over; lengths
+    that end in the first and the last of a block's tiles, on a block's end, one key, none."""
+    check(cuda, 6, h, hk, sq, 300, d, [300, 128, 17, 1, 0, 129], seed=sq + h)
+    check(cuda, 1, h, hk, sq, 64, d, None, seed=sq)
+    check(cuda, 2, h, hk, sq, 1030, d, [1030, 700], seed=h)
+
+
+@pytest.mark.parametrize("d", [32, 64, 128])
 @pytest.mark.parametrize("b,h,hk,sq,sk,lens", [
     (1, 8, 1, 500, 200, None), (1, 1, 1, 1000, 130, [90]), (2, 6, 1, 700, 300, [300, 0]),
     (3, 16, 2, 200, 1000, [1000, 64, 129]), (1, 2, 1, 2000, 2300, [2300]), (2, 4, 1, 1100, 64, [64, 1])])
