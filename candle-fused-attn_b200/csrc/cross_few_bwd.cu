@@ -10,8 +10,8 @@
 //
 // Bound by memory up to 16 rows: K, V are read and dK, dV written once, at 20 rows D flops a key against
 // 16 D bytes; at 32 by the products' issue. The tcgen05 pair, whose tiles are 64 queries, spends a block's
-// first loads, splits and last stores on 128 keys: [34, 24 over 8, 10, 64] over 1000 to 2000 keys 202 us here,
-// 332 there; [32, 8, 32, 64] over 500 to 1000 101 and 161.
+// first loads, splits and last stores on 128 keys: [34, 24 over 8, 10, 64] over 1000 to 2000 keys 219 us here,
+// 332 there; [32, 8, 32, 64] over 500 to 1000 108 and 161.
 #include "cfa_common.cuh"
 #include "tf32.cuh"
 
@@ -145,34 +145,20 @@ __global__ void __launch_bounds__(NT, 2) cross_few_bwd_kernel(const BwdArgs a) {
     const float* V = K + TK * D;
     // Scores' layout: keys g, g + 8 (x >> 1); queries 8 q + 2 t4, + 1 (x & 1).
     auto scores = [&](const float* A, const float* B, float (&s)[NQ][4]) {
-      float small[NQ][4];
+      clear(s);
 #pragma unroll
-      for (int q = 0; q < NQ; ++q)
+      for (int j = 0; j < J; j += 2) {
+        float c[NQ][4];
+        clear(c);
 #pragma unroll
-        for (int x = 0; x < 4; ++x) s[q][x] = small[q][x] = 0.0f;
+        for (int y = 0; y < 2; ++y) {
+          uint32_t ah[2][4], al[2][4];
+          split_rows(at_row(A, 0, j + y), at_row(A, 8, j + y), ah, al);
 #pragma unroll
-      for (int j = 0; j < J; ++j) {
-        uint32_t h0[4], h1[4], l0[4], l1[4];
-        split_tf32(at_row(A, 0, j), h0, l0);
-        split_tf32(at_row(A, 8, j), h1, l1);
-        const uint32_t ah[2][4] = {{h0[0], h1[0], h0[1], h1[1]}, {h0[2], h1[2], h0[3], h1[3]}};
-        const uint32_t al[2][4] = {{l0[0], l1[0], l0[1], l1[1]}, {l0[2], l1[2], l0[3], l1[3]}};
-#pragma unroll
-        for (int q = 0; q < NQ; ++q) {
-          uint32_t bh_[4], bl[4];
-          split_tf32(at_row(B, 8 * q, j), bh_, bl);
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            mma_tf32(small[q], al[x], bh_[2 * x], bh_[2 * x + 1]);
-            mma_tf32(s[q], ah[x], bh_[2 * x], bh_[2 * x + 1]);
-            mma_tf32(small[q], ah[x], bl[2 * x], bl[2 * x + 1]);
-          }
+          for (int q = 0; q < NQ; ++q) products(c[q], ah, al, at_row(B, 8 * q, j + y));
         }
+        add(s, c);
       }
-#pragma unroll
-      for (int q = 0; q < NQ; ++q)
-#pragma unroll
-        for (int x = 0; x < 4; ++x) s[q][x] += small[q][x];
     };
     // dst[keys][dims] = X^T Y for scores-shaped X (keys x queries) and Y [queries][dims], times f.
     auto rows_out = [&](const float (&x)[NQ][4], const float* Y, float* dst, float f) {
@@ -181,19 +167,12 @@ __global__ void __launch_bounds__(NT, 2) cross_few_bwd_kernel(const BwdArgs a) {
       for (int q = 0; q < NQ; ++q) split_tf32(make_float4(x[q][0], x[q][2], x[q][1], x[q][3]), xh[q], xl[q]);
 #pragma unroll
       for (int j = 0; j < JV; ++j) {
-        float c[4][4] = {};
+        float c[4][4], small[4][4];
+        clear(c);
+        clear(small);
 #pragma unroll
-        for (int q = 0; q < NQ; ++q) {
-          uint32_t yh[4], yl[4], zh[4], zl[4];
-          split_tf32(at_col(Y, q, 0, j), yh, yl);
-          split_tf32(at_col(Y, q, 1, j), zh, zl);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) mma_tf32(c[e], xl[q], yh[e], zh[e]);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) mma_tf32(c[e], xh[q], yl[e], zl[e]);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) mma_tf32(c[e], xh[q], yh[e], zh[e]);
-        }
+        for (int q = 0; q < NQ; ++q) products(small, c, xh[q], xl[q], at_col(Y, q, 0, j), at_col(Y, q, 1, j));
+        add(c, small);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           if (key0 + g + 8 * h >= a.Sk) continue;  // (rows past the length hold zeros)
@@ -224,28 +203,27 @@ __global__ void __launch_bounds__(NT, 2) cross_few_bwd_kernel(const BwdArgs a) {
     rows_out(ds, Qs, dkv, a.scale);
     __syncwarp();  // dS's rows in place
 #pragma unroll
-    for (int m = 0; m < MQ; ++m)
+    for (int m = 0; m < MQ; ++m) {
+      uint32_t xh[2][4], xl[2][4];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const float* at = ds_rows + (16 * m + g) * LS + 8 * i + 2 * t4;
         const float2 x = *reinterpret_cast<const float2*>(at);
         float2 y = make_float2(0.f, 0.f);  // (8 rows: the product's other 8 are none)
         if constexpr (NQ > 1) y = *reinterpret_cast<const float2*>(at + 8 * LS);
-        uint32_t xh[4], xl[4];
-        split_tf32(make_float4(x.x, y.x, x.y, y.y), xh, xl);
-#pragma unroll
-        for (int j = 0; j < JV; ++j) {
-          uint32_t yh[4], yl[4], zh[4], zl[4];
-          split_tf32(at_col(K, i, 0, j), yh, yl);
-          split_tf32(at_col(K, i, 1, j), zh, zl);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) mma_tf32(dq[m][j][e], xl, yh[e], zh[e]);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) mma_tf32(dq[m][j][e], xh, yl[e], zl[e]);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) mma_tf32(dq[m][j][e], xh, yh[e], zh[e]);
-        }
+        split_tf32(make_float4(x.x, y.x, x.y, y.y), xh[i], xl[i]);
       }
+#pragma unroll
+      for (int j = 0; j < JV; ++j) {
+        float c[4][4], small[4][4];
+        clear(c);
+        clear(small);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) products(small, c, xh[i], xl[i], at_col(K, i, 0, j), at_col(K, i, 1, j));
+        add(c, small);
+        add(dq[m][j], c);
+      }
+    }
     __syncwarp();  // dS's rows are read
   }
   __syncthreads();  // every warp's keys are read: their dQ take the place

@@ -6,15 +6,14 @@
 // S). Forward: 64 of them, 16 a warp, over key tiles of 64, online softmax.
 //
 // Products by mma.m16n8k8 on tf32 operands in two parts (tf32.cuh): hi hi + hi lo + lo hi, what is left out
-// below 2^-22 of the products' magnitudes; S's small products in a chain of their own, every tile's P V a
-// fresh accumulator folded by an fp32 FMA. Dims and keys are numbered within a product so that a lane reads
+// below 2^-22 of the products' magnitudes, in short sums (32 dims, keys or queries) that are added in fp32. Dims and keys are numbered within a product so that a lane reads
 // Q, K and V 16 bytes at a time (k = t, t + 4 are adjacent dims, or keys 2 t, 2 t + 1) and P's fragment is
 // S's. (head dims 64 and 32 run on tcgen05, whose three-part operands do not fit at 128.)
 //
 // Bound by the issue of splits and products, two warps a scheduler: at the rate of these products (a third
 // of tf32's: 96 TFLOP/s) the tensor core is busy for 0.5 to 0.6 of the time. [16, 8, 512 x 512, 128]:
-// forward 298 us (58 TFLOP/s), backward 862 us (50); by fp32 FMAs, as hd_ffma.cu has the fused attention's,
-// 442 and 1128 us. [2, 8, 2048 x 4096, 128]: 1.32 and 3.27 ms, for 1.70 and 4.33.
+// forward 303 us (57 TFLOP/s), backward 896 us (48); by fp32 FMAs, as hd_ffma.cu has the fused attention's,
+// 442 and 1128 us. [2, 8, 2048 x 4096, 128]: 1.32 and 3.40 ms, for 1.70 and 4.33.
 #include "cfa_common.cuh"
 #include "tf32.cuh"
 
@@ -93,29 +92,20 @@ __global__ void __launch_bounds__(NT, 2) cross_hd_fwd_kernel(const FwdArgs a) {
     cp_async_wait_all();
     __syncthreads();  // K in place; the last tile's V is read
     load_keys(Vs, LV, vp, a.v_ss, k0);
-    float ch[BN / 8][4], cl[BN / 8][4];  // rows g, g + 8; keys 8 i + 2 t4, + 1
+    float sc[BN / 8][4];  // rows g, g + 8; keys 8 i + 2 t4, + 1
+    clear(sc);
+#pragma unroll 1
+    for (int j = 0; j < D / 16; j += 2) {
+      float c[BN / 8][4];
+      clear(c);
 #pragma unroll
-    for (int i = 0; i < BN / 8; ++i)
+      for (int y = 0; y < 2; ++y) {
+        uint32_t ah[2][4], al[2][4];
+        split_rows(ld4(qa + 16 * (j + y)), ld4(qa + 8 * LQ + 16 * (j + y)), ah, al);
 #pragma unroll
-      for (int x = 0; x < 4; ++x) ch[i][x] = cl[i][x] = 0.0f;
-#pragma unroll 4
-    for (int j = 0; j < D / 16; ++j) {
-      uint32_t h0[4], h1[4], l0[4], l1[4];
-      split_tf32(ld4(qa + 16 * j), h0, l0);
-      split_tf32(ld4(qa + 8 * LQ + 16 * j), h1, l1);
-      const uint32_t ah[2][4] = {{h0[0], h1[0], h0[1], h1[1]}, {h0[2], h1[2], h0[3], h1[3]}};
-      const uint32_t al[2][4] = {{l0[0], l1[0], l0[1], l1[1]}, {l0[2], l1[2], l0[3], l1[3]}};
-#pragma unroll
-      for (int i = 0; i < BN / 8; ++i) {
-        uint32_t kh[4], kl[4];
-        split_tf32(ld4(ka + 8 * i * LQ + 16 * j), kh, kl);
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          mma_tf32(cl[i], al[x], kh[2 * x], kh[2 * x + 1]);
-          mma_tf32(ch[i], ah[x], kh[2 * x], kh[2 * x + 1]);
-          mma_tf32(cl[i], ah[x], kl[2 * x], kl[2 * x + 1]);
-        }
+        for (int i = 0; i < BN / 8; ++i) products(c[i], ah, al, ld4(ka + 8 * i * LQ + 16 * (j + y)));
       }
+      add(sc, c);
     }
     const bool edge = k0 + BN > SK;
     uint32_t ph[BN / 8][4], pl[BN / 8][4];  // P as A fragments: k = t4 is key 8 i + 2 t4, t4 + 4 the next
@@ -127,7 +117,7 @@ __global__ void __launch_bounds__(NT, 2) cross_hd_fwd_kernel(const FwdArgs a) {
       for (int i = 0; i < BN / 8; ++i)
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          s[i][x] = (cl[i][2 * h + x] + ch[i][2 * h + x]) * a.scale;
+          s[i][x] = sc[i][2 * h + x] * a.scale;
           if (edge && k0 + 8 * i + 2 * t4 + x >= SK) s[i][x] = -INFINITY;
           top = fmaxf(top, s[i][x]);
         }
@@ -153,23 +143,23 @@ __global__ void __launch_bounds__(NT, 2) cross_hd_fwd_kernel(const FwdArgs a) {
     if (k0 + BN < SK) load_keys(Ks, LQ, kp, a.k_ss, k0 + BN);
 #pragma unroll
     for (int j = 0; j < D / 32; ++j) {
-      float c[4][4] = {};
+      float small[4][4], large[4][4];
+      clear(small);
+      clear(large);
 #pragma unroll
       for (int i = 0; i < BN / 8; ++i) {
-        uint32_t xh[4], xl[4], yh[4], yl[4];
-        split_tf32(ld4(va + 8 * i * LV + 32 * j), xh, xl);
-        split_tf32(ld4(va + (8 * i + 1) * LV + 32 * j), yh, yl);
+        const float* at = va + 8 * i * LV + 32 * j;
+        products(small, large, ph[i], pl[i], ld4(at), ld4(at + LV));
+        if (i == BN / 16 - 1) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) mma_tf32(c[e], pl[i], xh[e], yh[e]);
+          for (int e = 0; e < 4; ++e)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) mma_tf32(c[e], ph[i], xl[e], yl[e]);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) mma_tf32(c[e], ph[i], xh[e], yh[e]);
+            for (int x = 0; x < 4; ++x) acc[j][e][x] = fmaf(acc[j][e][x], alpha[x >> 1], large[e][x]);
+          clear(large);
+        }
       }
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-#pragma unroll
-        for (int x = 0; x < 4; ++x) acc[j][e][x] = fmaf(acc[j][e][x], alpha[x >> 1], c[e][x]);
+      add(large, small);
+      add(acc[j], large);
     }
   }
 #pragma unroll
@@ -197,8 +187,7 @@ __global__ void __launch_bounds__(NT, 2) cross_hd_fwd_kernel(const FwdArgs a) {
 // warps. Per tile:
 //   1. warps 0-3 S = Q K^T (the forward's order) and P = e^(S scale - L), warps 4-7 dP = dO V^T and, with P
 //      out of shared memory, dS = P o (dP - D); both to shared memory, [query][key];
-//   2. warps 0-3 dV += P^T dO, warps 4-7 dK += dS^T Q, 16 keys a warp, every tile's product a fresh
-//      accumulator added in fp32;
+//   2. warps 0-3 dV += P^T dO, warps 4-7 dK += dS^T Q, 16 keys a warp, added in fp32;
 //   3. all: the tile's dQ partial dS K, 16 queries and half the dims a warp.
 // Key blocks, parts, dQ's order and the zeros of unattended keys are cross_bwd_tc.cu's. The operands' tiles
 // are read both by rows (products over the dims) and by columns: piece c of row r is piece c ^ swizzle(r),
@@ -333,29 +322,20 @@ __global__ void __launch_bounds__(BT, 1) cross_hd_bwd_kernel(const BwdArgs a) {
     {
       const float* As = (grp ? dOs : Qs) + 16 * wg * D;
       const float* Bs = grp ? Vs : Ks;
-      float ch[8][4], cl[8][4];
+      float sc[8][4];
+      clear(sc);
+#pragma unroll 1
+      for (int j = 0; j < D / 16; j += 2) {  // (the forward's sums)
+        float c[8][4];
+        clear(c);
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
+        for (int y = 0; y < 2; ++y) {
+          uint32_t ah[2][4], al[2][4];
+          split_rows(at_row(As, 0, j + y), at_row(As, 8, j + y), ah, al);
 #pragma unroll
-        for (int x = 0; x < 4; ++x) ch[i][x] = cl[i][x] = 0.0f;
-#pragma unroll 4
-      for (int j = 0; j < D / 16; ++j) {
-        uint32_t h0f[4], h1f[4], l0f[4], l1f[4];
-        split_tf32(at_row(As, 0, j), h0f, l0f);
-        split_tf32(at_row(As, 8, j), h1f, l1f);
-        const uint32_t ah[2][4] = {{h0f[0], h1f[0], h0f[1], h1f[1]}, {h0f[2], h1f[2], h0f[3], h1f[3]}};
-        const uint32_t al[2][4] = {{l0f[0], l1f[0], l0f[1], l1f[1]}, {l0f[2], l1f[2], l0f[3], l1f[3]}};
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          uint32_t kh[4], kl[4];
-          split_tf32(at_row(Bs, 8 * i, j), kh, kl);
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            mma_tf32(cl[i], al[x], kh[2 * x], kh[2 * x + 1]);
-            mma_tf32(ch[i], ah[x], kh[2 * x], kh[2 * x + 1]);
-            mma_tf32(cl[i], ah[x], kl[2 * x], kl[2 * x + 1]);
-          }
+          for (int i = 0; i < 8; ++i) products(c[i], ah, al, at_row(Bs, 8 * i, j + y));
         }
+        add(sc, c);
       }
       const int r0 = 16 * wg + g;
       if (grp == 0) {
@@ -368,7 +348,7 @@ __global__ void __launch_bounds__(BT, 1) cross_hd_bwd_kernel(const BwdArgs a) {
             float p[2];
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-              p[x] = ex2(fmaf(cl[i][2 * h + x] + ch[i][2 * h + x], a.scale, -L) * LOG2E);
+              p[x] = ex2(fmaf(sc[i][2 * h + x], a.scale, -L) * LOG2E);
               if (edge && !(q0 + r0 + 8 * h < rows && k0 + 8 * i + 2 * t4 + x < SK)) p[x] = 0.0f;
             }
             *reinterpret_cast<float2*>(Ps + (r0 + 8 * h) * LP + 8 * i + 2 * t4) = make_float2(p[0], p[1]);
@@ -384,8 +364,7 @@ __global__ void __launch_bounds__(BT, 1) cross_hd_bwd_kernel(const BwdArgs a) {
           for (int i = 0; i < 8; ++i) {
             const int at = (r0 + 8 * h) * LP + 8 * i + 2 * t4;
             const float2 p = *reinterpret_cast<const float2*>(Ps + at);
-            *reinterpret_cast<float2*>(dSs + at) = make_float2(p.x * (cl[i][2 * h] + ch[i][2 * h] - d),
-                                                               p.y * (cl[i][2 * h + 1] + ch[i][2 * h + 1] - d));
+            *reinterpret_cast<float2*>(dSs + at) = make_float2(p.x * (sc[i][2 * h] - d), p.y * (sc[i][2 * h + 1] - d));
           }
         }
         asm volatile("bar.sync 1, %0;" ::"n"(BT / 2) : "memory");  // dS in place for its warps; the others go on to dV
@@ -404,23 +383,19 @@ __global__ void __launch_bounds__(BT, 1) cross_hd_bwd_kernel(const BwdArgs a) {
       }
 #pragma unroll
       for (int j = 0; j < D / 32; ++j) {
-        float c[4][4] = {};
+        float small[4][4], large[4][4];
+        clear(small);
+        clear(large);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          uint32_t yh[4], yl[4], zh[4], zl[4];
-          split_tf32(at_col(Ys, i, 0, j), yh, yl);
-          split_tf32(at_col(Ys, i, 1, j), zh, zl);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) mma_tf32(c[e], xl[i], yh[e], zh[e]);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) mma_tf32(c[e], xh[i], yl[e], zl[e]);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) mma_tf32(c[e], xh[i], yh[e], zh[e]);
+          products(small, large, xh[i], xl[i], at_col(Ys, i, 0, j), at_col(Ys, i, 1, j));
+          if (i == 3) {
+            add(acc[j], large);
+            clear(large);
+          }
         }
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-#pragma unroll
-          for (int x = 0; x < 4; ++x) acc[j][e][x] += c[e][x];
+        add(large, small);
+        add(acc[j], large);
       }
     }
     __syncthreads();
@@ -439,22 +414,20 @@ __global__ void __launch_bounds__(BT, 1) cross_hd_bwd_kernel(const BwdArgs a) {
       }
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-#pragma unroll
-          for (int x = 0; x < 4; ++x) pq[j][e][x] = 0.0f;
+        float small[4][4], large[4][4];
+        clear(pq[j]);
+        clear(small);
+        clear(large);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          uint32_t yh[4], yl[4], zh[4], zl[4];
-          split_tf32(at_col(Ks, i, 0, 2 * grp + j), yh, yl);
-          split_tf32(at_col(Ks, i, 1, 2 * grp + j), zh, zl);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) mma_tf32(pq[j][e], xl[i], yh[e], zh[e]);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) mma_tf32(pq[j][e], xh[i], yl[e], zl[e]);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) mma_tf32(pq[j][e], xh[i], yh[e], zh[e]);
+          products(small, large, xh[i], xl[i], at_col(Ks, i, 0, 2 * grp + j), at_col(Ks, i, 1, 2 * grp + j));
+          if (i == 3) {
+            add(pq[j], large);
+            clear(large);
+          }
         }
+        add(large, small);
+        add(pq[j], large);
       }
     }
     auto partial = [&](int j, int h, int x) {
