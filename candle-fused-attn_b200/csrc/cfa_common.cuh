@@ -220,6 +220,12 @@ template <typename Args>
 __device__ __forceinline__ int cross_keys(const Args& a, int b) {
   return a.key_lengths ? min(max(a.key_lengths[b], 0), a.Sk) : a.Sk;
 }
+// The factor of cross attention's dQ and dK: the scale, or nothing where there is one key, whose weight is
+// one whatever its score (the sums would hold dP - D, which should cancel and do so to a rounding).
+template <typename Args>
+__device__ __forceinline__ float grad_scale(const Args& a, int keys) {
+  return keys == 1 ? 0.0f : a.scale;
+}
 
 // Another status into the host-visible flag (a page id outside the cache, found by a kernel).
 __device__ __forceinline__ void flag_error(int* sink, int status) {

@@ -82,6 +82,7 @@ __global__ void __launch_bounds__(NB, 1) cross_bwd_tc_kernel(const BwdArgs a) {
   const int rows = group * S, nqt = (rows + QT - 1) / QT;  // and their rows, in tiles
   const int SK = cross_keys(a, b);
   const int nkb = (SK + KB - 1) / KB;  // key blocks of this (batch, head) that take part
+  const float dscale = grad_scale(a, SK);
   float* dkv = a.dkv + static_cast<int64_t>(part) * a.part_stride;  // (parts: in the workspace)
   if (kb >= nkb) {  // no key of this block is attended: zeros, and no part in dQ's sums
     griddep_launch_dependents();
@@ -473,7 +474,7 @@ __global__ void __launch_bounds__(NB, 1) cross_bwd_tc_kernel(const BwdArgs a) {
               const float4 prev = __ldcg(dst + c4);
               v = make_float4(prev.x + v.x, prev.y + v.y, prev.z + v.z, prev.w + v.w);
             }
-            if (kb == last) v = make_float4(v.x * a.scale, v.y * a.scale, v.z * a.scale, v.w * a.scale);
+            if (kb == last) v = make_float4(v.x * dscale, v.y * dscale, v.z * dscale, v.w * dscale);
             __stcg(dst + c4, v);
           }
         }
@@ -511,8 +512,8 @@ __global__ void __launch_bounds__(NB, 1) cross_bwd_tc_kernel(const BwdArgs a) {
         reinterpret_cast<float4*>(sv + row * LDS + 16 * cg)[c4] =
             make_float4(dv[4 * c4], dv[4 * c4 + 1], dv[4 * c4 + 2], dv[4 * c4 + 3]);
         reinterpret_cast<float4*>(sk + row * LDS + 16 * cg)[c4] =
-            make_float4(dk[4 * c4] * a.scale, dk[4 * c4 + 1] * a.scale, dk[4 * c4 + 2] * a.scale,
-                        dk[4 * c4 + 3] * a.scale);
+            make_float4(dk[4 * c4] * dscale, dk[4 * c4 + 1] * dscale, dk[4 * c4 + 2] * dscale,
+                        dk[4 * c4 + 3] * dscale);
       }
     }
     __syncthreads();  // the dV, dK rows in place
@@ -558,7 +559,7 @@ __global__ void __launch_bounds__(NB, 1) cross_bwd_tc_kernel(const BwdArgs a) {
             v = make_float4(v.x + q.x, v.y + q.y, v.z + q.z, v.w + q.w);
           }
           reinterpret_cast<float4*>(dq_out + i * row_stride)[c4] =
-              make_float4(v.x * a.scale, v.y * a.scale, v.z * a.scale, v.w * a.scale);
+              make_float4(v.x * dscale, v.y * dscale, v.z * dscale, v.w * dscale);
         }
         if (!ok && tid == 0) flag_timeout(a.err, a.sink);
         return;
@@ -600,8 +601,7 @@ __global__ void __launch_bounds__(NB, 1) cross_bwd_tc_kernel(const BwdArgs a) {
           const int idx = base + u * NB;
           if (last[u] >= 0)
             reinterpret_cast<float4*>(dq_out + (idx / C4) * row_stride)[idx % C4] =
-                make_float4(v[u].x * a.scale, v[u].y * a.scale, v[u].z * a.scale,
-                            v[u].w * a.scale);
+                make_float4(v[u].x * dscale, v[u].y * dscale, v[u].z * dscale, v[u].w * dscale);
         }
       }
     };

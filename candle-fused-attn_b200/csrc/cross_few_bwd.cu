@@ -147,16 +147,13 @@ __global__ void __launch_bounds__(NT, 2) cross_few_bwd_kernel(const BwdArgs a) {
     auto scores = [&](const float* A, const float* B, float (&s)[NQ][4]) {
       clear(s);
 #pragma unroll
-      for (int j = 0; j < J; j += 2) {
+      for (int j = 0; j < J; ++j) {
         float c[NQ][4];
         clear(c);
+        uint32_t ah[2][4], al[2][4];
+        split_rows(at_row(A, 0, j), at_row(A, 8, j), ah, al);
 #pragma unroll
-        for (int y = 0; y < 2; ++y) {
-          uint32_t ah[2][4], al[2][4];
-          split_rows(at_row(A, 0, j + y), at_row(A, 8, j + y), ah, al);
-#pragma unroll
-          for (int q = 0; q < NQ; ++q) products(c[q], ah, al, at_row(B, 8 * q, j + y));
-        }
+        for (int q = 0; q < NQ; ++q) products(c[q], ah, al, at_row(B, 8 * q, j));
         add(s, c);
       }
     };
@@ -200,7 +197,7 @@ __global__ void __launch_bounds__(NT, 2) cross_few_bwd_kernel(const BwdArgs a) {
       }
     }
     rows_out(p, dOs, dkv + dv_at, 1.0f);
-    rows_out(ds, Qs, dkv, a.scale);
+    rows_out(ds, Qs, dkv, grad_scale(a, SK));
     __syncwarp();  // dS's rows in place
 #pragma unroll
     for (int m = 0; m < MQ; ++m) {

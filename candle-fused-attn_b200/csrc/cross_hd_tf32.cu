@@ -6,14 +6,15 @@
 // S). Forward: 64 of them, 16 a warp, over key tiles of 64, online softmax.
 //
 // Products by mma.m16n8k8 on tf32 operands in two parts (tf32.cuh): hi hi + hi lo + lo hi, what is left out
-// below 2^-22 of the products' magnitudes, in short sums (32 dims, keys or queries) that are added in fp32. Dims and keys are numbered within a product so that a lane reads
-// Q, K and V 16 bytes at a time (k = t, t + 4 are adjacent dims, or keys 2 t, 2 t + 1) and P's fragment is
-// S's. (head dims 64 and 32 run on tcgen05, whose three-part operands do not fit at 128.)
+// below 2^-22 of the products' magnitudes, in short sums (32 dims, keys or queries) that are added in fp32.
+// Dims and keys are numbered within a product so that a lane reads Q, K and V 16 bytes at a time (k = t, t + 4
+// are adjacent dims, or keys 2 t, 2 t + 1) and P's fragment is S's. (Head dims 64 and 32 run on tcgen05, whose
+// three-part operands do not fit at 128.)
 //
 // Bound by the issue of splits and products, two warps a scheduler: at the rate of these products (a third
 // of tf32's: 96 TFLOP/s) the tensor core is busy for 0.5 to 0.6 of the time. [16, 8, 512 x 512, 128]:
-// forward 303 us (57 TFLOP/s), backward 896 us (48); by fp32 FMAs, as hd_ffma.cu has the fused attention's,
-// 442 and 1128 us. [2, 8, 2048 x 4096, 128]: 1.32 and 3.40 ms, for 1.70 and 4.33.
+// forward 303 us (57 TFLOP/s), backward 889 us (48); by fp32 FMAs, as hd_ffma.cu has the fused attention's,
+// 442 and 1128 us. [2, 8, 2048 x 4096, 128]: 1.32 and 3.35 ms, for 1.70 and 4.33.
 #include "cfa_common.cuh"
 #include "tf32.cuh"
 
@@ -239,6 +240,7 @@ __global__ void __launch_bounds__(BT, 1) cross_hd_bwd_kernel(const BwdArgs a) {
   const int nqt = (rows + 63) / 64;
   const int SK = cross_keys(a, b);
   const int nkb = (SK + KB - 1) / KB;  // key blocks of this (batch, head) that take part
+  const float dscale = grad_scale(a, SK);
   float* dkv = a.dkv + static_cast<int64_t>(part) * a.part_stride;  // (parts: in the workspace)
   if (kb >= nkb) {  // no key of this block is attended: zeros, and no part in dQ's sums
     const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -480,7 +482,7 @@ __global__ void __launch_bounds__(BT, 1) cross_hd_bwd_kernel(const BwdArgs a) {
               const float4 p = __ldcg(at);
               v = make_float4(p.x + v.x, p.y + v.y, p.z + v.z, p.w + v.w);
             }
-            if (kb == last) v = make_float4(v.x * a.scale, v.y * a.scale, v.z * a.scale, v.w * a.scale);
+            if (kb == last) v = make_float4(v.x * dscale, v.y * dscale, v.z * dscale, v.w * dscale);
             __stcg(at, v);
           }
       }
@@ -513,7 +515,7 @@ __global__ void __launch_bounds__(BT, 1) cross_hd_bwd_kernel(const BwdArgs a) {
             v = make_float4(v.x + p.x, v.y + p.y, v.z + p.z, v.w + p.w);
           }
           *reinterpret_cast<float4*>(dq_out + i * row_stride + 4 * c4) =
-              make_float4(v.x * a.scale, v.y * a.scale, v.z * a.scale, v.w * a.scale);
+              make_float4(v.x * dscale, v.y * dscale, v.z * dscale, v.w * dscale);
         }
       }
     }
@@ -521,7 +523,7 @@ __global__ void __launch_bounds__(BT, 1) cross_hd_bwd_kernel(const BwdArgs a) {
 
   // grp 0 stores dV, grp 1 stores dK * scale.
   // (dkv [b, Sk, 2, Hk, D], dK first; rows past the length hold zeros.)
-  const float f = grp ? a.scale : 1.0f;
+  const float f = grp ? dscale : 1.0f;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const int r = k0 + 16 * wg + g + 8 * h;

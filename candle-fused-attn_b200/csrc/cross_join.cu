@@ -26,7 +26,8 @@ __global__ void __launch_bounds__(JT) cross_join_kernel(const BwdArgs a, int D, 
       const int64_t row = x / C4, bh = row / a.S;
       const int c4 = static_cast<int>(x - row * C4), i = static_cast<int>(row - bh * a.S);
       const int b = static_cast<int>(bh / a.H), head = static_cast<int>(bh - static_cast<int64_t>(b) * a.H);
-      const int nkb = (cross_keys(a, b) + key_block - 1) / key_block;
+      const int keys = cross_keys(a, b), nkb = (keys + key_block - 1) / key_block;
+      const float scale = grad_scale(a, keys);
       const float4* p = reinterpret_cast<const float4*>(a.dq_part) + (bh * a.n_kblocks * a.S + i) * C4 + c4;
       const int64_t step = static_cast<int64_t>(a.S) * C4;
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -34,7 +35,7 @@ __global__ void __launch_bounds__(JT) cross_join_kernel(const BwdArgs a, int D, 
 #pragma unroll 4
       for (int j = 1; j < nkb; ++j) v = add4(v, __ldcs(p + j * step));
       reinterpret_cast<float4*>(a.dq)[((static_cast<int64_t>(b) * a.S + i) * a.H + head) * C4 + c4] =
-          make_float4(v.x * a.scale, v.y * a.scale, v.z * a.scale, v.w * a.scale);
+          make_float4(v.x * scale, v.y * scale, v.z * scale, v.w * scale);
     } else {
       const int64_t y = x - n_dq;
       const float4* p = reinterpret_cast<const float4*>(a.dkv) + y;

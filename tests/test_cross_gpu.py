@@ -253,6 +253,16 @@ def test_empty(cuda):
     cfa.check_status()
 
 
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("sq", [3, 70, 700])
+def test_one_key_has_no_gradient(cuda, d, sq):
+    """Its weight is one whatever the score: dQ and dK are zeros, not what is left of a cancellation."""
+    _, _, o, (dq, dk, dv) = run(cuda, 2, 4, 2, sq, 130, d, [1, 130])
+    assert not dq[0].any() and not dk[0].any() and dv[0, :, 0].any() and dq[1].any() and dk[1].any()
+    _, _, o, (dq, dk, dv) = run(cuda, 2, 2, 2, sq, 1, d, None)
+    assert not dq.any() and not dk.any() and dv.any()
+
+
 def test_no_query_heads(cuda):
     """Key heads that no query reads: their gradients are zeros, whatever the memory held."""
     for h, sq in ((0, 3), (2, 0), (0, 0)):
