@@ -166,6 +166,19 @@ def test_bitwise_reruns_and_batches(cuda, d):
         assert torch.equal(oi[0], o[i]) and all(torch.equal(a[0], c[i]) for a, c in zip(gi, grads))
 
 
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("sq", [1, 7, 30])
+def test_few_rows_do_not_depend_on_the_batch(cuda, d, sq):
+    """Outputs and gradients of each batch element alone, bit for bit."""
+    lens = [900, 1, 0, 257, 64]
+    (q, k, v, dout, scale, lengths), _, o, grads = run(cuda, 5, 4, 4, sq, 900, d, lens, scale=0.1)
+    for i in range(5):
+        x = [t[i:i + 1].to(cuda).requires_grad_(True) for t in (q, k, v)]
+        o1 = cfa.cross_attention(*x, scale, key_lengths=lengths[i:i + 1])
+        g1 = torch.autograd.grad(o1, x, dout[i:i + 1].to(cuda))
+        assert torch.equal(o1[0], o[i]) and all(torch.equal(a[0], b[i]) for a, b in zip(g1, grads))
+
+
 def test_equal_lengths_match_the_fused_attention(cuda):
     """Keys as long as the queries, a head each: fused_attention's own result, bit for bit (at 128 the two
     run on different units)."""
