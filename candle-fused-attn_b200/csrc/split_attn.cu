@@ -19,15 +19,19 @@
 //   16-bit caches, up to 8 query rows: S^T = K Q^T and O^T += V^T P^T by mma.m16n8k16, the keys (dims)
 //     as the 16 rows and the query rows as the 8 columns: a column's softmax state then lives in the lanes
 //     that hold the column's output. fp32 queries enter in parts that keep their 24 bits (three
-//     bf16, or two fp16 under a power of two a row: 22 bits), p as two parts (16 bits of bf16, 22 of
-//     fp16) or, fp32 queries over bf16, three (24 bits), every tile's product a fresh accumulator
-//     folded by an fp32 FMA -- the tensor core's truncating sums never run longer than a tile.
+//     bf16, or two fp16 under a power of two a row: 22 bits), p as three parts over bf16 (24 bits) or
+//     two over fp16 (22), every tile's product a fresh accumulator
+//     folded by an fp32 FMA -- the tensor core's truncating sums never run longer than a tile. (p in two
+//     bf16 parts for bf16 outputs: 192.4 us where three take 195.8, but 0.19 % of the outputs are then not
+//     the bf16 number nearest the exact one, with three 0.016 %.)
 //     tcgen05 has no shape below 64 rows, and at a few rows the product is a small share of the
 //     tile's load time. Three stages of two blocks a SM (two of three blocks: 245 us for 204).
-//   16-bit caches, more rows: S = Q K^T and O += P V, 16 query rows as the 16 rows; the same parts. In
-//     blocks of 8 and of 16, 32 sequences of 100 to 8000 keys, four key heads, in us: 16 rows bf16 69
-//     and 56 (d 64), 113 and 81 (d 128), fp32 over bf16 75 and 68, 131 and 98; 40 rows bf16 d 128 270
-//     and 209. Bound by the issue of the products and the softmax, two warps a scheduler.
+//   16-bit caches, more rows: S = Q K^T and O += P V, 16 query rows as the 16 rows; the same parts, but p in
+//     two (16 bits) for bf16 outputs, whose own rounding is 2^-9: bound by the products' issue, a third part
+//     takes 16 rows bf16 from 56 to 65 us (d 64) and from 81 to 94 (d 128), for 0.21 % and 0.024 % of outputs
+//     that are not the nearest. In blocks of 8 and of 16, 32 sequences of 100 to 8000 keys, four key heads,
+//     in us: 16 rows bf16 69 and 56 (d 64), 113 and 81 (d 128), fp32 over bf16 75 and 68, 131 and 98; 40 rows
+//     bf16 d 128 270 and 209. Bound by the issue of the products and the softmax, two warps a scheduler.
 //   fp32 caches, three query rows and more: S = Q K^T and O += P V by mma.m16n8k8 on tf32 operands, 8 or
 //     16 query rows as the 16 rows. Every operand enters in two parts of 11 bits (x = hi + lo to 2^-22
 //     |x|; three or all four of the products of the parts), and dims and keys are numbered within a
@@ -40,7 +44,7 @@
 //     eight rows 121 and 66, 241 and 125; 16 rows, in blocks of 8 and of 16: 222 and 92, 461 and 169; one
 //     row of 64 sequences over 240 keys 11.7 and 17.
 // On one B200, with the join: 64 sequences of up to 8192 keys, 32 heads over 8, [page 16] bf16, d = 128
-// 193 us (5.8 TB/s); 2 of 131071 keys, fp32 over bf16, d = 64 55 us; 16 of 1000 to 6000 keys, 16 heads,
+// 196 us (5.7 TB/s); 2 of 131071 keys, fp32 over bf16, d = 64 55 us; 16 of 1000 to 6000 keys, 16 heads,
 // fp32, d = 64 79 us (5.9 TB/s). One sequence of 240 keys: 6.9 us.
 //
 // Order of summation: fixed by the sequence's length, the number of rows and the row alone (not by the
@@ -483,7 +487,7 @@ __global__ void __launch_bounds__(NT, 2)
   constexpr bool F32 = std::is_same_v<QT, float>;
   constexpr bool HALF = std::is_same_v<T, __half>;
   constexpr int QP = F32 ? (HALF ? 2 : 3) : 1;  // parts of q
-  constexpr int PP = F32 && !HALF ? 3 : 2;      // parts of p
+  constexpr int PP = HALF ? 2 : 3;              // parts of p
   constexpr int KS = D / 16;
   using QPair = std::conditional_t<F32, float2, uint32_t>;
   extern __shared__ __align__(128) unsigned char smem[];
