@@ -20,7 +20,7 @@
 //     as the 16 rows and the query rows as the 8 columns: a column's softmax state then lives in the lanes
 //     that hold the column's output. fp32 queries enter in parts that keep their 24 bits (three
 //     bf16, or two fp16 under a power of two a row: 22 bits), p as three parts over bf16 (24 bits) or
-//     two over fp16 (22), every tile's product a fresh accumulator
+//     two over fp16 (22; P_UP_F16), every tile's product a fresh accumulator
 //     folded by an fp32 FMA -- the tensor core's truncating sums never run longer than a tile. (p in two
 //     bf16 parts for bf16 outputs: 192.4 us where three take 195.8, but 0.19 % of the outputs are then not
 //     the bf16 number nearest the exact one, with three 0.016 %.)
@@ -72,6 +72,11 @@ constexpr int WARPS = 4;
 constexpr int NT = 32 * WARPS;
 constexpr int MAXR = 16;   // most query rows per block
 constexpr float LOG2E = 1.4426950408889634f;
+// fp16 caches: p, and with it the sums l and o, carries this factor, which o / l drops (no log-sum-exp is
+// written there). p's two fp16 parts then keep 22 bits from p = 2^-17 on and miss at most 2^-39 below; without
+// it the small part is subnormal below p = 2^-3 and the large one below 2^-14, both miss 2^-25, and a tail of
+// weights near 1e-7 beside one large weight counts in l but not in o.
+constexpr float P_UP_F16 = 16384.0f;
 
 // Keys per chunk, as a power of two, of a sequence of `len` keys in tiles of 2^tile_log keys: 16 tiles
 // (four a warp, 128 KB of keys and values) up to 16 chunks, then 32 tiles up to 256 chunks, then as many
@@ -488,6 +493,7 @@ __global__ void __launch_bounds__(NT, 2)
   constexpr bool HALF = std::is_same_v<T, __half>;
   constexpr int QP = F32 ? (HALF ? 2 : 3) : 1;  // parts of q
   constexpr int PP = HALF ? 2 : 3;              // parts of p
+  constexpr float P_UP = HALF ? P_UP_F16 : 1.0f;
   constexpr int KS = D / 16;
   using QPair = std::conditional_t<F32, float2, uint32_t>;
   extern __shared__ __align__(128) unsigned char smem[];
@@ -653,8 +659,8 @@ __global__ void __launch_bounds__(NT, 2)
       float ps0 = 0.0f, ps1 = 0.0f;
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
-        float2 x = make_float2(ex2((s[i][0] - u0) * LOG2E), ex2((s[i][1] - u1) * LOG2E));
-        float2 y = make_float2(ex2((s[i][2] - u0) * LOG2E), ex2((s[i][3] - u1) * LOG2E));
+        float2 x = make_float2(ex2((s[i][0] - u0) * LOG2E) * P_UP, ex2((s[i][1] - u1) * LOG2E) * P_UP);
+        float2 y = make_float2(ex2((s[i][2] - u0) * LOG2E) * P_UP, ex2((s[i][3] - u1) * LOG2E) * P_UP);
         ps0 += x.x + y.x;
         ps1 += x.y + y.y;
 #pragma unroll
@@ -763,6 +769,7 @@ __global__ void __launch_bounds__(NT, 2) split_rows_kernel(const SplitArgs a) {
   constexpr bool HALF = std::is_same_v<T, __half>;
   constexpr int QP = F32 ? (HALF ? 2 : 3) : 1;  // parts of q
   constexpr int PP = F32 && !HALF ? 3 : 2;      // parts of p
+  constexpr float P_UP = HALF ? P_UP_F16 : 1.0f;
   constexpr int JQ = (KS + WARPS - 1) / WARPS;  // this warp's share of q's columns
   using QPair = std::conditional_t<F32, float2, uint32_t>;
   extern __shared__ __align__(128) unsigned char smem[];
@@ -956,7 +963,8 @@ __global__ void __launch_bounds__(NT, 2) split_rows_kernel(const SplitArgs a) {
         for (int i = 0; i < MT; ++i)
 #pragma unroll
           for (int y = 0; y < 2; ++y) {
-            float2 v = make_float2(ex2((s[i][y][2 * h] - mu) * LOG2E), ex2((s[i][y][2 * h + 1] - mu) * LOG2E));
+            float2 v = make_float2(ex2((s[i][y][2 * h] - mu) * LOG2E) * P_UP,
+                                   ex2((s[i][y][2 * h + 1] - mu) * LOG2E) * P_UP);
             sum += v.x + v.y;
 #pragma unroll
             for (int p = 0; p < PP; ++p) {

@@ -50,3 +50,24 @@ def test_bf16_outputs_have_weights_of_24_bits(cuda, d, h):
     want = ((1.0 - p * c) / (1.0 + p))[:, None, None]
     lim = torch.finfo(BF16).eps / 2 * want.abs() + 12 * U / (1.0 + p)[:, None, None]
     assert bool(((o - want).abs() <= lim).all()), float(((o - want).abs() / lim).max())
+
+
+@pytest.mark.parametrize("qt", [F32, F16])
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("h", [2, 24])
+def test_a_tail_of_small_weights_over_fp16_counts(cuda, qt, d, h):
+    """One key takes nearly all of the weight and has the value 0; 600 others of e^-16 to e^-8 share values
+    near 1. A weight is off by 24 u (the argument, below 23, rounds once and its constant is off by a
+    quarter step: 20 u; 2^x: 4 u), its two parts by 2^-22 = 4 u of it and 2^-39; the sums of n terms in
+    chunks by (n / 16 + 64) u; l by 24 u."""
+    b, n = 4, 601
+    g = torch.Generator().manual_seed(d + h)
+    scores = (-16.0 + 8.0 * torch.rand(b, n, generator=g)).half().double()
+    v = (0.5 + torch.rand(b, n, d, generator=g)).half().double()
+    scores[:, 100], v[:, 100] = 0.0, 0.0
+    o = attend(cuda, scores, v, h, d, qt, F16)
+    want = torch.softmax(scores, 1)[:, None] @ v
+    lim = (24 + 4 + n / 16 + 64 + 24) * U * want + 2.0 ** -39 * v.sum(1, keepdim=True)
+    if qt == F16:
+        lim = lim + torch.finfo(F16).eps / 2 * want + 2.0 ** -25
+    assert bool(((o - want).abs() <= lim).all()), float(((o - want).abs() / lim).max())
