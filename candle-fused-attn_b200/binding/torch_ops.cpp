@@ -134,7 +134,16 @@ void one_device(const char* who, Tensors ts) {
     if (t->defined()) same &= t->get_device() == index, cuda &= t->is_cuda();
   REQUIRE(same, who, cuda ? ": tensors on different devices" : ": CUDA tensors required");
 }
+// A forward-mode tangent (torch.autograd.forward_ad) rides on a tensor without requires_grad: no result
+// here would carry it on, which reads as a derivative of zero.
+void no_tangent(const char* who, const char* what, Tensors ts) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  for (const Tensor* t : ts)
+    REQUIRE(!t->defined() || !t->_fw_grad(/*level=*/0).defined(), who, what,
+            ": has no forward-mode derivative");
+}
 void no_gradient(const char* who, const char* what, Tensors ts) {
+  no_tangent(who, what, ts);
   if (!at::GradMode::is_enabled()) return;
   for (const Tensor* t : ts)
     REQUIRE(!t->defined() || !t->requires_grad(), who, what,
@@ -376,6 +385,7 @@ void count(Py_ssize_t got, Py_ssize_t want) { REQUIRE(got == want, "_ops: ", wan
 Turn turn_of(const char* who, const Tensor& x, PyObject* const* a, int64_t b, int64_t s, int64_t d,
              int64_t heads) {
   REQUIRE(dtype_of(x) >= 0, who, ": f32, f16 or bf16 expected, got ", type_name(x));
+  no_tangent(who, "", {&x});
   Turn t{who, Tensor(), 0, tensor_of(a[1], who, "freqs"), double_of(a[2]), bool_of(a[3]), heads};
   check_freqs(who, t.freqs, d);
   if (!THPVariable_Check(a[0])) {
@@ -433,6 +443,7 @@ PyObject* cross_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   REQUIRE((m.hk ? m.h % m.hk : m.h) == 0, who, ": ", m.h, " query heads are no multiple of ", m.hk,
           " key heads");
   check_head_dim(m.d);
+  no_tangent(who, "", {&q, &k, &v});
   one_device(who, {&q, &k, &v, &lengths});
   int32_vector(who, "key_lengths", lengths, m.b);
   q = aligned_rows(q), k = aligned_rows(k), v = aligned_rows(v);
@@ -481,9 +492,9 @@ PyObject* paged_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
                            q.scalar_type() == k.scalar_type()),
           who, ": q [", b, ", h, ", s, ", ", d, "] of k's type expected, got ", type_name(q), " ", q.sizes());
   check_cache(who, k, kc, vc, table, lengths, fresh, b, hk, d);
-  one_device(who, {&k, &v, &kc, &vc, &table, &lengths, &fresh, &q, &freqs});
   no_gradient(who, "", {&q, &k, &v, &kc, &vc});
   if (freqs.defined()) check_freqs(who, freqs, d);
+  one_device(who, {&k, &v, &kc, &vc, &table, &lengths, &fresh, &q, &freqs});
   const Launch on(k);
   k = dense_rows(k), v = dense_rows(v);
   Tensor out;
@@ -523,8 +534,8 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const int64_t hk = kc.dim() == 4 ? kc.size(2) : 0;
   check_cache(who, q, kc, vc, table, lengths, fresh, b, hk, d);
   REQUIRE((hk ? h % hk : h) == 0, who, ": ", h, " query heads are no multiple of ", hk, " key heads");
-  one_device(who, {&q, &kc, &vc, &table, &lengths, &fresh});
   no_gradient(who, "", {&q, &kc, &vc});
+  one_device(who, {&q, &kc, &vc, &table, &lengths, &fresh});
   REQUIRE(kc.numel() == 0 || aligned(kc), who, ": k_cache: rows must be 16-byte aligned");
   REQUIRE(vc.numel() == 0 || aligned(vc), who, ": v_cache: rows must be 16-byte aligned");
   const Launch on(q);
