@@ -212,9 +212,12 @@ struct Launch {
 };
 
 // The gradients of a backward: where a graph of them is made (create_graph), one that says so when it is
-// differentiated in its turn -- the kernels record nothing.
-variable_list first_order(const Tensor& grad, variable_list grads) {
-  if (!at::GradMode::is_enabled() || !grad.requires_grad()) return grads;
+// differentiated in its turn -- the kernels record nothing. `sources`: what the gradients depend on.
+variable_list first_order(Tensors sources, variable_list grads) {
+  if (!at::GradMode::is_enabled()) return grads;
+  bool differentiable = false;
+  for (const Tensor* t : sources) differentiable |= t->requires_grad();
+  if (!differentiable) return grads;
   variable_list leaves;
   for (const Tensor& g : grads)
     if (g.defined()) leaves.push_back(g.detach().set_requires_grad(true));
@@ -279,7 +282,7 @@ struct Rotary : torch::autograd::Function<Rotary> {
     const int64_t layout = ctx->saved_data["layout"].toInt();
     const Turn t{layout > 1 ? "rotary_qkv" : "rotary", saved[1], ctx->saved_data["first"].toInt(), saved[0],
                  ctx->saved_data["amplitude"].toDouble(), (layout & 1) != 0, layout / 2};
-    return first_order(grads[0], {turn(grads[0], t, true), Tensor()});
+    return first_order({&grads[0]}, {turn(grads[0], t, true), Tensor()});  // (linear: no part of x in it)
   }
 };
 Tensor rotate(const Tensor& x, const Turn& t) {
@@ -350,8 +353,9 @@ struct Cross : torch::autograd::Function<Cross> {
                                m.sk, m.d, static_cast<float>(ctx->saved_data["scale"].toDouble()), on.stream),
                  "cross_attention");
     const std::array<int64_t, 4> size{m.b, m.hk, m.sk, m.d}, stride{m.sk * row, m.d, row, 1};
-    return first_order(grads[0], {dq, dkv.as_strided(size, stride), dkv.as_strided(size, stride, m.hk * m.d),
-                                  Tensor(), Tensor(), Tensor()});
+    return first_order({&grads[0], &q, &k, &v},
+                       {dq, dkv.as_strided(size, stride), dkv.as_strided(size, stride, m.hk * m.d), Tensor(),
+                        Tensor(), Tensor()});
   }
 };
 
