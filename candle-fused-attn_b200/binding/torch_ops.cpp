@@ -518,6 +518,9 @@ PyObject* paged_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
                                 ptr<int32_t>(fresh), ptr<double>(freqs), static_cast<float>(amplitude), b, h,
                                 hk, s, d, freqs.defined() ? 2 * freqs.numel() : 0, interleaved, on.stream),
                who);
+  // As every in-place operation: a backward that saved the cache before is told.
+  for (const Tensor* t : {&kc, &vc})
+    if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
   if (!q.defined()) Py_RETURN_NONE;
   return THPVariable_Wrap(out);
   END_HANDLE_TH_ERRORS

@@ -35,3 +35,38 @@ def test_a_rotation_of_a_constant_gradient_is_constant(cuda):
     assert not g.requires_grad
     (g.square().sum() + x.square().sum()).backward()
     assert torch.equal(x.grad, 2 * x)
+
+
+@pytest.mark.parametrize("which", ["k", "v"])
+def test_append_is_seen_as_an_in_place_write(cuda, which):
+    """A backward that saved the cache (or a view of it) before new tokens were written raises, as after any
+    in-place operation."""
+    pool = torch.randn(2, 3, 16, 2, 64, device=cuda)
+    caches = dict(k=pool[0], v=pool[1].clone())
+    w = torch.ones(64, device=cuda, requires_grad=True)
+    x = torch.randn(1, 2, 1, 64, device=cuda)
+    table, lengths = (torch.ones(1, n, dtype=torch.int32, device=cuda) for n in (3, 1))
+
+    def append():
+        cfa.paged_append(x, x, caches["k"], caches["v"], table, lengths.view(-1))
+
+    append()
+    y = (caches[which][1:] * w).sum()
+    y.backward(retain_graph=True)
+    with torch.no_grad():
+        append()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    cfa.check_status()
+
+
+def test_append_into_inference_tensors(cuda):
+    """They have no version to count."""
+    with torch.inference_mode():
+        k, v = torch.zeros(2, 3, 16, 2, 64, device=cuda).unbind(0)
+        x = torch.randn(1, 2, 1, 64, device=cuda)
+        table, lengths = torch.ones(1, 3, dtype=torch.int32, device=cuda), torch.ones(1, dtype=torch.int32, device=cuda)
+        cfa.paged_append(x, x, k, v, table, lengths)
+    cfa.paged_append(x, x, k, v, table, lengths)
+    assert torch.equal(k[1, 0], x[0, :, 0]) and torch.equal(v[1, 0], x[0, :, 0])
+    cfa.check_status()
