@@ -401,8 +401,9 @@ Turn turn_of(const char* who, const Tensor& x, PyObject* const* a, int64_t b, in
   REQUIRE(p.scalar_type() == at::kInt || p.scalar_type() == at::kLong, who,
           ": int32 or int64 positions expected");
   const int64_t n = p.dim();
-  REQUIRE((n == 1 && p.size(0) == s) || (n == 2 && (p.size(0) == b || p.size(0) == 1) && p.size(1) == s), who,
-          ": positions [", s, "] or [", b, ", ", s, "] expected, got ", p.sizes());
+  REQUIRE((n == 1 && p.size(0) == s) ||
+              (n == 2 && (p.size(0) == b || p.size(0) == 1) && (p.size(1) == s || (p.size(1) == 1 && p.size(0) == b))),
+          who, ": positions [", s, "], [", b, ", ", s, "] or [", b, ", 1] expected, got ", p.sizes());
   one_device(who, {&x, &t.freqs, &p});
   t.positions = n == 2 && p.size(0) == b && p.size(1) == s ? p : p.expand({b, s});
   return t;

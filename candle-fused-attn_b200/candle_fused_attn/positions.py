@@ -56,8 +56,9 @@ def rotary(x: torch.Tensor, positions: torch.Tensor | int, freqs: torch.Tensor, 
     """x with each head's first 2 len(freqs) dims turned by its position.
 
     x [batch, heads, seq, d] (queries or keys), f32, f16 or bf16 on CUDA, any strides, d <= 1024.
-    `positions`: int32 or int64 [seq] or [batch, seq] on the device, one a token, or the first (an int)
-    of consecutive ones. `freqs`: float64 radians a position (`rotary_frequencies`); pair j is
+    `positions`: int32 or int64 on the device, one a token ([seq] or [batch, seq]) or one for all of
+    a sequence's tokens ([batch, 1]: not the first of consecutive ones); or an int, the first of
+    consecutive ones. `freqs`: float64 radians a position (`rotary_frequencies`); pair j is
     (j, j + len(freqs)), or (2j, 2j + 1) with `interleaved`, and is turned by position * freqs[j] and
     scaled by `amplitude`; the dims past the pairs are copied. Angles are reduced in 64 bits, so far
     positions lose nothing. -> [batch, heads, seq, d], laid out as a dense [batch, seq, heads, d], of
