@@ -39,6 +39,8 @@ Failure detection: every device-side wait of the kernels is bounded. An expired 
 invalid) is written by the kernel into a page-locked host flag this module registers with the C
 ABI (`cfa_error_sink`), so the next call of any function here raises `FusedAttentionError`
 without synchronising; `check_status()` synchronises first and raises for the calls before it.
+A page id outside the cache or a length past its page table -- data of one sequence, which a kernel
+finds and leaves out -- is kept apart: no call fails for it, `check_status()` raises for it.
 """
 
 from __future__ import annotations
@@ -168,22 +170,29 @@ def _stream(dev: torch.device) -> int:
 _sink_tensor: torch.Tensor | None = None
 
 
-def _sink_flag() -> ctypes.c_int32:
-    """The registered page-locked flag (created and registered on first use, with CUDA up)."""
+_PAGE_FLAG = 16  # the page sink's word, on a cache line of its own
+
+
+def _sink_flag(word: int = 0) -> ctypes.c_int32:
+    """A registered page-locked flag (created and registered on first use, with CUDA up): of expired
+    waits, or (_PAGE_FLAG) of bad pages."""
     global _sink_tensor
     if _sink_tensor is None:
-        t = torch.zeros(1, dtype=torch.int32).pin_memory()
-        st = _abi.error_sink(t.data_ptr())
-        if st != _abi.CFA_OK:
-            raise FusedAttentionError(_abi.strerror(st))
+        t = torch.zeros(2 * _PAGE_FLAG, dtype=torch.int32).pin_memory()
+        for st in (_abi.error_sink(t.data_ptr()), _abi.page_sink(t.data_ptr() + 4 * _PAGE_FLAG)):
+            if st != _abi.CFA_OK:
+                raise FusedAttentionError(_abi.strerror(st))
         _sink_tensor = t
-    return ctypes.c_int32.from_address(_sink_tensor.data_ptr())
+    return ctypes.c_int32.from_address(_sink_tensor.data_ptr() + 4 * word)
 
 
 def _raise_if_expired() -> None:
     """Raise (once) for a bounded wait that expired in a kernel launched earlier: the flag is read
     as it stands, with no synchronisation, so kernels still running are not covered."""
-    flag = _sink_flag()
+    _raise_flag(_sink_flag())
+
+
+def _raise_flag(flag: ctypes.c_int32) -> None:
     code = flag.value
     if code != 0:
         flag.value = 0
@@ -192,9 +201,12 @@ def _raise_if_expired() -> None:
 
 def check_status(device: torch.device | int | None = None) -> None:
     """Synchronise `device` (default: the current one) and raise `FusedAttentionError` if a bounded
-    device-side wait of any earlier call expired (their results are then invalid)."""
+    device-side wait of any earlier call expired (their results are then invalid), or if an earlier
+    `paged_append` or `paged_attention` met a page id outside the cache or a length past its page
+    table (keys of that sequence were left out)."""
     torch.cuda.synchronize(device)
     _raise_if_expired()
+    _raise_flag(_sink_flag(_PAGE_FLAG))
 
 
 # ---------------------------------------------------------------------------------------------

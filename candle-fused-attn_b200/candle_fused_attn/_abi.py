@@ -56,6 +56,7 @@ EXPORTS = (
     "cfa_bwd_f32_d64_ffma",
     "cfa_bwd_noalloc_status",
     "cfa_error_sink",
+    "cfa_page_sink",
     "cfa_matmul_workspace_bytes",
     "cfa_matmul_f32",
     "cfa_matmul_status",
@@ -139,6 +140,8 @@ def load() -> ctypes.CDLL:
     lib.cfa_bwd_noalloc_status.argtypes = [_p]
     lib.cfa_error_sink.restype = ctypes.c_int
     lib.cfa_error_sink.argtypes = [_p]
+    lib.cfa_page_sink.restype = ctypes.c_int
+    lib.cfa_page_sink.argtypes = [_p]
     lib.cfa_fwd_status.restype = ctypes.c_int
     lib.cfa_fwd_status.argtypes = [_p]
     lib.cfa_matmul_workspace_bytes.restype = ctypes.c_size_t
@@ -290,6 +293,11 @@ def error_sink(host_ptr) -> int:
     """cfa_error_sink: register a page-locked host int (its address; None unregisters) that every
     bounded-wait expiry reaches without a synchronisation. Returns the status."""
     return load().cfa_error_sink(host_ptr)
+
+
+def page_sink(host_ptr) -> int:
+    """cfa_page_sink: the same for page ids outside the cache and lengths past the page table."""
+    return load().cfa_page_sink(host_ptr)
 
 
 def bwd_noalloc_status(stream) -> int:

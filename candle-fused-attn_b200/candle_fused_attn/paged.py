@@ -13,9 +13,9 @@ calls of a step:
     o = paged_attention(q, k_cache, v_cache, page_table, lengths, scale)
 
 Everything is read on the device when the kernels run: a captured CUDA graph of these lines can be
-replayed while the lengths grow, up to the table's width. A page id outside the cache, or a length
-past the table, raises `FusedAttentionError` on a later call (or in `check_status()`); the kernels
-leave such keys out.
+replayed while the lengths grow, up to the table's width. Where a page id lies outside the cache, or
+a length past the table, the kernels leave such keys out and go on; `check_status()` raises
+`FusedAttentionError` for it, and no other call does (it may serve another sequence).
 """
 
 from __future__ import annotations

@@ -34,6 +34,26 @@ DeviceOnce g_bwd_tc_once[kMaxDevices];
 enum class Pair { kTensorCore, kFfma };
 // The host-visible error flag of cfa_error_sink, as the device addresses it (nullptr: none).
 std::atomic<int*> g_sink{nullptr};
+// And that of cfa_page_sink.
+std::atomic<int*> g_page_sink{nullptr};
+
+int register_sink(std::atomic<int*>& sink, int* host_flag) {
+  if (host_flag == nullptr) {
+    sink.store(nullptr);
+    return CFA_OK;
+  }
+  if ((reinterpret_cast<uintptr_t>(host_flag) & 3u) != 0) return CFA_ERR_ALIGNMENT;
+  // Only page-locked host memory the device can address is accepted: a kernel's store to anything
+  // else would fault.
+  cudaPointerAttributes attr{};
+  if (cudaPointerGetAttributes(&attr, host_flag) != cudaSuccess) return CFA_ERR_CUDA;
+  if (attr.type != cudaMemoryTypeHost) return CFA_ERR_CUDA;
+  void* dev_ptr = nullptr;
+  if (cudaHostGetDevicePointer(&dev_ptr, host_flag, 0) != cudaSuccess || dev_ptr == nullptr)
+    return CFA_ERR_CUDA;
+  sink.store(static_cast<int*>(dev_ptr));
+  return CFA_OK;
+}
 
 int setup(DeviceOnce* table, cudaError_t (*fn)()) {
   int dev = 0;
@@ -222,11 +242,12 @@ int bwd_impl(const float* q, const int64_t q_strides[3], const float* k,
 
 namespace cfa {
 int* error_sink() { return g_sink.load(std::memory_order_relaxed); }
+int* page_sink() { return g_page_sink.load(std::memory_order_relaxed); }
 }  // namespace cfa
 
 extern "C" {
 
-int cfa_abi_version(void) { return (2 << 16) | 3; }
+int cfa_abi_version(void) { return (2 << 16) | 4; }
 
 const char* cfa_strerror(int status) {
   switch (status) {
@@ -429,23 +450,9 @@ int cfa_selftest_bounded_wait(void* workspace, int64_t timeout_ns, int blocks, v
   return e == cudaSuccess ? CFA_OK : CFA_ERR_LAUNCH;
 }
 
-int cfa_error_sink(int* host_flag) {
-  if (host_flag == nullptr) {
-    g_sink.store(nullptr);
-    return CFA_OK;
-  }
-  if ((reinterpret_cast<uintptr_t>(host_flag) & 3u) != 0) return CFA_ERR_ALIGNMENT;
-  // Only page-locked host memory the device can address is accepted: a kernel's store to anything
-  // else would fault.
-  cudaPointerAttributes attr{};
-  if (cudaPointerGetAttributes(&attr, host_flag) != cudaSuccess) return CFA_ERR_CUDA;
-  if (attr.type != cudaMemoryTypeHost) return CFA_ERR_CUDA;
-  void* dev_ptr = nullptr;
-  if (cudaHostGetDevicePointer(&dev_ptr, host_flag, 0) != cudaSuccess || dev_ptr == nullptr)
-    return CFA_ERR_CUDA;
-  g_sink.store(static_cast<int*>(dev_ptr));
-  return CFA_OK;
-}
+int cfa_error_sink(int* host_flag) { return register_sink(g_sink, host_flag); }
+
+int cfa_page_sink(int* host_flag) { return register_sink(g_page_sink, host_flag); }
 
 int cfa_fwd_status(void* stream) {
   if (cudaStreamSynchronize(static_cast<cudaStream_t>(stream)) != cudaSuccess) return CFA_ERR_CUDA;

@@ -221,6 +221,8 @@ cudaError_t launch_selftest_wait(int* ws, uint64_t short_ns, int blocks, int* si
 
 // The host-visible error flag registered with cfa_error_sink (its device address), or nullptr.
 int* error_sink();
+// That of cfa_page_sink.
+int* page_sink();
 
 // One-time per-device attribute set-up (dynamic shared memory limits).
 cudaError_t setup_fwd_attributes();

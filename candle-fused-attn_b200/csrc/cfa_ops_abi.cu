@@ -275,7 +275,6 @@ int cfa_cross_few_f32(const float* q, const int64_t q_strides[3], const float* k
   a.B = static_cast<int>(batch), a.H = static_cast<int>(heads), a.Hk = static_cast<int>(key_heads);
   a.S = static_cast<int>(seq), a.D = static_cast<int>(head_dim);
   a.scale = scale;
-  a.sink = cfa::error_sink();
   return status(cfa::launch_split_attention(a, CFA_F32, CFA_F32, workspace,
                                             static_cast<cudaStream_t>(stream)));
 }
@@ -362,7 +361,7 @@ int cfa_paged_append(const void* q, const int64_t q_strides[3], void* q_out,
   a.rot_heads = a.H;
   a.S = static_cast<int>(seq), a.D = static_cast<int>(head_dim), a.rot = static_cast<int>(rotary_dim);
   a.n_tokens = batch * seq;
-  a.sink = cfa::error_sink();
+  a.sink = cfa::page_sink();
   return status(cfa::launch_paged_append(a, dtype, cache_dtype, static_cast<cudaStream_t>(stream)));
 }
 
@@ -424,7 +423,7 @@ int cfa_paged_attention(const void* q, const int64_t q_strides[3], int dtype, co
   a.B = static_cast<int>(batch), a.H = static_cast<int>(heads), a.Hk = static_cast<int>(key_heads);
   a.S = static_cast<int>(seq), a.D = static_cast<int>(head_dim);
   a.scale = scale;
-  a.sink = cfa::error_sink();
+  a.sink = cfa::page_sink();
   return status(cfa::launch_split_attention(a, dtype, cache_dtype, workspace,
                                             static_cast<cudaStream_t>(stream)));
 }

@@ -52,7 +52,7 @@
 //
 // Masked keys are excluded rather than weighted by zero, so what lies behind a sequence's end or a
 // row's last key -- infinities and NaN among it -- never reaches a result. A page id outside the
-// pool is reported through the error sink and its keys are left out.
+// pool is reported through the page sink and its keys are left out.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 

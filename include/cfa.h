@@ -28,7 +28,7 @@
  *   cfa_matmul_workspace_bytes           the training step (examples/tutorial.rs:103-118) as a
  *   cfa_matmul_status                    tensor-core kernel
  *   cfa_cross_*, cfa_rotary,   operators beside the path (no counterpart): attention to another
- *   cfa_paged_*                            sequence, rotary positions, a paged cache and its attention
+ *   cfa_paged_*, cfa_page_sink             sequence, rotary positions, a paged cache and its attention
  *
  * Head dim 64 runs one kernel pair, as the reference does (src/cuda.rs:140-260): the tensor-core
  * pair (csrc/fwd_tc.cu, csrc/bwd_tc.cu). A backward must run on the forward's L of the same pair
@@ -254,6 +254,12 @@ int cfa_selftest_bounded_wait(void* workspace, int64_t timeout_ns, int blocks, v
  * it registered can run. Has no counterpart in the reference, whose waits have no bound. */
 int cfa_error_sink(int* host_flag);
 
+/* The same for the paged cache's operators: a kernel that meets a page id outside the cache or a
+ * length past its page table writes CFA_ERR_PAGE there. A word of its own, because it says something
+ * of one sequence's data, not of the results of others: nobody's next call need fail for it, and it
+ * cannot cover an expiry. */
+int cfa_page_sink(int* host_flag);
+
 /* The projection next to the attention: C = A B over fp32 on the tensor cores (three bf16 parts
  * per operand, six products, fp32 sums per 64-element window) -- the contraction of candle's
  * `Tensor::broadcast_matmul` in the reference's training step (examples/tutorial.rs:110: qkv =
@@ -354,7 +360,7 @@ int cfa_rotary(const void* x, const int64_t x_strides[3], void* y, const int64_t
  * that position (rotary_dim 0: not at all). q, if given, is rotated into q_out (rows that are no
  * token: zeros). `dtype`: q, k, v; the cache's type is the same or, for fp32 inputs, any. A token
  * without a page (an id outside 0 .. pages - 1, past the table, a negative position) is not written;
- * a bad page id is reported through cfa_error_sink (CFA_ERR_PAGE). Two tokens of a call must not
+ * a bad page id is reported through cfa_page_sink (CFA_ERR_PAGE). Two tokens of a call must not
  * share a slot. */
 int cfa_paged_append(const void* q, const int64_t q_strides[3], void* q_out,
                      const int64_t q_out_strides[3], const void* k, const int64_t k_strides[3],
@@ -372,7 +378,7 @@ int cfa_paged_append(const void* q, const int64_t q_strides[3], void* q_out,
  * `dtype`, 16-byte rows; o [batch, seq, heads, head_dim] dense, of `dtype`; rows that see nothing or
  * are no token: zeros. head_dim 32, 64 or 128; the cache's rows 16-byte aligned; types and heads as
  * above. Sums and softmax statistics are fp32. Keys on a bad page are left out and reported
- * (CFA_ERR_PAGE), and so is a length past the table. Workspace (256-byte aligned, no initialisation)
+ * (cfa_page_sink), and so is a length past the table. Workspace (256-byte aligned, no initialisation)
  * for max_keys = table_width * page_size. */
 size_t cfa_paged_attention_workspace_bytes(int64_t batch, int64_t heads, int64_t seq,
                                            int64_t max_keys, int64_t head_dim, int cache_dtype);
@@ -390,7 +396,7 @@ const char* cfa_strerror(int status);
 
 /* ABI version: (major << 16) | minor (2.0: one kernel pair per entry point, the error sink;
  * 2.1: the projection GEMM; 2.2: head dim 32 on the tensor cores, the generic CUDA-core pair;
- * 2.3: cross attention, rotary positions, the paged cache). */
+ * 2.3: cross attention, rotary positions, the paged cache; 2.4: the page sink). */
 int cfa_abi_version(void);
 
 #ifdef __cplusplus
