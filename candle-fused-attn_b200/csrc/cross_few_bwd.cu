@@ -223,6 +223,7 @@ __global__ void __launch_bounds__(NT, 2) cross_few_bwd_kernel(const BwdArgs a) {
     }
     __syncwarp();  // dS's rows are read
   }
+  cp_async_wait_all();  // (a warp that left at its first tile has the second one's copies in flight)
   __syncthreads();  // every warp's keys are read: their dQ take the place
 #pragma unroll
   for (int m = 0; m < MQ; ++m)
