@@ -70,8 +70,8 @@ int check_cross(int64_t B, int64_t H, int64_t Hk, int64_t Sq, int64_t Sk, int64_
   return CFA_OK;
 }
 
-// The cross backward's workspace: ticket and error flag, turn counters (one cleared range), D, where the
-// query tiles are cut into parts their dK, dV, and, in a workspace of `total_fast`, the dQ partials. The
+// The cross backward's workspace: ticket and error flag, turn counters, the slices' tickets (one cleared
+// range), D, where the query tiles are cut into parts a slice's dK, dV, and, in a workspace of `total_fast`, the dQ partials. The
 // parts follow from the shapes of one batch element: no sum depends on the batch.
 // dQ by partials (up to 4 GB of them) or by the turn chain, whose blocks wait for one another: the same
 // sums in the same order, but at [4, 16 over 4, 2048 x 8192, 64] 4.53 ms against 6.61, at 470 rows over
@@ -82,11 +82,16 @@ constexpr int64_t kCrossJoinBytes = 512 << 10;   // dQ partials of a (batch, key
 // 700 x 300, 64] 32, 51, 103 and 192 us; [8, 8, 512 x 512, 64] 122, 106, 106, 106; [2, 16 over 1, 1024 x
 // 1024, 64] 215, 215, 176, 1023.
 constexpr int kCrossPartTiles = 8;
+// Most bytes of the parts' dK and dV: with more (one part of 19 a batch element of [64, 16 over 1, 1024 x
+// 1024, 64] takes 0.5 MB, the batch 638), the batch goes in slices that use the same memory one after another,
+// the same bits as each element's are its own. A slice of that size is still many times what the SMs take at once.
+constexpr int64_t kCrossPartsBytes = int64_t(512) << 20;
 struct CrossLayout {
   int64_t n_zero;  // ints cleared before the backward
   size_t turn_off, dsum_off, kv_off, part_off, total, total_fast;
   bool join_dq;    // (with the partials)
   int n_parts;
+  int64_t slice, tickets;  // batch elements of a launch; where the slices' tickets are, in ints
   bool few;
 };
 CrossLayout cross_layout(int64_t B, int64_t H, int64_t Hk, int64_t Sq, int64_t Sk, int64_t D) {
@@ -101,10 +106,15 @@ CrossLayout cross_layout(int64_t B, int64_t H, int64_t Hk, int64_t Sq, int64_t S
   w.join_dq = w.n_parts > 1 || group * Sq > kCrossJoinBytes / row_bytes;
   w.turn_off = 256;
   const int64_t turns = B * Hk * tiles;
-  w.n_zero = 64 + turns;
-  w.dsum_off = w.turn_off + cfa::align256(static_cast<size_t>(turns) * 4);
+  const int64_t parts = w.n_parts > 1 ? w.n_parts * Sk * 2 * Hk * D * 4 : 0;  // bytes of an element's (< 2^50)
+  w.slice = parts == 0 ? B : std::max<int64_t>(1, std::min(B, kCrossPartsBytes / parts));
+  const int64_t slices = (B + w.slice - 1) / w.slice;
+  w.tickets = slices == 1 ? 0 : 64 + turns;
+  const int64_t counters = turns + (slices == 1 ? 0 : slices);
+  w.n_zero = 64 + counters;
+  w.dsum_off = w.turn_off + cfa::align256(static_cast<size_t>(counters) * 4);
   w.kv_off = w.dsum_off + cfa::align256(static_cast<size_t>(B * H * Sq) * 4);
-  w.total = w.kv_off + (w.n_parts > 1 ? static_cast<size_t>(w.n_parts) * B * Sk * 2 * Hk * D * 4 : 0);
+  w.total = w.kv_off + static_cast<size_t>(w.slice * parts);
   w.part_off = w.total;
   const int64_t queries = B * H * Sq;
   w.total_fast = w.total + (queries <= kCrossPartialBytes / row_bytes ? static_cast<size_t>(queries * row_bytes) : 0);
@@ -206,36 +216,46 @@ int cfa_cross_bwd_f32(const float* q, const int64_t q_strides[3], const float* k
                                  : cfa::launch_hd_bwd_prep(p, static_cast<int>(head_dim), s);
   if (e != cudaSuccess) return status(e);
 
-  cfa::BwdArgs a{};
-  a.q = q, a.k = k, a.v = v, a.d_o = d_o, a.lse = lse, a.dsum = p.dsum;
-  a.dq = dq, a.dkv = dkv;
-  a.ticket = ticket;
-  a.err = ticket + 1;
-  a.turn = reinterpret_cast<int*>(ws + lay.turn_off);
-  a.q_sb = q_strides[0], a.q_sh = q_strides[1], a.q_ss = q_strides[2];
-  a.k_sb = k_strides[0], a.k_sh = k_strides[1], a.k_ss = k_strides[2];
-  a.v_sb = v_strides[0], a.v_sh = v_strides[1], a.v_ss = v_strides[2];
-  a.do_sb = do_strides[0], a.do_sh = do_strides[1], a.do_ss = do_strides[2];
-  a.B = static_cast<int>(batch), a.H = static_cast<int>(heads), a.S = static_cast<int>(seq);
-  a.Hk = static_cast<int>(key_heads), a.Sk = static_cast<int>(key_seq);
-  a.key_lengths = key_lengths;
-  a.scale = scale;
-  a.n_qtiles = static_cast<int>((seq + 63) / 64);
-  a.timeout_ns = cfa::WAIT_TIMEOUT_NS;
-  a.sink = cfa::error_sink();
   // The dQ partials when the workspace holds them (the same results, bit for bit).
   const bool partials = lay.few || (lay.total_fast > lay.total && workspace_bytes >= lay.total_fast);
-  a.dq_part = partials ? reinterpret_cast<float*>(ws + lay.part_off) : nullptr;
-  a.n_parts = lay.n_parts;
-  a.join_dq = lay.few || (partials && lay.join_dq);
-  a.dkv_out = dkv;
-  if (lay.n_parts > 1) {
-    a.dkv = reinterpret_cast<float*>(ws + lay.kv_off);
-    a.part_stride = batch * key_seq * 2 * key_heads * head_dim;
+  const int64_t kb = head_dim == 128 ? 64 : 128, nkb = (key_seq + kb - 1) / kb;
+  const int64_t tiles = (heads / key_heads * seq + 63) / 64;
+  const int64_t dkv_size = key_seq * 2 * key_heads * head_dim;  // floats of a batch element's
+  for (int64_t b0 = 0, i = 0; b0 < batch; b0 += lay.slice, ++i) {
+    cfa::BwdArgs a{};
+    a.q = q + b0 * q_strides[0], a.k = k + b0 * k_strides[0], a.v = v + b0 * v_strides[0];
+    a.d_o = d_o + b0 * do_strides[0];
+    a.lse = lse + b0 * queries, a.dsum = p.dsum + b0 * queries;
+    a.dq = dq + b0 * queries * head_dim;
+    a.dkv = a.dkv_out = dkv + b0 * dkv_size;
+    a.ticket = ticket + lay.tickets + (lay.tickets ? i : 0);
+    a.err = ticket + 1;
+    a.turn = reinterpret_cast<int*>(ws + lay.turn_off) + b0 * key_heads * tiles;
+    a.q_sb = q_strides[0], a.q_sh = q_strides[1], a.q_ss = q_strides[2];
+    a.k_sb = k_strides[0], a.k_sh = k_strides[1], a.k_ss = k_strides[2];
+    a.v_sb = v_strides[0], a.v_sh = v_strides[1], a.v_ss = v_strides[2];
+    a.do_sb = do_strides[0], a.do_sh = do_strides[1], a.do_ss = do_strides[2];
+    const int64_t n = std::min(lay.slice, batch - b0);
+    a.B = static_cast<int>(n), a.H = static_cast<int>(heads), a.S = static_cast<int>(seq);
+    a.Hk = static_cast<int>(key_heads), a.Sk = static_cast<int>(key_seq);
+    a.key_lengths = key_lengths ? key_lengths + b0 : nullptr;
+    a.scale = scale;
+    a.n_qtiles = static_cast<int>((seq + 63) / 64);
+    a.timeout_ns = cfa::WAIT_TIMEOUT_NS;
+    a.sink = cfa::error_sink();
+    a.dq_part = partials ? reinterpret_cast<float*>(ws + lay.part_off) + b0 * queries * nkb * head_dim : nullptr;
+    a.n_parts = lay.n_parts;
+    a.join_dq = lay.few || (partials && lay.join_dq);
+    if (lay.n_parts > 1) {
+      a.dkv = reinterpret_cast<float*>(ws + lay.kv_off);
+      a.part_stride = n * dkv_size;
+    }
+    e = lay.few            ? cfa::launch_cross_few_bwd(a, static_cast<int>(head_dim), s)
+        : head_dim == 128  ? cfa::launch_cross_hd_bwd(a, s)
+                           : cfa::launch_cross_bwd_tc(a, static_cast<int>(head_dim), s);
+    if (e != cudaSuccess) return status(e);
   }
-  if (lay.few) return status(cfa::launch_cross_few_bwd(a, static_cast<int>(head_dim), s));
-  return status(head_dim == 128 ? cfa::launch_cross_hd_bwd(a, s)
-                                : cfa::launch_cross_bwd_tc(a, static_cast<int>(head_dim), s));
+  return CFA_OK;
 }
 
 size_t cfa_cross_few_workspace_bytes(int64_t batch, int64_t heads, int64_t seq, int64_t key_seq,

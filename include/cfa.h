@@ -308,7 +308,9 @@ int cfa_cross_fwd_f32(const float* q, const int64_t q_strides[3],
 
 /* Its backward, from the forward's o and lse: dq [batch, seq, heads, head_dim] and dkv [batch,
  * key_seq, 2, key_heads, head_dim] (dK, dV interleaved), dense, written whole (rows past a key
- * length: zeros). Scratch (256-byte aligned, no initialisation): at least the first size; with the
+ * length: zeros). Scratch (256-byte aligned, no initialisation): at least the first size (the sums of
+ * dK and dV over query tiles that are cut into parts take up to 512 MB of it, or one batch element's if
+ * that is more: a larger batch goes in slices, the same results); with the
  * second (up to 4 GB more; the first where the partials would take more) dQ goes by partials instead of
  * a chain of key blocks that wait for one another -- the same results, bit for bit, in less time.
  * cfa_bwd_status reads its error flag. */
