@@ -37,6 +37,7 @@ using torch::autograd::variable_list;
 // side of failure detection: where its flag is, and what raises for it.
 struct Abi {
   decltype(&cfa_cross_fwd_f32) cross_fwd;
+  decltype(&cfa_cross_bwd_workspace_bytes) cross_bwd_least;
   decltype(&cfa_cross_bwd_workspace_bytes_fast) cross_bwd_workspace;
   decltype(&cfa_cross_bwd_f32) cross_bwd;
   decltype(&cfa_cross_few_workspace_bytes) cross_few_workspace;
@@ -344,8 +345,16 @@ struct Cross : torch::autograd::Function<Cross> {
     const Tensor dq = merged_heads(m.b, m.h, m.sq, m.d, q);
     const int64_t row = 2 * m.hk * m.d;
     const Tensor dkv = empty({m.b, m.sk, 2, m.hk, m.d}, {m.sk * row, row, m.hk * m.d, m.d, 1}, q, at::kFloat);
-    const size_t n = abi.cross_bwd_workspace(m.b, m.h, m.hk, m.sq, m.sk, m.d);
-    const Tensor ws = workspace(n, q);
+    // With the dQ partials (up to 4 GB) or, where there is no room for them, without: the same bits.
+    size_t n = abi.cross_bwd_workspace(m.b, m.h, m.hk, m.sq, m.sk, m.d);
+    Tensor ws;
+    try {
+      ws = workspace(n, q);
+    } catch (const c10::OutOfMemoryError&) {
+      const size_t least = abi.cross_bwd_least(m.b, m.h, m.hk, m.sq, m.sk, m.d);
+      if (least == n) throw;
+      ws = workspace(n = least, q);
+    }
     check_status(abi.cross_bwd(ptr<float>(q), Strides3(q), ptr<float>(k), Strides3(k), ptr<float>(v),
                                Strides3(v), ptr<int32_t>(lengths), ptr<float>(o), ptr<float>(lse),
                                ptr<float>(g), Strides3(g), dq.mutable_data_ptr<float>(),
@@ -567,7 +576,7 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   constexpr Py_ssize_t entries = sizeof(Abi) / sizeof(void*);
   if (n != 4 || !PyTuple_Check(a[0]) || PyTuple_GET_SIZE(a[0]) != entries) {
-    PyErr_SetString(PyExc_TypeError, "bind: ten addresses, a class and two functions expected");
+    PyErr_SetString(PyExc_TypeError, "bind: eleven addresses, a class and two functions expected");
     return nullptr;
   }
   void* at[entries];

@@ -13,8 +13,8 @@ from . import FusedAttentionError, _abi, _raise_if_expired, _sink_flag
 
 # In the order of the extension's table.
 _ENTRY_POINTS = (
-    "cfa_cross_fwd_f32", "cfa_cross_bwd_workspace_bytes_fast", "cfa_cross_bwd_f32",
-    "cfa_cross_few_workspace_bytes", "cfa_cross_few_f32", "cfa_rotary", "cfa_paged_append",
+    "cfa_cross_fwd_f32", "cfa_cross_bwd_workspace_bytes", "cfa_cross_bwd_workspace_bytes_fast",
+    "cfa_cross_bwd_f32", "cfa_cross_few_workspace_bytes", "cfa_cross_few_f32", "cfa_rotary", "cfa_paged_append",
     "cfa_paged_attention_workspace_bytes", "cfa_paged_attention", "cfa_strerror")
 _FUNCTIONS = ("cross_attention", "paged_append", "paged_attention", "rotary", "rotary_qkv")
 

@@ -24,6 +24,7 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: fl
 
     Differentiable in q, k and v (dk, dv of a shared head are summed over its query heads). Few
     queries -- the single token of a decoding step -- take a kernel that splits the keys.
-    Bit-identical across reruns and batch splits.
+    The backward asks for up to 4 GB of scratch beside its gradients and goes on, with the same bits
+    but slower, where that cannot be had. Bit-identical across reruns and batch splits.
     """
     return _ops.cross_attention(q, k, v, scale, key_lengths)

@@ -53,3 +53,23 @@ def test_a_batch_whose_parts_take_slices(cuda, d, b, h, sq, sk):
     cfa.check_status()
     chain = (dq.transpose(1, 2), *(dkv[:, :, i].transpose(1, 2) for i in (0, 1)))
     assert torch.equal(out.transpose(1, 2), o) and all(torch.equal(a, c) for a, c in zip(chain, grads))
+
+
+def test_backward_without_room_for_its_partials(cuda):
+    """2 GB of dQ partials that the allocator refuses: the least workspace, the same bits."""
+    b, h, sq, sk, d = 4, 8, 4096, 8192, 64
+    x = [torch.randn(b, h, s, d, device=cuda, requires_grad=True) for s in (sq, sk, sk)]
+    o = cfa.cross_attention(*x, 0.125)
+    dout = torch.randn_like(o)
+    want = torch.autograd.grad(o, x, dout, retain_graph=True)
+    size = _abi.cross_bwd_workspace_bytes_fast(b, h, h, sq, sk, d)
+    assert size > 2 << 30 and _abi.cross_bwd_workspace_bytes(b, h, h, sq, sk, d) < 100 << 20
+    torch.cuda.empty_cache()
+    total = torch.cuda.get_device_properties(cuda).total_memory
+    torch.cuda.set_per_process_memory_fraction((torch.cuda.memory_reserved() + size // 2) / total)
+    try:
+        got = torch.autograd.grad(o, x, dout)
+    finally:
+        torch.cuda.set_per_process_memory_fraction(1.0)
+    assert all(torch.equal(a, c) for a, c in zip(got, want))
+    cfa.check_status()
