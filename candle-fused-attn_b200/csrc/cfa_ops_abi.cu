@@ -77,7 +77,13 @@ int check_cross(int64_t B, int64_t H, int64_t Hk, int64_t Sq, int64_t Sk, int64_
 // sums in the same order, but at [4, 16 over 4, 2048 x 8192, 64] 4.53 ms against 6.61, at 470 rows over
 // 6990 keys 157 us against 311.
 constexpr int64_t kCrossPartialBytes = int64_t(4) << 30;
-constexpr int64_t kCrossJoinBytes = 512 << 10;   // dQ partials of a (batch, key head) one block may sum
+// Most dQ partials of a (batch, key head) that its last block sums; more are summed by the join kernel. Last
+// block and join, in us, backward alone, at 64 dims: 256 KB [16, 8, 512 x 256] 107 and 106, 300 KB [64, 6, 240 x
+// 600] 378 and 374, the same over 100 to 600 keys 272 and 279, 375 KB [64, 6, 300 x 640] 444 and 437, 384 KB
+// [8, 8, 384 x 512] 83 and 79, 512 KB [8, 8, 512 x 512] 103 and 97, [8, 8 over 2, 128 x 512] 54 and 57, 1 MB
+// [4, 8, 512 x 1024] 113 and 96. At 128 dims always the join: 400 KB [32, 8, 200 x 256] 517 and 457, 480 KB [64,
+// 6, 240 x 240] 761 and 719, 512 KB [32, 8, 128 x 512] 540 and 491, 2 MB [16, 8, 512 x 512] 1027 and 880.
+constexpr int64_t kCrossJoinBytes = 320 << 10;
 // Fewest query tiles of a part: each reads its keys again. With 4, 8, 16 and without parts: [1, 8 over 2,
 // 700 x 300, 64] 32, 51, 103 and 192 us; [8, 8, 512 x 512, 64] 122, 106, 106, 106; [2, 16 over 1, 1024 x
 // 1024, 64] 215, 215, 176, 1023.
@@ -103,7 +109,7 @@ CrossLayout cross_layout(int64_t B, int64_t H, int64_t Hk, int64_t Sq, int64_t S
   const int64_t want = (cfa::LIN_SMS + nkb * Hk - 1) / (nkb * Hk);
   w.n_parts = static_cast<int>(std::max<int64_t>(1, std::min(want, tiles / kCrossPartTiles)));
   const int64_t row_bytes = nkb * D * 4;  // of one query's dQ partials (below 2^34)
-  w.join_dq = w.n_parts > 1 || group * Sq > kCrossJoinBytes / row_bytes;
+  w.join_dq = w.n_parts > 1 || D == 128 || group * Sq > kCrossJoinBytes / row_bytes;
   w.turn_off = 256;
   const int64_t turns = B * Hk * tiles;
   const int64_t parts = w.n_parts > 1 ? w.n_parts * Sk * 2 * Hk * D * 4 : 0;  // bytes of an element's (< 2^50)

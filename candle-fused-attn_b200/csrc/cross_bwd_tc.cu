@@ -13,10 +13,9 @@
 //    tiles are cut into parts of consecutive ones, a block each, whose dV, dK sums cross_join_kernel
 //    adds in order. (bwd_tc.cu's split tail would have one block fold every tile of the others: at 16
 //    heads over one, [2, 16, 1024, 64], that and one block's sum of all dQ partials took 1.2 of 1.5
-//    ms.) Where the dQ partials of a (batch, key head) exceed half a MB, or with parts, that kernel
+//    ms.) Where the dQ partials of a (batch, key head) exceed 320 KB, or with parts, that kernel
 //    sums them too, by all SMs; below, the key head's last block does, behind which the others run on
-//    ([64, 6, 240, 64] over 100 to 600 keys: 272 us so, 279 by the join; [8, 8, 512 x 512, 64]: 106
-//    against 100);
+//    ([64, 6, 240, 64] over 100 to 600 keys: 272 us so, 279 by the join; kCrossJoinBytes has more);
 //  - dQ [B, S, H, HD] and dK, dV [B, Sk, 2, Hk, HD] go to buffers of their own.
 // It is a kernel of its own, because at 96 registers a thread the fused attention's backward keeps
 // its registers only as it stands: as one template, that instance spilled or slowed by 0.2 to 3 %.

@@ -13,7 +13,7 @@
 //
 // Bound by the issue of splits and products, two warps a scheduler: at the rate of these products (a third
 // of tf32's: 96 TFLOP/s) the tensor core is busy for 0.5 to 0.6 of the time. [16, 8, 512 x 512, 128]:
-// forward 303 us (57 TFLOP/s), backward 889 us (48); by fp32 FMAs, as hd_ffma.cu has the fused attention's,
+// forward 303 us (57 TFLOP/s), backward 880 us (49); by fp32 FMAs, as hd_ffma.cu has the fused attention's,
 // 442 and 1128 us. [2, 8, 2048 x 4096, 128]: 1.32 and 3.35 ms, for 1.70 and 4.33.
 #include "cfa_common.cuh"
 #include "tf32.cuh"
@@ -190,7 +190,8 @@ __global__ void __launch_bounds__(NT, 2) cross_hd_fwd_kernel(const FwdArgs a) {
 //      out of shared memory, dS = P o (dP - D); both to shared memory, [query][key];
 //   2. warps 0-3 dV += P^T dO, warps 4-7 dK += dS^T Q, 16 keys a warp, added in fp32;
 //   3. all: the tile's dQ partial dS K, 16 queries and half the dims a warp.
-// Key blocks, parts, dQ's order and the zeros of unattended keys are cross_bwd_tc.cu's. The operands' tiles
+// Key blocks, parts, dQ's order and the zeros of unattended keys are cross_bwd_tc.cu's, the dQ partials
+// always cross_join_kernel's. The operands' tiles
 // are read both by rows (products over the dims) and by columns: piece c of row r is piece c ^ swizzle(r),
 // conflict-free for 16-byte reads of two rows' four pieces and of every other row's two.
 constexpr int BT = 256, KB = 64, LP = KB + 4;
@@ -257,7 +258,6 @@ __global__ void __launch_bounds__(BT, 1) cross_hd_bwd_kernel(const BwdArgs a) {
     return;
   }
   int* turn = a.turn + static_cast<int64_t>(bh) * nqt;       // turn chain: counters per tile
-  const int64_t row_stride = static_cast<int64_t>(a.H) * D;  // dq floats per (b, s)
 
   {
     const float* kp = a.k + b * a.k_sb + hk * a.k_sh;
@@ -491,33 +491,6 @@ __global__ void __launch_bounds__(BT, 1) cross_hd_bwd_kernel(const BwdArgs a) {
       __threadfence();  // ORDER: this block's dQ stores are visible before the turn passes on
       __syncthreads();
       if (tid == 0) st_release_gpu(turn + t, kb + 1);
-    }
-  }
-
-  if (no_wait && !a.join_dq) {  // (without join_dq there is one part)
-    // ORDER: partials visible GPU-wide before counting in; the last to count sums them all.
-    __threadfence();
-    __syncthreads();
-    if (tid == 0) s_int[1] = atomicAdd(a.turn + bh, 1);
-    __syncthreads();
-    if (s_int[1] == nkb - 1) {
-      __threadfence();
-      // DETERMINISM: (((p0 + p1) + p2) + ...) * scale over the contributing key blocks in order.
-      for (int hq = h0; hq < h0 + group; ++hq) {
-        const float* part = a.dq_part + (static_cast<int64_t>(b) * a.H + hq) * a.n_kblocks * S * D;
-        float* dq_out = a.dq + static_cast<int64_t>(b) * S * row_stride + hq * D;
-        for (int idx = tid; idx < S * C; idx += BT) {
-          const int i = idx / C, c4 = idx % C;
-          float4 v = __ldcg(reinterpret_cast<const float4*>(part + static_cast<int64_t>(i) * D + 4 * c4));
-          for (int j = 1; j < nkb; ++j) {
-            const float4 p = __ldcg(reinterpret_cast<const float4*>(
-                part + (static_cast<int64_t>(j) * S + i) * D + 4 * c4));
-            v = make_float4(v.x + p.x, v.y + p.y, v.z + p.z, v.w + p.w);
-          }
-          *reinterpret_cast<float4*>(dq_out + i * row_stride + 4 * c4) =
-              make_float4(v.x * dscale, v.y * dscale, v.z * dscale, v.w * dscale);
-        }
-      }
     }
   }
 
