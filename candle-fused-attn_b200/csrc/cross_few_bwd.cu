@@ -6,7 +6,7 @@
 //   dV = P^T dO and dK = scale dS^T Q, whole, to memory; dQ += dS K in registers,
 // the block's dQ partial summed over its warps in order, the key blocks' by cross_join_kernel. Products by
 // mma.m16n8k8 on two-part tf32 operands (tf32.cuh; hi hi + hi lo + lo hi), the keys as the 16 rows, the
-// queries as columns; P^T's and dS^T's fragments are those of the scores, dS's rows go through shared memory.
+// queries as columns; a score's products and sums in the order of the forward that made L (split_attn.cu); P^T's and dS^T's fragments are those of the scores, dS's rows go through shared memory.
 //
 // Bound by memory up to 16 rows: K, V are read and dK, dV written once, at 20 rows D flops a key against
 // 16 D bytes; at 32 by the products' issue. The tcgen05 pair, whose tiles are 64 queries, spends a block's
@@ -148,13 +148,28 @@ __global__ void __launch_bounds__(NT, 2) cross_few_bwd_kernel(const BwdArgs a) {
       clear(s);
 #pragma unroll
       for (int j = 0; j < J; ++j) {
-        float c[NQ][4];
-        clear(c);
         uint32_t ah[2][4], al[2][4];
         split_rows(at_row(A, 0, j), at_row(A, 8, j), ah, al);
+        if constexpr (NQ == 1) {  // (the forward has the parts of up to 8 rows in sums of their own)
+          uint32_t h[4], l[4];
+          split_tf32(at_row(B, 0, j), h, l);
+          float c[3][4];
+          clear(c);
 #pragma unroll
-        for (int q = 0; q < NQ; ++q) products(c[q], ah, al, at_row(B, 8 * q, j));
-        add(s, c);
+          for (int y = 0; y < 2; ++y) {
+            mma_tf32(c[0], al[y], h[2 * y], h[2 * y + 1]);
+            mma_tf32(c[1], ah[y], l[2 * y], l[2 * y + 1]);
+            mma_tf32(c[2], ah[y], h[2 * y], h[2 * y + 1]);
+          }
+#pragma unroll
+          for (int x = 0; x < 4; ++x) s[0][x] += (c[1][x] + c[0][x]) + c[2][x];
+        } else {
+          float c[NQ][4];
+          clear(c);
+#pragma unroll
+          for (int q = 0; q < NQ; ++q) products(c[q], ah, al, at_row(B, 8 * q, j));
+          add(s, c);
+        }
       }
     };
     // dst[keys][dims] = X^T Y for scores-shaped X (keys x queries) and Y [queries][dims], times f.

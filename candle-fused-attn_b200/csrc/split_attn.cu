@@ -37,12 +37,12 @@
 //     |x|; three or all four of the products of the parts), and dims and keys are numbered within a
 //     product so that a lane reads K and V 16 bytes at a time and P's fragment is S's. Three stages of
 //     two blocks a SM; bound by the issue of the splits and products at 16 rows.
-//   fp32 caches, one or two rows: 32 D / 1024 lanes a key for the scores, four dims a lane for the
-//     output, p through shared memory; packed FMAs. Two stages of three blocks a SM.
+//   fp32 caches, one or two rows (where no log-sum-exp is asked for): 32 D / 1024 lanes a key for the scores,
+//     four dims a lane for the output, p through shared memory; packed FMAs. Two stages of three blocks a SM.
 //     By FMAs and by products, 32 sequences of 100 to 8000 keys, four key heads, in us: one row 61 and
-//     64 (d 64), 107 and 120 (d 128), two rows 63 and 65, 115 and 121, four rows 79 and 65, 148 and 122,
-//     eight rows 121 and 66, 241 and 125; 16 rows, in blocks of 8 and of 16: 222 and 92, 461 and 169; one
-//     row of 64 sequences over 240 keys 11.7 and 17.
+//     64 (d 64), 107 and 120 (d 128), two rows 63 and 65, 115 and 121, four rows 79 and 66, 148 and 125,
+//     eight rows 121 and 67, 241 and 129; 16 rows, in blocks of 8 and of 16: 222 and 92, 461 and 171; one
+//     row of 64 sequences over 240 keys 11.7 and 16. (Training takes the products: the backward's scores.)
 // On one B200, with the join: 64 sequences of up to 8192 keys, 32 heads over 8, [page 16] bf16, d = 128
 // 196 us (5.7 TB/s); 2 of 131071 keys, fp32 over bf16, d = 64 55 us; 16 of 1000 to 6000 keys, 16 heads,
 // fp32, d = 64 79 us (5.9 TB/s). One sequence of 240 keys: 6.9 us.
@@ -1243,7 +1243,6 @@ __global__ void __launch_bounds__(NT, 2) split_f32_kernel(const SplitArgs a) {
   using R = RingOf<D, 4, 8 * HALVES>;
   constexpr int ST = R::ST, TK = R::TK;
   constexpr int NK = TK / 8, J = D / 16, JV = D / 32;
-  constexpr int CH = NK == 1 ? 2 : 1;          // chains of a score's large products (and of its small ones)
   constexpr int JQ = HALVES == 1 ? J : (J + WARPS - 1) / WARPS;  // this warp's share of q's columns
   extern __shared__ __align__(128) unsigned char smem[];
   const int tid = threadIdx.x, w = tid >> 5, lane = tid & 31;
@@ -1341,15 +1340,15 @@ __global__ void __launch_bounds__(NT, 2) split_f32_kernel(const SplitArgs a) {
       const unsigned char* vt = kt + R::KV;
       const int k0 = n.lo + TK * t;
 
-      // Scores: rows g, g + 8; keys 8 i + 2 t4, + 1. The small products in chains of their own,
-      // truncated at their magnitude.
-      float ch[NK][CH][4], cl[NK][CH][4];
+      // Scores: rows g, g + 8; keys 8 i + 2 t4, + 1, in sums of 16 dims, their products and additions in
+      // cross_few_bwd.cu's order: its e^(s - L) is then what L was made of. (With the dims in one chain of
+      // products, truncated at its own magnitude, and one or two rows by FMAs in training too, dV at scores of
+      // a hundred was 1e-5 off where it is 2e-6 now; 8 rows 126 us for 129 at d 128, 66.1 for 66.6 at 64.)
+      float s[NK][2 * HALVES];
 #pragma unroll
       for (int i = 0; i < NK; ++i)
 #pragma unroll
-        for (int x = 0; x < CH; ++x)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) ch[i][x][e] = cl[i][x][e] = 0.0f;
+        for (int x = 0; x < 2 * HALVES; ++x) s[i][x] = 0.0f;
       const unsigned char* ka = kt + g * R::RB + 16 * (t4 ^ (4 * (g & 1)));
       const unsigned char* kb = kt + g * R::RB + 16 * (t4 ^ (4 * (~g & 1)));
 #pragma unroll
@@ -1368,30 +1367,30 @@ __global__ void __launch_bounds__(NT, 2) split_f32_kernel(const SplitArgs a) {
         }
 #pragma unroll
         for (int i = 0; i < NK; ++i) {
-          uint32_t kh[4], kl[4];
-          split_tf32(*reinterpret_cast<const float4*>((j & 1 ? kb : ka) + 8 * i * R::RB + 128 * (j >> 1)),
-                     kh, kl);
+          const float4 key = *reinterpret_cast<const float4*>((j & 1 ? kb : ka) + 8 * i * R::RB + 128 * (j >> 1));
+          float c[4] = {0.f, 0.f, 0.f, 0.f};
+          if constexpr (HALVES == 2) {
+            products(c, ah, al, key);
 #pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            if constexpr (HALVES == 2) mma_tf32(cl[i][x % CH], al[x], kh[2 * x], kh[2 * x + 1]);
-            mma_tf32(cl[i][x % CH], ah[x], kl[2 * x], kl[2 * x + 1]);
-            mma_tf32(ch[i][x % CH], ah[x], kh[2 * x], kh[2 * x + 1]);
+            for (int x = 0; x < 4; ++x) s[i][x] += c[x];
+          } else {
+            uint32_t kh[4], kl[4];
+            float cl[4] = {0.f, 0.f, 0.f, 0.f};
+            split_tf32(key, kh, kl);
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              mma_tf32(cl, ah[x], kl[2 * x], kl[2 * x + 1]);
+              mma_tf32(c, ah[x], kh[2 * x], kh[2 * x + 1]);
+            }
+#pragma unroll
+            for (int x = 0; x < 2; ++x) s[i][x] += (c[2 + x] + cl[x]) + c[x];  // (not both small parts: cl[2 + x])
           }
         }
       }
-      float s[NK][2 * HALVES];
 #pragma unroll
       for (int i = 0; i < NK; ++i)
 #pragma unroll
-        for (int x = 0; x < 2 * HALVES; ++x) {
-          float small = cl[i][0][x], large = ch[i][0][x];
-          if constexpr (CH == 2) small += cl[i][CH - 1][x], large += ch[i][CH - 1][x];
-          if constexpr (HALVES == 1) {
-            small += ch[i][0][2 + x] + cl[i][0][2 + x];
-            if constexpr (CH == 2) small += ch[i][CH - 1][2 + x] + cl[i][CH - 1][2 + x];
-          }
-          s[i][x] = (small + large) * a.scale;
-        }
+        for (int x = 0; x < 2 * HALVES; ++x) s[i][x] *= a.scale;
       // (behind the products: their latency hides the next loads' issue)
       const unsigned now = ring.advance(stage == 0 ? ST - 1 : stage - 1);
       const bool edge = lim_min < min(k0 + TK, n.hi);
@@ -1680,8 +1679,8 @@ cudaError_t launch_d(const SplitArgs& a, int qd, int kd, cudaStream_t stream) {
   cudaError_t e;
   if (qd == CFA_F32) {
     if (kd == CFA_F32) {
-      e = a.rows == 1         ? launch_split<split_fma_kernel<D, 1>>(split_smem<D, 4, 1>(), a, stream)
-          : a.rows == 2       ? launch_split<split_fma_kernel<D, 2>>(split_smem<D, 4, 2>(), a, stream)
+      e = a.rows == 1 && !a.lse   ? launch_split<split_fma_kernel<D, 1>>(split_smem<D, 4, 1>(), a, stream)
+          : a.rows == 2 && !a.lse ? launch_split<split_fma_kernel<D, 2>>(split_smem<D, 4, 2>(), a, stream)
           : a.block_rows == 8 ? launch_split<split_f32_kernel<D, 1>>(split_smem<D, 4, 8>(), a, stream)
                               : launch_split<split_f32_kernel<D, 2>>(split_smem<D, 4, 16>(), a, stream);
     } else if (kd == CFA_F16) {

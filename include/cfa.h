@@ -329,7 +329,8 @@ int cfa_cross_bwd_f32(const float* q, const int64_t q_strides[3],
 
 /* The forward for few query rows a key head (single tokens): the same contract, split over the keys;
  * lse may be NULL. Any seq is right; past 16 rows a key head (seq * heads / key_heads) the keys are
- * read once for every 16. */
+ * read once for every 16. With an lse its scores are those of cfa_cross_bwd_f32 for up to 32 rows a key
+ * head, so that the weights e^(score - lse) there sum to one: a backward of so few rows takes this lse. */
 size_t cfa_cross_few_workspace_bytes(int64_t batch, int64_t heads, int64_t seq, int64_t key_seq,
                                      int64_t head_dim);
 int cfa_cross_few_f32(const float* q, const int64_t q_strides[3],

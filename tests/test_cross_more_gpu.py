@@ -1,12 +1,15 @@
 # SPDX-License-Identifier: MIT OR Apache-2.0
 """Cross attention at the sizes and scales that tests/test_cross_gpu.py leaves out; its band."""
 
+import math
+
 import pytest
 import torch
 
 import candle_fused_attn as cfa
 from candle_fused_attn import _abi
-from test_cross_gpu import check
+import formulas as ref
+from test_cross_gpu import check, run
 
 pytestmark = pytest.mark.gpu
 
@@ -72,4 +75,53 @@ def test_backward_without_room_for_its_partials(cuda):
     finally:
         torch.cuda.set_per_process_memory_fraction(1.0)
     assert all(torch.equal(a, c) for a, c in zip(got, want))
+    cfa.check_status()
+
+
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("h,hk,sq", [(2, 2, 1), (2, 2, 2), (4, 1, 2), (4, 2, 7), (2, 2, 32), (2, 2, 70)])
+@pytest.mark.parametrize("scale", [0.0, -0.125, 0.3, 1.0, 4.0])
+def test_scales_of_every_kernel(cuda, d, h, hk, sq, scale):
+    """Scores of up to a few hundreds, zero and negative scales, for every pair of kernels.
+
+    A score is off by delta = 44 u sum |q| |k| |scale|, u = 2^-24: two tf32 parts leave out 3 2^-22 = 12 u of a
+    product, short sums of 16 truncated steps 32 u (the three-part pair: 26 u in all). P = e^(s - L) is then off
+    by 2 delta (s and L), and dS = P (dP - D) by that of both its terms' absolute values, D once more by o's 2
+    delta: 4 delta of the formulas with absolute values, and the sums of the products themselves (64 + n) u.
+    Weights below fp32's smallest normal number, 2^-126, are zero: at scale 4 scores lie more than 87 below
+    their row's largest, and what such a weight multiplies is below 2^20 here (|g| |v| d, |q| or |k|, scale)."""
+    (q, k, v, dout, scale, _), _, o, grads = run(cuda, 2, h, hk, sq, 90, d, [90, 33], seed=d + sq, scale=scale)
+    clean = [torch.nan_to_num(t, nan=0.0) for t in (k, v)]
+    want, size = ref.cross(q, *clean, scale, [90, 33], dout)
+    group = h // hk
+    top = torch.matmul(q.double().abs(), clean[0].double().abs().repeat_interleave(group, 1).transpose(2, 3)).max()
+    u = 2.0 ** -24
+    rel = math.expm1(4 * 44 * u * float(top) * abs(scale)) + (64 + 90 + group * sq) * u
+    for name, g, w, a in zip(("o", "dq", "dk", "dv"), (o, *grads), want, size):
+        err = (g.detach().cpu().double() - w).abs()
+        assert bool((err <= rel * a + 2.0 ** (20 - 126)).all()), f"{name}: {float((err / a.clamp_min(1e-300)).max()):.2e} of {rel:.2e}"
+
+
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("sq", [1, 2, 5, 8, 9, 20, 32, 70])
+def test_large_scores_have_weights_that_sum_to_one(cuda, d, sq):
+    """The backward's weights e^(s - L), at scores near a hundred: their sum over the keys (what dV sums to for
+    gradients of one) is off from the number of rows only by what L and the forward's scaled scores are rounded
+    by, half a step of L each. Two uniform roundings are sqrt(2 / 3) of that in the mean square, 1.3 with what
+    else there is (2^x, a quarter at this size). Scores summed in another order would be off by far more.
+
+    One query row a head and batch element, or (from two on) rows that are copies of one another."""
+    b, h, n = 40, 4, 90
+    g = torch.Generator().manual_seed(d + sq)
+    q = torch.randn(b, h, 1, d, generator=g).expand(b, h, sq, d)
+    k, v = (torch.randn(b, h, n, d, generator=g) for _ in range(2))
+    scale = 32.0 / math.sqrt(d)
+    L = torch.logsumexp((q[:, :, :1].double() @ k.double().transpose(2, 3)) * scale, -1)
+    x = [t.to(cuda).requires_grad_(True) for t in (q, k, v)]
+    o = cfa.cross_attention(*x, scale)
+    dv, = torch.autograd.grad(o, x[2], torch.ones_like(o))
+    total = dv[..., 0].cpu().double().sum(2) / sq
+    step = 2.0 ** (torch.floor(torch.log2(L.abs())) - 24).squeeze(-1)
+    off = (((total - 1.0) / step) ** 2).mean().sqrt()
+    assert float(L.min()) > 16 and float(off) <= 1.3, float(off)
     cfa.check_status()
