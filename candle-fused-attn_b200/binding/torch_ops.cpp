@@ -66,8 +66,7 @@ struct Gil {
   PyErr_SetString(error_class, message.c_str());
   throw_python();
 }
-// Pieces of a message. (Not by a stream: a number through one crashed here, in a process whose libraries
-// bring C++ runtimes of their own.)
+// Pieces of a message.
 std::string text(const char* s) { return s; }
 std::string text(int64_t n) { return std::to_string(n); }
 std::string text(at::IntArrayRef sizes) {

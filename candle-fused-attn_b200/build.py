@@ -92,13 +92,21 @@ def build_host(force: bool = False, verbose: bool = False) -> Path:
     return HOST_OUT
 
 
+def cxx_runtime() -> list[str]:
+    """The shared libstdc++ of this process, which torch runs on. A compiler that has only a static one would
+    give the extension a C++ runtime of its own: its exceptions are caught by torch's, and a number written to
+    a stream crashed on the other one's locale."""
+    with open("/proc/self/maps") as f:
+        return sorted({line.split()[-1] for line in f if "/libstdc++.so" in line})
+
+
 def build_ops(force: bool = False, verbose: bool = False) -> Path:
     """_ops.so: binding/torch_ops.cpp against the headers and libraries of the installed torch (which is
     loaded before it, so no path to them is kept; a torch newer than the extension rebuilds it)."""
     import torch
 
     base = Path(torch.__file__).resolve().parent
-    deps = [OPS_SOURCE, ROOT / "include" / "cfa.h", base / "version.py"]
+    deps = [OPS_SOURCE, ROOT / "include" / "cfa.h", base / "version.py", Path(__file__)]
     if not force and OPS_OUT.exists() and all(
             p.stat().st_mtime <= OPS_OUT.stat().st_mtime for p in deps):
         return OPS_OUT
@@ -109,7 +117,7 @@ def build_ops(force: bool = False, verbose: bool = False) -> Path:
            "-isystem", str(base / "include" / "torch" / "csrc" / "api" / "include"),
            "-isystem", str(cuda / "include"), "-isystem", sysconfig.get_paths()["include"],
            "-o", str(OPS_OUT), str(OPS_SOURCE), "-L", str(base / "lib"), "-ltorch_python", "-ltorch",
-           "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda"]
+           "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda", *cxx_runtime()]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if verbose or r.returncode != 0:
         sys.stderr.write(r.stdout + r.stderr)

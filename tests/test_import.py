@@ -2,9 +2,12 @@
 """Importing the package loads no native library; the operators' extension is loaded by the first call of
 one of them, and without it the rest works."""
 
+import shutil
 import subprocess
 import sys
 from pathlib import Path
+
+import pytest
 
 PACKAGE = Path(__file__).resolve().parents[1] / "candle-fused-attn_b200"
 
@@ -75,3 +78,16 @@ ts = [threading.Thread(target=call) for _ in range(8)]
 print(seen)
 """)
     assert out.count("FusedAttentionError") == 8
+
+
+def test_the_extension_has_no_cxx_runtime_of_its_own():
+    """It throws what torch catches: one libstdc++ in the process, none inside the extension."""
+    readelf = shutil.which("readelf")
+    if readelf is None:
+        pytest.skip("no readelf")
+    lib = str(PACKAGE / "candle_fused_attn" / "_ops.so")
+    needed = subprocess.run([readelf, "-dW", lib], capture_output=True, text=True, check=True).stdout
+    assert "[libstdc++.so.6]" in needed
+    names = subprocess.run([readelf, "--dyn-syms", "-W", lib], capture_output=True, text=True, check=True).stdout
+    own = [x.split()[-1] for x in names.splitlines() if "__cxa_throw" in x or "_ZNSt6locale" in x]
+    assert own and all(" UND " in x for x in names.splitlines() if "__cxa_throw" in x or "_ZNSt6locale" in x), own
