@@ -1,6 +1,10 @@
 # SPDX-License-Identifier: MIT OR Apache-2.0
 """What autograd sees of the operators on the GPU: second derivatives, in-place writes."""
 
+import subprocess
+import sys
+from pathlib import Path
+
 import pytest
 import torch
 
@@ -70,3 +74,33 @@ def test_append_into_inference_tensors(cuda):
     cfa.paged_append(x, x, k, v, table, lengths)
     assert torch.equal(k[1, 0], x[0, :, 0]) and torch.equal(v[1, 0], x[0, :, 0])
     cfa.check_status()
+
+
+@pytest.mark.parametrize("op", ["cross", "rotary"])
+def test_a_failed_capture_is_an_error(cuda, op):
+    """A backward captured while an eager graph of the same leaf lives: torch synchronises with the stream of
+    that graph's gradient node, which ends the capture (plain operations fare alike). It has to come out as an
+    error, and calls have to go on."""
+    package = Path(__file__).resolve().parents[1] / "candle-fused-attn_b200"
+    code = f"""
+import sys, warnings; sys.path.insert(0, {str(package)!r}); warnings.simplefilter("ignore")
+import torch, candle_fused_attn as cfa
+freqs, _ = cfa.rotary_frequencies(64)
+k = torch.randn(1, 2, 90, 64, device="cuda")
+op = dict(cross=lambda x: cfa.cross_attention(x, k, k, 0.1), rotary=lambda x: cfa.rotary(x, 3, freqs))[{op!r}]
+x = torch.randn(1, 2, 40, 64, device="cuda", requires_grad=True)
+want, = torch.autograd.grad(op(x).square().sum(), x)
+eager = op(x)
+try:
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        op(x).square().sum().backward()
+except RuntimeError as e:
+    print("refused")
+eager.square().sum().backward()
+x.grad = None
+op(x).square().sum().backward()
+cfa.check_status()
+print("same" if torch.equal(x.grad, want) else "other")
+"""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and r.stdout.endswith("same\n"), r.stdout + r.stderr
