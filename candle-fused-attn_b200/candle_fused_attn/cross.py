@@ -19,7 +19,9 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: fl
     strides (rows that are not 16-byte aligned are copied first); heads a multiple of key_heads:
     query head i reads key head i // (heads // key_heads). `key_lengths`: int32 [batch] on the
     device, how many keys each batch element has (values are held within 0 .. sk); what lies behind
-    them is not read into any result, and a query without a key gives zeros and no gradient.
+    them is not read into any result, and a query without a key gives zeros and no gradient. What a
+    query does see is to be finite (operands enter the tensor cores in parts, and with an infinity the
+    result may be NaN where the formula has a value, in its own batch element).
     -> [batch, heads, sq, d], laid out as a dense [batch, sq, heads, d].
 
     Differentiable in q, k and v (dk, dv of a shared head are summed over its query heads). Few

@@ -55,7 +55,10 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     cache's key heads. Query i of a sequence's n (n = s, or new_lengths[b]) sees its first
     lengths[b] - n + i + 1 keys: all of them for a single token. The cache's rows must be 16-byte
     aligned. -> [batch, heads, s, d], laid out as a dense [batch, s, heads, d], of q's type; zeros
-    where a query sees no key or a padded row is no query. The keys are split into chunks by the
+    where a query sees no key or a padded row is no query. What a query sees is to be finite (with an
+    infinity the result may be NaN where the formula has a value, in its own sequence; what none sees
+    may be anything).
+    The keys are split into chunks by the
     sequence's own length and joined in order: bit-identical across reruns and batches. Softmax
     statistics and sums are fp32. No gradients.
     """

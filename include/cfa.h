@@ -296,8 +296,10 @@ int cfa_matmul_status(void* stream);
  * [batch, key_heads, key_seq, head_dim], the (batch, head, seq) strides as for cfa_fwd_f32 (16-byte
  * rows); head_dim 32, 64 or 128; heads a multiple of key_heads (query head h reads key head
  * h / (heads / key_heads)). key_lengths: [batch] int32 on the device, the keys of each batch element
- * (held within 0 .. key_seq), or NULL: all; what lies behind them is never read into a result. A
- * row without a key: O = 0, L = -inf, no gradient. o: [batch, seq, heads, head_dim] dense; lse
+ * (held within 0 .. key_seq), or NULL: all; what lies behind them is never read into a result. What a
+ * row does see is to be finite: operands enter the products in parts, and with an infinity (or a number that
+ * rounds to one in 11 bits) the result may be NaN where the formula has a value, in its own batch
+ * element. A row without a key: O = 0, L = -inf, no gradient. o: [batch, seq, heads, head_dim] dense; lse
  * [batch, heads, seq] dense. Tensor-core kernels. */
 int cfa_cross_fwd_f32(const float* q, const int64_t q_strides[3],
                       const float* k, const int64_t k_strides[3],
@@ -380,7 +382,8 @@ int cfa_paged_append(const void* q, const int64_t q_strides[3], void* q_out,
  * i of n sees the sequence's first lengths[b] - n + i + 1 keys. q [batch, heads, seq, head_dim] of
  * `dtype`, 16-byte rows; o [batch, seq, heads, head_dim] dense, of `dtype`; rows that see nothing or
  * are no token: zeros. head_dim 32, 64 or 128; the cache's rows 16-byte aligned; types and heads as
- * above. Sums and softmax statistics are fp32. Keys on a bad page are left out and reported
+ * above. Sums and softmax statistics are fp32; visible keys and values are to be finite, as for
+ * cfa_cross_fwd_f32. Keys on a bad page are left out and reported
  * (cfa_page_sink), and so is a length past the table. Workspace (256-byte aligned, no initialisation)
  * for max_keys = table_width * page_size. */
 size_t cfa_paged_attention_workspace_bytes(int64_t batch, int64_t heads, int64_t seq,

@@ -125,3 +125,25 @@ def test_large_scores_have_weights_that_sum_to_one(cuda, d, sq):
     off = (((total - 1.0) / step) ** 2).mean().sqrt()
     assert float(L.min()) > 16 and float(off) <= 1.3, float(off)
     cfa.check_status()
+
+
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("sq", [1, 7, 40])
+def test_a_visible_infinity_stays_in_its_batch_element(cuda, d, sq):
+    """In outputs and gradients: an infinite value or key of one element leaves the others their bits."""
+    g = torch.Generator().manual_seed(sq)
+    x = [torch.randn(3, 2, s, d, generator=g).to(cuda) for s in (sq, 90, 90)]
+    dout = torch.randn(3, 2, sq, d, generator=g).to(cuda)
+
+    def step():
+        y = [t.clone().requires_grad_(True) for t in x]
+        o = cfa.cross_attention(*y, 0.125)
+        return (o.detach(), *torch.autograd.grad(o, y, dout))
+
+    want = step()
+    for which in (1, 2):
+        x[which][1, 0, 40, 5] = math.inf
+        got = step()
+        x[which][1, 0, 40, 5] = 0.0
+        assert all(torch.equal(a[[0, 2]], c[[0, 2]]) for a, c in zip(got, want))
+    cfa.check_status()

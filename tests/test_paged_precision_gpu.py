@@ -71,3 +71,28 @@ def test_a_tail_of_small_weights_over_fp16_counts(cuda, qt, d, h):
     if qt == F16:
         lim = lim + torch.finfo(F16).eps / 2 * want + 2.0 ** -25
     assert bool(((o - want).abs() <= lim).all()), float(((o - want).abs() / lim).max())
+
+
+@pytest.mark.parametrize("qt,kt", [(F32, F32), (F32, BF16), (F32, F16), (F16, F16), (BF16, BF16)])
+@pytest.mark.parametrize("h", [1, 2, 8, 24])
+def test_a_visible_infinity_stays_in_its_sequence(cuda, qt, kt, h):
+    """An infinite value: its dim of that sequence is not finite, everything else as without it. An infinite
+    key (scores of both signs: a weight of zero, or none that is defined): the other sequences as without it."""
+    g = torch.Generator().manual_seed(h)
+    k, v = ([torch.randn(1, n, 64, generator=g).to(kt) for n in (100, 100, 700)] for _ in range(2))
+    q = torch.randn(3, h, 1, 64, generator=g).to(qt).to(cuda)
+
+    def attend():
+        kc, vc, table, lengths = (t.to(cuda) for t in ref.paged(k, v, 16, torch.Generator().manual_seed(1), kt))
+        return cfa.paged_attention(q, kc, vc, table, lengths, 0.125)
+
+    want = attend()
+    v[1][0, 40, 7] = math.inf
+    got = attend()
+    assert not got[1, :, 0, 7].isfinite().any()
+    got[1, :, 0, 7] = want[1, :, 0, 7]
+    assert torch.equal(got, want)
+    v[1][0, 40, 7] = 0.0
+    k[1][0, 40, 7] = math.inf
+    assert torch.equal(attend()[[0, 2]], want[[0, 2]])
+    cfa.check_status()
