@@ -25,7 +25,8 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, *, scaling: str |
       the fastest left alone);
     - "yarn": by the turns a frequency makes over `original_length` positions: above beta_fast as it
       is, below beta_slow divided by factor, linear in the turns between; amplitude
-      0.1 ln(factor) + 1.
+      0.1 ln(factor) + 1. (A model trained with a ramp over the index j between rounded bounds has
+      other frequencies in between: pass its own as `freqs`.)
     """
     who = "rotary_frequencies"
     require(rotary_dim > 0 and rotary_dim % 2 == 0, who,

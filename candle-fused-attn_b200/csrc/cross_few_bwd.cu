@@ -6,12 +6,14 @@
 //   dV = P^T dO and dK = scale dS^T Q, whole, to memory; dQ += dS K in registers,
 // the block's dQ partial summed over its warps in order, the key blocks' by cross_join_kernel. Products by
 // mma.m16n8k8 on two-part tf32 operands (tf32.cuh; hi hi + hi lo + lo hi), the keys as the 16 rows, the
-// queries as columns; a score's products and sums in the order of the forward that made L (split_attn.cu); P^T's and dS^T's fragments are those of the scores, dS's rows go through shared memory.
+// queries as columns; a score's products and sums in the order of the forward that made L (split_attn.cu).
+// P^T's and dS^T's fragments are those of the scores, dS's rows go through shared memory.
 //
-// Bound by memory up to 16 rows: K, V are read and dK, dV written once, at 20 rows D flops a key against
-// 16 D bytes; at 32 by the products' issue. The tcgen05 pair, whose tiles are 64 queries, spends a block's
-// first loads, splits and last stores on 128 keys: [34, 24 over 8, 10, 64] over 1000 to 2000 keys 219 us here,
-// 332 there; [32, 8, 32, 64] over 500 to 1000 108 and 161.
+// K, V are read and dK, dV written once, at 20 rows D flops a key against 16 D bytes: 4.3 TB/s at 8 rows
+// ([32, 8, 8, 64] over 1000 keys, 61 us), 3.3 at 16, 2.1 at 30, where the products' issue bounds it. The
+// tcgen05 pair, whose tiles are 64 queries, spends a block's first loads, splits and last stores on 128 keys:
+// [34, 24 over 8, 10, 64] over 1000 to 2000 keys 219 us here, 332 there; [32, 8, 32, 64] over 500 to 1000 108
+// and 161.
 #include "cfa_common.cuh"
 #include "tf32.cuh"
 

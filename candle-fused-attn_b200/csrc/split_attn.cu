@@ -576,7 +576,8 @@ __global__ void __launch_bounds__(NT, 2)
         }
     }
     const int lim0 = row_limit(a, n, n.r0 + 2 * qc), lim1 = row_limit(a, n, n.r0 + 2 * qc + 1);
-    // The fewest keys that a row of the block sees: a tile that ends behind it masks row by row.
+    // What the sequence's first new token sees, the fewest of all: a tile that ends behind it masks row by
+    // row, in every block (a prompt's every tile: its value products are then issued once a row).
     const int lim_min = a.causal ? max(n.len - n.n_new + 1, 0) : n.len;
 
     float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
@@ -870,7 +871,8 @@ __global__ void __launch_bounds__(NT, 2) split_rows_kernel(const SplitArgs a) {
     const int tiles = (n.hi - n.lo + TK - 1) / TK;
     const float qscale[2] = {a.scale * up[0], a.scale * up[1]};
     const int lim[2] = {row_limit(a, n, n.r0 + g), row_limit(a, n, n.r0 + g + 8)};
-    // The fewest keys that a row of the block sees: a tile that ends behind it masks row by row.
+    // What the sequence's first new token sees, the fewest of all: a tile that ends behind it masks row by
+    // row, in every block (a prompt's every tile: its value products are then issued once a row).
     const int lim_min = a.causal ? max(n.len - n.n_new + 1, 0) : n.len;
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
     float acc[KS][2][4];  // rows g, g + 8: dims 16 mt + 8 y + 2 t4, + 1
@@ -1320,7 +1322,8 @@ __global__ void __launch_bounds__(NT, 2) split_f32_kernel(const SplitArgs a) {
     int lim[HALVES];
 #pragma unroll
     for (int h = 0; h < HALVES; ++h) lim[h] = row_limit(a, n, n.r0 + g + 8 * h);
-    // The fewest keys that a row of the block sees: a tile that ends behind it masks row by row.
+    // What the sequence's first new token sees, the fewest of all: a tile that ends behind it masks row by
+    // row, in every block (a prompt's every tile: its value products are then issued once a row).
     const int lim_min = a.causal ? max(n.len - n.n_new + 1, 0) : n.len;
     float m[HALVES], l[HALVES];
     float acc[JV][4][2 * HALVES];  // rows g (, g + 8): dims 32 j + 8 t4 + e (, + 4)
