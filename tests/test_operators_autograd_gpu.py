@@ -9,6 +9,7 @@ import pytest
 import torch
 
 import candle_fused_attn as cfa
+from candle_fused_attn import _abi
 
 pytestmark = pytest.mark.gpu
 
@@ -104,3 +105,33 @@ print("same" if torch.equal(x.grad, want) else "other")
 """
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and r.stdout.endswith("same\n"), r.stdout + r.stderr
+
+
+@pytest.mark.parametrize("op", ["cross", "rotary"])
+def test_an_error_in_a_backward_is_raised(cuda, op):
+    """A bounded wait of an earlier kernel expires between forward and backward: the backward, in autograd's own
+    thread, raises what a call does, and the next one runs."""
+    freqs, _ = cfa.rotary_frequencies(64, device=cuda)
+    x = torch.randn(1, 2, 40, 64, device=cuda, requires_grad=True)
+    o = cfa.cross_attention(x, x, x, 0.1) if op == "cross" else cfa.rotary(x, 3, freqs)
+    want, = torch.autograd.grad(o.square().sum(), x, retain_graph=True)
+    ws = torch.zeros(256, dtype=torch.uint8, device=cuda)
+    stream = torch.cuda.current_stream().cuda_stream
+    assert _abi.selftest_bounded_wait(ws.data_ptr(), 20_000_000, 2, stream) == _abi.CFA_OK
+    torch.cuda.synchronize()
+    with pytest.raises(cfa.FusedAttentionError, match="expired"):
+        torch.autograd.grad(o.square().sum(), x, retain_graph=True)
+    got, = torch.autograd.grad(o.square().sum(), x)
+    assert torch.equal(got, want)
+    cfa.check_status()
+
+
+def test_function_transforms_are_refused(cuda):
+    """Tensors of torch.func have no memory of their own: an error, not a wrong result."""
+    freqs, _ = cfa.rotary_frequencies(64, device=cuda)
+    x = torch.randn(2, 1, 2, 9, 64, device=cuda)
+    for call in (lambda t: cfa.cross_attention(t, t, t, 0.1), lambda t: cfa.rotary(t, 3, freqs)):
+        for run in (lambda: torch.vmap(call)(x), lambda: torch.func.grad(lambda t: call(t).sum())(x[0]),
+                    lambda: torch.func.jvp(call, (x[0],), (x[0],))):
+            with pytest.raises(RuntimeError):
+                run()
